@@ -133,7 +133,7 @@ def _quantised(x):
     """int8 codes and the f32 scale of each last-dimension row."""
     a = x.abs().amax(-1, keepdim=True)
     zero = a < MIN_AMAX
-    code = torch.where(zero, torch.zeros_like(x), torch.round(x * (127.0 / a.masked_fill(zero, 1.0))))
+    code = torch.where(zero, torch.zeros_like(x), torch.round(x * (torch.full_like(a, 127.0) / a.masked_fill(zero, 1.0))))
     return code.to(torch.int8), torch.where(zero, torch.zeros_like(a), a / 127.0)[..., 0]
 
 
