@@ -6,6 +6,14 @@ this package is its tensor-level host binding, mirroring the reference's public 
 """
 from ._lib import Iq2Error, LIB_PATH
 from .activation_quant import ActivationQuantConfig, ActivationQuantMode
+from .attention import (
+    KvCache,
+    attention_decode,
+    attention_decode_workspace_bytes,
+    attention_prefill,
+    kv_cache_read,
+    kv_cache_write,
+)
 from .iq2_matmul import (
     Iq2MatmulOp,
     Iq2MatmulVariant,
@@ -29,7 +37,11 @@ __all__ = [
     "Iq2Error",
     "Iq2MatmulOp",
     "Iq2MatmulVariant",
+    "KvCache",
     "LIB_PATH",
+    "attention_decode",
+    "attention_decode_workspace_bytes",
+    "attention_prefill",
     "device_check",
     "iq2_dequantize",
     "iq2_dequantize_to_f16",
@@ -41,5 +53,7 @@ __all__ = [
     "iq2_xs_matmul",
     "iq2_xxs_matmul",
     "iq3_s_matmul",
+    "kv_cache_read",
+    "kv_cache_write",
     "workspace_bytes",
 ]

@@ -26,6 +26,7 @@ IQ2_ERR_TIMEOUT = 11
 IQ2_COMM_ID_BYTES = 128
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
+KV_INT8 = 3
 ACT_QUANT_OFF, ACT_QUANT_W8A8, ACT_QUANT_W4A8 = 0, 1, 2
 
 # Every symbol the headers (include/candelora_iq2.h, include/candelora_iq2_testing.h) declare,
@@ -55,6 +56,12 @@ SIGNATURES = {
     "iq2_comm_check": ([_vp], _int),
     "iq2_matmul_grouped_sharded_workspace_size": ([_vp, _u32, _u32, _int, _int], _sz),
     "iq2_matmul_grouped_sharded": ([_vp, _vp, _u32, _u32, _int, _vp, _sz, _vp], _int),
+    "iq2_kv_cache_write": ([_vp, _vp, _vp], _int),
+    "iq2_kv_cache_read": ([_vp, _vp, _u32, _u32, _vp, _vp, _u32, _vp, _vp, _int, _vp], _int),
+    "iq2_attention_prefill_workspace_size": ([_vp], _sz),
+    "iq2_attention_prefill": ([_vp, _vp, _sz, _vp], _int),
+    "iq2_attention_decode_workspace_size": ([_vp, _u32, _u32], _sz),
+    "iq2_attention_decode": ([_vp, _vp, _vp, _sz, _vp], _int),
 }
 
 
@@ -64,6 +71,42 @@ class Iq2MatmulProblem(ctypes.Structure):
     _fields_ = [("x", ctypes.c_void_p), ("weight_bytes", ctypes.c_void_p), ("weight_bytes_len", ctypes.c_size_t),
                 ("weight_scales", ctypes.c_void_p), ("weight_scales_len", ctypes.c_size_t),
                 ("out_dim", ctypes.c_uint32), ("in_dim", ctypes.c_uint32), ("out", ctypes.c_void_p)]
+
+
+class KvCacheStruct(ctypes.Structure):
+    """struct iq2_kv_cache."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("num_pages", _u32), ("kv_heads", _u32),
+                ("page_size", _u32), ("head_dim", _u32), ("dtype", _int)]
+
+
+class Rows(ctypes.Structure):
+    """struct iq2_rows."""
+
+    _fields_ = [("data", _vp), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class KvTokens(ctypes.Structure):
+    """struct iq2_kv_tokens."""
+
+    _fields_ = [("k", Rows), ("v", Rows), ("q", Rows), ("dtype", _int), ("tokens", _u32), ("q_heads", _u32),
+                ("slots", _vp), ("positions", _vp), ("cos", _vp), ("sin", _vp), ("rope_len", _u32),
+                ("interleaved", _int), ("q_out", _vp), ("q_out_dtype", _int)]
+
+
+class AttentionPrompts(ctypes.Structure):
+    """struct iq2_attention_prompts."""
+
+    _fields_ = [("q", Rows), ("k", Rows), ("v", Rows), ("dtype", _int), ("sequences", _u32), ("q_tokens", _u32),
+                ("k_tokens", _u32), ("q_heads", _u32), ("kv_heads", _u32), ("head_dim", _u32), ("cu_seqlens_q", _vp),
+                ("cu_seqlens_k", _vp), ("causal", _int), ("scale", ctypes.c_float), ("out", _vp)]
+
+
+class AttentionTokens(ctypes.Structure):
+    """struct iq2_attention_tokens."""
+
+    _fields_ = [("q", Rows), ("dtype", _int), ("batch", _u32), ("q_heads", _u32), ("table_width", _u32),
+                ("block_table", _vp), ("seq_lens", _vp), ("scale", ctypes.c_float), ("out", _vp)]
 
 
 class Iq2Error(RuntimeError):

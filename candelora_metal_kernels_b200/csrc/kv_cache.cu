@@ -1,0 +1,233 @@
+// The paged key-value cache: the write of new tokens (with the rotation of q and k, and the quantisation of an int8
+// cache) and the read of cached tokens back into packed tensors. Both move each byte once and are bound by HBM.
+//
+// Rotation, for the pair (a, b) = (x[i], x[i + d/2]) ("half") or (x[2i], x[2i + 1]) (interleaved):
+//     a' = a c - b s,  b' = b c + a s,  c = cos[position][i], s = sin[position][i],
+// with every product and sum rounded by itself in f32, so that a result does not depend on how the compiler fuses.
+// int8 rows (one token and head): m = max |x|, scale = m / 127, code = rint(x * (127 / m)); m < 2^-100 gives zeros (the
+// quotient would overflow), and a row with an infinity or NaN gets a NaN scale, so that it reads back as NaN.
+#include "attention_internal.h"
+#include "iq2xxs_common.cuh"
+
+#include <algorithm>
+
+namespace iq2 {
+
+namespace {
+
+constexpr int KW_THREADS = 256;
+constexpr float MIN_AMAX = 7.88860905e-31f;  // 2^-100
+
+__device__ __forceinline__ float4 load4(const void* base, int64_t i, int dtype, bool vec) {
+    if (dtype == kF32) {
+        const float* p = static_cast<const float*>(base) + i;
+        if (vec) return __ldg(reinterpret_cast<const float4*>(p));
+        return make_float4(p[0], p[1], p[2], p[3]);
+    }
+    const uint16_t* p = static_cast<const uint16_t*>(base) + i;
+    uint32_t lo, hi;
+    if (vec) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+        lo = w.x, hi = w.y;
+    } else {
+        lo = p[0] | ((uint32_t)p[1] << 16), hi = p[2] | ((uint32_t)p[3] << 16);
+    }
+    if (dtype == kF16) {
+        const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+        return make_float4(a.x, a.y, b.x, b.y);
+    }
+    return make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u), __uint_as_float(hi << 16),
+                       __uint_as_float(hi & 0xFFFF0000u));
+}
+
+__device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
+    if (dtype == kF16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Four values at element i of a 16-byte aligned tensor (i a multiple of 4).
+__device__ __forceinline__ void store4(void* base, int64_t i, int dtype, float4 x) {
+    if (dtype == kF32) *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = x;
+    else
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + i) =
+            make_uint2(pack16(x.x, x.y, dtype), pack16(x.z, x.w, dtype));
+}
+
+__device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
+    const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s)), y = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
+    a = x, b = y;
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t codes4(float4 x, float inv) {
+    const int a = __float2int_rn(__fmul_rn(x.x, inv)), b = __float2int_rn(__fmul_rn(x.y, inv));
+    const int c = __float2int_rn(__fmul_rn(x.z, inv)), d = __float2int_rn(__fmul_rn(x.w, inv));
+    return (a & 0xFF) | ((b & 0xFF) << 8) | ((c & 0xFF) << 16) | ((uint32_t)d << 24);
+}
+
+// LANES threads (a power of two >= d / 8) take one row: lane l holds elements 4l..4l+3 of each half, so that a pair of
+// either rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head) with the heads
+// of q, then k, then v.
+template <int LANES>
+__global__ void __launch_bounds__(KW_THREADS) kv_write_kernel(const KvWriteParams p, uint32_t token0, uint32_t rows) {
+    const uint32_t r = blockIdx.x * (KW_THREADS / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+    const uint32_t heads = p.q_heads + 2 * p.c.heads, half = p.c.d / 2;
+    const bool live = r < rows;
+    const uint32_t t = token0 + (live ? r / heads : 0u);
+    uint32_t h = live ? r % heads : 0u;
+    const bool is_q = h < p.q_heads, is_v = h >= p.q_heads + p.c.heads;
+    if (!is_q) h -= is_v ? p.q_heads + p.c.heads : p.q_heads;
+    const int64_t slot = live && !is_q ? (int64_t)p.slots[t] : 0;
+    const bool wanted = live && (is_q || (slot >= 0 && slot < (int64_t)p.c.pages * p.c.page_size));
+    const bool active = wanted && lane * 8 < p.c.d;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    if (active) {
+        const RowsView& in = is_q ? p.q : is_v ? p.v : p.k;
+        const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * 4;
+        a = load4(in.p, at, p.dtype, p.vec);
+        b = load4(in.p, at + half, p.dtype, p.vec);
+        if (p.cos != nullptr && !is_v) {
+            const uint32_t pos = min((uint32_t)max(p.positions[t], 0), p.rope_len - 1);
+            const int64_t row = (int64_t)pos * half;
+            if (p.interleaved) {
+                const int64_t i0 = row + lane * 2, i1 = i0 + half / 2;
+                rotate(a.x, a.y, p.cos[i0], p.sin[i0]);
+                rotate(a.z, a.w, p.cos[i0 + 1], p.sin[i0 + 1]);
+                rotate(b.x, b.y, p.cos[i1], p.sin[i1]);
+                rotate(b.z, b.w, p.cos[i1 + 1], p.sin[i1 + 1]);
+            } else {
+                const float4 c = load4(p.cos, row + lane * 4, kF32, p.vec), s = load4(p.sin, row + lane * 4, kF32, p.vec);
+                rotate(a.x, b.x, c.x, s.x);
+                rotate(a.y, b.y, c.y, s.y);
+                rotate(a.z, b.z, c.z, s.z);
+                rotate(a.w, b.w, c.w, s.w);
+            }
+        }
+    }
+    if (is_q) {
+        if (active) {
+            const int64_t at = ((int64_t)t * p.q_heads + h) * p.c.d + lane * 4;
+            store4(p.q_out, at, p.q_out_dtype, a);
+            store4(p.q_out, at + half, p.q_out_dtype, b);
+        }
+        if (p.c.dtype != kInt8) return;
+    }
+    const int64_t page = slot / p.c.page_size;
+    const int64_t row = wanted ? (page * p.c.heads + h) * p.c.page_size + (slot - page * p.c.page_size) : 0;
+    void* const cache = is_v ? p.c.v : p.c.k;
+    if (p.c.dtype != kInt8) {
+        if (active) {
+            store4(cache, row * p.c.d + lane * 4, p.c.dtype, a);
+            store4(cache, row * p.c.d + lane * 4 + half, p.c.dtype, b);
+        }
+        return;
+    }
+    float m = max_nan(max_nan(max_nan(fabsf(a.x), fabsf(a.y)), max_nan(fabsf(a.z), fabsf(a.w))),
+                      max_nan(max_nan(fabsf(b.x), fabsf(b.y)), max_nan(fabsf(b.z), fabsf(b.w))));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (is_q || !active) return;
+    const bool finite = m < __int_as_float(0x7F800000), zero = m < MIN_AMAX;
+    const float inv = finite && !zero ? __fdiv_rn(127.0f, m) : 0.0f;
+    int8_t* const dst = static_cast<int8_t*>(cache) + row * p.c.d + lane * 4;
+    *reinterpret_cast<uint32_t*>(dst) = finite ? codes4(a, inv) : 0u;
+    *reinterpret_cast<uint32_t*>(dst + half) = finite ? codes4(b, inv) : 0u;
+    if (lane == 0)
+        (is_v ? p.c.v_scale : p.c.k_scale)[row] =
+            !finite ? __int_as_float(0x7FC00000) : zero ? 0.0f : __fdiv_rn(m, 127.0f);
+}
+
+template <int LANES>
+cudaError_t launch_write(const KvWriteParams& p, cudaStream_t stream) {
+    const uint32_t heads = p.q_heads + 2 * p.c.heads;
+    const uint32_t chunk = std::max(1u, 0x7FFFFFFFu / heads);  // rows of a launch stay below 2^31
+    for (uint64_t t0 = 0; t0 < p.tokens; t0 += chunk) {
+        const uint32_t rows = std::min<uint64_t>(chunk, p.tokens - t0) * heads, per = KW_THREADS / LANES;
+        kv_write_kernel<LANES><<<rows / per + (rows % per != 0), KW_THREADS, 0, stream>>>(p, (uint32_t)t0, rows);
+    }
+    return cudaGetLastError();
+}
+
+// ---- read ----
+constexpr int KR_TOKENS = 32;  // tokens of a block
+
+__device__ __forceinline__ void read8(const KvCacheView& c, const void* src, const float* scale, int64_t row, uint32_t col,
+                                      float (&x)[8]) {
+    const int64_t at = row * c.d + col;
+    if (c.dtype == kInt8) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const int8_t*>(src) + at));
+        const float s = __ldg(scale + row);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] = __fmul_rn((float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3))), s);
+        return;
+    }
+    const float4 a = load4(src, at, c.dtype, true), b = load4(src, at + 4, c.dtype, true);
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+
+__global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const KvReadParams p) {
+    __shared__ int64_t first[KR_TOKENS];  // each token's row of head 0 in the cache, -1: none (its rows are zeros)
+    const uint32_t t0 = blockIdx.x * KR_TOKENS;
+    if (threadIdx.x < KR_TOKENS && t0 + threadIdx.x < p.total) {
+        const int32_t t = (int32_t)(t0 + threadIdx.x);
+        uint32_t lo = 0, hi = p.seqs;  // the sequence whose [cu[b], cu[b + 1]) holds t
+        while (lo < hi) {
+            const uint32_t mid = (lo + hi) / 2;
+            if (__ldg(p.cu + mid + 1) <= t) lo = mid + 1;
+            else hi = mid;
+        }
+        int64_t row = -1;
+        if (lo < p.seqs && t >= __ldg(p.cu + lo)) {
+            const int64_t pos = (int64_t)(t - __ldg(p.cu + lo)) + (p.starts ? p.starts[lo] : 0);
+            const int64_t col = pos / p.c.page_size;
+            if (pos >= 0 && col < p.table_width) {
+                const int32_t page = p.block_table[(int64_t)lo * p.table_width + col];
+                if (page >= 0 && (uint32_t)page < p.c.pages)
+                    row = (int64_t)page * p.c.heads * p.c.page_size + (pos - col * p.c.page_size);
+            }
+        }
+        first[threadIdx.x] = row;
+    }
+    __syncthreads();
+    const uint32_t chunks = p.c.d / 8, per_token = p.c.heads * chunks;
+    const uint32_t n = min((uint32_t)KR_TOKENS, p.total - t0) * per_token;
+    for (uint32_t i = threadIdx.x; i < n; i += KW_THREADS) {
+        const uint32_t t = i / per_token, rest = i - t * per_token, h = rest / chunks, col = (rest - h * chunks) * 8;
+        const int64_t row0 = first[t], out = (int64_t)t0 * per_token * 8 + (int64_t)i * 8;
+        float k[8] = {}, v[8] = {};
+        if (row0 >= 0) {
+            const int64_t row = row0 + (int64_t)h * p.c.page_size;
+            read8(p.c, p.c.k, p.c.k_scale, row, col, k);
+            read8(p.c, p.c.v, p.c.v_scale, row, col, v);
+        }
+        store4(p.k_out, out, p.out_dtype, make_float4(k[0], k[1], k[2], k[3]));
+        store4(p.k_out, out + 4, p.out_dtype, make_float4(k[4], k[5], k[6], k[7]));
+        store4(p.v_out, out, p.out_dtype, make_float4(v[0], v[1], v[2], v[3]));
+        store4(p.v_out, out + 4, p.out_dtype, make_float4(v[4], v[5], v[6], v[7]));
+    }
+}
+
+}  // namespace
+
+cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream) {
+    if (p.c.d > 64) return launch_write<16>(p, stream);
+    if (p.c.d > 32) return launch_write<8>(p, stream);
+    return launch_write<4>(p, stream);
+}
+
+cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream) {
+    kv_read_kernel<<<(p.total + KR_TOKENS - 1) / KR_TOKENS, KW_THREADS, 0, stream>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace iq2

@@ -13,6 +13,10 @@ const SOURCES: &[&str] = &[
     "iq2xxs_noalloc.cu",
     "iq2xxs_sharded.cu",
     "iq2_variants.cu",
+    "attention_capi.cu",
+    "kv_cache.cu",
+    "attention_decode.cu",
+    "attention_prefill.cu",
 ];
 
 fn main() {
@@ -42,7 +46,13 @@ fn main() {
     let lib = out.join("libcandelora_iq2.a");
     let status = Command::new(&nvcc).arg("-lib").arg("-o").arg(&lib).args(&objs).status().unwrap();
     assert!(status.success(), "nvcc -lib failed");
-    for h in ["iq2xxs_common.cuh", "iq2xxs_codebook.h", "iq2xxs_internal.h", "iq2_variant_grids.h"] {
+    for h in [
+        "iq2xxs_common.cuh",
+        "iq2xxs_codebook.h",
+        "iq2xxs_internal.h",
+        "iq2_variant_grids.h",
+        "attention_internal.h",
+    ] {
         println!("cargo:rerun-if-changed={}", csrc.join(h).display());
     }
     println!("cargo:rerun-if-changed={}", include.join("candelora_iq2.h").display());

@@ -44,6 +44,88 @@ pub struct Iq2MatmulProblem {
     pub out: *mut f32,
 }
 
+pub const IQ2_KV_INT8: c_int = 3;
+
+/// struct iq2_kv_cache (a paged key-value cache).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Iq2KvCache {
+    pub k: *mut c_void,
+    pub v: *mut c_void,
+    pub k_scale: *mut f32,
+    pub v_scale: *mut f32,
+    pub num_pages: u32,
+    pub kv_heads: u32,
+    pub page_size: u32,
+    pub head_dim: u32,
+    pub dtype: c_int,
+}
+
+/// struct iq2_rows (a [tokens, heads, head_dim] tensor, strides in elements).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Iq2Rows {
+    pub data: *const c_void,
+    pub token_stride: i64,
+    pub head_stride: i64,
+}
+
+/// struct iq2_kv_tokens (new tokens for a cache).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Iq2KvTokens {
+    pub k: Iq2Rows,
+    pub v: Iq2Rows,
+    pub q: Iq2Rows,
+    pub dtype: c_int,
+    pub tokens: u32,
+    pub q_heads: u32,
+    pub slots: *const i32,
+    pub positions: *const i32,
+    pub cos: *const f32,
+    pub sin: *const f32,
+    pub rope_len: u32,
+    pub interleaved: c_int,
+    pub q_out: *mut c_void,
+    pub q_out_dtype: c_int,
+}
+
+/// struct iq2_attention_prompts (packed prompts).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Iq2AttentionPrompts {
+    pub q: Iq2Rows,
+    pub k: Iq2Rows,
+    pub v: Iq2Rows,
+    pub dtype: c_int,
+    pub sequences: u32,
+    pub q_tokens: u32,
+    pub k_tokens: u32,
+    pub q_heads: u32,
+    pub kv_heads: u32,
+    pub head_dim: u32,
+    pub cu_seqlens_q: *const i32,
+    pub cu_seqlens_k: *const i32,
+    pub causal: c_int,
+    pub scale: f32,
+    pub out: *mut c_void,
+}
+
+/// struct iq2_attention_tokens (one new token for each sequence).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Iq2AttentionTokens {
+    pub q: Iq2Rows,
+    pub dtype: c_int,
+    pub batch: u32,
+    pub q_heads: u32,
+    pub table_width: u32,
+    pub block_table: *const i32,
+    pub seq_lens: *const i32,
+    pub scale: f32,
+    pub out: *mut c_void,
+}
+
 #[link(name = "candelora_iq2", kind = "static")]
 extern "C" {
     pub fn iq2_last_error() -> *const c_char;
@@ -174,6 +256,35 @@ extern "C" {
         count: u32,
         m: u32,
         x_dtype: c_int,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn iq2_kv_cache_write(cache: *const Iq2KvCache, tokens: *const Iq2KvTokens, stream: *mut c_void) -> c_int;
+    pub fn iq2_kv_cache_read(
+        cache: *const Iq2KvCache,
+        block_table: *const i32,
+        table_width: u32,
+        sequences: u32,
+        starts: *const i32,
+        cu_seqlens: *const i32,
+        total: u32,
+        k_out: *mut c_void,
+        v_out: *mut c_void,
+        out_dtype: c_int,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn iq2_attention_prefill_workspace_size(prompts: *const Iq2AttentionPrompts) -> usize;
+    pub fn iq2_attention_prefill(
+        prompts: *const Iq2AttentionPrompts,
+        workspace: *mut c_void,
+        workspace_bytes: usize,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn iq2_attention_decode_workspace_size(cache: *const Iq2KvCache, batch: u32, q_heads: u32) -> usize;
+    pub fn iq2_attention_decode(
+        cache: *const Iq2KvCache,
+        tokens: *const Iq2AttentionTokens,
         workspace: *mut c_void,
         workspace_bytes: usize,
         stream: *mut c_void,

@@ -264,6 +264,117 @@ int iq2_matmul_grouped_sharded(iq2_comm_t comm, const iq2_matmul_problem* proble
                                uint32_t m, int x_dtype, void* workspace, size_t workspace_bytes,
                                iq2_stream_t stream);
 
+/*
+ * Attention over the projections' outputs (no reference counterpart: the reference ends at the
+ * projections). q [tokens, q_heads, head_dim], k and v [tokens, kv_heads, head_dim], query head h
+ * reading key head h / (q_heads / kv_heads); q_heads is a multiple of kv_heads, at most 128 times
+ * as many. head_dim is a multiple of 16, at most 128.
+ */
+
+/* Element type of a cache: IQ2_DTYPE_F16, IQ2_DTYPE_BF16, or int8 codes with one f32 scale for
+ * each token and head. */
+#define IQ2_KV_INT8 3
+
+/*
+ * A paged key-value cache: k and v [num_pages, kv_heads, page_size, head_dim], contiguous and
+ * 16-byte aligned; k_scale and v_scale f32 [num_pages, kv_heads, page_size], for IQ2_KV_INT8 only.
+ * Any page_size. Token `pos` of a sequence lies in page block_table[pos / page_size], row
+ * pos % page_size. A block table is int32 [sequences, table_width] on the device; entries outside
+ * [0, num_pages) are never followed: their tokens take no part in an attention and read as zeros.
+ */
+typedef struct iq2_kv_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    uint32_t num_pages, kv_heads, page_size, head_dim;
+    int dtype; /* IQ2_DTYPE_F16, IQ2_DTYPE_BF16 or IQ2_KV_INT8 */
+} iq2_kv_cache;
+
+/* Rows of a [tokens, heads, head_dim] tensor whose last dimension is contiguous: strides in
+ * elements, so that q, k and v may be slices of one projection's output. */
+typedef struct iq2_rows {
+    const void* data;
+    int64_t token_stride, head_stride;
+} iq2_rows;
+
+/* New tokens for a cache (iq2_kv_cache_write). */
+typedef struct iq2_kv_tokens {
+    iq2_rows k, v, q;           /* f32, f16 or bf16 (dtype); q.data NULL: no queries           */
+    int dtype;
+    uint32_t tokens, q_heads;
+    const int32_t* slots;       /* [tokens] page * page_size + row; a slot outside the cache
+                                   (e.g. -1) writes nothing; no two tokens share a slot        */
+    const int32_t* positions;   /* [tokens] row of cos / sin (clamped to the tables)           */
+    const float* cos;           /* [rope_len, head_dim / 2], or NULL: no rotation              */
+    const float* sin;
+    uint32_t rope_len;
+    int interleaved;            /* pairs (2i, 2i + 1), as in GGUF files, not (i, i + d / 2)    */
+    void* q_out;                /* [tokens, q_heads, head_dim] contiguous, 16-byte aligned     */
+    int q_out_dtype;
+} iq2_kv_tokens;
+
+/*
+ * Rotates q and k by their positions, writes q to q_out and k and v to their slots of the cache,
+ * in one launch. 16-bit caches round once; int8 rows (one token and head) hold
+ * rint(x * (127 / max|x|)) and the scale max|x| / 127, a row with an infinity or NaN a NaN scale.
+ */
+int iq2_kv_cache_write(const iq2_kv_cache* cache, const iq2_kv_tokens* tokens, iq2_stream_t stream);
+
+/*
+ * Cached tokens -> packed k_out, v_out [total, kv_heads, head_dim] in out_dtype: rows
+ * [cu_seqlens[b], cu_seqlens[b + 1]) are tokens starts[b], starts[b] + 1, ... of sequence b
+ * (starts NULL: from 0). cu_seqlens int32 [sequences + 1], ascending. Rows of no sequence are zeros.
+ */
+int iq2_kv_cache_read(const iq2_kv_cache* cache, const int32_t* block_table, uint32_t table_width,
+                      uint32_t sequences, const int32_t* starts, const int32_t* cu_seqlens,
+                      uint32_t total, void* k_out, void* v_out, int out_dtype, iq2_stream_t stream);
+
+/* Attention of packed prompts (iq2_attention_prefill). */
+typedef struct iq2_attention_prompts {
+    iq2_rows q, k, v;            /* f16 or bf16 (dtype); 16-byte aligned, strides a multiple of 8 */
+    int dtype;
+    uint32_t sequences, q_tokens, k_tokens, q_heads, kv_heads, head_dim;
+    const int32_t* cu_seqlens_q; /* [sequences + 1], ascending from 0                            */
+    const int32_t* cu_seqlens_k;
+    int causal;                  /* key j is seen by query i when j <= i + Lk - Lq               */
+    float scale;                 /* of q . k; 0: 1 / sqrt(head_dim)                              */
+    void* out;                   /* [q_tokens, q_heads, head_dim] contiguous, dtype              */
+} iq2_attention_prompts;
+
+/* Bytes of device scratch iq2_attention_prefill needs. */
+size_t iq2_attention_prefill_workspace_size(const iq2_attention_prompts* prompts);
+
+/*
+ * out = softmax(scale q k^T) v for every sequence, f32 statistics and accumulation. Keys may be
+ * more than queries (a later chunk of a prompt) or fewer; a query that sees no key gets zeros.
+ * What a masked key or value holds (other sequences' tokens, infinities, NaN) has no effect.
+ */
+int iq2_attention_prefill(const iq2_attention_prompts* prompts, void* workspace, size_t workspace_bytes,
+                          iq2_stream_t stream);
+
+/* One new token for each sequence over its cached tokens (iq2_attention_decode). */
+typedef struct iq2_attention_tokens {
+    iq2_rows q;                  /* [batch, q_heads, head_dim] f32, f16 or bf16 (dtype)          */
+    int dtype;
+    uint32_t batch, q_heads, table_width;
+    const int32_t* block_table;  /* [batch, table_width]                                         */
+    const int32_t* seq_lens;     /* [batch] cached tokens, the new one among them (clamped to
+                                    table_width * page_size)                                     */
+    float scale;                 /* of q . k; 0: 1 / sqrt(head_dim)                              */
+    void* out;                   /* [batch, q_heads, head_dim] contiguous, dtype                 */
+} iq2_attention_tokens;
+
+/* Bytes of device scratch iq2_attention_decode needs (it does not depend on the lengths). */
+size_t iq2_attention_decode_workspace_size(const iq2_kv_cache* cache, uint32_t batch, uint32_t q_heads);
+
+/*
+ * out = softmax(scale q k^T) v, f32 statistics and accumulation, any q type over any cache type.
+ * A sequence of length 0 gets zeros.
+ */
+int iq2_attention_decode(const iq2_kv_cache* cache, const iq2_attention_tokens* tokens, void* workspace,
+                         size_t workspace_bytes, iq2_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
