@@ -185,8 +185,10 @@ def kv_cache_read(cache: KvCache, block_table: torch.Tensor, cu_seqlens: torch.T
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """`t`, or a copy of it where a row does not start on a 16-byte boundary (the loads of whole tiles need that)."""
-    if (t.data_ptr() | t.stride(0) * 2 | t.stride(1) * 2) % 16 == 0:
+    """`t`, or a copy of it where rows do not start on 16-byte boundaries of their own (whole tiles are loaded)."""
+    heads, tokens = t.stride(1), t.stride(0)
+    if t.data_ptr() % 16 == 0 and (t.shape[1] == 1 or (heads > 0 and heads % 8 == 0)) and \
+            (t.shape[0] <= 1 or (tokens > 0 and tokens % 8 == 0)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 

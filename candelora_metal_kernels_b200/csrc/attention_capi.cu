@@ -176,9 +176,13 @@ int iq2_attention_prefill(const iq2_attention_prompts* t, void* workspace, size_
                                   {"cu_seqlens_k", t->cu_seqlens_k, 4}})) != IQ2_OK)
         return rc;
     if (t->k_tokens > 0 && (rc = check_pointers(op, {{"k", t->k.data, 16}, {"v", t->v.data, 16}})) != IQ2_OK) return rc;
-    for (const iq2_rows* r : {&t->q, &t->k, &t->v})
-        if (r->token_stride < 0 || r->head_stride < 0 || !rows_aligned(*r, 2, 16))
+    for (const iq2_rows* r : {&t->q, &t->k, &t->v}) {
+        const uint32_t tokens = r == &t->q ? t->q_tokens : t->k_tokens, heads = r == &t->q ? t->q_heads : t->kv_heads;
+        if ((tokens > 1 && r->token_stride <= 0) || (heads > 1 && r->head_stride <= 0))
+            return capi_fail(IQ2_ERR_INVALID_ARGUMENT, "%s: strides are not positive", op);
+        if ((tokens > 1 && r->token_stride % 8 != 0) || (heads > 1 && r->head_stride % 8 != 0))
             return capi_fail(IQ2_ERR_INVALID_ARGUMENT, "%s: rows are not 16-byte aligned", op);
+    }
     const iq2::PrefillParams p = prefill_params(t, scale);
     const int sms = iq2::capi_num_sms();
     if ((rc = check_workspace(op, workspace, workspace_bytes, iq2::attention_prefill_workspace(p, sms))) != IQ2_OK) return rc;

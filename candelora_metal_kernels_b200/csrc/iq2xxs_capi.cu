@@ -322,6 +322,12 @@ int iq2_device_check(void) {
     unsigned int status = 0;
     const cudaError_t e = (cudaError_t)iq2::gemm_take_status(&status);
     if (e != cudaSuccess) return cuda_fail("iq2_device_check", e);
+    if ((status & 0xFFu) == 0u && status != 0u)
+        return fail(IQ2_ERR_TIMEOUT,
+                    "iq2_device_check: a prefill attention gave up on a pipeline wait (status 0x%x:%s%s%s%s); the outputs "
+                    "of that call are incomplete",
+                    status, (status & 0x100u) ? " loaded tiles" : "", (status & 0x200u) ? " stage release" : "",
+                    (status & 0x400u) ? " probabilities" : "", (status & 0x800u) ? " products" : "");
     if (status != 0u)
         return fail(IQ2_ERR_TIMEOUT,
                     "iq2_device_check: a prefill GEMM gave up on a pipeline wait (status 0x%x:%s%s%s%s%s%s); the "

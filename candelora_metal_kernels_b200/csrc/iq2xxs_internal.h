@@ -94,6 +94,10 @@ int gemm_take_status(unsigned int* status);
 // whose "weights written" arrival is withheld (0: none).
 void gemm_testing_set_stall(uint64_t wait_limit_ns, uint32_t stall_stage);
 
+// The same status word for other kernels with bounded waits (attention_prefill.cu), their wait bound, and the test
+// hook's stage.
+cudaError_t device_status(unsigned int** word, uint64_t* wait_ns, uint32_t* stall);
+
 // The current CUDA context of the calling thread (a CUcontext, as an opaque handle; nullptr when
 // none): caches of device addresses are keyed on it so that a new primary context (after
 // cudaDeviceReset) is looked up again.

@@ -52,6 +52,7 @@ fn main() {
         "iq2xxs_internal.h",
         "iq2_variant_grids.h",
         "attention_internal.h",
+        "tcgen05.cuh",
     ] {
         println!("cargo:rerun-if-changed={}", csrc.join(h).display());
     }

@@ -332,7 +332,7 @@ int iq2_kv_cache_read(const iq2_kv_cache* cache, const int32_t* block_table, uin
 
 /* Attention of packed prompts (iq2_attention_prefill). */
 typedef struct iq2_attention_prompts {
-    iq2_rows q, k, v;            /* f16 or bf16 (dtype); 16-byte aligned, strides a multiple of 8 */
+    iq2_rows q, k, v;            /* f16 or bf16 (dtype); 16-byte aligned, strides multiples of 8  */
     int dtype;
     uint32_t sequences, q_tokens, k_tokens, q_heads, kv_heads, head_dim;
     const int32_t* cu_seqlens_q; /* [sequences + 1], ascending from 0                            */

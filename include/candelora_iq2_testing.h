@@ -18,7 +18,9 @@ extern "C" {
  * every CTA whose "weights written" arrival the decode warps withhold. The MMA thread's wait on
  * that stage then runs out after wait_limit_ns (a flag that nothing sets): the kernel records the
  * timeout in the device status that iq2_device_check reports, stops issuing work, waits (bounded)
- * for what it already issued and frees its tensor memory. stall_stage = 0 restores normal runs.
+ * for what it already issued and frees its tensor memory. Prefill attentions take the same bound;
+ * their stall_stage is a key tile (1-based) whose probabilities one warpgroup withholds.
+ * stall_stage = 0 restores normal runs.
  */
 int iq2_testing_set_gemm_stall(uint64_t wait_limit_ns, uint32_t stall_stage);
 

@@ -15,6 +15,7 @@ import torch
 
 import attention_reference as ref
 import candelora_metal_kernels_b200 as c
+from candelora_metal_kernels_b200 import _lib
 
 pytestmark = pytest.mark.gpu
 BF16, F16, F32, I8 = torch.bfloat16, torch.float16, torch.float32, torch.int8
@@ -132,6 +133,27 @@ def test_prefill_large_scores():
     got = c.attention_prefill(q, k, v, lens.cuda()).double().cpu()
     # a score of 2000 is held to 2^-24 * 2000 by its last rounding alone and to some 2^-12 over the sum: 1 % of p
     assert (got - want).norm() / want.norm() < 0.02
+
+
+def test_prefill_wait_that_runs_out_is_reported_and_the_context_stays_usable():
+    """With the test hook one warpgroup withholds the probabilities of a key tile: the wait on them runs out after 20 ms,
+    device_check reports it once, and the same call is right again afterwards. No GPU fault is involved."""
+    lib = _lib.load()
+    q, k, v = randn((700, 4, 128), 1, BF16), randn((700, 2, 128), 2, BF16), randn((700, 2, 128), 3, BF16)
+    lens = cu([700]).cuda()
+    want = c.attention_prefill(q, k, v, lens)
+    c.device_check()
+    for tile in (1, 3):
+        assert lib.iq2_testing_set_gemm_stall(20_000_000, tile) == _lib.IQ2_OK
+        try:
+            c.attention_prefill(q, k, v, lens)
+            with pytest.raises(c.Iq2Error, match="prefill attention gave up.*probabilities") as e:
+                c.device_check()
+            assert e.value.code == _lib.IQ2_ERR_TIMEOUT
+        finally:
+            lib.iq2_testing_set_gemm_stall(0, 0)
+        c.device_check()
+        assert torch.equal(c.attention_prefill(q, k, v, lens), want)
 
 
 # ---- one token over the cache ----
