@@ -18,18 +18,20 @@ import torch
 
 from . import _lib
 from ._lib import Iq2Error
-from .iq2_matmul import _X_DTYPES, _bail, _stream_handle
+from .iq2_matmul import _X_DTYPES, _bail
 
 _KV_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.int8: _lib.KV_INT8}
 
 
 def _call(device: torch.device, fn, *args) -> None:
     """fn(*args, stream) on `device`, which the C ABI expects to be the current one."""
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, _stream_handle(device))
+    index = device.index
+    stream = torch._C._cuda_getCurrentRawStream(index)  # current_stream(device).cuda_stream without the Stream object
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, _stream_handle(device))
+            rc = fn(*args, stream)
     if rc != _lib.IQ2_OK:
         _lib.check(rc)
 

@@ -49,22 +49,22 @@ struct DecodeShape {
     static constexpr int SMEM = AD_WARPS * RING + Q_BYTES + 4 * PART * 4 + AD_HEADS * 4;
 };
 
-// A workspace record for each block: whether its first part begins inside an item (whose earlier parts other blocks have).
+// What join_kernel's block of the same number has to join: the parts of blocks c0 to c1 of one item, block c0's being its
+// part number `slot` (0: its first, 1: its last), the others' their first. c1 = 0: nothing.
 struct JoinRecord {
-    uint64_t unit0, all;      // the item's first unit, and the units of all items
-    uint32_t b, item, units;  // sequence, item of the sequence, the item's units (0: no such part)
+    uint32_t b, item, c0, c1, slot;
 };
-
 inline size_t records_bytes(uint32_t blocks) { return (blocks * sizeof(JoinRecord) + 255) / 256 * 256; }
 
-__device__ __forceinline__ uint64_t part_start(uint32_t block, uint32_t blocks, uint64_t units) { return units * block / blocks; }
-// The block whose part holds `unit`.
-__device__ __forceinline__ uint32_t block_of(uint64_t unit, uint32_t blocks, uint64_t units) {
-    uint32_t c = (uint32_t)(unit * blocks / units);
-    while (c + 1 < blocks && part_start(c + 1, blocks, units) <= unit) ++c;
-    while (c > 0 && part_start(c, blocks, units) > unit) --c;
-    return c;
-}
+// The units are dealt as evenly as whole units go: the first units % blocks blocks take one more than the others.
+struct Deal {
+    uint64_t each, more;  // units / blocks, units % blocks
+    __device__ __forceinline__ uint64_t start(uint32_t block) const { return block * each + min((uint64_t)block, more); }
+    __device__ __forceinline__ uint32_t block_of(uint64_t unit) const {
+        const uint64_t big = more * (each + 1);
+        return (uint32_t)(unit < big ? unit / (each + 1) : more + (unit - big) / each);
+    }
+};
 
 __device__ __forceinline__ uint32_t seq_len(const DecodeParams& p, uint32_t b) {
     const uint64_t most = min((uint64_t)p.table_width * p.c.page_size, (uint64_t)0x7FFFFFFF);
@@ -181,60 +181,61 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     const uint32_t d = p.c.d, group = p.q_heads / p.c.heads, items = p.c.heads * chunks_of_heads;
     pdl_launch_dependents();
 
-    // ---- this block's part of the line ----
-    __shared__ uint64_t warp_sum[AD_WARPS];
-    __shared__ Cursor first;
-    uint64_t mine = 0;
-    for (uint32_t b = threadIdx.x; b < p.batch; b += AD_THREADS) mine += (seq_len(p, b) + UNIT - 1) / UNIT;
-    for (int o = 16; o > 0; o /= 2) mine += __shfl_xor_sync(0xFFFFFFFFu, mine, o);
-    if (lane == 0) warp_sum[warp] = mine;
+    // ---- this block's part of the line (every warp works it out for itself) ----
     // the ring starts as zeros: chunks past head_dim are never copied, and the matrix instructions read them
     if (d < DP)
-        for (uint32_t i = threadIdx.x; i < AD_WARPS * S::RING / 16; i += AD_THREADS)
-            *reinterpret_cast<uint4*>(smem + i * 16) = make_uint4(0, 0, 0, 0);
-    __syncthreads();
+        for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
     uint64_t units = 0;
-    for (int w = 0; w < AD_WARPS; ++w) units += warp_sum[w];
+    for (uint32_t b = lane; b < p.batch; b += 32) units += (seq_len(p, b) + UNIT - 1) / UNIT;
+    for (int o = 16; o > 0; o /= 2) units += __shfl_xor_sync(0xFFFFFFFFu, units, o);
     units *= items;
-    const uint64_t u0 = part_start(blockIdx.x, gridDim.x, units), u1 = part_start(blockIdx.x + 1, gridDim.x, units);
+    const Deal deal{units / gridDim.x, units % gridDim.x};
+    const uint64_t u0 = deal.start(blockIdx.x), u1 = deal.start(blockIdx.x + 1);
     // sequences of length 0: zeros
     for (uint32_t b = blockIdx.x; b < p.batch; b += gridDim.x)
         if (seq_len(p, b) == 0)
             for (uint32_t i = threadIdx.x; i < p.q_heads * d; i += AD_THREADS)
                 store_elem(p.out, (int64_t)b * p.q_heads * d + i, p.dtype, 0.f);
-    if (threadIdx.x == 0) records[blockIdx.x].units = 0;
-    if (u0 >= u1) return;
-    // the sequence that holds unit u0: the lengths again, a warp's worth at a time
-    if (warp == 0) {
-        uint64_t before = 0;
-        for (uint32_t b0 = 0; b0 < p.batch; b0 += 32) {
-            const uint32_t len = b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0u;
-            const uint32_t own = (len + UNIT - 1) / UNIT;
-            uint64_t upto = (uint64_t)own * items;
-            for (int o = 1; o < 32; o *= 2) {
-                const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-                if (lane >= (uint32_t)o) upto += x;
-            }
-            const bool here = before + upto > u0 && before + upto - (uint64_t)own * items <= u0;
-            if (here) {
-                const uint64_t rest = u0 - (before + upto - (uint64_t)own * items);
-                Cursor c;
-                c.unit = u0, c.end = u1, c.b = b0 + lane, c.len = len, c.units = own;
-                c.item = (uint32_t)(rest / own), c.k = (uint32_t)(rest % own);
-                c.cut();
-                first = c;
-            }
-            if (__any_sync(0xFFFFFFFFu, here)) break;
-            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
-        }
+    if (u0 >= u1) {
+        if (threadIdx.x == 0) records[blockIdx.x].c1 = 0;
+        return;
     }
-    __syncthreads();
-    Cursor cur = first, pre = first;
-    if (threadIdx.x == 0 && cur.k > 0) records[blockIdx.x] = {cur.unit - cur.k, units, cur.b, cur.item, cur.units};
+    Cursor cur{};
+    uint64_t before = 0;  // units of the sequences before
+    for (uint32_t b0 = 0;; b0 += 32) {
+        const uint32_t len = b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0u, own = (len + UNIT - 1) / UNIT;
+        uint64_t upto = (uint64_t)own * items;
+        for (int o = 1; o < 32; o *= 2) {
+            const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+            if (lane >= (uint32_t)o) upto += x;
+        }
+        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + upto > u0);
+        if (hit != 0) {
+            const int at = __ffs(hit) - 1;
+            cur.b = b0 + at;
+            cur.len = __shfl_sync(0xFFFFFFFFu, len, at), cur.units = __shfl_sync(0xFFFFFFFFu, own, at);
+            const uint32_t rest = (uint32_t)(u0 - before - __shfl_sync(0xFFFFFFFFu, upto - (uint64_t)own * items, at));
+            cur.item = rest / cur.units, cur.k = rest % cur.units;
+            break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    cur.unit = u0, cur.end = u1;
+    cur.cut();
+    Cursor pre = cur;
+    if (threadIdx.x == 0) {
+        // the first block whose part begins inside an item joins it
+        const uint64_t unit0 = u0 - cur.k;
+        const uint32_t c0 = cur.k > 0 ? deal.block_of(unit0) : blockIdx.x;
+        JoinRecord r{cur.b, cur.item, c0, 0, 0};
+        if (c0 + 1 == blockIdx.x) r.c1 = deal.block_of(unit0 + cur.units - 1), r.slot = deal.start(c0) == unit0 ? 0 : 1;
+        records[blockIdx.x] = r;
+    }
 
     // ---- the copies: tile `i` (TOK tokens) of pre's piece of an item, one page lookup ahead ----
     uint8_t* const ring = smem + warp * S::RING;
     const uint32_t ring_u32 = smem_u32(ring);
+    if (d < DP) __syncwarp();
     uint32_t pre_i = warp, pre_page = 0;  // the tile to copy next and this lane's token's page number
     auto pre_tokens = [&](const Cursor& c) { return min(c.len, (c.k + c.n) * UNIT) - c.k * UNIT; };
     auto find_tile = [&]() {  // the next tile of this warp, and its page numbers under way
@@ -288,24 +289,28 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         copy_tile(stage);
         find_tile();
     };
+    // q of an item, a warp a head: loaded while the copies before it are under way
+    float q_next[DP / 32];
+    auto load_q = [&](const Cursor& c) {
+        const uint32_t kv = c.item / chunks_of_heads, h0 = kv * group + (c.item % chunks_of_heads) * AD_HEADS;
+        const bool has = warp < min((uint32_t)AD_HEADS, (kv + 1) * group - h0);
+        const int64_t at = (int64_t)c.b * p.q.token_stride + (int64_t)(h0 + warp) * p.q.head_stride;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) q_next[i] = has && lane + i * 32 < d ? load_elem(p.q.p, at + lane + i * 32, p.dtype) : 0.f;
+    };
     find_tile();
+    load_q(cur);
     for (int s = 0; s < AD_STAGES - 1; ++s) copy_and_find(s);
     int stage = 0;
 
     while (!cur.done()) {
-        // ---- q of the item: two 16-bit pieces of each head, one warp a head ----
+        // ---- q of the item: two 16-bit pieces of each head ----
         const uint32_t kv_head = cur.item / chunks_of_heads, head0 = kv_head * group + (cur.item % chunks_of_heads) * AD_HEADS;
         const uint32_t heads = min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
         {
             float x[DP / 32], top = 0.f;
 #pragma unroll
-            for (int i = 0; i < DP / 32; ++i) {
-                const uint32_t e = lane + i * 32;
-                x[i] = warp < heads && e < d
-                           ? load_elem(p.q.p, (int64_t)cur.b * p.q.token_stride + (int64_t)(head0 + warp) * p.q.head_stride + e, p.dtype)
-                           : 0.f;
-                top = fmaxf(top, fabsf(x[i]));
-            }
+            for (int i = 0; i < DP / 32; ++i) x[i] = q_next[i], top = fmaxf(top, fabsf(x[i]));
             float up = 1.f, down = 1.f;  // 2^e and 2^-e
             if (!BF) {
                 for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
@@ -451,6 +456,10 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
 
+        Cursor next = cur;
+        next.next<UNIT>(p, items);
+        if (!next.done()) load_q(next);
+
         // ---- the eight warps' (o, m, l) of the item, through four slots of shared memory ----
         auto put = [&](float* slot) {
 #pragma unroll
@@ -505,46 +514,48 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                 if (!whole && lane == 0) part[AD_HEADS * DP + h] = mx, part[AD_HEADS * DP + AD_HEADS + h] = sum;
             }
         }
-        cur.next<UNIT>(p, items);
+        cur = next;
         if (!cur.done()) __syncthreads();  // the slots and q are written again
     }
     cp_async_wait<0>();
 }
 
-// One block for each block of decode_kernel whose part begins inside an item: the first such block of an item joins the
-// item's parts, (o, m, l) = sum over them of 2^(m_c - max) (o_c, l_c). A warp a head.
+// The parts of an item that several blocks had: (o, m, l) = sum over them of 2^(m_c - max) (o_c, l_c), in the blocks'
+// order. A block a record, a warp a head.
 template <int DP>
-__global__ void __launch_bounds__(AD_THREADS)
-    join_kernel(const DecodeParams p, const float* __restrict__ parts, const JoinRecord* __restrict__ records,
-                uint32_t chunks_of_heads) {
+__global__ void __launch_bounds__(AD_THREADS, 1)
+    join_kernel(const DecodeParams p, const float* __restrict__ parts, const JoinRecord* __restrict__ records, uint32_t chunks_of_heads) {
     constexpr int PART = AD_HEADS * (DP + 2);
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     pdl_wait();
     const JoinRecord r = records[blockIdx.x];
-    if (r.units == 0) return;
-    const uint32_t blocks = gridDim.x, d = p.c.d, group = p.q_heads / p.c.heads;
-    const uint64_t units = r.all;
-    const uint32_t c0 = block_of(r.unit0, blocks, units);
-    if (blockIdx.x != c0 + 1) {  // blocks between (without work, or earlier parts of this item) leave it to the first
-        for (uint32_t c = c0 + 1; c < blockIdx.x; ++c)
-            if (records[c].units != 0) return;
-    }
-    const uint32_t c1 = block_of(r.unit0 + r.units - 1, blocks, units);
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (r.c1 == 0) return;
+    const uint32_t d = p.c.d, group = p.q_heads / p.c.heads;
     const uint32_t kv_head = r.item / chunks_of_heads, head0 = kv_head * group + (r.item % chunks_of_heads) * AD_HEADS;
     if (warp >= min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0)) return;
-    auto slot = [&](uint32_t c) { return parts + ((uint64_t)c * 2 + (c == c0 && part_start(c, blocks, units) != r.unit0 ? 1 : 0)) * PART; };
-    float mx = -INFINITY;
-    for (uint32_t c = c0 + lane; c <= c1; c += 32)
-        if (part_start(c, blocks, units) < part_start(c + 1, blocks, units)) mx = fmaxf(mx, slot(c)[AD_HEADS * DP + warp]);
-    for (int o = 16; o > 0; o /= 2) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
-    float y[DP / 32] = {}, sum = 0.f;
-    for (uint32_t c = c0; c <= c1; ++c) {
-        if (part_start(c, blocks, units) >= part_start(c + 1, blocks, units)) continue;
-        const float* const s = slot(c);
-        const float w = mx == -INFINITY ? 0.f : exp2_approx(s[AD_HEADS * DP + warp] - mx);
-        sum += s[AD_HEADS * DP + AD_HEADS + warp] * w;
+    auto slot = [&](uint32_t c) { return parts + ((uint64_t)c * 2 + (c == r.c0 ? r.slot : 0)) * PART; };
+    float y[DP / 32] = {}, sum = 0.f, mx = -INFINITY;
+    // lanes hold the maxima and sums of 32 parts; the parts' o are added with their weights
+    for (uint32_t c1 = r.c0; c1 <= r.c1; c1 += 32) {
+        const uint32_t n = min(r.c1 + 1 - c1, 32u);
+        const float m = lane < n ? slot(c1 + lane)[AD_HEADS * DP + warp] : -INFINITY;
+        const float l = lane < n ? slot(c1 + lane)[AD_HEADS * DP + AD_HEADS + warp] : 0.f;
+        float top = fmaxf(m, mx);
+        for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
+        const float keep = top == -INFINITY ? 0.f : exp2_approx(mx - top), w = top == -INFINITY ? 0.f : exp2_approx(m - top);
+        mx = top;
+        float add = w * l;
+        for (int o = 16; o > 0; o /= 2) add += __shfl_xor_sync(0xFFFFFFFFu, add, o);
+        sum = sum * keep + add;
 #pragma unroll
-        for (int i = 0; i < DP / 32; ++i) y[i] += s[warp * DP + lane + i * 32] * w;
+        for (int i = 0; i < DP / 32; ++i) y[i] *= keep;
+#pragma unroll 4
+        for (uint32_t c = 0; c < n; ++c) {
+            const float* const o = slot(c1 + c) + warp * DP + lane;
+            const float wc = __shfl_sync(0xFFFFFFFFu, w, c);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) y[i] += o[i * 32] * wc;
+        }
     }
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i)

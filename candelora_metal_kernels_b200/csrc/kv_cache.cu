@@ -121,8 +121,8 @@ __global__ void __launch_bounds__(KW_THREADS) kv_write_kernel(const KvWriteParam
         }
         if (p.c.dtype != kInt8) return;
     }
-    const int64_t page = slot / p.c.page_size;
-    const int64_t row = wanted ? (page * p.c.heads + h) * p.c.page_size + (slot - page * p.c.page_size) : 0;
+    const uint32_t page = (uint32_t)slot / p.c.page_size;
+    const int64_t row = wanted ? ((int64_t)page * p.c.heads + h) * p.c.page_size + ((uint32_t)slot - page * p.c.page_size) : 0;
     void* const cache = is_v ? p.c.v : p.c.k;
     if (p.c.dtype != kInt8) {
         if (active) {
@@ -158,27 +158,57 @@ cudaError_t launch_write(const KvWriteParams& p, cudaStream_t stream) {
 }
 
 // ---- read ----
-constexpr int KR_TOKENS = 32;  // tokens of a block
+// A block takes `tokens` tokens: it finds their rows in the cache, then groups of LANES threads (a power of two >= d / 8)
+// copy a row of K and V each, eight elements a thread, KR_BATCH rows' loads in flight.
+constexpr int KR_MOST = 32, KR_BATCH = 4;
 
-__device__ __forceinline__ void read8(const KvCacheView& c, const void* src, const float* scale, int64_t row, uint32_t col,
-                                      float (&x)[8]) {
-    const int64_t at = row * c.d + col;
+struct Eight {
+    uint4 w;  // 8 16-bit elements; or the 8 codes in x, y and the scale in z
+};
+__device__ __forceinline__ Eight read8(const KvCacheView& c, const void* src, const float* scale, int64_t row, uint32_t col) {
+    Eight e;
     if (c.dtype == kInt8) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const int8_t*>(src) + at));
-        const float s = __ldg(scale + row);
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            x[i] = __fmul_rn((float)(int8_t)((i < 4 ? w.x : w.y) >> (8 * (i & 3))), s);
-        return;
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const int8_t*>(src) + row * c.d + col));
+        e.w = make_uint4(w.x, w.y, __float_as_uint(__ldg(scale + row)), 0u);
+    } else {
+        e.w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + row * c.d + col));
     }
-    const float4 a = load4(src, at, c.dtype, true), b = load4(src, at + 4, c.dtype, true);
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+    return e;
 }
 
-__global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const KvReadParams p) {
-    __shared__ int64_t first[KR_TOKENS];  // each token's row of head 0 in the cache, -1: none (its rows are zeros)
-    const uint32_t t0 = blockIdx.x * KR_TOKENS;
-    if (threadIdx.x < KR_TOKENS && t0 + threadIdx.x < p.total) {
+__device__ __forceinline__ float2 widen16(uint32_t v, int dtype) {
+    if (dtype == kF16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+}
+
+__device__ __forceinline__ void write8(void* out, int64_t at, int out_dtype, const Eight& e, int dtype) {
+    if (out_dtype == dtype) {  // 16-bit to the same type: the bits
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = e.w;
+        return;
+    }
+    float x[8];
+    if (dtype == kInt8) {
+        const float s = __uint_as_float(e.w.z);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn((float)(int8_t)((i < 4 ? e.w.x : e.w.y) >> (8 * (i & 3))), s);
+    } else {
+        const float2 a = widen16(e.w.x, dtype), b = widen16(e.w.y, dtype), c = widen16(e.w.z, dtype), d = widen16(e.w.w, dtype);
+        x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y, x[4] = c.x, x[5] = c.y, x[6] = d.x, x[7] = d.y;
+    }
+    if (out_dtype == kF32) {
+        float4* const o = reinterpret_cast<float4*>(static_cast<float*>(out) + at);
+        o[0] = make_float4(x[0], x[1], x[2], x[3]), o[1] = make_float4(x[4], x[5], x[6], x[7]);
+        return;
+    }
+    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) =
+        make_uint4(pack16(x[0], x[1], out_dtype), pack16(x[2], x[3], out_dtype), pack16(x[4], x[5], out_dtype), pack16(x[6], x[7], out_dtype));
+}
+
+template <int LANES>
+__global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const KvReadParams p, uint32_t tokens) {
+    __shared__ int64_t first[KR_MOST];  // each token's row of head 0 in the cache, -1: none (its rows are zeros)
+    const uint32_t t0 = blockIdx.x * tokens;
+    if (threadIdx.x < tokens && t0 + threadIdx.x < p.total) {
         const int32_t t = (int32_t)(t0 + threadIdx.x);
         uint32_t lo = 0, hi = p.seqs;  // the sequence whose [cu[b], cu[b + 1]) holds t
         while (lo < hi) {
@@ -189,32 +219,49 @@ __global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const KvReadParams 
         int64_t row = -1;
         if (lo < p.seqs && t >= __ldg(p.cu + lo)) {
             const int64_t pos = (int64_t)(t - __ldg(p.cu + lo)) + (p.starts ? p.starts[lo] : 0);
-            const int64_t col = pos / p.c.page_size;
-            if (pos >= 0 && col < p.table_width) {
+            const uint32_t col = (uint32_t)pos / p.c.page_size;
+            if (pos >= 0 && pos <= INT32_MAX && col < p.table_width) {
                 const int32_t page = p.block_table[(int64_t)lo * p.table_width + col];
                 if (page >= 0 && (uint32_t)page < p.c.pages)
-                    row = (int64_t)page * p.c.heads * p.c.page_size + (pos - col * p.c.page_size);
+                    row = (int64_t)page * p.c.heads * p.c.page_size + ((uint32_t)pos - col * p.c.page_size);
             }
         }
         first[threadIdx.x] = row;
     }
     __syncthreads();
-    const uint32_t chunks = p.c.d / 8, per_token = p.c.heads * chunks;
-    const uint32_t n = min((uint32_t)KR_TOKENS, p.total - t0) * per_token;
-    for (uint32_t i = threadIdx.x; i < n; i += KW_THREADS) {
-        const uint32_t t = i / per_token, rest = i - t * per_token, h = rest / chunks, col = (rest - h * chunks) * 8;
-        const int64_t row0 = first[t], out = (int64_t)t0 * per_token * 8 + (int64_t)i * 8;
-        float k[8] = {}, v[8] = {};
-        if (row0 >= 0) {
-            const int64_t row = row0 + (int64_t)h * p.c.page_size;
-            read8(p.c, p.c.k, p.c.k_scale, row, col, k);
-            read8(p.c, p.c.v, p.c.v_scale, row, col, v);
+    constexpr uint32_t GROUPS = KW_THREADS / LANES;
+    const uint32_t col = threadIdx.x % LANES * 8, rows = min(tokens, p.total - t0) * p.c.heads;
+    if (col >= p.c.d) return;
+    for (uint32_t r0 = threadIdx.x / LANES; r0 < rows; r0 += GROUPS * KR_BATCH) {
+        Eight k[KR_BATCH], v[KR_BATCH];
+#pragma unroll
+        for (int i = 0; i < KR_BATCH; ++i) {
+            const uint32_t r = r0 + i * GROUPS, t = r / p.c.heads;
+            k[i].w = v[i].w = make_uint4(0, 0, 0, 0);
+            if (r < rows && first[t] >= 0) {
+                const int64_t row = first[t] + (int64_t)(r - t * p.c.heads) * p.c.page_size;
+                k[i] = read8(p.c, p.c.k, p.c.k_scale, row, col);
+                v[i] = read8(p.c, p.c.v, p.c.v_scale, row, col);
+            }
         }
-        store4(p.k_out, out, p.out_dtype, make_float4(k[0], k[1], k[2], k[3]));
-        store4(p.k_out, out + 4, p.out_dtype, make_float4(k[4], k[5], k[6], k[7]));
-        store4(p.v_out, out, p.out_dtype, make_float4(v[0], v[1], v[2], v[3]));
-        store4(p.v_out, out + 4, p.out_dtype, make_float4(v[4], v[5], v[6], v[7]));
+#pragma unroll
+        for (int i = 0; i < KR_BATCH; ++i) {
+            const uint32_t r = r0 + i * GROUPS;
+            if (r >= rows) break;
+            const int64_t at = ((int64_t)t0 * p.c.heads + r) * p.c.d + col;
+            write8(p.k_out, at, p.out_dtype, k[i], p.c.dtype);
+            write8(p.v_out, at, p.out_dtype, v[i], p.c.dtype);
+        }
     }
+}
+
+template <int LANES>
+cudaError_t launch_read(const KvReadParams& p, cudaStream_t stream) {
+    // up to 32 tokens a block (the look-up of their rows is done once for all heads), fewer where that leaves the SMs idle
+    uint32_t tokens = KR_MOST;
+    while (tokens > 1 && (p.total + tokens - 1) / tokens < 4 * 148) tokens /= 2;
+    kv_read_kernel<LANES><<<(p.total + tokens - 1) / tokens, KW_THREADS, 0, stream>>>(p, tokens);
+    return cudaGetLastError();
 }
 
 }  // namespace
@@ -226,8 +273,9 @@ cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream) {
 }
 
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream) {
-    kv_read_kernel<<<(p.total + KR_TOKENS - 1) / KR_TOKENS, KW_THREADS, 0, stream>>>(p);
-    return cudaGetLastError();
+    if (p.c.d > 64) return launch_read<16>(p, stream);
+    if (p.c.d > 32) return launch_read<8>(p, stream);
+    return launch_read<4>(p, stream);
 }
 
 }  // namespace iq2
