@@ -5,6 +5,7 @@ There is no fallback: if the CUDA library is missing, loading fails loudly.
 from __future__ import annotations
 
 import ctypes
+import struct
 import threading
 from pathlib import Path
 
@@ -80,33 +81,12 @@ class KvCacheStruct(ctypes.Structure):
                 ("page_size", _u32), ("head_dim", _u32), ("dtype", _int)]
 
 
-class Rows(ctypes.Structure):
-    """struct iq2_rows."""
-
-    _fields_ = [("data", _vp), ("token_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
-
-
-class KvTokens(ctypes.Structure):
-    """struct iq2_kv_tokens."""
-
-    _fields_ = [("k", Rows), ("v", Rows), ("q", Rows), ("dtype", _int), ("tokens", _u32), ("q_heads", _u32),
-                ("slots", _vp), ("positions", _vp), ("cos", _vp), ("sin", _vp), ("rope_len", _u32),
-                ("interleaved", _int), ("q_out", _vp), ("q_out_dtype", _int)]
-
-
-class AttentionPrompts(ctypes.Structure):
-    """struct iq2_attention_prompts."""
-
-    _fields_ = [("q", Rows), ("k", Rows), ("v", Rows), ("dtype", _int), ("sequences", _u32), ("q_tokens", _u32),
-                ("k_tokens", _u32), ("q_heads", _u32), ("kv_heads", _u32), ("head_dim", _u32), ("cu_seqlens_q", _vp),
-                ("cu_seqlens_k", _vp), ("causal", _int), ("scale", ctypes.c_float), ("out", _vp)]
-
-
-class AttentionTokens(ctypes.Structure):
-    """struct iq2_attention_tokens."""
-
-    _fields_ = [("q", Rows), ("dtype", _int), ("batch", _u32), ("q_heads", _u32), ("table_width", _u32),
-                ("block_table", _vp), ("seq_lens", _vp), ("scale", ctypes.c_float), ("out", _vp)]
+# The attention operators' argument structs, packed in the header's field order with C alignment (iq2_rows: a pointer and
+# two int64 strides). Packing bytes is several times cheaper than filling a ctypes.Structure, and these calls are short.
+_ROWS = "Pqq"
+KV_TOKENS = struct.Struct("@" + 3 * _ROWS + "iIIPPPPIiPi0q")           # iq2_kv_tokens
+ATTENTION_PROMPTS = struct.Struct("@" + 3 * _ROWS + "iIIIIIIPPifP")    # iq2_attention_prompts
+ATTENTION_TOKENS = struct.Struct("@" + _ROWS + "iIIIPPfP")             # iq2_attention_tokens
 
 
 class Iq2Error(RuntimeError):

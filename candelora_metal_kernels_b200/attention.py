@@ -20,6 +20,7 @@ from . import _lib
 from ._lib import Iq2Error
 from .iq2_matmul import _X_DTYPES, _bail
 
+_PREFILL_DTYPES = (torch.float16, torch.bfloat16)
 _KV_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.int8: _lib.KV_INT8}
 
 
@@ -36,34 +37,36 @@ def _call(device: torch.device, fn, *args) -> None:
         _lib.check(rc)
 
 
-def _on(op: str, device: torch.device, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            _bail(_lib.IQ2_ERR_DEVICE, f"{op} device mismatch: {name}={t.device}, expected {device}")
+def _on(op: str, device: torch.device, name: str, t: torch.Tensor) -> None:
+    if t.device != device:
+        _bail(_lib.IQ2_ERR_DEVICE, f"{op} device mismatch: {name}={t.device}, expected {device}")
 
 
-def _indices(op: str, name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
+def _indices(op: str, device: torch.device, name: str, t: torch.Tensor, dims: int) -> torch.Tensor:
+    if t.device != device:
+        _on(op, device, name, t)
     if t.dtype != torch.int32 or t.dim() != dims:
         _bail(_lib.IQ2_ERR_DTYPE, f"{op} expects {name} as an int32 tensor of rank {dims}, got {t.dtype} {list(t.shape)}")
     return t if t.is_contiguous() else t.contiguous()
 
 
-def _rows(op: str, name: str, t: torch.Tensor, heads: int | None, dim: int) -> torch.Tensor:
+def _rows(op: str, device: torch.device, name: str, t: torch.Tensor, heads: int | None, dim: int) -> torch.Tensor:
     """`t` as [tokens, heads, dim] with a contiguous last dimension (a copy where it is not)."""
-    if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
+    if t.device != device:
+        _on(op, device, name, t)
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != dim or (heads is not None and shape[1] != heads):
         _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op} expects {name} of shape [tokens, {heads if heads else 'heads'}, {dim}], "
-                                             f"got {list(t.shape)}")
+                                             f"got {list(shape)}")
     return t if t.stride(2) == 1 else t.contiguous()
 
 
-def _rows_struct(t: torch.Tensor) -> _lib.Rows:
-    return _lib.Rows(t.data_ptr(), t.stride(0), t.stride(1))
-
-
-def _out(op: str, out, shape, dtype, device) -> torch.Tensor:
+def _out(op: str, out, shape, dtype, device, like: torch.Tensor | None = None) -> torch.Tensor:
     if out is None:
+        if like is not None and like.dtype == dtype and like.is_contiguous():
+            return torch.empty_like(like)  # the cheapest way to a tensor of this shape
         return torch.empty(shape, dtype=dtype, device=device)
-    if tuple(out.shape) != tuple(shape) or out.dtype != dtype or not out.is_contiguous() or out.device != device:
+    if out.shape != shape or out.dtype != dtype or not out.is_contiguous() or out.device != device:
         _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: out must be a contiguous {dtype} {list(shape)} tensor on {device}")
     return out
 
@@ -81,7 +84,9 @@ class KvCache:
                                                  f"head_dim], got {list(k.shape)} and {list(v.shape)}")
         if k.device.type != "cuda":
             _bail(_lib.IQ2_ERR_DEVICE, f"{op} requires a CUDA device")
-        _on(op, k.device, v=v, k_scale=k_scale, v_scale=v_scale)
+        for name, t in (("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
+            if t is not None:
+                _on(op, k.device, name, t)
         if k.dtype not in _KV_DTYPES or v.dtype != k.dtype:
             _bail(_lib.IQ2_ERR_DTYPE, f"{op} unsupported cache dtype: {k.dtype}, {v.dtype}")
         if k.dtype == torch.int8:
@@ -122,41 +127,43 @@ def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     default)."""
     op = "kv_cache_write"
     d, device = cache.head_dim, cache.device
-    _on(op, device, k=k, v=v, slots=slots, q=q, positions=positions, cos=cos, sin=sin)
-    k, v = _rows(op, "k", k, cache.kv_heads, d), _rows(op, "v", v, cache.kv_heads, d)
-    tokens = k.shape[0]
-    if k.dtype not in _X_DTYPES or v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
-        _bail(_lib.IQ2_ERR_DTYPE, f"{op} expects q, k and v in one of f32, f16 and bf16, got {k.dtype} and {v.dtype}"
+    k, v = _rows(op, device, "k", k, cache.kv_heads, d), _rows(op, device, "v", v, cache.kv_heads, d)
+    slots = _indices(op, device, "slots", slots, 1)
+    tokens, dtype = k.shape[0], k.dtype
+    if dtype not in _X_DTYPES or v.dtype != dtype or (q is not None and q.dtype != dtype):
+        _bail(_lib.IQ2_ERR_DTYPE, f"{op} expects q, k and v in one of f32, f16 and bf16, got {dtype} and {v.dtype}"
                                   f"{'' if q is None else f' and {q.dtype}'}")
-    slots = _indices(op, "slots", slots, 1)
-    args = _lib.KvTokens(k=_rows_struct(k), v=_rows_struct(v), dtype=_X_DTYPES[k.dtype], tokens=tokens,
-                         slots=slots.data_ptr(), interleaved=int(interleaved))
-    counts = {"v": v.shape[0], "slots": slots.shape[0]}
+    same = v.shape[0] == tokens and slots.shape[0] == tokens
+    rows_q, out_ptr, out_code, rope = (0, 0, 0, 0), 0, 0, (0, 0, 0, 0)
     if q is not None:
-        q = _rows(op, "q", q, None, d)
-        counts["q"] = q.shape[0]
-        q_dtype = q_dtype or q.dtype
+        q = _rows(op, device, "q", q, None, d)
+        same = same and q.shape[0] == tokens
+        q_dtype = q_dtype or dtype
         if q_dtype not in _X_DTYPES:
             _bail(_lib.IQ2_ERR_DTYPE, f"{op} unsupported q dtype: {q_dtype}")
-        q_out = _out(op, q_out, q.shape, q_dtype, device)
-        args.q, args.q_heads = _rows_struct(q), q.shape[1]
-        args.q_out, args.q_out_dtype = q_out.data_ptr(), _X_DTYPES[q_dtype]
+        q_out = _out(op, q_out, q.shape, q_dtype, device, q)
+        rows_q, out_ptr, out_code = (q.data_ptr(), q.stride(0), q.stride(1), q.shape[1]), q_out.data_ptr(), _X_DTYPES[q_dtype]
     elif q_out is not None or q_dtype is not None:
         _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: q_out and q_dtype go with q")
     if cos is not None or sin is not None or positions is not None:
         if cos is None or sin is None or positions is None:
             _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: cos, sin and positions go together")
-        for t in (cos, sin):
+        for name, t in (("cos", cos), ("sin", sin)):
+            _on(op, device, name, t)
             if t.dtype != torch.float32 or t.dim() != 2 or t.shape != cos.shape or t.shape[1] * 2 != d or not t.is_contiguous():
                 _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op} expects contiguous f32 cos and sin [rows, {d // 2}], got "
                                                      f"{t.dtype} {list(t.shape)}")
-        positions = _indices(op, "positions", positions, 1)
-        counts["positions"] = positions.shape[0]
-        args.positions, args.cos, args.sin, args.rope_len = positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0]
-    if any(n != tokens for n in counts.values()):
-        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: k has {tokens} tokens, the others {counts}")
+        positions = _indices(op, device, "positions", positions, 1)
+        same = same and positions.shape[0] == tokens
+        rope = (positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), cos.shape[0])
+    if not same:
+        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: k has {tokens} tokens, v {v.shape[0]}, slots {slots.shape[0]}"
+                                             f"{'' if q is None else f', q {q.shape[0]}'}"
+                                             f"{'' if positions is None else f', positions {positions.shape[0]}'}")
     if tokens:
-        _call(device, _lib.load().iq2_kv_cache_write, cache._ptr, ctypes.addressof(args))
+        args = _lib.KV_TOKENS.pack(k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), *rows_q[:3],
+                                   _X_DTYPES[dtype], tokens, rows_q[3], slots.data_ptr(), *rope, interleaved, out_ptr, out_code)
+        _call(device, _lib.load().iq2_kv_cache_write, cache._ptr, args)
     return q_out
 
 
@@ -167,10 +174,9 @@ def kv_cache_read(cache: KvCache, block_table: torch.Tensor, cu_seqlens: torch.T
     sequence whose pages are block_table[b] (int32 [sequences, width]). Rows of no sequence are zeros."""
     op = "kv_cache_read"
     device = cache.device
-    _on(op, device, block_table=block_table, cu_seqlens=cu_seqlens, starts=starts)
-    table, cu = _indices(op, "block_table", block_table, 2), _indices(op, "cu_seqlens", cu_seqlens, 1)
+    table, cu = _indices(op, device, "block_table", block_table, 2), _indices(op, device, "cu_seqlens", cu_seqlens, 1)
     seqs, width = table.shape
-    starts = None if starts is None else _indices(op, "starts", starts, 1)
+    starts = None if starts is None else _indices(op, device, "starts", starts, 1)
     if cu.shape[0] != seqs + 1 or (starts is not None and starts.shape[0] != seqs):
         _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: block_table has {seqs} sequences, cu_seqlens {cu.shape[0]} entries")
     if dtype is None:
@@ -205,28 +211,32 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     op = "attention_prefill"
     if q.device.type != "cuda":
         _bail(_lib.IQ2_ERR_DEVICE, f"{op} requires a CUDA device")
-    cu_seqlens_k = cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k
-    device = q.device
-    _on(op, device, k=k, v=v, cu_seqlens_q=cu_seqlens_q, cu_seqlens_k=cu_seqlens_k)
-    if q.dtype not in (torch.float16, torch.bfloat16) or k.dtype != q.dtype or v.dtype != q.dtype:
-        _bail(_lib.IQ2_ERR_DTYPE, f"{op} expects q, k and v all in f16 or all in bf16, got {q.dtype}, {k.dtype}, {v.dtype}")
-    q = _rows(op, "q", q, None, q.shape[-1])
+    device, dtype = q.device, q.dtype
+    if dtype not in _PREFILL_DTYPES or k.dtype != dtype or v.dtype != dtype:
+        _bail(_lib.IQ2_ERR_DTYPE, f"{op} expects q, k and v all in f16 or all in bf16, got {dtype}, {k.dtype}, {v.dtype}")
+    q = _rows(op, device, "q", q, None, q.shape[-1])
     tokens, heads, d = q.shape
-    k = _rows(op, "k", k, None, d)
-    v = _rows(op, "v", v, k.shape[1], d)
-    if v.shape[0] != k.shape[0]:
-        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: k has {k.shape[0]} tokens, v {v.shape[0]}")
-    cu_q, cu_k = _indices(op, "cu_seqlens_q", cu_seqlens_q, 1), _indices(op, "cu_seqlens_k", cu_seqlens_k, 1)
-    if cu_q.shape[0] != cu_k.shape[0] or cu_q.shape[0] == 0:
-        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: cu_seqlens_q and cu_seqlens_k have {cu_q.shape[0]} and {cu_k.shape[0]} entries")
+    k = _rows(op, device, "k", k, None, d)
+    keys, kv_heads, _ = k.shape
+    v = _rows(op, device, "v", v, kv_heads, d)
+    if v.shape[0] != keys:
+        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: k has {keys} tokens, v {v.shape[0]}")
+    cu_q = cu_k = _indices(op, device, "cu_seqlens_q", cu_seqlens_q, 1)
+    if cu_seqlens_k is not None:
+        cu_k = _indices(op, device, "cu_seqlens_k", cu_seqlens_k, 1)
+    entries = cu_q.shape[0]
+    if cu_k.shape[0] != entries or entries == 0:
+        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: cu_seqlens_q and cu_seqlens_k have {entries} and {cu_k.shape[0]} entries")
     q, k, v = _aligned_rows(q), _aligned_rows(k), _aligned_rows(v)
-    out = _out(op, out, q.shape, q.dtype, device)
-    args = _lib.AttentionPrompts(_rows_struct(q), _rows_struct(k), _rows_struct(v), _X_DTYPES[q.dtype], cu_q.shape[0] - 1,
-                                 tokens, k.shape[0], heads, k.shape[1], d, cu_q.data_ptr(), cu_k.data_ptr(), int(causal),
-                                 _scale(op, scale), out.data_ptr())
+    out = _out(op, out, q.shape, dtype, device, q)
+    args = _lib.ATTENTION_PROMPTS.pack(
+        q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1),
+        _X_DTYPES[dtype], entries - 1, tokens, keys, heads, kv_heads, d, cu_q.data_ptr(), cu_k.data_ptr(), causal,
+        _scale(op, scale), out.data_ptr())
     lib = _lib.load()
-    ws, ws_len, _keep = _scratch(lib.iq2_attention_prefill_workspace_size(ctypes.addressof(args)), workspace, device)
-    _call(device, lib.iq2_attention_prefill, ctypes.addressof(args), ws, ws_len)
+    if workspace is None:
+        workspace = _scratch(lib.iq2_attention_prefill_workspace_size(args), device)
+    _call(device, lib.iq2_attention_prefill, args, *_buffer(workspace))
     return out
 
 
@@ -238,13 +248,12 @@ def _scale(op: str, scale: float | None) -> float:
     return scale
 
 
-def _scratch(need: int, workspace, device):
-    """(pointer, length, tensor to keep) of a workspace of `need` bytes: the caller's, or a new one."""
-    if need == 0:
-        return None, 0, None
-    if workspace is None or workspace.numel() < need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    return workspace.data_ptr(), workspace.numel(), workspace
+def _scratch(need: int, device):
+    return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+
+
+def _buffer(workspace: torch.Tensor | None):
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
 
 
 def attention_decode_workspace_bytes(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor) -> int:
@@ -261,18 +270,20 @@ def attention_decode(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor,
     shape and dtype; the accumulation is in f32."""
     op = "attention_decode"
     device = cache.device
-    _on(op, device, q=q, block_table=block_table, seq_lens=seq_lens)
-    q = _rows(op, "q", q, None, cache.head_dim)
-    batch, heads, _ = q.shape
-    if q.dtype not in _X_DTYPES:
-        _bail(_lib.IQ2_ERR_DTYPE, f"{op} unsupported q dtype: {q.dtype}")
-    table, lens = _indices(op, "block_table", block_table, 2), _indices(op, "seq_lens", seq_lens, 1)
-    if table.shape[0] != batch or lens.shape[0] != batch:
-        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: q has a batch of {batch}, block_table {table.shape[0]}, seq_lens {lens.shape[0]}")
-    out = _out(op, out, q.shape, q.dtype, device)
-    args = _lib.AttentionTokens(_rows_struct(q), _X_DTYPES[q.dtype], batch, heads, table.shape[1], table.data_ptr(),
-                                lens.data_ptr(), _scale(op, scale), out.data_ptr())
+    q = _rows(op, device, "q", q, None, cache.head_dim)
+    batch, heads, _ = shape = q.shape
+    dtype = q.dtype
+    if dtype not in _X_DTYPES:
+        _bail(_lib.IQ2_ERR_DTYPE, f"{op} unsupported q dtype: {dtype}")
+    table, lens = _indices(op, device, "block_table", block_table, 2), _indices(op, device, "seq_lens", seq_lens, 1)
+    tables, width = table.shape
+    if tables != batch or lens.shape[0] != batch:
+        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: q has a batch of {batch}, block_table {tables}, seq_lens {lens.shape[0]}")
+    out = _out(op, out, shape, dtype, device, q)
+    args = _lib.ATTENTION_TOKENS.pack(q.data_ptr(), q.stride(0), q.stride(1), _X_DTYPES[dtype], batch, heads, width,
+                                      table.data_ptr(), lens.data_ptr(), _scale(op, scale), out.data_ptr())
     lib = _lib.load()
-    ws, ws_len, _keep = _scratch(lib.iq2_attention_decode_workspace_size(cache._ptr, batch, heads), workspace, device)
-    _call(device, lib.iq2_attention_decode, cache._ptr, ctypes.addressof(args), ws, ws_len)
+    if workspace is None:
+        workspace = _scratch(attention_decode_workspace_bytes(q, cache, block_table), device)
+    _call(device, lib.iq2_attention_decode, cache._ptr, args, *_buffer(workspace))
     return out

@@ -56,16 +56,6 @@ struct JoinRecord {
 };
 inline size_t records_bytes(uint32_t blocks) { return (blocks * sizeof(JoinRecord) + 255) / 256 * 256; }
 
-// The units are dealt as evenly as whole units go: the first units % blocks blocks take one more than the others.
-struct Deal {
-    uint64_t each, more;  // units / blocks, units % blocks
-    __device__ __forceinline__ uint64_t start(uint32_t block) const { return block * each + min((uint64_t)block, more); }
-    __device__ __forceinline__ uint32_t block_of(uint64_t unit) const {
-        const uint64_t big = more * (each + 1);
-        return (uint32_t)(unit < big ? unit / (each + 1) : more + (unit - big) / each);
-    }
-};
-
 __device__ __forceinline__ uint32_t seq_len(const DecodeParams& p, uint32_t b) {
     const uint64_t most = min((uint64_t)p.table_width * p.c.page_size, (uint64_t)0x7FFFFFFF);
     return (uint32_t)min((uint64_t)max(__ldg(p.seq_lens + b), 0), most);
@@ -159,8 +149,13 @@ struct Cursor {
         if (done()) return;
         if (++item == items) {
             item = 0;
-            do len = seq_len(p, ++b);
-            while (len == 0);
+            do {
+                if (++b >= p.batch) {  // (not reached while the lengths stay as they were)
+                    unit = end;
+                    return;
+                }
+                len = seq_len(p, b);
+            } while (len == 0);
             units = (len + UNIT - 1) / UNIT;
         }
         cut();
@@ -189,7 +184,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     for (uint32_t b = lane; b < p.batch; b += 32) units += (seq_len(p, b) + UNIT - 1) / UNIT;
     for (int o = 16; o > 0; o /= 2) units += __shfl_xor_sync(0xFFFFFFFFu, units, o);
     units *= items;
-    const Deal deal{units / gridDim.x, units % gridDim.x};
+    const Deal deal(units, gridDim.x);
     const uint64_t u0 = deal.start(blockIdx.x), u1 = deal.start(blockIdx.x + 1);
     // sequences of length 0: zeros
     for (uint32_t b = blockIdx.x; b < p.batch; b += gridDim.x)
@@ -203,6 +198,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     Cursor cur{};
     uint64_t before = 0;  // units of the sequences before
     for (uint32_t b0 = 0;; b0 += 32) {
+        if (b0 >= p.batch) return;  // (not reached while the lengths stay as they were)
         const uint32_t len = b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0u, own = (len + UNIT - 1) / UNIT;
         uint64_t upto = (uint64_t)own * items;
         for (int o = 1; o < 32; o *= 2) {
@@ -570,6 +566,9 @@ cudaError_t launch(const DecodeParams& p, uint8_t* workspace, uint32_t blocks, c
     JoinRecord* const records = reinterpret_cast<JoinRecord*>(workspace);
     float* const parts = reinterpret_cast<float*>(workspace + records_bytes(blocks));
     cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e != cudaSuccess) return e;
+    // (the second kernel keeps the first one's split of shared memory: changing it would drain the SMs twice a call)
+    e = cudaFuncSetAttribute(join_kernel<DP>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
     decode_kernel<DP, KIND><<<blocks, AD_THREADS, S::SMEM, stream>>>(p, parts, records, chunks);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;

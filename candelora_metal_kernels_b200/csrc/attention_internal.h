@@ -71,4 +71,20 @@ struct PrefillParams {
 size_t attention_prefill_workspace(const PrefillParams& p, int num_sms);
 cudaError_t launch_attention_prefill(const PrefillParams& p, void* workspace, int num_sms, cudaStream_t stream);
 
+#ifdef __CUDACC__
+// A line of work units dealt to blocks as evenly as whole units go: the first units % blocks blocks take one more than the
+// others, each a contiguous part.
+struct Deal {
+    uint64_t each, more;
+    __device__ __forceinline__ Deal(uint64_t units, uint32_t blocks) : each(units / blocks), more(units % blocks) {}
+    __device__ __forceinline__ uint64_t start(uint32_t block) const {
+        return block * each + (block < more ? (uint64_t)block : more);
+    }
+    __device__ __forceinline__ uint32_t block_of(uint64_t unit) const {
+        const uint64_t big = more * (each + 1);
+        return (uint32_t)(unit < big ? unit / (each + 1) : more + (unit - big) / each);
+    }
+};
+#endif
+
 }  // namespace iq2
