@@ -14,9 +14,13 @@
 // so the second piece, which gives f32 activations 22 bits (f16 pieces) or 16 (bf16 pieces), costs no instruction.
 //   * bf16 caches take bf16 pieces (their range); f16 and int8 caches f16 pieces of q / 2^e, 2^e the power of two above
 //     the head's largest |q|: pieces of at least 22 bits at any magnitude.
-//   * int8 codes become f16 by one byte permute (1024 + code + 128, exact) and one subtraction a pair; the key scale
-//     multiplies s. The value scale w_j multiplies p, with the running maximum taken over s_j + log2 w_j so that p w stays
-//     at most about 1, the range of its f16 pieces; the sum of p itself stays f32.
+//   * A bf16 cache under f32 activations takes a third piece (a second pair of products), or p would end at 2^-17.
+//   * int8 codes: the byte code + 128 with a zero byte above it is the f16 number (code + 128) 2^-24 (a subnormal, exact and
+//     full speed in the matrix instructions), so a pair costs half an exclusive or and one byte permute. The 128s are taken
+//     off as products with the constant 128 2^-24: S starts from minus them, O has them as one more column of P V.
+//   * The key scale multiplies s, the value scale multiplies p. The reference m of a head's exponents moves when a product
+//     p w exceeds 2^8 (it starts where the first tile's largest is 1), so that p w keeps to the range of f16; the sum of p
+//     itself is f32.
 // The maxima, sums, s, p and o are f32.
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"
@@ -29,13 +33,17 @@ namespace {
 
 constexpr int AD_WARPS = 8, AD_THREADS = AD_WARPS * 32, AD_STAGES = 3;
 constexpr int AD_HEADS = 8;                     // query heads of an item
-constexpr float AD_MIN_SCALE = 7.88860905e-31f;  // 2^-100: the smallest value scale the maximum goes by
+constexpr float AD_MIN_SCALE = 7.88860905e-31f;  // 2^-100: the smallest value scale (a row held as zeros has 0)
+constexpr float AD_LAZY = 256.f;                 // how far p times the value scale may grow before the reference moves
+constexpr uint32_t CODE_ZERO = 0x00800080u;      // two codes of 0 as f16: 128 2^-24
+constexpr float CODE_UNIT = 16777216.f;          // 2^24
 constexpr float LOG2E = 1.44269504f;
 
 enum CacheKind { CK_F16, CK_BF16, CK_INT8 };
 
-template <int DP, int KIND>
+template <int DP, int KIND, bool THIRD>
 struct DecodeShape {
+    static constexpr int PIECES = THIRD ? 3 : 2;
     static constexpr int ESIZE = KIND == CK_INT8 ? 1 : 2;
     static constexpr int TOK = KIND == CK_INT8 ? 32 : 16;  // tokens of a warp's stage: 8 KB of K and V at DP = 128
     static constexpr int UNIT = TOK * AD_WARPS;
@@ -44,7 +52,7 @@ struct DecodeShape {
     static constexpr int SCALES = KIND == CK_INT8 ? TOK * 8 : 0;
     static constexpr int STAGE = 2 * TOK * ROW + SCALES;
     static constexpr int RING = AD_STAGES * STAGE;
-    static constexpr int Q_BYTES = 2 * AD_HEADS * DP * 2;
+    static constexpr int Q_BYTES = PIECES * AD_HEADS * DP * 2;
     static constexpr int PART = AD_HEADS * (DP + 2);       // floats of one (o, max, sum)
     static constexpr int SMEM = AD_WARPS * RING + Q_BYTES + 4 * PART * 4 + AD_HEADS * 4;
 };
@@ -55,6 +63,15 @@ struct JoinRecord {
     uint32_t b, item, c0, c1, slot;
 };
 inline size_t records_bytes(uint32_t blocks) { return (blocks * sizeof(JoinRecord) + 255) / 256 * 256; }
+
+struct DecodeArgs {
+    DecodeParams p;
+    float* parts;
+    JoinRecord* records;
+    double inv_blocks;                      // 1 / the blocks of the launch
+    uint32_t chunks_of_heads, page_magic;   // token / page_size = (token page_magic) >> 32 + page_shift (tokens below 2^31)
+    int page_shift;                         // -1: pages of one token
+};
 
 __device__ __forceinline__ uint32_t seq_len(const DecodeParams& p, uint32_t b) {
     const uint64_t most = min((uint64_t)p.table_width * p.c.page_size, (uint64_t)0x7FFFFFFF);
@@ -116,11 +133,10 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
                  : "r"(addr));
 }
 
-// Two bytes of biased codes (code + 128) -> two f16 codes: 0x6400 | byte is 1024 + byte.
-__device__ __forceinline__ uint32_t codes_to_half2(uint32_t biased, uint32_t sel) {
-    const uint32_t u = prmt(biased, 0x64646464u, sel);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t*>(&h);
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
 
 // Byte offset of 16-byte chunk c of row r in a K or V stage. The readers of a phase must meet eight different 16-byte
@@ -162,18 +178,20 @@ struct Cursor {
     }
 };
 
-template <int DP, int KIND>
+template <int DP, int KIND, bool THIRD>
 __global__ void __launch_bounds__(AD_THREADS, 1)
-    decode_kernel(const DecodeParams p, float* __restrict__ parts, JoinRecord* __restrict__ records, uint32_t chunks_of_heads) {
-    using S = DecodeShape<DP, KIND>;
-    constexpr bool BF = KIND == CK_BF16;
+    decode_kernel(const __grid_constant__ DecodeArgs a) {
+    using S = DecodeShape<DP, KIND, THIRD>;
+    constexpr bool BF = KIND == CK_BF16, I8 = KIND == CK_INT8;
     constexpr int TOK = S::TOK, UNIT = S::UNIT, NT = DP / 8, KS = DP / 16, ST = TOK / 8;
+    constexpr uint32_t ALL = TOK == 32 ? 0xFFFFFFFFu : (1u << TOK) - 1;
+    const DecodeParams& p = a.p;
     extern __shared__ __align__(128) uint8_t smem[];
-    uint8_t* const q_smem = smem + AD_WARPS * S::RING;                     // [8 heads][2 pieces][DP] 16-bit
+    uint8_t* const q_smem = smem + AD_WARPS * S::RING;                     // [8 heads][pieces][DP] 16-bit
     float* const part_smem = reinterpret_cast<float*>(q_smem + S::Q_BYTES);  // 4 x (o, max, sum)
     float* const q_factor = part_smem + 4 * S::PART;                       // [8] scale log2(e) 2^e
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    const uint32_t d = p.c.d, group = p.q_heads / p.c.heads, items = p.c.heads * chunks_of_heads;
+    const uint32_t d = p.c.d, group = p.q_heads / p.c.heads, items = p.c.heads * a.chunks_of_heads;
     pdl_launch_dependents();
 
     // ---- this block's part of the line (every warp works it out for itself) ----
@@ -181,26 +199,34 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     if (d < DP)
         for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
     uint64_t units = 0;
-    for (uint32_t b = lane; b < p.batch; b += 32) units += (seq_len(p, b) + UNIT - 1) / UNIT;
+#pragma unroll 1
+    for (uint32_t b0 = 0; b0 < p.batch; b0 += 32) {
+        const uint32_t b = b0 + lane, len = b < p.batch ? seq_len(p, b) : 1u;
+        units += b < p.batch ? (len + UNIT - 1) / UNIT : 0u;
+        // sequences of length 0: zeros, a block a sequence
+        uint32_t empty = __ballot_sync(0xFFFFFFFFu, len == 0 && b % gridDim.x == blockIdx.x);
+        for (; empty != 0; empty &= empty - 1)
+            for (uint32_t i = threadIdx.x; i < p.q_heads * d; i += AD_THREADS)
+                store_elem(p.out, (int64_t)(b0 + __ffs(empty) - 1) * p.q_heads * d + i, p.dtype, 0.f);
+    }
+#pragma unroll 1
     for (int o = 16; o > 0; o /= 2) units += __shfl_xor_sync(0xFFFFFFFFu, units, o);
     units *= items;
-    const Deal deal(units, gridDim.x);
-    const uint64_t u0 = deal.start(blockIdx.x), u1 = deal.start(blockIdx.x + 1);
-    // sequences of length 0: zeros
-    for (uint32_t b = blockIdx.x; b < p.batch; b += gridDim.x)
-        if (seq_len(p, b) == 0)
-            for (uint32_t i = threadIdx.x; i < p.q_heads * d; i += AD_THREADS)
-                store_elem(p.out, (int64_t)b * p.q_heads * d + i, p.dtype, 0.f);
+    uint64_t each = (uint64_t)((double)units * a.inv_blocks);  // units / blocks, rounded up
+    while (each * gridDim.x < units) ++each;
+    const uint64_t u0 = min(blockIdx.x * each, units), u1 = min(u0 + each, units);
     if (u0 >= u1) {
-        if (threadIdx.x == 0) records[blockIdx.x].c1 = 0;
+        if (threadIdx.x == 0) a.records[blockIdx.x].c1 = 0;
         return;
     }
     Cursor cur{};
     uint64_t before = 0;  // units of the sequences before
+#pragma unroll 1
     for (uint32_t b0 = 0;; b0 += 32) {
         if (b0 >= p.batch) return;  // (not reached while the lengths stay as they were)
         const uint32_t len = b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0u, own = (len + UNIT - 1) / UNIT;
         uint64_t upto = (uint64_t)own * items;
+#pragma unroll 1
         for (int o = 1; o < 32; o *= 2) {
             const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
             if (lane >= (uint32_t)o) upto += x;
@@ -220,19 +246,26 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     cur.cut();
     Cursor pre = cur;
     if (threadIdx.x == 0) {
-        // the first block whose part begins inside an item joins it
+        // the first block whose part begins inside an item joins it: the block before it has the item's first unit
         const uint64_t unit0 = u0 - cur.k;
-        const uint32_t c0 = cur.k > 0 ? deal.block_of(unit0) : blockIdx.x;
-        JoinRecord r{cur.b, cur.item, c0, 0, 0};
-        if (c0 + 1 == blockIdx.x) r.c1 = deal.block_of(unit0 + cur.units - 1), r.slot = deal.start(c0) == unit0 ? 0 : 1;
-        records[blockIdx.x] = r;
+        JoinRecord r{cur.b, cur.item, blockIdx.x - 1, 0, 0};
+        if (cur.k > 0 && u0 - each <= unit0) {
+            r.c1 = blockIdx.x, r.slot = u0 - each == unit0 ? 0 : 1;
+            while ((r.c1 + 1) * each < unit0 + cur.units) ++r.c1;
+        }
+        a.records[blockIdx.x] = r;
     }
 
     // ---- the copies: tile `i` (TOK tokens) of pre's piece of an item, one page lookup ahead ----
     uint8_t* const ring = smem + warp * S::RING;
     const uint32_t ring_u32 = smem_u32(ring);
     if (d < DP) __syncwarp();
-    uint32_t pre_i = warp, pre_page = 0;  // the tile to copy next and this lane's token's page number
+    // a tile's rows lie side by side in one page, or each lane looks one row up
+    const bool side_by_side = p.c.page_size % TOK == 0;
+    const uint32_t row_bytes = d * S::ESIZE, chunk = lane % S::CHUNKS, row0 = lane / S::CHUNKS;
+    constexpr int ROWS = 32 / S::CHUNKS;  // rows that the warp copies at a time
+    auto page_of = [&](uint32_t tok) { return a.page_shift < 0 ? tok : __umulhi(tok, a.page_magic) >> a.page_shift; };
+    uint32_t pre_i = warp, pre_page = 0, pre_first = 0;  // the tile to copy next, its page, the first token of that page
     auto pre_tokens = [&](const Cursor& c) { return min(c.len, (c.k + c.n) * UNIT) - c.k * UNIT; };
     auto find_tile = [&]() {  // the next tile of this warp, and its page numbers under way
         while (!pre.done() && pre_i * TOK >= pre_tokens(pre)) {
@@ -240,55 +273,73 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             pre_i = warp;
         }
         if (pre.done()) return;
-        const uint32_t tok = pre.k * UNIT + pre_i * TOK + lane;
-        if (lane < TOK && tok < pre.len)
-            pre_page = (uint32_t)__ldg(p.block_table + (int64_t)pre.b * p.table_width + tok / p.c.page_size);
+        const uint32_t tok = pre.k * UNIT + pre_i * TOK + (side_by_side ? 0 : lane);
+        if (tok < pre.len) {
+            const uint32_t at = page_of(tok);
+            pre_first = at * p.c.page_size;
+            pre_page = (uint32_t)__ldg(p.block_table + (int64_t)pre.b * p.table_width + at);
+        }
     };
+    // Copies the tile and returns a bit for each token that takes part: rows of tokens past the end, or of pages outside
+    // the cache, are zeros, and what such pages hold cannot matter.
     auto copy_tile = [&](uint32_t stage) {
-        if (!pre.done()) {
-            const uint32_t tok = pre.k * UNIT + pre_i * TOK + lane, h = pre.item / chunks_of_heads;
-            const bool valid = lane < TOK && tok < pre.len && pre_page < p.c.pages;
-            const int64_t row = valid ? ((int64_t)pre_page * p.c.heads + h) * p.c.page_size + tok % p.c.page_size : -1;
-            const uint32_t dst = ring_u32 + stage * S::STAGE;
-            const uint32_t c = lane % S::CHUNKS, r0 = lane / S::CHUNKS;
-            const uint32_t row_bytes = d * S::ESIZE;
-            const bool inside = c * 16 < row_bytes;
+        const uint32_t tok = pre.k * UNIT + pre_i * TOK, h = pre.item / a.chunks_of_heads, dst = ring_u32 + stage * S::STAGE;
+        const uint32_t left = pre.len - tok, in_page = tok + (side_by_side ? 0 : lane) - pre_first;
+        const int64_t row = ((int64_t)pre_page * p.c.heads + h) * p.c.page_size + in_page;
+        const uint8_t *const k = static_cast<const uint8_t*>(p.c.k), *const v = static_cast<const uint8_t*>(p.c.v);
+        const bool inside = chunk * 16 < row_bytes;
+        uint32_t here = ALL;
+        if (side_by_side && left >= TOK && pre_page < p.c.pages) {
+            const int64_t off = row * row_bytes + row0 * row_bytes + chunk * 16;
+            const uint8_t *pk = k + off, *pv = v + off;
+            if (inside) {
 #pragma unroll
-            for (int i = 0; i < TOK * S::CHUNKS / 32; ++i) {
-                const uint32_t r = r0 + i * (32 / S::CHUNKS);
-                const int64_t src = __shfl_sync(0xFFFFFFFFu, row, r);
-                const int64_t off = src < 0 ? 0 : src * row_bytes + c * 16;
-                if (inside) {  // a token that takes no part is zeros: what its page holds cannot matter
-                    cp_async_16(dst + stage_offset<S::CHUNKS, KIND == CK_INT8>(r, c), static_cast<const uint8_t*>(p.c.k) + off, src < 0 ? 0 : 16);
-                    cp_async_16(dst + TOK * S::ROW + stage_offset<S::CHUNKS, false>(r, c), static_cast<const uint8_t*>(p.c.v) + off, src < 0 ? 0 : 16);
+                for (int i = 0; i < TOK / ROWS; ++i, pk += ROWS * row_bytes, pv += ROWS * row_bytes) {
+                    cp_async_16(dst + stage_offset<S::CHUNKS, I8>(row0 + i * ROWS, chunk), pk);
+                    cp_async_16(dst + TOK * S::ROW + stage_offset<S::CHUNKS, false>(row0 + i * ROWS, chunk), pv);
                 }
             }
-            if (KIND == CK_INT8) {
-                const int64_t off = row < 0 ? 0 : row;
-                cp_async_4(dst + 2 * TOK * S::ROW + lane * 4, p.c.k_scale + off, row < 0 ? 0 : 4);
-                cp_async_4(dst + 2 * TOK * S::ROW + TOK * 4 + lane * 4, p.c.v_scale + off, row < 0 ? 0 : 4);
+            if (I8) {
+                cp_async_4(dst + 2 * TOK * S::ROW + lane * 4, p.c.k_scale + row + lane, 4);
+                cp_async_4(dst + 2 * TOK * S::ROW + TOK * 4 + lane * 4, p.c.v_scale + row + lane, 4);
             }
-            pre_i += AD_WARPS;
+        } else {
+            const bool valid = lane < TOK && lane < left && pre_page < p.c.pages;
+            here = __ballot_sync(0xFFFFFFFFu, valid);
+            const int64_t mine = !valid ? -1 : side_by_side ? row + lane : row;
+#pragma unroll 1
+            for (int i = 0; i < TOK / ROWS; ++i) {
+                const uint32_t r = row0 + i * ROWS;
+                const int64_t src = __shfl_sync(0xFFFFFFFFu, mine, r);
+                const int64_t off = src < 0 ? 0 : src * row_bytes + chunk * 16;
+                if (inside) {
+                    cp_async_16(dst + stage_offset<S::CHUNKS, I8>(r, chunk), k + off, src < 0 ? 0 : 16);
+                    cp_async_16(dst + TOK * S::ROW + stage_offset<S::CHUNKS, false>(r, chunk), v + off, src < 0 ? 0 : 16);
+                }
+            }
+            if (I8) {
+                cp_async_4(dst + 2 * TOK * S::ROW + lane * 4, p.c.k_scale + (valid ? mine : 0), valid ? 4 : 0);
+                cp_async_4(dst + 2 * TOK * S::ROW + TOK * 4 + lane * 4, p.c.v_scale + (valid ? mine : 0), valid ? 4 : 0);
+            }
         }
-        cp_async_commit();
+        pre_i += AD_WARPS;
+        return here;
     };
-    // Tokens whose page is outside the cache are rare and take no part: a bit for each token of a stage.
     uint32_t present[AD_STAGES] = {};
     auto copy_and_find = [&](int stage) {
         if (!pre.done()) {
-            const uint32_t tok = pre.k * UNIT + pre_i * TOK + lane;
-            const uint32_t bits = __ballot_sync(0xFFFFFFFFu, lane < TOK && tok < pre.len && pre_page < p.c.pages);
+            const uint32_t here = copy_tile(stage);
 #pragma unroll
             for (int s = 0; s < AD_STAGES; ++s)
-                if (s == stage) present[s] = bits;
+                if (s == stage) present[s] = here;
+            find_tile();
         }
-        copy_tile(stage);
-        find_tile();
+        cp_async_commit();
     };
     // q of an item, a warp a head: loaded while the copies before it are under way
     float q_next[DP / 32];
     auto load_q = [&](const Cursor& c) {
-        const uint32_t kv = c.item / chunks_of_heads, h0 = kv * group + (c.item % chunks_of_heads) * AD_HEADS;
+        const uint32_t kv = c.item / a.chunks_of_heads, h0 = kv * group + (c.item % a.chunks_of_heads) * AD_HEADS;
         const bool has = warp < min((uint32_t)AD_HEADS, (kv + 1) * group - h0);
         const int64_t at = (int64_t)c.b * p.q.token_stride + (int64_t)(h0 + warp) * p.q.head_stride;
 #pragma unroll
@@ -296,56 +347,59 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     };
     find_tile();
     load_q(cur);
+#pragma unroll 1
     for (int s = 0; s < AD_STAGES - 1; ++s) copy_and_find(s);
     int stage = 0;
 
     while (!cur.done()) {
-        // ---- q of the item: two 16-bit pieces of each head ----
-        const uint32_t kv_head = cur.item / chunks_of_heads, head0 = kv_head * group + (cur.item % chunks_of_heads) * AD_HEADS;
+        // ---- q of the item: the 16-bit pieces of each head ----
+        const uint32_t kv_head = cur.item / a.chunks_of_heads, head0 = kv_head * group + (cur.item % a.chunks_of_heads) * AD_HEADS;
         const uint32_t heads = min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
         {
-            float x[DP / 32], top = 0.f;
-#pragma unroll
-            for (int i = 0; i < DP / 32; ++i) x[i] = q_next[i], top = fmaxf(top, fabsf(x[i]));
-            float up = 1.f, down = 1.f;  // 2^e and 2^-e
+            float top = 0.f, up = 1.f, down = 1.f;  // 2^e and 2^-e
             if (!BF) {
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) top = fmaxf(top, fabsf(q_next[i]));
                 for (int o = 16; o > 0; o /= 2) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, o));
                 const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -125), 126);
                 if (top > 0.f && top < INFINITY) up = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(127 - e) << 23);
             }
-            __nv_bfloat16* const qb = reinterpret_cast<__nv_bfloat16*>(q_smem) + warp * 2 * DP;
-            __half* const qh = reinterpret_cast<__half*>(q_smem) + warp * 2 * DP;
+            uint16_t* const q = reinterpret_cast<uint16_t*>(q_smem) + warp * S::PIECES * DP;
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) {
-                const float y = x[i] * down;
-                if (BF) {
-                    qb[lane + i * 32] = __float2bfloat16_rn(y);
-                    qb[DP + lane + i * 32] = __float2bfloat16_rn(y - __bfloat162float(qb[lane + i * 32]));
-                } else {
-                    qh[lane + i * 32] = __float2half_rn(y);
-                    qh[DP + lane + i * 32] = __float2half_rn(y - __half2float(qh[lane + i * 32]));
+                float rest = q_next[i] * down;
+#pragma unroll
+                for (int piece = 0; piece < S::PIECES; ++piece) {
+                    const uint32_t h = pack_pair<BF>(rest, 0.f);
+                    q[piece * DP + lane + i * 32] = (uint16_t)h;
+                    rest -= unpack_pair<BF>(h).x;
                 }
             }
-            if (lane == 0) q_factor[warp] = p.scale * LOG2E * up;
+            if (lane == 0) q_factor[warp] = p.scale * LOG2E * up * (I8 ? CODE_UNIT : 1.f);
         }
         __syncthreads();
         // A fragments of S: k index 16 ks + 2t (+1, +8, +9). For int8 the k index is a relabelled dimension, so that a
         // thread's codes of four k steps are 16 consecutive bytes of its row.
+        auto k_lo = [&](int ks) { return I8 ? (t + 4 * (ks / 4)) * 16 + (ks % 4) * 4 : ks * 16 + t * 2; };
+        const uint32_t* const q_row = reinterpret_cast<const uint32_t*>(q_smem) + g * S::PIECES * (DP / 2);
         uint32_t qa[KS][4];
+        float minus[4] = {0.f, 0.f, 0.f, 0.f};  // where S starts: minus its products with the 128s
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const uint32_t lo = KIND == CK_INT8 ? (t + 4 * (ks / 4)) * 16 + (ks % 4) * 4 : ks * 16 + t * 2;
-            const uint32_t hi = KIND == CK_INT8 ? lo + 2 : lo + 8;
-            const uint32_t* const row = reinterpret_cast<const uint32_t*>(q_smem + g * 4 * DP);
-            qa[ks][0] = row[lo / 2], qa[ks][1] = row[DP / 2 + lo / 2];
-            qa[ks][2] = row[hi / 2], qa[ks][3] = row[DP / 2 + hi / 2];
+            const uint32_t lo = k_lo(ks) / 2, hi = lo + (I8 ? 1 : 4);
+            qa[ks][0] = q_row[lo], qa[ks][1] = q_row[DP / 2 + lo];
+            qa[ks][2] = q_row[hi], qa[ks][3] = q_row[DP / 2 + hi];
+            if (I8) mma16816<BF>(minus, qa[ks], CODE_ZERO, CODE_ZERO);
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) minus[j] = -minus[j];
         const float factor = q_factor[g];
-        float o[NT][4], m = -INFINITY, l = 0.f;
+        float o[NT][4], o_off[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
         const uint32_t tokens = pre_tokens(cur);
+#pragma unroll 1
         for (uint32_t i = warp; i * TOK < tokens; i += AD_WARPS) {
             cp_async_wait<AD_STAGES - 2>();
             __syncwarp();
@@ -358,20 +412,23 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 
             float s[ST][4];
 #pragma unroll
-            for (int n = 0; n < ST; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-            if (KIND == CK_INT8) {
+            for (int n = 0; n < ST; ++n)
 #pragma unroll
-                for (int n = 0; n < ST; ++n)
+                for (int j = 0; j < 4; ++j) s[n][j] = minus[j];
+            if (I8) {
 #pragma unroll
-                    for (int q4 = 0; q4 < KS / 4; ++q4) {
-                        const uint4 w = ld_shared_v4<0>(k_at + stage_offset<S::CHUNKS, true>(n * 8 + g, t + 4 * q4));
-                        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+                for (int q4 = 0; q4 < KS / 4; ++q4) {
+                    uint4 w[ST];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t u = x[j] ^ 0x80808080u;
-                            mma16816<BF>(s[n], qa[q4 * 4 + j], codes_to_half2(u, 0x4140u), codes_to_half2(u, 0x4342u));
+                    for (int n = 0; n < ST; ++n) w[n] = ld_shared_v4<0>(k_at + stage_offset<S::CHUNKS, true>(n * 8 + g, t + 4 * q4));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int n = 0; n < ST; ++n) {
+                            const uint32_t u = (j == 0 ? w[n].x : j == 1 ? w[n].y : j == 2 ? w[n].z : w[n].w) ^ 0x80808080u;
+                            mma16816<BF>(s[n], qa[q4 * 4 + j], prmt(u, 0u, 0x4140u), prmt(u, 0u, 0x4342u));
                         }
-                    }
+                }
             } else {
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) {
@@ -379,52 +436,89 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                     ldmatrix4(r, k_at + stage_offset<S::CHUNKS, false>((lane / 16) * 8 + lane % 8, ks * 2 + (lane / 8) % 2));
                     mma16816<BF>(s[0], qa[ks], r[0], r[1]);
                     mma16816<BF>(s[1], qa[ks], r[2], r[3]);
+                    if (THIRD) {
+                        const uint32_t third[4] = {q_row[DP + k_lo(ks) / 2], 0u, q_row[DP + k_lo(ks) / 2 + 4], 0u};
+                        mma16816<BF>(s[0], third, r[0], r[1]);
+                        mma16816<BF>(s[1], third, r[2], r[3]);
+                    }
                 }
             }
 
-            // p = 2^(s - m), this thread's tokens 8 n + 2 t, + 1 of head g
-            float x[ST][2], vs[ST][2], top = -INFINITY;
-#pragma unroll
-            for (int n = 0; n < ST; ++n)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const uint32_t r = n * 8 + t * 2 + j;
-                    float y = (s[n][j] + s[n][j + 2]) * factor, rank = 0.f;
-                    vs[n][j] = 1.f;
-                    if (KIND == CK_INT8) {
-                        const float* const sc = reinterpret_cast<const float*>(ring + stage * S::STAGE + 2 * TOK * S::ROW);
-                        y *= sc[r];
-                        vs[n][j] = sc[TOK + r];
-                        rank = __log2f(fmaxf(vs[n][j], AD_MIN_SCALE));
-                    }
-                    x[n][j] = (here >> r) & 1u ? y : -INFINITY;
-                    top = fmaxf(top, x[n][j] + rank);
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-            if (__any_sync(0xFFFFFFFFu, top > m)) {
-                const float next = fmaxf(m, top), keep = next == -INFINITY ? 1.f : exp2_approx(m - next);
-                m = next;
-                l *= keep;
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) o[n][j] *= keep;
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            uint32_t pa[TOK / 16][4];
+            // x = log2(e) scale q . k, this thread's tokens 8 n + 2 t, + 1 of head g; w = 2^(x - m) times the value scale
+            float x[ST][2], e[ST][2], w[ST][2], vs[ST][2];
+            const float2* const scales = reinterpret_cast<const float2*>(ring + stage * S::STAGE + 2 * TOK * S::ROW) + t;
 #pragma unroll
             for (int n = 0; n < ST; ++n) {
-                const float e0 = exp2_approx(x[n][0] - base), e1 = exp2_approx(x[n][1] - base);
-                l += e0 + e1;
-                const float w0 = e0 * vs[n][0], w1 = e1 * vs[n][1];
-                const uint32_t high = pack_pair<BF>(w0, w1);
-                const float2 back = unpack_pair<BF>(high);
+                float2 ks2 = make_float2(factor, factor), vs2 = make_float2(1.f, 1.f);
+                if (I8) {
+                    const float2 sk = scales[n * 4], sv = scales[TOK / 2 + n * 4];
+                    ks2 = make_float2(sk.x * factor, sk.y * factor);
+                    vs2 = make_float2(max_nan(sv.x, AD_MIN_SCALE), max_nan(sv.y, AD_MIN_SCALE));
+                }
+                x[n][0] = (s[n][0] + s[n][2]) * ks2.x, x[n][1] = (s[n][1] + s[n][3]) * ks2.y;
+                vs[n][0] = vs2.x, vs[n][1] = vs2.y;
+            }
+            if (here != ALL) {
+#pragma unroll
+                for (int n = 0; n < ST; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (!((here >> (n * 8 + t * 2 + j)) & 1u)) x[n][j] = -INFINITY;
+            }
+            // The reference does as a rule: the products are made with it, and made again in the rare case that it moves.
+            for (;;) {
+                const float base = m == -INFINITY ? 0.f : m;
+                float top = 0.f;
+#pragma unroll
+                for (int n = 0; n < ST; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        e[n][j] = exp2_approx(x[n][j] - base);
+                        w[n][j] = I8 ? e[n][j] * vs[n][j] : e[n][j];
+                        top = fmaxf(top, w[n][j]);
+                    }
+                if (!__any_sync(0xFFFFFFFFu, top > AD_LAZY || m == -INFINITY)) break;
+                // the largest x + log2(value scale) of the head's tokens
+                float most = -INFINITY;
+#pragma unroll
+                for (int n = 0; n < ST; ++n)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) most = fmaxf(most, I8 ? x[n][j] + __log2f(vs[n][j]) : x[n][j]);
+                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+                const float next = fmaxf(m, most), keep = m == -INFINITY ? 0.f : exp2_approx(m - next);
+                const bool moved = next > m;
+                if (!__any_sync(0xFFFFFFFFu, moved)) break;
+                if (moved) {
+                    m = next;
+                    l *= keep;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[n][j] *= keep;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o_off[j] *= keep;
+                }
+            }
+            uint32_t pa[TOK / 16][4], pa3[TOK / 16][4];
+#pragma unroll
+            for (int n = 0; n < ST; ++n) {
+                l += e[n][0] + e[n][1];
+                const uint32_t high = pack_pair<BF>(w[n][0], w[n][1]);
+                const float2 h = unpack_pair<BF>(high);
+                const uint32_t low = pack_pair<BF>(w[n][0] - h.x, w[n][1] - h.y);
                 pa[n / 2][(n % 2) * 2] = high;
-                pa[n / 2][(n % 2) * 2 + 1] = pack_pair<BF>(w0 - back.x, w1 - back.y);
+                pa[n / 2][(n % 2) * 2 + 1] = low;
+                if (THIRD) {
+                    const float2 h2 = unpack_pair<BF>(low);
+                    pa3[n / 2][(n % 2) * 2] = pack_pair<BF>(w[n][0] - h.x - h2.x, w[n][1] - h.y - h2.y);
+                    pa3[n / 2][(n % 2) * 2 + 1] = 0u;
+                }
             }
 
-            if (KIND == CK_INT8) {
+            if (I8) {
+#pragma unroll
+                for (int ks = 0; ks < TOK / 16; ++ks) mma16816<BF>(o_off, pa[ks], CODE_ZERO, CODE_ZERO);
 #pragma unroll
                 for (int c = 0; c < S::CHUNKS; ++c) {
                     uint32_t r[4];  // chunk c of tokens 0-7, 8-15, 16-23, 24-31; each word: dimensions 2g, 2g + 1 of two tokens
@@ -433,8 +527,8 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                     for (int j = 0; j < 4; ++j) r[j] ^= 0x80808080u;
 #pragma unroll
                     for (int ks = 0; ks < TOK / 16; ++ks) {
-                        mma16816<BF>(o[c * 2], pa[ks], codes_to_half2(r[ks * 2], 0x4240u), codes_to_half2(r[ks * 2 + 1], 0x4240u));
-                        mma16816<BF>(o[c * 2 + 1], pa[ks], codes_to_half2(r[ks * 2], 0x4341u), codes_to_half2(r[ks * 2 + 1], 0x4341u));
+                        mma16816<BF>(o[c * 2], pa[ks], prmt(r[ks * 2], 0u, 0x4240u), prmt(r[ks * 2 + 1], 0u, 0x4240u));
+                        mma16816<BF>(o[c * 2 + 1], pa[ks], prmt(r[ks * 2], 0u, 0x4341u), prmt(r[ks * 2 + 1], 0u, 0x4341u));
                     }
                 }
             } else {
@@ -444,10 +538,20 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                     ldmatrix4_trans(r, v_at + stage_offset<S::CHUNKS, false>(lane % 16, c + lane / 16));
                     mma16816<BF>(o[c], pa[0], r[0], r[1]);
                     mma16816<BF>(o[c + 1], pa[0], r[2], r[3]);
+                    if (THIRD) {
+                        mma16816<BF>(o[c], pa3[0], r[0], r[1]);
+                        mma16816<BF>(o[c + 1], pa3[0], r[2], r[3]);
+                    }
                 }
             }
             __syncwarp();
             stage = stage == AD_STAGES - 1 ? 0 : stage + 1;
+        }
+        if (I8) {  // the 128s off, and the codes' unit on
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[n][j] = (o[n][j] - o_off[j]) * CODE_UNIT;
         }
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
@@ -472,13 +576,13 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         if (warp < 4) {
             float* const slot = part_smem + warp * S::PART;
             const float m2 = slot[AD_HEADS * DP + g], l2 = slot[AD_HEADS * DP + AD_HEADS + g];
-            const float both = fmaxf(m, m2), a = both == -INFINITY ? 0.f : exp2_approx(m - both), b = both == -INFINITY ? 0.f : exp2_approx(m2 - both);
-            l = l * a + l2 * b, m = both;
+            const float both = fmaxf(m, m2), f1 = both == -INFINITY ? 0.f : exp2_approx(m - both), f2 = both == -INFINITY ? 0.f : exp2_approx(m2 - both);
+            l = l * f1 + l2 * f2, m = both;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint32_t e0 = KIND == CK_INT8 ? (n / 2) * 16 + n % 2 + t * 4 : n * 8 + t * 2, e1 = e0 + (KIND == CK_INT8 ? 2 : 1);
-                o[n][0] = (o[n][0] + o[n][2]) * a + slot[g * DP + e0] * b, o[n][2] = 0.f;
-                o[n][1] = (o[n][1] + o[n][3]) * a + slot[g * DP + e1] * b, o[n][3] = 0.f;
+                o[n][0] = (o[n][0] + o[n][2]) * f1 + slot[g * DP + e0] * f2, o[n][2] = 0.f;
+                o[n][1] = (o[n][1] + o[n][3]) * f1 + slot[g * DP + e1] * f2, o[n][3] = 0.f;
             }
             __syncwarp();
             put(slot);
@@ -486,7 +590,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         __syncthreads();
         {
             const bool whole = cur.k == 0 && cur.n == cur.units;
-            float* const part = parts + ((uint64_t)blockIdx.x * 2 + (cur.unit == u0 ? 0 : 1)) * S::PART;
+            float* const part = a.parts + ((uint64_t)blockIdx.x * 2 + (cur.unit == u0 ? 0 : 1)) * S::PART;
             const uint32_t h = warp;  // a warp a head
             float mx = -INFINITY, w[4], sum = 0.f;
 #pragma unroll
@@ -520,16 +624,18 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 // order. A block a record, a warp a head.
 template <int DP>
 __global__ void __launch_bounds__(AD_THREADS, 1)
-    join_kernel(const DecodeParams p, const float* __restrict__ parts, const JoinRecord* __restrict__ records, uint32_t chunks_of_heads) {
+    join_kernel(const __grid_constant__ DecodeArgs a) {
+    const DecodeParams& p = a.p;
+    const uint32_t chunks_of_heads = a.chunks_of_heads;
     constexpr int PART = AD_HEADS * (DP + 2);
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     pdl_wait();
-    const JoinRecord r = records[blockIdx.x];
+    const JoinRecord r = a.records[blockIdx.x];
     if (r.c1 == 0) return;
     const uint32_t d = p.c.d, group = p.q_heads / p.c.heads;
     const uint32_t kv_head = r.item / chunks_of_heads, head0 = kv_head * group + (r.item % chunks_of_heads) * AD_HEADS;
     if (warp >= min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0)) return;
-    auto slot = [&](uint32_t c) { return parts + ((uint64_t)c * 2 + (c == r.c0 ? r.slot : 0)) * PART; };
+    auto slot = [&](uint32_t c) { return a.parts + ((uint64_t)c * 2 + (c == r.c0 ? r.slot : 0)) * PART; };
     float y[DP / 32] = {}, sum = 0.f, mx = -INFINITY;
     // lanes hold the maxima and sums of 32 parts; the parts' o are added with their weights
     for (uint32_t c1 = r.c0; c1 <= r.c1; c1 += 32) {
@@ -559,18 +665,15 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             store_elem(p.out, ((int64_t)r.b * p.q_heads + head0 + warp) * d + lane + i * 32, p.dtype, sum == 0.f ? 0.f : y[i] / sum);
 }
 
-template <int DP, int KIND>
-cudaError_t launch(const DecodeParams& p, uint8_t* workspace, uint32_t blocks, cudaStream_t stream) {
-    using S = DecodeShape<DP, KIND>;
-    const uint32_t chunks = (p.q_heads / p.c.heads + AD_HEADS - 1) / AD_HEADS;
-    JoinRecord* const records = reinterpret_cast<JoinRecord*>(workspace);
-    float* const parts = reinterpret_cast<float*>(workspace + records_bytes(blocks));
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    if (e != cudaSuccess) return e;
+template <int DP, int KIND, bool THIRD>
+cudaError_t launch(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
+    using S = DecodeShape<DP, KIND, THIRD>;
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP, KIND, THIRD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     // (the second kernel keeps the first one's split of shared memory: changing it would drain the SMs twice a call)
-    e = cudaFuncSetAttribute(join_kernel<DP>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(join_kernel<DP>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
-    decode_kernel<DP, KIND><<<blocks, AD_THREADS, S::SMEM, stream>>>(p, parts, records, chunks);
+    decode_kernel<DP, KIND, THIRD><<<blocks, AD_THREADS, S::SMEM, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -581,15 +684,14 @@ cudaError_t launch(const DecodeParams& p, uint8_t* workspace, uint32_t blocks, c
     cfg.stream = stream;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<DP>, p, static_cast<const float*>(parts),
-                              static_cast<const JoinRecord*>(records), chunks);
+    return cudaLaunchKernelEx(&cfg, join_kernel<DP>, a);
 }
 
 template <int DP>
-cudaError_t launch_kind(const DecodeParams& p, uint8_t* ws, uint32_t blocks, cudaStream_t stream) {
-    if (p.c.dtype == kInt8) return launch<DP, CK_INT8>(p, ws, blocks, stream);
-    if (p.c.dtype == kBf16) return launch<DP, CK_BF16>(p, ws, blocks, stream);
-    return launch<DP, CK_F16>(p, ws, blocks, stream);
+cudaError_t launch_kind(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
+    if (a.p.c.dtype == kInt8) return launch<DP, CK_INT8, false>(a, blocks, stream);
+    if (a.p.c.dtype == kF16) return launch<DP, CK_F16, false>(a, blocks, stream);
+    return a.p.dtype == kF32 ? launch<DP, CK_BF16, true>(a, blocks, stream) : launch<DP, CK_BF16, false>(a, blocks, stream);
 }
 
 }  // namespace
@@ -600,7 +702,13 @@ size_t attention_decode_workspace(uint32_t, uint32_t, uint32_t, uint32_t d, int 
 
 cudaError_t launch_attention_decode(const DecodeParams& p, void* workspace, int num_sms, cudaStream_t stream) {
     uint8_t* const ws = static_cast<uint8_t*>(workspace);
-    return p.c.d > 64 ? launch_kind<128>(p, ws, num_sms, stream) : launch_kind<64>(p, ws, num_sms, stream);
+    DecodeArgs a{p, reinterpret_cast<float*>(ws + records_bytes(num_sms)), reinterpret_cast<JoinRecord*>(ws), 1.0 / num_sms,
+                 (p.q_heads / p.c.heads + AD_HEADS - 1) / AD_HEADS, 0, -1};
+    // division by page_size as a product: with 2^s the power of two at or above it, floor(2^(31 + s) / page_size) + 1 is
+    // exact for every token below 2^31
+    while (a.page_shift < 31 && (1ull << (a.page_shift + 1)) < p.c.page_size) ++a.page_shift;
+    if (a.page_shift >= 0) a.page_magic = (uint32_t)((1ull << (32 + a.page_shift)) / p.c.page_size + 1);
+    return p.c.d > 64 ? launch_kind<128>(a, num_sms, stream) : launch_kind<64>(a, num_sms, stream);
 }
 
 }  // namespace iq2
