@@ -2,9 +2,9 @@
 //     s_j = scale q . k_j,  o = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max)   over the sequence's tokens j < length.
 //
 // Bound by HBM: every cached byte is read once and feeds 2 G multiply-adds (G query heads share a key head). An item is
-// one sequence, one key head and up to eight of its query heads; the items' lengths, cut into units of 8 warps x TOK
-// tokens, form one line of work that the thread blocks (one an SM) take equal, contiguous parts of, whatever the lengths
-// are. The lengths are on the device, so every block sums them up itself. A part that is not a whole item leaves its
+// one sequence, one key head and up to eight of its query heads; the items, each as long as its tokens in units of 4 TOK
+// and AD_ITEM_COST more, form one line of work that the thread blocks (one an SM) take equal, contiguous parts of, whatever
+// the lengths are. The lengths are on the device, so every block sums them up itself. A part that is not a whole item leaves its
 // (max, sum, o) in the workspace, and join_kernel adds the parts of an item up in the order of the blocks.
 //
 // Inside a block each warp streams its own TOK tokens (K and V rows) through a ring of cp.async stages, across the items'
@@ -33,6 +33,9 @@ namespace {
 
 constexpr int AD_WARPS = 8, AD_THREADS = AD_WARPS * 32, AD_STAGES = 3;
 constexpr int AD_HEADS = 8;                     // query heads of an item
+// Units' time that starting and ending an item costs. Measured with 1 / 2 / 3: 128 x 4096 tokens 219 / 216 / 214 us,
+// 1 x 100001 49.7 / 48.6 / 47.9 us.
+constexpr uint32_t AD_ITEM_COST = 3;
 constexpr float AD_MIN_SCALE = 7.88860905e-31f;  // 2^-100: the smallest value scale (a row held as zeros has 0)
 constexpr float AD_LAZY = 256.f;                 // how far p times the value scale may grow before the reference moves
 constexpr uint32_t CODE_ZERO = 0x00800080u;      // two codes of 0 as f16: 128 2^-24
@@ -46,7 +49,7 @@ struct DecodeShape {
     static constexpr int PIECES = THIRD ? 3 : 2;
     static constexpr int ESIZE = KIND == CK_INT8 ? 1 : 2;
     static constexpr int TOK = KIND == CK_INT8 ? 32 : 16;  // tokens of a warp's stage: 8 KB of K and V at DP = 128
-    static constexpr int UNIT = TOK * AD_WARPS;
+    static constexpr int UNIT = TOK * 4;                   // tokens that the line of work is cut at: 32 KB at DP = 128
     static constexpr int ROW = DP * ESIZE;                 // bytes of a padded K or V row
     static constexpr int CHUNKS = ROW / 16;
     static constexpr int SCALES = KIND == CK_INT8 ? TOK * 8 : 0;
@@ -150,14 +153,22 @@ __device__ __forceinline__ uint32_t stage_offset(uint32_t r, uint32_t c) {
     return (r * CHUNKS + (PLAIN ? c ^ ((r & 1) * 4) : c ^ (r & 7))) * 16;
 }
 
-// The line of work from one unit on: the item it is in and the tokens [t0, t1) of that item up to the end of the part.
+// The line of work from one unit on: the item it is in and the tokens [t0, t1) of that item in the part. An item's first
+// AD_ITEM_COST units have no tokens; a part that ends inside them has none (the next block has the item).
 struct Cursor {
     uint64_t unit, end;
     uint32_t b, item, len, units;  // the sequence, its item (key head, group of query heads), tokens and units an item
-    uint32_t k;                    // first unit of the item in the part
-    uint32_t n;                    // units of the item in the part
-    __device__ __forceinline__ void cut() { n = (uint32_t)min((uint64_t)(units - k), end - unit); }
+    uint32_t k, n;                 // first unit of the item in the part, and how many
+    uint32_t t0, t1;
+    template <int UNIT>
+    __device__ __forceinline__ void cut() {
+        n = (uint32_t)min((uint64_t)(units - k), end - unit);
+        t0 = (max(k, AD_ITEM_COST) - AD_ITEM_COST) * UNIT, t1 = min((max(k + n, AD_ITEM_COST) - AD_ITEM_COST) * UNIT, len);
+    }
+    template <int UNIT>
+    static __device__ __forceinline__ uint32_t units_of(uint32_t len_) { return len_ == 0 ? 0 : (len_ + UNIT - 1) / UNIT + AD_ITEM_COST; }
     __device__ __forceinline__ bool done() const { return unit >= end; }
+    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == len; }
     template <int UNIT>
     __device__ __forceinline__ void next(const DecodeParams& p, uint32_t items) {
         unit += n;
@@ -172,9 +183,10 @@ struct Cursor {
                 }
                 len = seq_len(p, b);
             } while (len == 0);
-            units = (len + UNIT - 1) / UNIT;
+            units = units_of<UNIT>(len);
         }
-        cut();
+        cut<UNIT>();
+        if (t0 == t1) unit = end;
     }
 };
 
@@ -199,62 +211,65 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     if (d < DP)
         for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
     uint64_t units = 0;
+    uint32_t len = 0;  // of sequence b0 + lane
 #pragma unroll 1
     for (uint32_t b0 = 0; b0 < p.batch; b0 += 32) {
-        const uint32_t b = b0 + lane, len = b < p.batch ? seq_len(p, b) : 1u;
-        units += b < p.batch ? (len + UNIT - 1) / UNIT : 0u;
+        const uint32_t b = b0 + lane;
+        len = b < p.batch ? seq_len(p, b) : 0u;
+        units += Cursor::units_of<UNIT>(len);
         // sequences of length 0: zeros, a block a sequence
-        uint32_t empty = __ballot_sync(0xFFFFFFFFu, len == 0 && b % gridDim.x == blockIdx.x);
+        uint32_t empty = __ballot_sync(0xFFFFFFFFu, len == 0 && b < p.batch && b % gridDim.x == blockIdx.x);
+#pragma unroll 1
         for (; empty != 0; empty &= empty - 1)
+#pragma unroll 1
             for (uint32_t i = threadIdx.x; i < p.q_heads * d; i += AD_THREADS)
                 store_elem(p.out, (int64_t)(b0 + __ffs(empty) - 1) * p.q_heads * d + i, p.dtype, 0.f);
     }
-#pragma unroll 1
+#pragma unroll
     for (int o = 16; o > 0; o /= 2) units += __shfl_xor_sync(0xFFFFFFFFu, units, o);
     units *= items;
     uint64_t each = (uint64_t)((double)units * a.inv_blocks);  // units / blocks, rounded up
     while (each * gridDim.x < units) ++each;
     const uint64_t u0 = min(blockIdx.x * each, units), u1 = min(u0 + each, units);
-    if (u0 >= u1) {
-        if (threadIdx.x == 0) a.records[blockIdx.x].c1 = 0;
-        return;
-    }
     Cursor cur{};
-    uint64_t before = 0;  // units of the sequences before
+    if (u0 < u1) {
+        uint64_t before = 0;  // units of the sequences before
 #pragma unroll 1
-    for (uint32_t b0 = 0;; b0 += 32) {
-        if (b0 >= p.batch) return;  // (not reached while the lengths stay as they were)
-        const uint32_t len = b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0u, own = (len + UNIT - 1) / UNIT;
-        uint64_t upto = (uint64_t)own * items;
-#pragma unroll 1
-        for (int o = 1; o < 32; o *= 2) {
-            const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-            if (lane >= (uint32_t)o) upto += x;
+        for (uint32_t b0 = 0; b0 < p.batch; b0 += 32) {
+            if (p.batch > 32) len = b0 + lane < p.batch ? seq_len(p, b0 + lane) : 0u;
+            const uint32_t own = Cursor::units_of<UNIT>(len);
+            uint64_t upto = (uint64_t)own * items;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const uint64_t x = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                if (lane >= (uint32_t)o) upto += x;
+            }
+            const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + upto > u0);
+            if (hit != 0) {
+                const int at = __ffs(hit) - 1;
+                cur.b = b0 + at;
+                cur.len = __shfl_sync(0xFFFFFFFFu, len, at), cur.units = __shfl_sync(0xFFFFFFFFu, own, at);
+                const uint32_t rest = (uint32_t)(u0 - before - __shfl_sync(0xFFFFFFFFu, upto - (uint64_t)own * items, at));
+                cur.item = rest / cur.units, cur.k = rest % cur.units;
+                cur.unit = u0, cur.end = u1;
+                cur.cut<UNIT>();
+                break;
+            }
+            before += __shfl_sync(0xFFFFFFFFu, upto, 31);
         }
-        const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + upto > u0);
-        if (hit != 0) {
-            const int at = __ffs(hit) - 1;
-            cur.b = b0 + at;
-            cur.len = __shfl_sync(0xFFFFFFFFu, len, at), cur.units = __shfl_sync(0xFFFFFFFFu, own, at);
-            const uint32_t rest = (uint32_t)(u0 - before - __shfl_sync(0xFFFFFFFFu, upto - (uint64_t)own * items, at));
-            cur.item = rest / cur.units, cur.k = rest % cur.units;
-            break;
-        }
-        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
-    cur.unit = u0, cur.end = u1;
-    cur.cut();
-    Cursor pre = cur;
     if (threadIdx.x == 0) {
-        // the first block whose part begins inside an item joins it: the block before it has the item's first unit
+        // the first block whose part begins inside an item's tokens joins it: the block before it has the first of them
         const uint64_t unit0 = u0 - cur.k;
         JoinRecord r{cur.b, cur.item, blockIdx.x - 1, 0, 0};
-        if (cur.k > 0 && u0 - each <= unit0) {
-            r.c1 = blockIdx.x, r.slot = u0 - each == unit0 ? 0 : 1;
+        if (cur.t0 > 0 && u0 - each <= unit0 + AD_ITEM_COST) {
+            r.c1 = blockIdx.x, r.slot = u0 - each >= unit0 ? 0 : 1;
             while ((r.c1 + 1) * each < unit0 + cur.units) ++r.c1;
         }
         a.records[blockIdx.x] = r;
     }
+    if (cur.t0 == cur.t1) return;  // nothing, or nothing but an item's start
+    Cursor pre = cur;
 
     // ---- the copies: tile `i` (TOK tokens) of pre's piece of an item, one page lookup ahead ----
     uint8_t* const ring = smem + warp * S::RING;
@@ -266,25 +281,32 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     constexpr int ROWS = 32 / S::CHUNKS;  // rows that the warp copies at a time
     auto page_of = [&](uint32_t tok) { return a.page_shift < 0 ? tok : __umulhi(tok, a.page_magic) >> a.page_shift; };
     uint32_t pre_i = warp, pre_page = 0, pre_first = 0;  // the tile to copy next, its page, the first token of that page
-    auto pre_tokens = [&](const Cursor& c) { return min(c.len, (c.k + c.n) * UNIT) - c.k * UNIT; };
+    uint32_t lane_page = 0, ahead = 0;                    // pages of this warp's next 32 tiles, a lane each; tiles since
+    auto look_up = [&](uint32_t tok, uint32_t& page) {
+        if (tok < pre.t1) page = (uint32_t)__ldg(p.block_table + (int64_t)pre.b * p.table_width + page_of(tok));
+    };
     auto find_tile = [&]() {  // the next tile of this warp, and its page numbers under way
-        while (!pre.done() && pre_i * TOK >= pre_tokens(pre)) {
+        bool fresh = ahead == 32;
+        while (!pre.done() && pre.t0 + pre_i * TOK >= pre.t1) {
             pre.next<UNIT>(p, items);
-            pre_i = warp;
+            pre_i = warp, fresh = true;
         }
         if (pre.done()) return;
-        const uint32_t tok = pre.k * UNIT + pre_i * TOK + (side_by_side ? 0 : lane);
-        if (tok < pre.len) {
-            const uint32_t at = page_of(tok);
-            pre_first = at * p.c.page_size;
-            pre_page = (uint32_t)__ldg(p.block_table + (int64_t)pre.b * p.table_width + at);
+        const uint32_t tok = pre.t0 + pre_i * TOK;
+        if (side_by_side) {
+            if (fresh || pre_i == warp) look_up(tok + lane * (AD_WARPS * TOK), lane_page), ahead = 0;
+            pre_page = __shfl_sync(0xFFFFFFFFu, lane_page, ahead++);
+            pre_first = page_of(tok) * p.c.page_size;
+        } else {
+            look_up(tok + lane, pre_page);
+            pre_first = page_of(tok + lane) * p.c.page_size;
         }
     };
     // Copies the tile and returns a bit for each token that takes part: rows of tokens past the end, or of pages outside
     // the cache, are zeros, and what such pages hold cannot matter.
     auto copy_tile = [&](uint32_t stage) {
-        const uint32_t tok = pre.k * UNIT + pre_i * TOK, h = pre.item / a.chunks_of_heads, dst = ring_u32 + stage * S::STAGE;
-        const uint32_t left = pre.len - tok, in_page = tok + (side_by_side ? 0 : lane) - pre_first;
+        const uint32_t tok = pre.t0 + pre_i * TOK, h = pre.item / a.chunks_of_heads, dst = ring_u32 + stage * S::STAGE;
+        const uint32_t left = pre.t1 - tok, in_page = tok + (side_by_side ? 0 : lane) - pre_first;
         const int64_t row = ((int64_t)pre_page * p.c.heads + h) * p.c.page_size + in_page;
         const uint8_t *const k = static_cast<const uint8_t*>(p.c.k), *const v = static_cast<const uint8_t*>(p.c.v);
         const bool inside = chunk * 16 < row_bytes;
@@ -398,7 +420,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
-        const uint32_t tokens = pre_tokens(cur);
+        const uint32_t tokens = cur.t1 - cur.t0;
 #pragma unroll 1
         for (uint32_t i = warp; i * TOK < tokens; i += AD_WARPS) {
             cp_async_wait<AD_STAGES - 2>();
@@ -589,7 +611,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         }
         __syncthreads();
         {
-            const bool whole = cur.k == 0 && cur.n == cur.units;
+            const bool whole = cur.whole();
             float* const part = a.parts + ((uint64_t)blockIdx.x * 2 + (cur.unit == u0 ? 0 : 1)) * S::PART;
             const uint32_t h = warp;  // a warp a head
             float mx = -INFINITY, w[4], sum = 0.f;
@@ -651,7 +673,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         sum = sum * keep + add;
 #pragma unroll
         for (int i = 0; i < DP / 32; ++i) y[i] *= keep;
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t c = 0; c < n; ++c) {
             const float* const o = slot(c1 + c) + warp * DP + lane;
             const float wc = __shfl_sync(0xFFFFFFFFu, w, c);
