@@ -72,8 +72,8 @@ struct DecodeArgs {
     float* parts;
     JoinRecord* records;
     double inv_blocks;                      // 1 / the blocks of the launch
-    uint32_t chunks_of_heads, page_magic;   // token / page_size = (token page_magic) >> 32 + page_shift (tokens below 2^31)
-    int page_shift;                         // -1: pages of one token
+    uint32_t chunks_of_heads;
+    Divisor by_page;                        // tokens of a page
 };
 
 __device__ __forceinline__ uint32_t seq_len(const DecodeParams& p, uint32_t b) {
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     const bool side_by_side = p.c.page_size % TOK == 0;
     const uint32_t row_bytes = d * S::ESIZE, chunk = lane % S::CHUNKS, row0 = lane / S::CHUNKS;
     constexpr int ROWS = 32 / S::CHUNKS;  // rows that the warp copies at a time
-    auto page_of = [&](uint32_t tok) { return a.page_shift < 0 ? tok : __umulhi(tok, a.page_magic) >> a.page_shift; };
+    auto page_of = [&](uint32_t tok) { return a.by_page.quotient(tok); };
     uint32_t pre_i = warp, pre_page = 0, pre_first = 0;  // the tile to copy next, its page, the first token of that page
     uint32_t lane_page = 0, ahead = 0;                    // pages of this warp's next 32 tiles, a lane each; tiles since
     auto look_up = [&](uint32_t tok, uint32_t& page) {
@@ -724,12 +724,8 @@ size_t attention_decode_workspace(uint32_t, uint32_t, uint32_t, uint32_t d, int 
 
 cudaError_t launch_attention_decode(const DecodeParams& p, void* workspace, int num_sms, cudaStream_t stream) {
     uint8_t* const ws = static_cast<uint8_t*>(workspace);
-    DecodeArgs a{p, reinterpret_cast<float*>(ws + records_bytes(num_sms)), reinterpret_cast<JoinRecord*>(ws), 1.0 / num_sms,
-                 (p.q_heads / p.c.heads + AD_HEADS - 1) / AD_HEADS, 0, -1};
-    // division by page_size as a product: with 2^s the power of two at or above it, floor(2^(31 + s) / page_size) + 1 is
-    // exact for every token below 2^31
-    while (a.page_shift < 31 && (1ull << (a.page_shift + 1)) < p.c.page_size) ++a.page_shift;
-    if (a.page_shift >= 0) a.page_magic = (uint32_t)((1ull << (32 + a.page_shift)) / p.c.page_size + 1);
+    const DecodeArgs a{p, reinterpret_cast<float*>(ws + records_bytes(num_sms)), reinterpret_cast<JoinRecord*>(ws), 1.0 / num_sms,
+                 (p.q_heads / p.c.heads + AD_HEADS - 1) / AD_HEADS, Divisor::of(p.c.page_size)};
     return p.c.d > 64 ? launch_kind<128>(a, num_sms, stream) : launch_kind<64>(a, num_sms, stream);
 }
 

@@ -10,6 +10,22 @@ namespace iq2 {
 // Element types, numbered as IQ2_DTYPE_* of the C ABI; a cache adds int8 (IQ2_KV_INT8).
 constexpr int kF32 = 0, kF16 = 1, kBf16 = 2, kInt8 = 3;
 
+// Division of n < 2^31 by a divisor that is known before the launch, as a product: with 2^s the power of two at or above
+// the divisor, floor(n / divisor) = (n magic) >> (31 + s) for magic = floor(2^(31 + s) / divisor) + 1.
+struct Divisor {
+    uint32_t magic;
+    int32_t shift;  // s - 1, -1 for a divisor of 1
+    static Divisor of(uint32_t divisor) {
+        Divisor d{0, -1};
+        while (d.shift < 31 && (1ull << (d.shift + 1)) < divisor) ++d.shift;
+        if (d.shift >= 0) d.magic = (uint32_t)((1ull << (32 + d.shift)) / divisor + 1);
+        return d;
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t quotient(uint32_t n) const { return shift < 0 ? n : __umulhi(n, magic) >> shift; }
+#endif
+};
+
 // A paged cache (iq2_kv_cache): k, v [pages][heads][page_size][d], k_scale, v_scale f32 [pages][heads][page_size]
 // for int8 codes. Token `pos` of a sequence lives in page block_table[pos / page_size], row pos % page_size.
 struct KvCacheView {
@@ -35,6 +51,7 @@ struct KvWriteParams {
     int dtype, q_out_dtype;
     bool interleaved;
     bool vec;  // every row of the inputs and tables starts on a 16-byte boundary (8 for 16-bit rows)
+    Divisor by_heads, by_page;  // set by the launch: heads of a token (q, k and v), tokens of a page
 };
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);
 
@@ -70,21 +87,5 @@ struct PrefillParams {
 };
 size_t attention_prefill_workspace(const PrefillParams& p, int num_sms);
 cudaError_t launch_attention_prefill(const PrefillParams& p, void* workspace, int num_sms, cudaStream_t stream);
-
-#ifdef __CUDACC__
-// A line of work units dealt to blocks as evenly as whole units go: the first units % blocks blocks take one more than the
-// others, each a contiguous part.
-struct Deal {
-    uint64_t each, more;
-    __device__ __forceinline__ Deal(uint64_t units, uint32_t blocks) : each(units / blocks), more(units % blocks) {}
-    __device__ __forceinline__ uint64_t start(uint32_t block) const {
-        return block * each + (block < more ? (uint64_t)block : more);
-    }
-    __device__ __forceinline__ uint32_t block_of(uint64_t unit) const {
-        const uint64_t big = more * (each + 1);
-        return (uint32_t)(unit < big ? unit / (each + 1) : more + (unit - big) / each);
-    }
-};
-#endif
 
 }  // namespace iq2

@@ -16,18 +16,21 @@ namespace iq2 {
 namespace {
 
 constexpr int KW_THREADS = 256;
+
 constexpr float MIN_AMAX = 7.88860905e-31f;  // 2^-100
 
+// Four values at element i. ONCE: they are not read again (the cache lines give way first).
+template <bool ONCE>
 __device__ __forceinline__ float4 load4(const void* base, int64_t i, int dtype, bool vec) {
     if (dtype == kF32) {
         const float* p = static_cast<const float*>(base) + i;
-        if (vec) return __ldg(reinterpret_cast<const float4*>(p));
+        if (vec) return ONCE ? __ldcs(reinterpret_cast<const float4*>(p)) : __ldg(reinterpret_cast<const float4*>(p));
         return make_float4(p[0], p[1], p[2], p[3]);
     }
     const uint16_t* p = static_cast<const uint16_t*>(base) + i;
     uint32_t lo, hi;
     if (vec) {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+        const uint2 w = ONCE ? __ldcs(reinterpret_cast<const uint2*>(p)) : __ldg(reinterpret_cast<const uint2*>(p));
         lo = w.x, hi = w.y;
     } else {
         lo = p[0] | ((uint32_t)p[1] << 16), hi = p[2] | ((uint32_t)p[3] << 16);
@@ -69,43 +72,42 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 }
 
 __device__ __forceinline__ uint32_t codes4(float4 x, float inv) {
-    const int a = __float2int_rn(__fmul_rn(x.x, inv)), b = __float2int_rn(__fmul_rn(x.y, inv));
-    const int c = __float2int_rn(__fmul_rn(x.z, inv)), d = __float2int_rn(__fmul_rn(x.w, inv));
-    return (a & 0xFF) | ((b & 0xFF) << 8) | ((c & 0xFF) << 16) | ((uint32_t)d << 24);
+    // 1.5 * 2^23 more rounds |x inv| <= 127 to the nearest integer (ties to even) and leaves it in the low byte
+    auto code = [&](float y) { return __float_as_uint(__fadd_rn(__fmul_rn(y, inv), 12582912.0f)); };
+    return prmt(prmt(code(x.x), code(x.y), 0x0040u), prmt(code(x.z), code(x.w), 0x0040u), 0x5410u);
 }
 
-// LANES threads (a power of two >= d / 8) take one row: lane l holds elements 4l..4l+3 of each half, so that a pair of
-// either rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head) with the heads
-// of q, then k, then v.
+// LANES threads (a power of two >= d / 8) take a row: lane l holds elements 4l..4l+3 of each half, so that a pair of either
+// rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head) with the heads of q, then
+// k, then v. A
+// thread has one row (two or three in flight: 2048 tokens 16.5 / 18.5 against 14.5 us); instructions bind next to HBM, so
+// that divisions are products and codes are rounded by an addition.
 template <int LANES>
-__global__ void __launch_bounds__(KW_THREADS) kv_write_kernel(const KvWriteParams p, uint32_t token0, uint32_t rows) {
-    const uint32_t r = blockIdx.x * (KW_THREADS / LANES) + threadIdx.x / LANES, lane = threadIdx.x % LANES;
+__global__ void __launch_bounds__(KW_THREADS) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
+    const uint32_t lane = threadIdx.x % LANES, r = blockIdx.x * (KW_THREADS / LANES) + threadIdx.x / LANES;
     const uint32_t heads = p.q_heads + 2 * p.c.heads, half = p.c.d / 2;
-    const bool live = r < rows;
-    const uint32_t t = token0 + (live ? r / heads : 0u);
-    uint32_t h = live ? r % heads : 0u;
-    const bool is_q = h < p.q_heads, is_v = h >= p.q_heads + p.c.heads;
-    if (!is_q) h -= is_v ? p.q_heads + p.c.heads : p.q_heads;
-    const int64_t slot = live && !is_q ? (int64_t)p.slots[t] : 0;
-    const bool wanted = live && (is_q || (slot >= 0 && slot < (int64_t)p.c.pages * p.c.page_size));
-    const bool active = wanted && lane * 8 < p.c.d;
+    const bool live = r < rows, active = live && lane * 8 < p.c.d;
+    const uint32_t in_launch = p.by_heads.quotient(r), t = token0 + in_launch, head = r - in_launch * heads;
+    const bool is_q = head < p.q_heads, is_v = head >= p.q_heads + p.c.heads;
+    const uint32_t h = head - (is_q ? 0 : is_v ? p.q_heads + p.c.heads : p.q_heads);
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    int32_t slot = 0;
     if (active) {
         const RowsView& in = is_q ? p.q : is_v ? p.v : p.k;
         const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * 4;
-        a = load4(in.p, at, p.dtype, p.vec);
-        b = load4(in.p, at + half, p.dtype, p.vec);
+        a = load4<true>(in.p, at, p.dtype, p.vec);
+        b = load4<true>(in.p, at + half, p.dtype, p.vec);
+        if (!is_q) slot = __ldg(p.slots + t);
         if (p.cos != nullptr && !is_v) {
-            const uint32_t pos = min((uint32_t)max(p.positions[t], 0), p.rope_len - 1);
-            const int64_t row = (int64_t)pos * half;
+            const int64_t row = (int64_t)min((uint32_t)max(__ldg(p.positions + t), 0), p.rope_len - 1) * half;
             if (p.interleaved) {
                 const int64_t i0 = row + lane * 2, i1 = i0 + half / 2;
-                rotate(a.x, a.y, p.cos[i0], p.sin[i0]);
-                rotate(a.z, a.w, p.cos[i0 + 1], p.sin[i0 + 1]);
-                rotate(b.x, b.y, p.cos[i1], p.sin[i1]);
-                rotate(b.z, b.w, p.cos[i1 + 1], p.sin[i1 + 1]);
+                rotate(a.x, a.y, __ldg(p.cos + i0), __ldg(p.sin + i0));
+                rotate(a.z, a.w, __ldg(p.cos + i0 + 1), __ldg(p.sin + i0 + 1));
+                rotate(b.x, b.y, __ldg(p.cos + i1), __ldg(p.sin + i1));
+                rotate(b.z, b.w, __ldg(p.cos + i1 + 1), __ldg(p.sin + i1 + 1));
             } else {
-                const float4 c = load4(p.cos, row + lane * 4, kF32, p.vec), s = load4(p.sin, row + lane * 4, kF32, p.vec);
+                const float4 c = load4<false>(p.cos, row + lane * 4, kF32, p.vec), s = load4<false>(p.sin, row + lane * 4, kF32, p.vec);
                 rotate(a.x, b.x, c.x, s.x);
                 rotate(a.y, b.y, c.y, s.y);
                 rotate(a.z, b.z, c.z, s.z);
@@ -121,29 +123,30 @@ __global__ void __launch_bounds__(KW_THREADS) kv_write_kernel(const KvWriteParam
         }
         if (p.c.dtype != kInt8) return;
     }
-    const uint32_t page = (uint32_t)slot / p.c.page_size;
-    const int64_t row = wanted ? ((int64_t)page * p.c.heads + h) * p.c.page_size + ((uint32_t)slot - page * p.c.page_size) : 0;
+    const bool wanted = active && !is_q && slot >= 0 && (uint64_t)slot < (uint64_t)p.c.pages * p.c.page_size;
+    const uint32_t page = p.by_page.quotient((uint32_t)slot & 0x7FFFFFFFu);
+    const int64_t row = ((int64_t)page * p.c.heads + h) * p.c.page_size + ((uint32_t)slot - page * p.c.page_size);
     void* const cache = is_v ? p.c.v : p.c.k;
     if (p.c.dtype != kInt8) {
-        if (active) {
+        if (wanted) {
             store4(cache, row * p.c.d + lane * 4, p.c.dtype, a);
             store4(cache, row * p.c.d + lane * 4 + half, p.c.dtype, b);
         }
         return;
     }
+    // (the whole warp shuffles)
     float m = max_nan(max_nan(max_nan(fabsf(a.x), fabsf(a.y)), max_nan(fabsf(a.z), fabsf(a.w))),
                       max_nan(max_nan(fabsf(b.x), fabsf(b.y)), max_nan(fabsf(b.z), fabsf(b.w))));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (is_q || !active) return;
+    if (!wanted) return;
     const bool finite = m < __int_as_float(0x7F800000), zero = m < MIN_AMAX;
     const float inv = finite && !zero ? __fdiv_rn(127.0f, m) : 0.0f;
     int8_t* const dst = static_cast<int8_t*>(cache) + row * p.c.d + lane * 4;
     *reinterpret_cast<uint32_t*>(dst) = finite ? codes4(a, inv) : 0u;
     *reinterpret_cast<uint32_t*>(dst + half) = finite ? codes4(b, inv) : 0u;
     if (lane == 0)
-        (is_v ? p.c.v_scale : p.c.k_scale)[row] =
-            !finite ? __int_as_float(0x7FC00000) : zero ? 0.0f : __fdiv_rn(m, 127.0f);
+        (is_v ? p.c.v_scale : p.c.k_scale)[row] = !finite ? __int_as_float(0x7FC00000) : zero ? 0.0f : __fdiv_rn(m, 127.0f);
 }
 
 template <int LANES>
@@ -205,7 +208,7 @@ __device__ __forceinline__ void write8(void* out, int64_t at, int out_dtype, con
 }
 
 template <int LANES>
-__global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const KvReadParams p, uint32_t tokens) {
+__global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const __grid_constant__ KvReadParams p, uint32_t tokens) {
     __shared__ int64_t first[KR_MOST];  // each token's row of head 0 in the cache, -1: none (its rows are zeros)
     const uint32_t t0 = blockIdx.x * tokens;
     if (threadIdx.x < tokens && t0 + threadIdx.x < p.total) {
@@ -266,7 +269,9 @@ cudaError_t launch_read(const KvReadParams& p, cudaStream_t stream) {
 
 }  // namespace
 
-cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream) {
+cudaError_t launch_kv_write(const KvWriteParams& params, cudaStream_t stream) {
+    KvWriteParams p = params;
+    p.by_heads = Divisor::of(p.q_heads + 2 * p.c.heads), p.by_page = Divisor::of(p.c.page_size);
     if (p.c.d > 64) return launch_write<16>(p, stream);
     if (p.c.d > 32) return launch_write<8>(p, stream);
     return launch_write<4>(p, stream);
