@@ -22,7 +22,7 @@ SOURCES = ["iq2xxs_capi.cu", "iq2xxs_gemv.cu", "iq2xxs_gemm.cu", "iq2xxs_dequant
            "iq2xxs_sharded.cu", "iq2_variants.cu", "attention_capi.cu", "kv_cache.cu", "attention_decode.cu",
            "attention_prefill.cu"]
 HEADERS = ["iq2xxs_common.cuh", "iq2xxs_codebook.h", "iq2xxs_internal.h", "iq2_variant_grids.h", "attention_internal.h",
-           "tcgen05.cuh"]
+           "tcgen05.cuh", "attention_parts.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -17,7 +17,9 @@
 //   * A bf16 cache under f32 activations takes a third piece (a second pair of products), or p would end at 2^-17.
 //   * int8 codes: the byte code + 128 with a zero byte above it is the f16 number (code + 128) 2^-24 (a subnormal, exact and
 //     full speed in the matrix instructions), so a pair costs half an exclusive or and one byte permute. The 128s are taken
-//     off as products with the constant 128 2^-24: S starts from minus them, O has them as one more column of P V.
+//     off as products with the constant 128 2^-24: S starts from minus them, O has them as one more column of P V. The
+//     sums are some four times as large for it, which f32 activations would notice (8e-6 against 1e-6 over the whole):
+//     for those a byte with 0x64 above it is 1024 + code + 128, and a subtraction makes it the code itself.
 //   * The key scale multiplies s, the value scale multiplies p. The reference m of a head's exponents moves when a product
 //     p w exceeds 2^8 (it starts where the first tile's largest is 1), so that p w keeps to the range of f16; the sum of p
 //     itself is f32.
@@ -44,9 +46,9 @@ constexpr float LOG2E = 1.44269504f;
 
 enum CacheKind { CK_F16, CK_BF16, CK_INT8 };
 
-template <int DP, int KIND, bool THIRD>
+template <int DP, int KIND, bool WIDE>
 struct DecodeShape {
-    static constexpr int PIECES = THIRD ? 3 : 2;
+    static constexpr int PIECES = WIDE && KIND == CK_BF16 ? 3 : 2;
     static constexpr int ESIZE = KIND == CK_INT8 ? 1 : 2;
     static constexpr int TOK = KIND == CK_INT8 ? 32 : 16;  // tokens of a warp's stage: 8 KB of K and V at DP = 128
     static constexpr int UNIT = TOK * 4;                   // tokens that the line of work is cut at: 32 KB at DP = 128
@@ -136,6 +138,15 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t (&r)[4], uint32_t addr)
                  : "r"(addr));
 }
 
+// Two bytes of codes + 128 as f16: (code + 128) 2^-24, or the codes themselves.
+template <bool SHIFTED>
+__device__ __forceinline__ uint32_t code_pair(uint32_t bytes, uint32_t sel) {
+    if (SHIFTED) return prmt(bytes, 0u, sel);
+    const uint32_t u = prmt(bytes, 0x64646464u, sel);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -190,11 +201,12 @@ struct Cursor {
     }
 };
 
-template <int DP, int KIND, bool THIRD>
+template <int DP, int KIND, bool WIDE>
 __global__ void __launch_bounds__(AD_THREADS, 1)
     decode_kernel(const __grid_constant__ DecodeArgs a) {
-    using S = DecodeShape<DP, KIND, THIRD>;
-    constexpr bool BF = KIND == CK_BF16, I8 = KIND == CK_INT8;
+    using S = DecodeShape<DP, KIND, WIDE>;
+    // WIDE: f32 activations
+    constexpr bool BF = KIND == CK_BF16, I8 = KIND == CK_INT8, THIRD = BF && WIDE, SHIFTED = I8 && !WIDE;
     constexpr int TOK = S::TOK, UNIT = S::UNIT, NT = DP / 8, KS = DP / 16, ST = TOK / 8;
     constexpr uint32_t ALL = TOK == 32 ? 0xFFFFFFFFu : (1u << TOK) - 1;
     const DecodeParams& p = a.p;
@@ -397,7 +409,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                     rest -= unpack_pair<BF>(h).x;
                 }
             }
-            if (lane == 0) q_factor[warp] = p.scale * LOG2E * up * (I8 ? CODE_UNIT : 1.f);
+            if (lane == 0) q_factor[warp] = p.scale * LOG2E * up * (SHIFTED ? CODE_UNIT : 1.f);
         }
         __syncthreads();
         // A fragments of S: k index 16 ks + 2t (+1, +8, +9). For int8 the k index is a relabelled dimension, so that a
@@ -411,7 +423,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             const uint32_t lo = k_lo(ks) / 2, hi = lo + (I8 ? 1 : 4);
             qa[ks][0] = q_row[lo], qa[ks][1] = q_row[DP / 2 + lo];
             qa[ks][2] = q_row[hi], qa[ks][3] = q_row[DP / 2 + hi];
-            if (I8) mma16816<BF>(minus, qa[ks], CODE_ZERO, CODE_ZERO);
+            if (SHIFTED) mma16816<BF>(minus, qa[ks], CODE_ZERO, CODE_ZERO);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) minus[j] = -minus[j];
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 #pragma unroll
                         for (int n = 0; n < ST; ++n) {
                             const uint32_t u = (j == 0 ? w[n].x : j == 1 ? w[n].y : j == 2 ? w[n].z : w[n].w) ^ 0x80808080u;
-                            mma16816<BF>(s[n], qa[q4 * 4 + j], prmt(u, 0u, 0x4140u), prmt(u, 0u, 0x4342u));
+                            mma16816<BF>(s[n], qa[q4 * 4 + j], code_pair<SHIFTED>(u, 0x4140u), code_pair<SHIFTED>(u, 0x4342u));
                         }
                 }
             } else {
@@ -540,7 +552,8 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 
             if (I8) {
 #pragma unroll
-                for (int ks = 0; ks < TOK / 16; ++ks) mma16816<BF>(o_off, pa[ks], CODE_ZERO, CODE_ZERO);
+                for (int ks = 0; ks < TOK / 16; ++ks)
+                    if (SHIFTED) mma16816<BF>(o_off, pa[ks], CODE_ZERO, CODE_ZERO);
 #pragma unroll
                 for (int c = 0; c < S::CHUNKS; ++c) {
                     uint32_t r[4];  // chunk c of tokens 0-7, 8-15, 16-23, 24-31; each word: dimensions 2g, 2g + 1 of two tokens
@@ -549,8 +562,8 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                     for (int j = 0; j < 4; ++j) r[j] ^= 0x80808080u;
 #pragma unroll
                     for (int ks = 0; ks < TOK / 16; ++ks) {
-                        mma16816<BF>(o[c * 2], pa[ks], prmt(r[ks * 2], 0u, 0x4240u), prmt(r[ks * 2 + 1], 0u, 0x4240u));
-                        mma16816<BF>(o[c * 2 + 1], pa[ks], prmt(r[ks * 2], 0u, 0x4341u), prmt(r[ks * 2 + 1], 0u, 0x4341u));
+                        mma16816<BF>(o[c * 2], pa[ks], code_pair<SHIFTED>(r[ks * 2], 0x4240u), code_pair<SHIFTED>(r[ks * 2 + 1], 0x4240u));
+                        mma16816<BF>(o[c * 2 + 1], pa[ks], code_pair<SHIFTED>(r[ks * 2], 0x4341u), code_pair<SHIFTED>(r[ks * 2 + 1], 0x4341u));
                     }
                 }
             } else {
@@ -569,7 +582,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             __syncwarp();
             stage = stage == AD_STAGES - 1 ? 0 : stage + 1;
         }
-        if (I8) {  // the 128s off, and the codes' unit on
+        if (SHIFTED) {  // the 128s off, and the codes' unit on
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -687,15 +700,15 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             store_elem(p.out, ((int64_t)r.b * p.q_heads + head0 + warp) * d + lane + i * 32, p.dtype, sum == 0.f ? 0.f : y[i] / sum);
 }
 
-template <int DP, int KIND, bool THIRD>
+template <int DP, int KIND, bool WIDE>
 cudaError_t launch(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
-    using S = DecodeShape<DP, KIND, THIRD>;
-    cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP, KIND, THIRD>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    using S = DecodeShape<DP, KIND, WIDE>;
+    cudaError_t e = cudaFuncSetAttribute(decode_kernel<DP, KIND, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     // (the second kernel keeps the first one's split of shared memory: changing it would drain the SMs twice a call)
     if (e == cudaSuccess)
         e = cudaFuncSetAttribute(join_kernel<DP>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
-    decode_kernel<DP, KIND, THIRD><<<blocks, AD_THREADS, S::SMEM, stream>>>(a);
+    decode_kernel<DP, KIND, WIDE><<<blocks, AD_THREADS, S::SMEM, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -711,9 +724,10 @@ cudaError_t launch(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
 
 template <int DP>
 cudaError_t launch_kind(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
-    if (a.p.c.dtype == kInt8) return launch<DP, CK_INT8, false>(a, blocks, stream);
+    const bool wide = a.p.dtype == kF32;
+    if (a.p.c.dtype == kInt8) return wide ? launch<DP, CK_INT8, true>(a, blocks, stream) : launch<DP, CK_INT8, false>(a, blocks, stream);
     if (a.p.c.dtype == kF16) return launch<DP, CK_F16, false>(a, blocks, stream);
-    return a.p.dtype == kF32 ? launch<DP, CK_BF16, true>(a, blocks, stream) : launch<DP, CK_BF16, false>(a, blocks, stream);
+    return wide ? launch<DP, CK_BF16, true>(a, blocks, stream) : launch<DP, CK_BF16, false>(a, blocks, stream);
 }
 
 }  // namespace

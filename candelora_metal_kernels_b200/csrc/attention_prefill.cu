@@ -12,7 +12,8 @@
 // K and V tiles arrive by TMA (128-byte swizzle, no multicast) in one ring, K_0 V_0 K_1 V_1 ..., across items.
 //   * Work: one block an SM stays for the whole call. The items, each as long as its keys and AP_ITEM_COST more, form one
 //     line, of which each block takes an equal contiguous part (short calls: whole items, see Work). A part that is
-//     not a whole item leaves (o, m, l) in the workspace and join_kernel adds an item's parts up in the blocks' order.
+//     not a whole item leaves (o, m, l) in the workspace, unless it is the item's last one: that adds the parts up
+//     (attention_parts.cuh), beside the other blocks' work and without a launch or a wait of its own.
 //   * Lazy rescaling: the reference m of a row moves only when a score exceeds it by more than 2^8 (p stays below 256,
 //     far inside both types' range), so O in TMEM is rescaled a few times a row instead of once a tile.
 //   * Masked keys are replaced by -inf before the maximum (never added to), so that whatever K holds there cannot matter.
@@ -21,6 +22,7 @@
 //     rows see become zeros too, and the epilogue adds them back to exactly the rows that see them.
 // Every wait is bounded by wall time (device_status); a block that gives up still drains its copies and frees its TMEM.
 #include "attention_internal.h"
+#include "attention_parts.cuh"
 #include "iq2xxs_internal.h"
 #include "tcgen05.cuh"
 
@@ -43,7 +45,7 @@ constexpr int32_t AP_ITEM_COST = 3 * AP_KEYS, AP_SPLIT_COST = 3 * AP_KEYS;
 constexpr int AP_REGS_SOFTMAX = 208, AP_REGS_OTHER = 88;
 static_assert(8 * AP_REGS_SOFTMAX + 4 * AP_REGS_OTHER <= 12 * 168, "register shares");
 
-constexpr int AP_PARTS = 4, AP_PART_BYTES = 64;  // parts of items on their way between the warps
+constexpr int AP_PARTS = 4, AP_PART_BYTES = 80;  // parts of items on their way between the warps
 
 template <int DP>
 struct PrefillShape {
@@ -56,17 +58,10 @@ struct PrefillShape {
 // A part of an item in the workspace: o [d / 4][256 rows][4], then the rows' references (in powers of two) and sums.
 constexpr uint32_t part_floats(int dp) { return AP_ITEM_ROWS * (dp + 2); }
 
-// What join_kernel's block of the same number has to join: an item's parts in blocks c0 to c1, block c0's being its part
-// number `slot` (0: its first, 1: its last), the others' their first. c1 = 0: nothing.
-struct JoinRecord {
-    int32_t q0, lq, tok0;
-    uint32_t kv_head, c0, c1, slot;
-};
-
 struct PrefillArgs {
     RowsView v;
     void* out;
-    JoinRecord* records;
+    unsigned long long *flags, token;  // see attention_parts.cuh
     float* parts;
     const int32_t *cu_q, *cu_k;
     unsigned int* status;
@@ -269,7 +264,8 @@ struct Work {
     // the item, and the key tiles [j0, j1) of its n in this part
     uint32_t b, kv_head;
     int32_t tok0, n, j0, j1;
-    int32_t pos, to;  // the part of the item's length
+    int32_t pos, to;     // the part of the item's length
+    uint64_t at, each;   // where the part begins in the line, and the blocks' share of it
     uint64_t left;    // of the block's part of the line, from this part on (whole items: their number)
     bool by_items;
     // its sequence and tiles
@@ -324,7 +320,7 @@ struct Work {
     // The next part that has key tiles (the first or last bit of an item may have none).
     __device__ __forceinline__ void next(const PrefillArgs& p) {
         do {
-            left -= by_items ? 1 : (uint64_t)(to - pos);
+            left -= by_items ? 1 : (uint64_t)(to - pos), at += (uint64_t)(to - pos);
             if (done()) return;
             pos = 0;
             if (++kv_head == p.kv_heads) {
@@ -344,6 +340,15 @@ struct Work {
             }
             enter_item(p);
         } while (j0 == j1);
+    }
+    // The blocks that have key tiles of the item, and whether it is the first of block c0 (slot 0) or its last (slot 1).
+    __device__ __forceinline__ void sharers(uint32_t* c0, uint32_t* c1, uint32_t* slot) const {
+        *c0 = *c1 = blockIdx.x, *slot = 0;
+        if (whole()) return;
+        const uint64_t item = at - (uint64_t)pos, first = item + AP_ITEM_COST, last = first + (uint32_t)((n - 1) * AP_KEYS);
+        while (*c0 * each > first) --*c0;
+        while ((*c1 + 1) * each <= last) ++*c1;
+        *slot = *c0 * each >= item ? 0 : 1;
     }
     // The block's part of the line; false if there is none. (Runs once, but from a cold instruction cache: without 64-bit
     // divisions it is a quarter of the code.) Every block but the last has `each` of the line.
@@ -370,8 +375,8 @@ struct Work {
         const uint32_t item_share = (items + gridDim.x - 1) / gridDim.x;
         const uint64_t share = (uint64_t)((double)total * p.inv_blocks) + 1;  // a little over its part of the line
         by_items = (uint64_t)item_share * (uint32_t)(AP_ITEM_COST + longest) <= share + AP_SPLIT_COST;
-        const uint64_t each = by_items ? item_share : max(share, (uint64_t)AP_KEYS), all = by_items ? items : total;
-        const uint64_t u0 = min(blockIdx.x * each, all);
+        each = by_items ? item_share : max(share, (uint64_t)AP_KEYS), at = blockIdx.x * each;
+        const uint64_t all = by_items ? items : total, u0 = min(at, all);
         left = min(u0 + each, all) - u0;
         if (left == 0) return false;
 #pragma unroll 1
@@ -413,16 +418,6 @@ struct Work {
             kv_head = (uint32_t)rest / length, pos = (int32_t)((uint32_t)rest % length);
         }
         enter_item(p);
-        // The first block that begins inside an item's key tiles joins the item: the block before it has the first of them.
-        JoinRecord r{q0, lq, tok0, kv_head, blockIdx.x - 1, 0, 0};
-        const uint64_t item0 = u0 - (uint64_t)pos;
-        if (j0 > 0 && j0 < j1 && u0 - each <= item0 + AP_ITEM_COST) {
-            const uint64_t last = item0 + (uint32_t)(AP_ITEM_COST + (n - 1) * AP_KEYS);  // where its last tile begins
-            r.c1 = blockIdx.x;
-            while ((r.c1 + 1) * each <= last) ++r.c1;
-            r.slot = u0 - each >= item0 ? 0 : 1;
-        }
-        if (lane == 0) p.records[blockIdx.x] = r;
         if (j0 == j1) next(p);
         return !done();
     }
@@ -435,6 +430,7 @@ struct Part {
     int32_t row0, tokens;              // the item's first token in the packed tensors; tokens of the sequence from it on
     int32_t seen0, keys;               // keys that the first token sees less one (before clamping to 0 .. keys)
     int32_t k0, kv_head, whole, more;  // more = 0: no further part
+    uint32_t c0, c1, slot;             // see PartSet
 };
 static_assert(sizeof(Part) <= AP_PART_BYTES, "a part's place");
 
@@ -464,8 +460,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     auto part_full = [&](uint32_t s) { return more + 120 + s * 8; };
     auto part_empty = [&](uint32_t s) { return more + 120 + (AP_PARTS + s) * 8; };
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    pdl_launch_dependents();
 
+    if (threadIdx.x < 2 * PART_WARPS) p.flags[blockIdx.x * 2 * PART_WARPS + threadIdx.x] = 0ull;  // (this block's own)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(q_full(i), 1), mbar_init(q_empty(i), 1), mbar_init(s_full(i), 1), mbar_init(o_full(i), 1);
@@ -505,10 +501,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             bool ok = true;
             uint32_t slot = 0, lap = 0, written = 0;
             Work w;
-            if (!w.begin(p)) {
-                w.left = 0;
-                if (lane == 0) p.records[blockIdx.x].c1 = 0;
-            }
+            if (!w.begin(p)) w.left = 0;
             auto load_kv = [&](const CUtensorMap* map, int32_t j) {
                 if (lap > 0 && ok) ok = __all_sync(0xFFFFFFFFu, wait_bar(empty(slot), (lap - 1) & 1, p, AP_RELEASE, abort_flag));
                 if (!ok) return;
@@ -537,9 +530,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 if (written >= AP_PARTS) ok = __all_sync(0xFFFFFFFFu, wait_bar(part_empty(s), (written / AP_PARTS - 1) & 1, p, AP_RELEASE, abort_flag));
                 if (!ok) break;
                 more_parts = !w.done();
+                uint32_t c0 = 0, c1 = 0, first_slot = 0;
+                if (more_parts) w.sharers(&c0, &c1, &first_slot);
                 if (lane == 0) {
                     parts[s] = {w.j0, w.j1, w.end(0), w.end(1), w.masked, w.least, w.most, w.q0 + w.tok0, w.lq - w.tok0,
-                                p.causal ? w.tok0 + w.lk - w.lq : w.lk - 1, w.lk, w.k0, (int32_t)w.kv_head, w.whole() ? 1 : 0, more_parts ? 1 : 0};
+                                p.causal ? w.tok0 + w.lk - w.lq : w.lk - 1, w.lk, w.k0, (int32_t)w.kv_head, w.whole() ? 1 : 0, more_parts ? 1 : 0, c0, c1, first_slot};
                     mbar_arrive(part_full(s));
                 }
                 if (!more_parts) break;
@@ -780,46 +775,86 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 tc_fence_after();
             }
             if (!ok) break;
-            // O / l to the output, or O, its reference and l to the workspace
+            // O / l to the output; or O, its reference and l to the workspace; or the sum of the item's parts to the output
             const bool whole = w.whole != 0, odd = any && *odd_values != 0u;
-            float* const part_o = p.parts + ((uint64_t)blockIdx.x * 2 + (part > 0 ? 1 : 0)) * part_floats(DP);
             const uint32_t item_row = i * AP_ROWS + row;
-            const float inv = seen > 0 ? __fdividef(1.0f, l) : 0.f;
-            const uint64_t inv2 = pair(inv, inv);
             uint16_t* const out = static_cast<uint16_t*>(p.out) +
                                   ((int64_t)(w.row0 + row_tok) * p.q_heads + w.kv_head * (int)p.group + (int)row_head) * p.d;
-            if (!whole) {
-                part_o[AP_ITEM_ROWS * DP + item_row] = m * p.c;
-                part_o[AP_ITEM_ROWS * (DP + 1) + item_row] = l;
-            }
-            if (!any && whole) {
-                if (valid)
-                    for (int c = 0; c < (int)p.d; c += 16) store32(out + c, make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0), p.out32);
-            } else if (any) {  // (the join leaves out parts without steps: their reference is -inf)
-#pragma unroll 2
-                for (int c = 0; c < DP; c += 32) {
-                    float o[32];
-                    tmem_ld32_async(o_col(i) + lanes + c, o);
-                    tmem_ld_wait();
-                    pin32(o);
-                    if (valid && !whole) {
-#pragma unroll
-                        for (int x = 0; x < 32; x += 4)
-                            *reinterpret_cast<float4*>(part_o + ((c + x) / 4 * AP_ITEM_ROWS + item_row) * 4) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
-                    } else if (valid) {
-                        uint32_t v[16];
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) {  // (o of a row that sees no key is 0, and so is inv)
-                            const uint64_t y = mul2(pair(o[2 * x], o[2 * x + 1]), inv2);
-                            v[x] = pack2<BF>(first_of(y), second_of(y));
-                        }
-#pragma unroll
-                        for (int x = 0; x < 2; ++x)
-                            if (c + x * 16 < (int)p.d)
-                                store32(out + c + x * 16, make_uint4(v[8 * x], v[8 * x + 1], v[8 * x + 2], v[8 * x + 3]),
-                                        make_uint4(v[8 * x + 4], v[8 * x + 5], v[8 * x + 6], v[8 * x + 7]), p.out32);
+            const PartSet set{p.flags, p.token, w.c0, w.c1, w.slot, blockIdx.x, warp};
+            auto part_at = [&](uint32_t c) { return p.parts + (uint64_t)set.part(c) * part_floats(DP) + item_row; };
+            // (one loop for all three, since code that is not cached costs more than its branches)
+            enum { WHOLE, LEAVE, JOIN };
+            int what = whole ? WHOLE : set.others_done() ? JOIN : LEAVE;
+            const float mine = m * p.c;
+            for (;;) {
+                float top = mine, sum = l;
+                float* const part_o = p.parts + ((uint64_t)blockIdx.x * 2 + (part > 0 ? 1 : 0)) * part_floats(DP);
+                auto ref_of = [&](uint32_t c) { return c == set.self ? mine : __ldcg(part_at(c) + AP_ITEM_ROWS * DP); };
+                if (what == LEAVE) part_o[AP_ITEM_ROWS * DP + item_row] = mine, part_o[AP_ITEM_ROWS * (DP + 1) + item_row] = l;
+                if (what == JOIN) {
+#pragma unroll 1
+                    for (uint32_t c = set.c0; c <= set.c1; ++c) top = fmaxf(top, ref_of(c));
+                    sum = 0.f;
+#pragma unroll 1
+                    for (uint32_t c = set.c0; c <= set.c1; ++c) {
+                        const float mc = ref_of(c), lc = c == set.self ? l : __ldcg(part_at(c) + AP_ITEM_ROWS * (DP + 1));
+                        sum += mc == -INFINITY ? lc : ex2(mc - top) * lc;  // (-inf: no key of the part is seen, or its scores are NaN)
                     }
-                    __syncwarp();
+                }
+                // a row that sees no key: zeros (its O is 0, too); NaN scores throughout: the sum is NaN
+                const float inv = top == -INFINITY && sum == 0.f ? 0.f : __fdividef(1.0f, sum);
+                const uint64_t inv2 = pair(inv, inv);
+                if (any || what != LEAVE) {  // (a part without steps of the tile has no O: its references are -inf)
+#pragma unroll 1
+                    for (int c = 0; c < DP; c += 32) {
+                        float o[32];
+                        if (any) {
+                            tmem_ld32_async(o_col(i) + lanes + c, o);
+                            tmem_ld_wait();
+                            pin32(o);
+                        } else {
+#pragma unroll
+                            for (int x = 0; x < 32; ++x) o[x] = 0.f;
+                        }
+                        if (what == LEAVE) {
+#pragma unroll
+                            for (int x = 0; x < 32; x += 4)
+                                *reinterpret_cast<float4*>(part_o + ((c + x) / 4 * AP_ITEM_ROWS + item_row) * 4) = make_float4(o[x], o[x + 1], o[x + 2], o[x + 3]);
+                        } else {
+                            if (what == JOIN) {
+                                float y[32];
+#pragma unroll
+                                for (int x = 0; x < 32; ++x) y[x] = 0.f;
+#pragma unroll 1
+                                for (uint32_t b = set.c0; b <= set.c1; ++b) {
+                                    const float mc = ref_of(b);
+                                    if (mc == -INFINITY) continue;
+                                    const float wb = ex2(mc - top);
+                                    const float* const src = part_at(b) - item_row + (c / 4 * AP_ITEM_ROWS + item_row) * 4;
+#pragma unroll
+                                    for (int x = 0; x < 32; x += 4) {
+                                        const float4 z = b == set.self ? make_float4(o[x], o[x + 1], o[x + 2], o[x + 3])
+                                                                       : __ldcg(reinterpret_cast<const float4*>(src + x * AP_ITEM_ROWS));
+                                        y[x] += z.x * wb, y[x + 1] += z.y * wb, y[x + 2] += z.z * wb, y[x + 3] += z.w * wb;
+                                    }
+                                }
+#pragma unroll
+                                for (int x = 0; x < 32; ++x) o[x] = y[x];
+                            }
+                            uint32_t v[16];
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) {
+                                const uint64_t y = mul2(pair(o[2 * x], o[2 * x + 1]), inv2);
+                                v[x] = pack2<BF>(first_of(y), second_of(y));
+                            }
+#pragma unroll
+                            for (int x = 0; x < 2; ++x)
+                                if (valid && c + x * 16 < (int)p.d)
+                                    store32(out + c + x * 16, make_uint4(v[8 * x], v[8 * x + 1], v[8 * x + 2], v[8 * x + 3]),
+                                            make_uint4(v[8 * x + 4], v[8 * x + 5], v[8 * x + 6], v[8 * x + 7]), p.out32);
+                        }
+                        __syncwarp();
+                    }
                 }
                 // infinities and NaN that the guard took out, back into the rows that see them
                 if (odd && valid) {
@@ -831,17 +866,20 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                         for (int x = 0; x < (int)p.d; ++x) {
                             const float f = BF ? __uint_as_float((uint32_t)v[x] << 16) : half_bits_to_float(v[x]);
                             if (fabsf(f) < INFINITY) continue;
-                            if (whole) {
+                            if (what == LEAVE) {
+                                part_o[(x / 4 * AP_ITEM_ROWS + item_row) * 4 + x % 4] += f;
+                            } else {
                                 const float y = BF ? __uint_as_float((uint32_t)out[x] << 16) : half_bits_to_float(out[x]);
                                 out[x] = (uint16_t)pack2<BF>(y + f, 0.f);
-                            } else {
-                                part_o[(x / 4 * AP_ITEM_ROWS + item_row) * 4 + x % 4] += f;
                             }
                         }
                     }
                 }
                 __syncwarp();
+                if (what != LEAVE || !set.show()) break;
+                what = JOIN;
             }
+            if (what == JOIN) set.clear();
             if (any) {
                 tc_fence_before();
                 __syncwarp();
@@ -859,45 +897,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             if (q_issued[i] > 0) mbar_wait(q_full(i), (q_issued[i] - 1) & 1, p.status, AP_LOAD, p.wait_ns);
         for (uint32_t x = issued > SLOTS ? issued - SLOTS : 0; x < issued; ++x)
             mbar_wait(full(x % SLOTS), (x / SLOTS) & 1, p.status, AP_LOAD, p.wait_ns);
-    }
-}
-
-// The parts of an item that several blocks had: (o, m, l) = sum over them of 2^(m_c - max) (o_c, l_c), in the blocks' order.
-// A block a record; a thread takes eight columns of a row, a warp's rows lie side by side in the parts.
-template <int DP, bool BF>
-__global__ void __launch_bounds__(AP_ITEM_ROWS, 1) join_kernel(const __grid_constant__ PrefillArgs p) {
-    pdl_wait();
-    const JoinRecord r = p.records[blockIdx.x];
-    if (r.c1 == 0) return;
-    const uint32_t row = threadIdx.x, in_tile = row % AP_ROWS;
-    const int32_t tok = r.tok0 + (int32_t)(row / AP_ROWS * p.tpt + in_tile / p.group);
-    if (in_tile >= p.tpt * p.group || tok >= r.lq) return;
-    auto part = [&](uint32_t c) { return p.parts + ((uint64_t)c * 2 + (c == r.c0 ? r.slot : 0)) * part_floats(DP); };
-    float top = -INFINITY, sum = 0.f;
-    for (uint32_t c = r.c0; c <= r.c1; ++c) top = fmaxf(top, part(c)[AP_ITEM_ROWS * DP + row]);
-    for (uint32_t c = r.c0; c <= r.c1; ++c) {
-        const float m = part(c)[AP_ITEM_ROWS * DP + row], l = part(c)[AP_ITEM_ROWS * (DP + 1) + row];
-        sum += m == -INFINITY ? l : ex2(m - top) * l;
-    }
-    const bool none = top == -INFINITY && sum == 0.f;  // the row sees no key
-    const float inv = 1.0f / sum;
-    uint16_t* const out = static_cast<uint16_t*>(p.out) + ((int64_t)(r.q0 + tok) * p.q_heads + r.kv_head * p.group + in_tile % p.group) * p.d;
-    const uint32_t columns = (p.d / 8 + gridDim.y - 1) / gridDim.y * 8, first = blockIdx.y * columns;
-    for (uint32_t d0 = first; d0 < min(first + columns, p.d); d0 += 8) {
-        float y[8] = {};
-        for (uint32_t c = r.c0; c <= r.c1; ++c) {
-            const float m = part(c)[AP_ITEM_ROWS * DP + row], w = ex2(m - top);
-            if (m == -INFINITY) continue;
-            const float4 a = *reinterpret_cast<const float4*>(part(c) + (d0 / 4 * AP_ITEM_ROWS + row) * 4);
-            const float4 b = *reinterpret_cast<const float4*>(part(c) + ((d0 / 4 + 1) * AP_ITEM_ROWS + row) * 4);
-            y[0] += a.x * w, y[1] += a.y * w, y[2] += a.z * w, y[3] += a.w * w;
-            y[4] += b.x * w, y[5] += b.y * w, y[6] += b.z * w, y[7] += b.w * w;
-        }
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (!none)
-            v = make_uint4(pack2<BF>(y[0] * inv, y[1] * inv), pack2<BF>(y[2] * inv, y[3] * inv), pack2<BF>(y[4] * inv, y[5] * inv),
-                           pack2<BF>(y[6] * inv, y[7] * inv));
-        *reinterpret_cast<uint4*>(out + d0) = v;
     }
 }
 
@@ -924,8 +923,6 @@ bool encode_rows(CUtensorMap* map, const RowsView& r, uint32_t d, uint32_t inner
     return e == CUDA_SUCCESS;
 }
 
-inline size_t records_bytes(uint32_t blocks) { return (blocks * sizeof(JoinRecord) + 255) / 256 * 256; }
-constexpr unsigned AP_JOIN_SLICES = 4;  // blocks of join_kernel that share an item's columns
 
 template <int DP, bool BF>
 cudaError_t launch(const PrefillParams& p, uint8_t* workspace, unsigned blocks, cudaStream_t stream) {
@@ -935,8 +932,8 @@ cudaError_t launch(const PrefillParams& p, uint8_t* workspace, unsigned blocks, 
     if (e != cudaSuccess) return e;
     if (encode_fn() == nullptr) return cudaErrorNotSupported;
     a.v = p.v, a.out = p.out, a.cu_q = p.cu_q, a.cu_k = p.cu_k;
-    a.records = reinterpret_cast<JoinRecord*>(workspace);
-    a.parts = reinterpret_cast<float*>(workspace + records_bytes(blocks));
+    a.flags = reinterpret_cast<unsigned long long*>(workspace), a.token = call_token();
+    a.parts = reinterpret_cast<float*>(workspace + part_flags_bytes(blocks));
     a.seqs = p.seqs, a.q_tokens = p.q_tokens, a.k_tokens = p.k_tokens, a.q_heads = p.q_heads, a.kv_heads = p.kv_heads;
     a.group = p.q_heads / p.kv_heads, a.tpt = AP_ROWS / a.group, a.d = p.d;
     a.inv_blocks = 1.0 / blocks;
@@ -950,27 +947,14 @@ cudaError_t launch(const PrefillParams& p, uint8_t* workspace, unsigned blocks, 
         return cudaErrorInvalidValue;
     e = cudaFuncSetAttribute(prefill_kernel<DP, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return e;
-    // (the second kernel keeps the first one's split of shared memory: changing it would drain the SMs twice a call)
-    e = cudaFuncSetAttribute(join_kernel<DP, BF>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-    if (e != cudaSuccess) return e;
     prefill_kernel<DP, BF><<<blocks, AP_THREADS, S::SMEM, stream>>>(qm, km, vm, a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks, AP_JOIN_SLICES);
-    cfg.blockDim = dim3(AP_ITEM_ROWS);
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, join_kernel<DP, BF>, a);
+    return cudaGetLastError();
 }
 
 }  // namespace
 
 size_t attention_prefill_workspace(const PrefillParams& p, int num_sms) {
-    return records_bytes(num_sms) + (size_t)num_sms * 2 * part_floats(p.d > 64 ? 128 : 64) * sizeof(float);
+    return part_flags_bytes(num_sms) + (size_t)num_sms * 2 * part_floats(p.d > 64 ? 128 : 64) * sizeof(float);
 }
 
 cudaError_t launch_attention_prefill(const PrefillParams& p, void* workspace, int num_sms, cudaStream_t stream) {

@@ -53,6 +53,7 @@ fn main() {
         "iq2_variant_grids.h",
         "attention_internal.h",
         "tcgen05.cuh",
+        "attention_parts.cuh",
     ] {
         println!("cargo:rerun-if-changed={}", csrc.join(h).display());
     }
