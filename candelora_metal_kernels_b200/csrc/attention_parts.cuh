@@ -15,8 +15,8 @@ namespace iq2 {
 constexpr uint32_t PART_WARPS = 8;
 inline size_t part_flags_bytes(uint32_t blocks) { return ((size_t)blocks * 2 * PART_WARPS * sizeof(unsigned long long) + 255) / 256 * 256; }
 
-// The parts of an item: blocks c0 to c1, block c0's being its part number `slot` (0: its first, 1: its last), the others'
-// their first; this warp's share of this block's (c = self).
+// The parts of an item: blocks c0 to c1, block c0's in its place `slot` (1 where it has begun in an earlier item), the others'
+// in their place 0; this warp's share of this block's (c = self).
 struct PartSet {
     unsigned long long* flags;
     unsigned long long token;

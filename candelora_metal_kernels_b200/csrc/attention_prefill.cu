@@ -341,7 +341,8 @@ struct Work {
             enter_item(p);
         } while (j0 == j1);
     }
-    // The blocks that have key tiles of the item, and whether it is the first of block c0 (slot 0) or its last (slot 1).
+    // The blocks that have key tiles of the item, and the place of block c0's part: 1 where that block begins in an earlier
+    // item (which then has place 0, if it has key tiles there).
     __device__ __forceinline__ void sharers(uint32_t* c0, uint32_t* c1, uint32_t* slot) const {
         *c0 = *c1 = blockIdx.x, *slot = 0;
         if (whole()) return;
@@ -701,7 +702,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         bool ok = true;
         Part w;
 #pragma unroll 1
-        for (int part = 0; ok && next_part(w); ++part) {
+        while (ok && next_part(w)) {
             const int32_t end = i == 0 ? w.end0 : w.end1;
             const bool valid = row < p.tpt * p.group && row_tok < w.tokens;
             const int32_t seen = !valid ? 0 : p.causal ? max(min(w.seen0 + row_tok + 1, w.keys), 0) : w.keys;
@@ -788,7 +789,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             const float mine = m * p.c;
             for (;;) {
                 float top = mine, sum = l;
-                float* const part_o = p.parts + ((uint64_t)blockIdx.x * 2 + (part > 0 ? 1 : 0)) * part_floats(DP);
+                float* const part_o = p.parts + (uint64_t)set.part(set.self) * part_floats(DP);
                 auto ref_of = [&](uint32_t c) { return c == set.self ? mine : __ldcg(part_at(c) + AP_ITEM_ROWS * DP); };
                 if (what == LEAVE) part_o[AP_ITEM_ROWS * DP + item_row] = mine, part_o[AP_ITEM_ROWS * (DP + 1) + item_row] = l;
                 if (what == JOIN) {

@@ -72,6 +72,18 @@ def test_prefill(lq, lk, hq, hkv, d, causal, dtype):
     check_prefill(q, k, v, cu_q, cu_k, got, causal=causal)
 
 
+@pytest.mark.parametrize("lq,lk", [([702], None), ([601], [1202]), ([333, 901], None), ([64], [9000]), ([17, 700, 450], [3017, 700, 2450])])
+def test_prefill_items_cut_between_blocks(lq, lk):
+    """Enough work that blocks end and begin inside items, also inside an item's last key tile."""
+    lk = lq if lk is None else lk
+    q, k, v = (randn((sum(n), h, 16), 20 + i, BF16) for i, (n, h) in enumerate([(lq, 32), (lk, 8), (lk, 8)]))
+    cu_q, cu_k = cu(lq), cu(lk)
+    got = c.attention_prefill(q, k, v, cu_q.cuda(), cu_k.cuda())
+    check_prefill(q, k, v, cu_q, cu_k, got)
+    for _ in range(3):
+        assert torch.equal(c.attention_prefill(q, k, v, cu_q.cuda(), cu_k.cuda()), got)
+
+
 def test_prefill_slices_of_one_projection():
     """q, k and v as strided slices of [tokens, (hq + 2 hkv) d], and slices whose rows are not 16-byte aligned."""
     hq, hkv, d, lens = 8, 2, 64, [150, 31]
