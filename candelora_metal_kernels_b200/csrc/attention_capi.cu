@@ -136,8 +136,7 @@ int iq2_kv_cache_write(const iq2_kv_cache* cache, const iq2_kv_tokens* t, iq2_st
     p.slots = t->slots, p.positions = t->positions, p.cos = rope ? t->cos : nullptr, p.sin = t->sin, p.q_out = t->q_out;
     p.tokens = t->tokens, p.q_heads = has_q ? t->q_heads : 0, p.rope_len = t->rope_len;
     p.dtype = t->dtype, p.q_out_dtype = t->q_out_dtype, p.interleaved = t->interleaved != 0;
-    const size_t wide = 4 * e;
-    p.vec = rows_aligned(t->k, e, wide) && rows_aligned(t->v, e, wide) && (!has_q || rows_aligned(t->q, e, wide)) &&
+    p.vec = rows_aligned(t->k, e, 16) && rows_aligned(t->v, e, 16) && (!has_q || rows_aligned(t->q, e, 16)) &&
             (!rope || (reinterpret_cast<uintptr_t>(t->cos) % 16 == 0 && reinterpret_cast<uintptr_t>(t->sin) % 16 == 0));
     const cudaError_t err = iq2::launch_kv_write(p, reinterpret_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? IQ2_OK : capi_cuda_fail(op, err);

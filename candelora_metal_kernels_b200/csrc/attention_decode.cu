@@ -24,6 +24,13 @@
 //     p w exceeds 2^8 (it starts where the first tile's largest is 1), so that p w keeps to the range of f16; the sum of p
 //     itself is f32.
 // The maxima, sums, s, p and o are f32.
+//
+// Measured (8 key heads, 128 elements): 128 sequences of up to 4096 tokens, bf16 cache, 214 us: 6260 GB/s, 0.96 of the copy
+// rate; one of 100001 tokens, int8 cache and 8 query heads a key head, 48 us: 4430 GB/s, of which about 8 us are start,
+// merge of the warps and join, and in the stream the widening of the codes binds as well (issue slots 48 % used); 16 of up to
+// 2048, int8, f32 q, 22 us, of which the stream is 7; one of 333 tokens 9.6 us, latencies one after another. The parts added
+// up inside this kernel (by the block that finishes last) instead of by a dependent launch: 11.4 and 53.8 us for the last and
+// the second of these.
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"
 

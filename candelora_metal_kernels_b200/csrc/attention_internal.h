@@ -53,7 +53,7 @@ struct KvWriteParams {
     uint32_t tokens, q_heads, rope_len;
     int dtype, q_out_dtype;
     bool interleaved;
-    bool vec;  // every row of the inputs and tables starts on a 16-byte boundary (8 for 16-bit rows)
+    bool vec;  // every row of the inputs and tables starts on a 16-byte boundary
     Divisor by_heads, by_page;  // set by the launch: heads of a token (q, k and v), tokens of a page
 };
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);

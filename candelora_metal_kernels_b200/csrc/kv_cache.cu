@@ -6,6 +6,9 @@
 // with every product and sum rounded by itself in f32, so that a result does not depend on how the compiler fuses.
 // int8 rows (one token and head): m = max |x|, scale = m / 127, code = rint(x * (127 / m)); m < 2^-100 gives zeros (the
 // quotient would overflow), and a row with an infinity or NaN gets a NaN scale, so that it reads back as NaN.
+// Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 13.2 us, 5820 GB/s of bytes in
+// and out; of 8800 tokens, f32 into an int8 cache, with the read back 66.8 us, 5430 GB/s; read of 89091 tokens of an int8 cache
+// to bf16 96 us, 5750 GB/s.
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"
 
@@ -19,28 +22,54 @@ constexpr int KW_THREADS = 256;
 
 constexpr float MIN_AMAX = 7.88860905e-31f;  // 2^-100
 
-// Four values at element i. ONCE: they are not read again (the cache lines give way first).
-template <bool ONCE>
-__device__ __forceinline__ float4 load4(const void* base, int64_t i, int dtype, bool vec) {
-    if (dtype == kF32) {
-        const float* p = static_cast<const float*>(base) + i;
-        if (vec) return ONCE ? __ldcs(reinterpret_cast<const float4*>(p)) : __ldg(reinterpret_cast<const float4*>(p));
-        return make_float4(p[0], p[1], p[2], p[3]);
+// 16 bytes of a row at element i, as they lie in memory: the loads of a thread are all on their way before the first is
+// widened. They are not read again, so that the cache lines give way first.
+template <int IN>
+__device__ __forceinline__ uint4 load16(const void* base, int64_t i, bool vec) {
+    if (IN == kF32) {
+        const uint32_t* p = static_cast<const uint32_t*>(base) + i;
+        return vec ? __ldcs(reinterpret_cast<const uint4*>(p)) : make_uint4(p[0], p[1], p[2], p[3]);
     }
     const uint16_t* p = static_cast<const uint16_t*>(base) + i;
-    uint32_t lo, hi;
-    if (vec) {
-        const uint2 w = ONCE ? __ldcs(reinterpret_cast<const uint2*>(p)) : __ldg(reinterpret_cast<const uint2*>(p));
-        lo = w.x, hi = w.y;
+    if (vec) return __ldcs(reinterpret_cast<const uint4*>(p));
+    return make_uint4(p[0] | ((uint32_t)p[1] << 16), p[2] | ((uint32_t)p[3] << 16), p[4] | ((uint32_t)p[5] << 16), p[6] | ((uint32_t)p[7] << 16));
+}
+
+__device__ __forceinline__ float2 widen16(uint32_t v, int dtype) {
+    if (dtype == kF16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+}
+
+template <int IN, int V>
+__device__ __forceinline__ void widen(const uint4& w, float (&x)[V]) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (V == 4) {
+            x[i] = __uint_as_float(u[i]);
+        } else {
+            const float2 f = widen16(u[i], IN);
+            x[2 * i % V] = f.x, x[(2 * i + 1) % V] = f.y;
+        }
+    }
+}
+
+// N values of a cosine or sine row.
+template <int N>
+__device__ __forceinline__ void load_angles(const float* p, bool vec, float (&x)[N]) {
+    if (!vec) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = __ldg(p + i);
+    } else if (N == 2) {
+        const float2 f = __ldg(reinterpret_cast<const float2*>(p));
+        x[0] = f.x, x[1] = f.y;
     } else {
-        lo = p[0] | ((uint32_t)p[1] << 16), hi = p[2] | ((uint32_t)p[3] << 16);
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(p + i));
+            x[i] = f.x, x[i + 1] = f.y, x[(i + 2) % N] = f.z, x[(i + 3) % N] = f.w;
+        }
     }
-    if (dtype == kF16) {
-        const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo)), b = __half22float2(*reinterpret_cast<__half2*>(&hi));
-        return make_float4(a.x, a.y, b.x, b.y);
-    }
-    return make_float4(__uint_as_float(lo << 16), __uint_as_float(lo & 0xFFFF0000u), __uint_as_float(hi << 16),
-                       __uint_as_float(hi & 0xFFFF0000u));
 }
 
 __device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
@@ -52,12 +81,21 @@ __device__ __forceinline__ uint32_t pack16(float a, float b, int dtype) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Four values at element i of a 16-byte aligned tensor (i a multiple of 4).
-__device__ __forceinline__ void store4(void* base, int64_t i, int dtype, float4 x) {
-    if (dtype == kF32) *reinterpret_cast<float4*>(static_cast<float*>(base) + i) = x;
-    else
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(base) + i) =
-            make_uint2(pack16(x.x, x.y, dtype), pack16(x.z, x.w, dtype));
+// V values at element i (a multiple of V) of a 16-byte aligned tensor.
+template <int V>
+__device__ __forceinline__ void store_values(void* base, int64_t i, int dtype, const float (&x)[V]) {
+    if (dtype == kF32) {
+        float4* const o = reinterpret_cast<float4*>(static_cast<float*>(base) + i);
+#pragma unroll
+        for (int j = 0; j < V; j += 4) o[j / 4] = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+        return;
+    }
+    uint32_t w[V / 2];
+#pragma unroll
+    for (int j = 0; j < V / 2; ++j) w[j] = pack16(x[2 * j], x[2 * j + 1], dtype);
+    uint16_t* const o = static_cast<uint16_t*>(base) + i;
+    if (V == 4) *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+    else *reinterpret_cast<uint4*>(o) = make_uint4(w[0], w[1], w[2 % (V / 2)], w[3 % (V / 2)]);
 }
 
 __device__ __forceinline__ void rotate(float& a, float& b, float c, float s) {
@@ -71,57 +109,62 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-__device__ __forceinline__ uint32_t codes4(float4 x, float inv) {
+__device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
     // 1.5 * 2^23 more rounds |x inv| <= 127 to the nearest integer (ties to even) and leaves it in the low byte
     auto code = [&](float y) { return __float_as_uint(__fadd_rn(__fmul_rn(y, inv), 12582912.0f)); };
-    return prmt(prmt(code(x.x), code(x.y), 0x0040u), prmt(code(x.z), code(x.w), 0x0040u), 0x5410u);
+    return prmt(prmt(code(x[0]), code(x[1]), 0x0040u), prmt(code(x[2]), code(x[3]), 0x0040u), 0x5410u);
 }
 
-// LANES threads (a power of two >= d / 8) take a row: lane l holds elements 4l..4l+3 of each half, so that a pair of either
-// rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head) with the heads of q, then
-// k, then v. A
-// thread has one row (two or three in flight: 2048 tokens 16.5 / 18.5 against 14.5 us); instructions bind next to HBM, so
-// that divisions are products and codes are rounded by an addition.
-template <int LANES>
+// LANES threads (a power of two >= d / 2V) take a row: lane l holds the V elements from Vl of each half, 16 bytes of the input,
+// so that a pair of either rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head)
+// with the heads of q, then k, then v. A thread has one row (two or three in flight: 2048 tokens 16.5 / 18.5 against 14.5 us);
+// instructions bind next to HBM, so that divisions are products, codes are rounded by an addition, and the input's type is
+// the kernel's (widened as it came, in pieces of eight bytes, bf16 rows of 8800 tokens took 61.5 us into a bf16 cache, not 42.8).
+template <int LANES, int IN>
 __global__ void __launch_bounds__(KW_THREADS) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
+    constexpr int V = IN == kF32 ? 4 : 8;
     const uint32_t lane = threadIdx.x % LANES, r = blockIdx.x * (KW_THREADS / LANES) + threadIdx.x / LANES;
     const uint32_t heads = p.q_heads + 2 * p.c.heads, half = p.c.d / 2;
-    const bool live = r < rows, active = live && lane * 8 < p.c.d;
+    const bool live = r < rows, active = live && lane * (2 * V) < p.c.d;
     const uint32_t in_launch = p.by_heads.quotient(r), t = token0 + in_launch, head = r - in_launch * heads;
     const bool is_q = head < p.q_heads, is_v = head >= p.q_heads + p.c.heads;
     const uint32_t h = head - (is_q ? 0 : is_v ? p.q_heads + p.c.heads : p.q_heads);
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    float a[V] = {}, b[V] = {};
     int32_t slot = 0;
     if (active) {
         const RowsView& in = is_q ? p.q : is_v ? p.v : p.k;
-        const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * 4;
-        a = load4<true>(in.p, at, p.dtype, p.vec);
-        b = load4<true>(in.p, at + half, p.dtype, p.vec);
+        const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * V;
+        const uint4 wa = load16<IN>(in.p, at, p.vec), wb = load16<IN>(in.p, at + half, p.vec);
         if (!is_q) slot = __ldg(p.slots + t);
-        if (p.cos != nullptr && !is_v) {
-            const int64_t row = (int64_t)min((uint32_t)max(__ldg(p.positions + t), 0), p.rope_len - 1) * half;
-            if (p.interleaved) {
-                const int64_t i0 = row + lane * 2, i1 = i0 + half / 2;
-                rotate(a.x, a.y, __ldg(p.cos + i0), __ldg(p.sin + i0));
-                rotate(a.z, a.w, __ldg(p.cos + i0 + 1), __ldg(p.sin + i0 + 1));
-                rotate(b.x, b.y, __ldg(p.cos + i1), __ldg(p.sin + i1));
-                rotate(b.z, b.w, __ldg(p.cos + i1 + 1), __ldg(p.sin + i1 + 1));
-            } else {
-                const float4 c = load4<false>(p.cos, row + lane * 4, kF32, p.vec), s = load4<false>(p.sin, row + lane * 4, kF32, p.vec);
-                rotate(a.x, b.x, c.x, s.x);
-                rotate(a.y, b.y, c.y, s.y);
-                rotate(a.z, b.z, c.z, s.z);
-                rotate(a.w, b.w, c.w, s.w);
-            }
+        const bool rotated = p.cos != nullptr && !is_v;
+        const int64_t row = rotated ? (int64_t)min((uint32_t)max(__ldg(p.positions + t), 0), p.rope_len - 1) * half : 0;
+        if (!rotated) {
+            widen<IN>(wa, a), widen<IN>(wb, b);
+        } else if (p.interleaved) {
+            const int64_t i0 = row + lane * (V / 2), i1 = i0 + half / 2;
+            float c0[V / 2], s0[V / 2], c1[V / 2], s1[V / 2];
+            load_angles(p.cos + i0, p.vec, c0), load_angles(p.sin + i0, p.vec, s0);
+            load_angles(p.cos + i1, p.vec, c1), load_angles(p.sin + i1, p.vec, s1);
+            widen<IN>(wa, a), widen<IN>(wb, b);
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) rotate(a[2 * i], a[2 * i + 1], c0[i], s0[i]), rotate(b[2 * i], b[2 * i + 1], c1[i], s1[i]);
+        } else {
+            float c[V], s[V];
+            load_angles(p.cos + row + lane * V, p.vec, c), load_angles(p.sin + row + lane * V, p.vec, s);
+            widen<IN>(wa, a), widen<IN>(wb, b);
+#pragma unroll
+            for (int i = 0; i < V; ++i) rotate(a[i], b[i], c[i], s[i]);
         }
     }
-    if (is_q) {
-        if (active) {
-            const int64_t at = ((int64_t)t * p.q_heads + h) * p.c.d + lane * 4;
-            store4(p.q_out, at, p.q_out_dtype, a);
-            store4(p.q_out, at + half, p.q_out_dtype, b);
-        }
-        if (p.c.dtype != kInt8) return;
+    if (is_q && active) {
+        const int64_t at = ((int64_t)t * p.q_heads + h) * p.c.d + lane * V;
+        store_values(p.q_out, at, p.q_out_dtype, a);
+        store_values(p.q_out, at + half, p.q_out_dtype, b);
+    }
+    if (p.c.dtype != kInt8) {
+        if (is_q) return;
+    } else if (__all_sync(0xFFFFFFFFu, is_q)) {  // (a warp that goes on shuffles as a whole)
+        return;
     }
     const bool wanted = active && !is_q && slot >= 0 && (uint64_t)slot < (uint64_t)p.c.pages * p.c.page_size;
     const uint32_t page = p.by_page.quotient((uint32_t)slot & 0x7FFFFFFFu);
@@ -129,40 +172,58 @@ __global__ void __launch_bounds__(KW_THREADS) kv_write_kernel(const __grid_const
     void* const cache = is_v ? p.c.v : p.c.k;
     if (p.c.dtype != kInt8) {
         if (wanted) {
-            store4(cache, row * p.c.d + lane * 4, p.c.dtype, a);
-            store4(cache, row * p.c.d + lane * 4 + half, p.c.dtype, b);
+            store_values(cache, row * p.c.d + lane * V, p.c.dtype, a);
+            store_values(cache, row * p.c.d + lane * V + half, p.c.dtype, b);
         }
         return;
     }
-    // (the whole warp shuffles)
-    float m = max_nan(max_nan(max_nan(fabsf(a.x), fabsf(a.y)), max_nan(fabsf(a.z), fabsf(a.w))),
-                      max_nan(max_nan(fabsf(b.x), fabsf(b.y)), max_nan(fabsf(b.z), fabsf(b.w))));
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) m = max_nan(m, max_nan(fabsf(a[i]), fabsf(b[i])));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
     if (!wanted) return;
     const bool finite = m < __int_as_float(0x7F800000), zero = m < MIN_AMAX;
     const float inv = finite && !zero ? __fdiv_rn(127.0f, m) : 0.0f;
-    int8_t* const dst = static_cast<int8_t*>(cache) + row * p.c.d + lane * 4;
-    *reinterpret_cast<uint32_t*>(dst) = finite ? codes4(a, inv) : 0u;
-    *reinterpret_cast<uint32_t*>(dst + half) = finite ? codes4(b, inv) : 0u;
+    int8_t* const dst = static_cast<int8_t*>(cache) + row * p.c.d + lane * V;
+    uint32_t code[V / 2];
+#pragma unroll
+    for (int i = 0; i < V; i += 4) code[i / 4] = finite ? codes4(a + i, inv) : 0u, code[(V + i) / 4] = finite ? codes4(b + i, inv) : 0u;
+    if (V == 4) {
+        *reinterpret_cast<uint32_t*>(dst) = code[0];
+        *reinterpret_cast<uint32_t*>(dst + half) = code[1];
+    } else {
+        *reinterpret_cast<uint2*>(dst) = make_uint2(code[0], code[1]);
+        *reinterpret_cast<uint2*>(dst + half) = make_uint2(code[2 % (V / 2)], code[3 % (V / 2)]);
+    }
     if (lane == 0)
         (is_v ? p.c.v_scale : p.c.k_scale)[row] = !finite ? __int_as_float(0x7FC00000) : zero ? 0.0f : __fdiv_rn(m, 127.0f);
 }
 
-template <int LANES>
+template <int LANES, int IN>
 cudaError_t launch_write(const KvWriteParams& p, cudaStream_t stream) {
     const uint32_t heads = p.q_heads + 2 * p.c.heads;
     const uint32_t chunk = std::max(1u, 0x7FFFFFFFu / heads);  // rows of a launch stay below 2^31
     for (uint64_t t0 = 0; t0 < p.tokens; t0 += chunk) {
         const uint32_t rows = std::min<uint64_t>(chunk, p.tokens - t0) * heads, per = KW_THREADS / LANES;
-        kv_write_kernel<LANES><<<rows / per + (rows % per != 0), KW_THREADS, 0, stream>>>(p, (uint32_t)t0, rows);
+        kv_write_kernel<LANES, IN><<<rows / per + (rows % per != 0), KW_THREADS, 0, stream>>>(p, (uint32_t)t0, rows);
     }
     return cudaGetLastError();
 }
 
+template <int IN>
+cudaError_t launch_write_of(const KvWriteParams& p, cudaStream_t stream) {
+    constexpr int MOST = IN == kF32 ? 16 : 8;  // lanes of a row of 128 elements
+    if (p.c.d > 64) return launch_write<MOST, IN>(p, stream);
+    if (p.c.d > 32) return launch_write<MOST / 2, IN>(p, stream);
+    return launch_write<MOST / 4, IN>(p, stream);
+}
+
 // ---- read ----
 // A block takes `tokens` tokens: it finds their rows in the cache, then groups of LANES threads (a power of two >= d / 8)
-// copy a row of K and V each, eight elements a thread, KR_BATCH rows' loads in flight.
+// copy a row of K and V each, eight elements a thread, KR_BATCH rows' loads in flight. An int8 cache is read at one byte for
+// two written, and the stores bind (codes widened by byte permutes instead of conversions: 96.0 us as well; stores that give
+// way in the cache: 96.6).
 constexpr int KR_MOST = 32, KR_BATCH = 4;
 
 struct Eight {
@@ -177,11 +238,6 @@ __device__ __forceinline__ Eight read8(const KvCacheView& c, const void* src, co
         e.w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(src) + row * c.d + col));
     }
     return e;
-}
-
-__device__ __forceinline__ float2 widen16(uint32_t v, int dtype) {
-    if (dtype == kF16) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
 }
 
 __device__ __forceinline__ void write8(void* out, int64_t at, int out_dtype, const Eight& e, int dtype) {
@@ -272,9 +328,8 @@ cudaError_t launch_read(const KvReadParams& p, cudaStream_t stream) {
 cudaError_t launch_kv_write(const KvWriteParams& params, cudaStream_t stream) {
     KvWriteParams p = params;
     p.by_heads = Divisor::of(p.q_heads + 2 * p.c.heads), p.by_page = Divisor::of(p.c.page_size);
-    if (p.c.d > 64) return launch_write<16>(p, stream);
-    if (p.c.d > 32) return launch_write<8>(p, stream);
-    return launch_write<4>(p, stream);
+    if (p.dtype == kF32) return launch_write_of<kF32>(p, stream);
+    return p.dtype == kF16 ? launch_write_of<kF16>(p, stream) : launch_write_of<kBf16>(p, stream);
 }
 
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream) {
