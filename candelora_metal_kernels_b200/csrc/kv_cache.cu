@@ -6,8 +6,8 @@
 // with every product and sum rounded by itself in f32, so that a result does not depend on how the compiler fuses.
 // int8 rows (one token and head): m = max |x|, scale = m / 127, code = rint(x * (127 / m)); m < 2^-100 gives zeros (the
 // quotient would overflow), and a row with an infinity or NaN gets a NaN scale, so that it reads back as NaN.
-// Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 13.2 us, 5820 GB/s of bytes in
-// and out; of 8800 tokens, f32 into an int8 cache, with the read back 66.8 us, 5430 GB/s; read of 89091 tokens of an int8 cache
+// Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 12.8 to 13.3 us, 5980 GB/s at best of bytes in
+// and out; of 8800 tokens, f32 into an int8 cache, with the read back 66.9 us, 5420 GB/s; read of 89091 tokens of an int8 cache
 // to bf16 96 us, 5750 GB/s.
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"
@@ -119,9 +119,11 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
 // so that a pair of either rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head)
 // with the heads of q, then k, then v. A thread has one row (two or three in flight: 2048 tokens 16.5 / 18.5 against 14.5 us);
 // instructions bind next to HBM, so that divisions are products, codes are rounded by an addition, and the input's type is
-// the kernel's (widened as it came, in pieces of eight bytes, bf16 rows of 8800 tokens took 61.5 us into a bf16 cache, not 42.8).
+// the kernel's (widened as it came, in pieces of eight bytes, bf16 rows of 8800 tokens took 61.5 us into a bf16 cache, not 43.6).
+// Blocks of an SM: eight for f32 rows (8800 tokens into a bf16 cache 54.0 us; with all the registers that the compiler likes
+// 58.8), six for the 16 values of a thread that 16-bit rows make (43.6 us; five 45.0, seven 44.9, with spills).
 template <int LANES, int IN>
-__global__ void __launch_bounds__(KW_THREADS) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
+__global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
     constexpr int V = IN == kF32 ? 4 : 8;
     const uint32_t lane = threadIdx.x % LANES, r = blockIdx.x * (KW_THREADS / LANES) + threadIdx.x / LANES;
     const uint32_t heads = p.q_heads + 2 * p.c.heads, half = p.c.d / 2;
