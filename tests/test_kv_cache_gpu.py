@@ -80,6 +80,24 @@ def test_write_strided_and_unaligned_rows(pad):
     assert torch.equal(at_slots(cache.v, pos), v.cpu().half())
 
 
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("pad", [0, 8, 4, 1])
+def test_write_16_bit_rows_off_the_boundaries(pad, dtype, pairs):
+    """16-bit slices of one projection that start on multiples of 16, 8 or 2 bytes: the same values, and codes, from all."""
+    hq, hkv, d, tokens = 4, 2, 96, 21
+    rows = randn((tokens, (hq + 2 * hkv) * d + pad), 2).to(dtype).cuda()
+    q, k, v = (x.unflatten(1, (-1, d)) for x in rows[:, pad:].split([hq * d, hkv * d, hkv * d], 1))
+    slots = torch.arange(tokens, dtype=torch.int32).cuda()
+    cos, sin = (x.cuda() for x in tables(40, d))
+    cache = c.KvCache.empty(3, hkv, 8, d, I8)
+    out = c.kv_cache_write(cache, k, v, slots, q=q, positions=slots, cos=cos, sin=sin, interleaved=pairs, q_dtype=F32)
+    pos = slots.cpu()
+    assert torch.equal(out.cpu(), ref.rotated(q.cpu().float(), pos, cos.cpu(), sin.cpu(), pairs))
+    for got, x in ((cache.k, ref.rotated(k.cpu().float(), pos, cos.cpu(), sin.cpu(), pairs)), (cache.v, v.cpu().float())):
+        assert torch.equal(at_slots(got, pos), ref.quantised(x)[0])
+
+
 def test_write_rows_that_do_not_quantise():
     """Zeros, subnormal rows, infinities and NaN."""
     x = randn((6, 1, 64), 1)
