@@ -5,8 +5,8 @@
 // key head packed beside each other (TPT = 128 / G tokens a tile), so that each K and V tile that is loaded serves all of
 // them and short prompts still fill the rows. Over tiles of 128 keys, with the running maximum and sum of a softmax:
 //   S_i = Q_i K^T   tcgen05.mma, M = N = 128, into TMEM (f32)                          one MMA warp for both tiles
-//   P_i = 2^(c S - m), rounded to the inputs' 16-bit type (one unit of 2^-8 or 2^-11, as the output's own rounding),
-//         written over S_i in TMEM; the sum is of the f32 values                        a warpgroup a tile, a thread a row
+//   P_i = 2^(c S - m), rounded to the inputs' 16-bit type (by 2^-8 or 2^-11 of itself, as the output's own rounding; f16 see
+//         below), written over S_i in TMEM; the sum is of the f32 values                a warpgroup a tile, a thread a row
 //   O_i += P_i V    tcgen05.mma with A = P_i from TMEM, V as the N-major operand
 // The two tiles alternate on the tensor core: while one warpgroup computes its exponentials the other's products run.
 // K and V tiles arrive by TMA (128-byte swizzle, no multicast) in one ring, K_0 V_0 K_1 V_1 ..., across items.
@@ -14,8 +14,11 @@
 //     line, of which each block takes an equal contiguous part (short calls: whole items, see Work). A part that is
 //     not a whole item leaves (o, m, l) in the workspace, unless it is the item's last one: that adds the parts up
 //     (attention_parts.cuh), beside the other blocks' work and without a launch or a wait of its own.
-//   * Lazy rescaling: the reference m of a row moves only when a score exceeds it by more than 2^8 (p stays below 256,
-//     far inside both types' range), so O in TMEM is rescaled a few times a row instead of once a tile.
+//   * Lazy rescaling: the reference m of a row moves only when a score exceeds it by more than 2^8 (bf16) or 2^4 (f16), so
+//     that O in TMEM is rescaled a few times a row instead of once a tile. f16 has no exponents to spare: where one token
+//     takes nearly all of a row's weight, the output may be made of p far below it. So p is 2^11 at the reference (2^15 at
+//     most) and keeps its eleven bits down to 2^-25 of the row's largest, 17.3 nats; below that its last bit is 2^-35 of the
+//     largest. 512 tokens after 7001 in f16 take 274 us with this, 264 with 2^8 above 2^7, 282 with 2^2 above 2^13.
 //   * Masked keys are replaced by -inf before the maximum (never added to), so that whatever K holds there cannot matter.
 //     V needs more, since 0 * NaN is NaN: two guard warps look through the V tiles that hold keys some row does not see.
 //     Rows past the last visible key (other sequences' tokens) become zeros; infinities and NaN of keys that only some
@@ -42,7 +45,11 @@ namespace {
 constexpr int AP_ROWS = 128, AP_KEYS = 128;
 constexpr int AP_MMA_WARP = 8, AP_TMA_WARP = 9, AP_GUARD_WARP = 10, AP_THREADS = 12 * 32;  // warps 0-7: softmax
 constexpr uint32_t AP_LOAD = 0x100u, AP_RELEASE = 0x200u, AP_PROB = 0x400u, AP_PRODUCT = 0x800u;  // status bits
-constexpr float AP_LAZY = 8.0f;  // how far (in powers of two) a score may exceed its row's reference
+// In powers of two: how far a score may exceed its row's reference, and p at the reference (f16: together below its 2^16).
+template <bool BF>
+constexpr float ap_lazy = BF ? 8.f : 4.f;
+template <bool BF>
+constexpr float ap_top = BF ? 0.f : 11.f;
 constexpr int AP_FIRST = 6;      // of the eight steps of 16 keys of P V, those that begin before the rest of P is there
 constexpr int AP_ITEM_ROWS = 2 * AP_ROWS;
 // Keys' time that an item costs besides its keys, and that leaving and joining a part costs. Measured: 16384 tokens
@@ -736,7 +743,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) tops[x] = fmaxf(fmaxf(tops[x], s[c + x]), s[c + x + 4]);
                 const float top = fmaxf(fmaxf(fmaxf(tops[0], s[124]), fmaxf(tops[1], s[125])), fmaxf(fmaxf(tops[2], s[126]), fmaxf(tops[3], s[127])));
-                const bool move = (top - m) * p.c > AP_LAZY || (m == -INFINITY && top > m);
+                const bool move = (top - m) * p.c > ap_lazy<BF> || (m == -INFINITY && top > m);
                 if (__any_sync(0xFFFFFFFFu, move)) {
                     const float next = fmaxf(m, top), keep = next == m ? 1.f : ex2((m - next) * p.c);
                     m = next;
@@ -753,7 +760,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                         tmem_st16(o_col(i) + lanes + c, bits);
                     }
                 }
-                const float base = m == -INFINITY ? 0.f : m * p.c;
+                const float base = m == -INFINITY ? 0.f : m * p.c - ap_top<BF>;
                 const uint64_t base2 = pair(-base, -base);
                 uint64_t sums[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
