@@ -13,16 +13,19 @@
 //   O = P V     rows 0-7: the high pieces of p, rows 8-15: the low pieces
 // so the second piece, which gives f32 activations 22 bits (f16 pieces) or 16 (bf16 pieces), costs no instruction.
 //   * bf16 caches take bf16 pieces (their range); f16 and int8 caches f16 pieces of q / 2^e, 2^e the power of two above
-//     the head's largest |q|: pieces of at least 22 bits at any magnitude.
+//     the head's largest |q|. A low piece is held times 2^11, which the sum of the two rows takes off, so that it is not
+//     held among f16's smallest numbers; and the largest p is 2^7 to 2^15. So q keeps 22 bits down to 2^-14 of the head's
+//     largest and p (times its value scale) down to 2^-21 of the largest, and what is smaller is off by no more than 2^-36 and
+//     2^-43 of those: a token that takes all of the weight leaves the others' digits as they are (2^-25 without the two).
 //   * A bf16 cache under f32 activations takes a third piece (a second pair of products), or p would end at 2^-17.
 //   * int8 codes: the byte code + 128 with a zero byte above it is the f16 number (code + 128) 2^-24 (a subnormal, exact and
 //     full speed in the matrix instructions), so a pair costs half an exclusive or and one byte permute. The 128s are taken
 //     off as products with the constant 128 2^-24: S starts from minus them, O has them as one more column of P V. The
 //     sums are some four times as large for it, which f32 activations would notice (8e-6 against 1e-6 over the whole):
 //     for those a byte with 0x64 above it is 1024 + code + 128, and a subtraction makes it the code itself.
-//   * The key scale multiplies s, the value scale multiplies p. The reference m of a head's exponents moves when a product
-//     p w exceeds 2^8 (it starts where the first tile's largest is 1), so that p w keeps to the range of f16; the sum of p
-//     itself is f32.
+//   * The key scale multiplies s, the value scale w multiplies p. The reference m of a head's exponents moves when a product
+//     p w has grown by more than 2^8, so that p w keeps to the range of f16; the sum of p itself is f32 (int8 caches: held by
+//     2^-16 of itself, since p alone may reach 2^115).
 // The maxima, sums, s, p and o are f32.
 //
 // Measured (8 key heads, 128 elements): 128 sequences of up to 4096 tokens, bf16 cache, 214 us: 6260 GB/s, 0.96 of the copy
@@ -46,7 +49,14 @@ constexpr int AD_HEADS = 8;                     // query heads of an item
 // 1 x 100001 49.7 / 48.6 / 47.9 us.
 constexpr uint32_t AD_ITEM_COST = 3;
 constexpr float AD_MIN_SCALE = 7.88860905e-31f;  // 2^-100: the smallest value scale (a row held as zeros has 0)
-constexpr float AD_LAZY = 256.f;                 // how far p times the value scale may grow before the reference moves
+// p times the value scale: the power of two that it has at the reference, and how far it may grow before that moves.
+template <bool BF>
+constexpr float AD_TOP = BF ? 0.f : 7.f;
+template <bool BF>
+constexpr float AD_LAZY = BF ? 256.f : 32768.f;
+template <bool BF>
+constexpr float AD_LOW = BF ? 1.f : 2048.f;      // what low pieces are held times
+constexpr float AD_SUM = 1.f / 65536.f;          // int8 caches: what the sums of p, and with them o, are held times
 constexpr uint32_t CODE_ZERO = 0x00800080u;      // two codes of 0 as f16: 128 2^-24
 constexpr float CODE_UNIT = 16777216.f;          // 2^24
 constexpr float LOG2E = 1.44269504f;
@@ -413,7 +423,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                 for (int piece = 0; piece < S::PIECES; ++piece) {
                     const uint32_t h = pack_pair<BF>(rest, 0.f);
                     q[piece * DP + lane + i * 32] = (uint16_t)h;
-                    rest -= unpack_pair<BF>(h).x;
+                    rest = (rest - unpack_pair<BF>(h).x) * AD_LOW<BF>;
                 }
             }
             if (lane == 0) q_factor[warp] = p.scale * LOG2E * up * (SHIFTED ? CODE_UNIT : 1.f);
@@ -434,6 +444,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) minus[j] = -minus[j];
+        auto joined = [](float high, float low) { return fmaf(low, 1.f / AD_LOW<BF>, high); };
         const float factor = q_factor[g];
         float o[NT][4], o_off[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -496,7 +507,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                     ks2 = make_float2(sk.x * factor, sk.y * factor);
                     vs2 = make_float2(max_nan(sv.x, AD_MIN_SCALE), max_nan(sv.y, AD_MIN_SCALE));
                 }
-                x[n][0] = (s[n][0] + s[n][2]) * ks2.x, x[n][1] = (s[n][1] + s[n][3]) * ks2.y;
+                x[n][0] = joined(s[n][0], s[n][2]) * ks2.x, x[n][1] = joined(s[n][1], s[n][3]) * ks2.y;
                 vs[n][0] = vs2.x, vs[n][1] = vs2.y;
             }
             if (here != ALL) {
@@ -508,7 +519,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             }
             // The reference does as a rule: the products are made with it, and made again in the rare case that it moves.
             for (;;) {
-                const float base = m == -INFINITY ? 0.f : m;
+                const float base = m == -INFINITY ? 0.f : m - AD_TOP<BF>;
                 float top = 0.f;
 #pragma unroll
                 for (int n = 0; n < ST; ++n)
@@ -518,7 +529,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                         w[n][j] = I8 ? e[n][j] * vs[n][j] : e[n][j];
                         top = fmaxf(top, w[n][j]);
                     }
-                if (!__any_sync(0xFFFFFFFFu, top > AD_LAZY || m == -INFINITY)) break;
+                if (!__any_sync(0xFFFFFFFFu, top > AD_LAZY<BF> || m == -INFINITY)) break;
                 // the largest x + log2(value scale) of the head's tokens
                 float most = -INFINITY;
 #pragma unroll
@@ -544,10 +555,10 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             uint32_t pa[TOK / 16][4], pa3[TOK / 16][4];
 #pragma unroll
             for (int n = 0; n < ST; ++n) {
-                l += e[n][0] + e[n][1];
+                l = fmaf(e[n][0] + e[n][1], I8 ? AD_SUM : 1.f, l);
                 const uint32_t high = pack_pair<BF>(w[n][0], w[n][1]);
                 const float2 h = unpack_pair<BF>(high);
-                const uint32_t low = pack_pair<BF>(w[n][0] - h.x, w[n][1] - h.y);
+                const uint32_t low = pack_pair<BF>((w[n][0] - h.x) * AD_LOW<BF>, (w[n][1] - h.y) * AD_LOW<BF>);
                 pa[n / 2][(n % 2) * 2] = high;
                 pa[n / 2][(n % 2) * 2 + 1] = low;
                 if (THIRD) {
@@ -589,11 +600,11 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             __syncwarp();
             stage = stage == AD_STAGES - 1 ? 0 : stage + 1;
         }
-        if (SHIFTED) {  // the 128s off, and the codes' unit on
+        if (I8) {  // the 128s off, and the codes' unit and the sums' on
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[n][j] = (o[n][j] - o_off[j]) * CODE_UNIT;
+                for (int j = 0; j < 4; ++j) o[n][j] = SHIFTED ? (o[n][j] - o_off[j]) * (CODE_UNIT * AD_SUM) : o[n][j] * AD_SUM;
         }
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
@@ -608,8 +619,8 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             for (int n = 0; n < NT; ++n) {
                 // int8: accumulator columns are the even and odd dimensions of a 16-dimension chunk
                 const uint32_t e0 = KIND == CK_INT8 ? (n / 2) * 16 + n % 2 + t * 4 : n * 8 + t * 2, e1 = e0 + (KIND == CK_INT8 ? 2 : 1);
-                slot[g * DP + e0] = o[n][0] + o[n][2];
-                slot[g * DP + e1] = o[n][1] + o[n][3];
+                slot[g * DP + e0] = joined(o[n][0], o[n][2]);
+                slot[g * DP + e1] = joined(o[n][1], o[n][3]);
             }
             if (t == 0) slot[AD_HEADS * DP + g] = m, slot[AD_HEADS * DP + AD_HEADS + g] = l;
         };
@@ -623,8 +634,8 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint32_t e0 = KIND == CK_INT8 ? (n / 2) * 16 + n % 2 + t * 4 : n * 8 + t * 2, e1 = e0 + (KIND == CK_INT8 ? 2 : 1);
-                o[n][0] = (o[n][0] + o[n][2]) * f1 + slot[g * DP + e0] * f2, o[n][2] = 0.f;
-                o[n][1] = (o[n][1] + o[n][3]) * f1 + slot[g * DP + e1] * f2, o[n][3] = 0.f;
+                o[n][0] = joined(o[n][0], o[n][2]) * f1 + slot[g * DP + e0] * f2, o[n][2] = 0.f;
+                o[n][1] = joined(o[n][1], o[n][3]) * f1 + slot[g * DP + e1] * f2, o[n][3] = 0.f;
             }
             __syncwarp();
             put(slot);
