@@ -21,8 +21,10 @@
 //   * int8 codes: the byte code + 128 with a zero byte above it is the f16 number (code + 128) 2^-24 (a subnormal, exact and
 //     full speed in the matrix instructions), so a pair costs half an exclusive or and one byte permute. The 128s are taken
 //     off as products with the constant 128 2^-24: S starts from minus them, O has them as one more column of P V. The
-//     sums are some four times as large for it, which f32 activations would notice (8e-6 against 1e-6 over the whole):
-//     for those a byte with 0x64 above it is 1024 + code + 128, and a subtraction makes it the code itself.
+//     sums are some four times as large for it (hundreds of times where one channel of q stands far above the others and
+//     the keys have little there), which the 2^-8 of bf16 activations hides. For f32 and f16 ones (8e-6 against 1e-6 over
+//     the whole) a byte with 0x64 above it is 1024 + code + 128, and a subtraction makes it the code itself: 51.0 instead of
+//     49.2 us for 100001 tokens.
 //   * The key scale multiplies s, the value scale w multiplies p. The reference m of a head's exponents moves when a product
 //     p w has grown by more than 2^8, so that p w keeps to the range of f16; the sum of p itself is f32 (int8 caches: held by
 //     2^-16 of itself, since p alone may reach 2^115).
@@ -222,7 +224,7 @@ template <int DP, int KIND, bool WIDE>
 __global__ void __launch_bounds__(AD_THREADS, 1)
     decode_kernel(const __grid_constant__ DecodeArgs a) {
     using S = DecodeShape<DP, KIND, WIDE>;
-    // WIDE: f32 activations
+    // WIDE: f32 activations, and f16 ones over int8 codes
     constexpr bool BF = KIND == CK_BF16, I8 = KIND == CK_INT8, THIRD = BF && WIDE, SHIFTED = I8 && !WIDE;
     constexpr int TOK = S::TOK, UNIT = S::UNIT, NT = DP / 8, KS = DP / 16, ST = TOK / 8;
     constexpr uint32_t ALL = TOK == 32 ? 0xFFFFFFFFu : (1u << TOK) - 1;
@@ -743,7 +745,7 @@ cudaError_t launch(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
 template <int DP>
 cudaError_t launch_kind(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
     const bool wide = a.p.dtype == kF32;
-    if (a.p.c.dtype == kInt8) return wide ? launch<DP, CK_INT8, true>(a, blocks, stream) : launch<DP, CK_INT8, false>(a, blocks, stream);
+    if (a.p.c.dtype == kInt8) return a.p.dtype != kBf16 ? launch<DP, CK_INT8, true>(a, blocks, stream) : launch<DP, CK_INT8, false>(a, blocks, stream);
     if (a.p.c.dtype == kF16) return launch<DP, CK_F16, false>(a, blocks, stream);
     return wide ? launch<DP, CK_BF16, true>(a, blocks, stream) : launch<DP, CK_BF16, false>(a, blocks, stream);
 }

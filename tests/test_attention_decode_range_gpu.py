@@ -50,7 +50,7 @@ def test_decode_sink(tokens, dtype, cache_dtype, gap):
 
 
 @pytest.mark.parametrize("cache_dtype", [F16, I8])
-@pytest.mark.parametrize("dtype", [F32])
+@pytest.mark.parametrize("dtype", [F32, F16])
 def test_decode_small_channels_beside_a_large_one(dtype, cache_dtype):
     """One channel of q is 2^12 and no key has anything there: the scores are made of the other channels."""
     gen = torch.Generator().manual_seed(3)
