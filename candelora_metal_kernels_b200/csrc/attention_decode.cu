@@ -27,7 +27,7 @@
 //     49.2 us for 100001 tokens.
 //   * The key scale multiplies s, the value scale w multiplies p. The reference m of a head's exponents moves when a product
 //     p w has grown by more than 2^8, so that p w keeps to the range of f16; the sum of p itself is f32 (int8 caches: held by
-//     2^-16 of itself, since p alone may reach 2^115).
+//     2^-16 of itself, since p alone may reach 2^122).
 // The maxima, sums, s, p and o are f32.
 //
 // Measured (8 key heads, 128 elements): 128 sequences of up to 4096 tokens, bf16 cache, 214 us: 6260 GB/s, 0.96 of the copy
@@ -50,7 +50,9 @@ constexpr int AD_HEADS = 8;                     // query heads of an item
 // Units' time that starting and ending an item costs. Measured with 1 / 2 / 3: 128 x 4096 tokens 219 / 216 / 214 us,
 // 1 x 100001 49.7 / 48.6 / 47.9 us.
 constexpr uint32_t AD_ITEM_COST = 3;
-constexpr float AD_MIN_SCALE = 7.88860905e-31f;  // 2^-100: the smallest value scale (a row held as zeros has 0)
+// 2^-107, just below the smallest value scale that a row of the cache has (its largest value, 2^-100 or more, over 127). A row of
+// zeros has 0 and counts as this, so that the reference stays finite; its codes are zeros.
+constexpr float AD_MIN_SCALE = 6.16297582e-33f;
 // p times the value scale: the power of two that it has at the reference, and how far it may grow before that moves.
 template <bool BF>
 constexpr float AD_TOP = BF ? 0.f : 7.f;
