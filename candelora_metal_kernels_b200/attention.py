@@ -217,7 +217,7 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     """softmax(scale q k^T) v of packed sequences: q [q_tokens, q_heads, head_dim], k, v [k_tokens, kv_heads, head_dim],
     f16 or bf16, sequence b holding the rows [cu_seqlens[b], cu_seqlens[b + 1]) (int32; cu_seqlens_k: those of q). With
     `causal`, query i of Lq sees the keys j <= i + Lk - Lq of Lk. scale: 1 / sqrt(head_dim) by default. Queries that see
-    no key give zeros. Returns q's shape and dtype."""
+    no key give zeros, and rows of no sequence are zeros. Returns q's shape and dtype."""
     op = "attention_prefill"
     if not q.is_cuda:
         _bail(_lib.IQ2_ERR_DEVICE, f"{op} requires a CUDA device")

@@ -653,6 +653,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
         } else {
             const uint32_t tid = threadIdx.x - AP_GUARD_WARP * 32;
+            // rows of no sequence (before the first or after the last one) are zeros
+            const uint32_t first = (uint32_t)min(max(__ldg(p.cu_q), 0), (int32_t)p.q_tokens);
+            const uint32_t last_end = (uint32_t)min(max(__ldg(p.cu_q + p.seqs), 0), (int32_t)p.q_tokens);
+            const uint32_t row_chunks = p.q_heads * (p.d / 8);  // of 16 bytes
+#pragma unroll 1
+            for (uint32_t r = blockIdx.x; r < first + (p.q_tokens - last_end); r += gridDim.x) {
+                uint4* const out = static_cast<uint4*>(p.out) + (int64_t)(r < first ? r : last_end + (r - first)) * row_chunks;
+#pragma unroll 1
+                for (uint32_t x = tid; x < row_chunks; x += 64) out[x] = make_uint4(0, 0, 0, 0);
+            }
             uint32_t vs = 1, v_lap = 0, guards = 0;
             bool ok = true;
             Part w;

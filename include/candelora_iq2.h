@@ -335,7 +335,7 @@ typedef struct iq2_attention_prompts {
     iq2_rows q, k, v;            /* f16 or bf16 (dtype); 16-byte aligned, strides multiples of 8  */
     int dtype;
     uint32_t sequences, q_tokens, k_tokens, q_heads, kv_heads, head_dim;
-    const int32_t* cu_seqlens_q; /* [sequences + 1], ascending from 0                            */
+    const int32_t* cu_seqlens_q; /* [sequences + 1], ascending                                   */
     const int32_t* cu_seqlens_k;
     int causal;                  /* key j is seen by query i when j <= i + Lk - Lq               */
     float scale;                 /* of q . k; 0: 1 / sqrt(head_dim)                              */
@@ -347,7 +347,8 @@ size_t iq2_attention_prefill_workspace_size(const iq2_attention_prompts* prompts
 
 /*
  * out = softmax(scale q k^T) v for every sequence, f32 statistics and accumulation. Keys may be
- * more than queries (a later chunk of a prompt) or fewer; a query that sees no key gets zeros.
+ * more than queries (a later chunk of a prompt) or fewer; a query that sees no key gets zeros, and
+ * so do rows of no sequence (before cu_seqlens_q[0], or from cu_seqlens_q[sequences] on).
  * What a masked key or value holds (other sequences' tokens, infinities, NaN) has no effect.
  */
 int iq2_attention_prefill(const iq2_attention_prompts* prompts, void* workspace, size_t workspace_bytes,
