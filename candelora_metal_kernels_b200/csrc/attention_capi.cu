@@ -1,7 +1,5 @@
 // C ABI of the attention operators (declared in include/candelora_iq2.h): the checks of their arguments, in the order
 // dimensions, device, types, layout, buffers; the kernels are in kv_cache.cu, attention_prefill.cu and attention_decode.cu.
-#include <atomic>
-#include <chrono>
 #include <cinttypes>
 #include <cmath>
 #include <initializer_list>
@@ -92,22 +90,6 @@ int check_workspace(const char* op, const void* workspace, size_t bytes, size_t 
 }
 
 }  // namespace
-
-namespace iq2 {
-
-uint64_t call_token() {
-    // a counter from a start of its own in every process, its bits spread (the finalizer of splitmix64): no small number, no
-    // pattern that other data in the workspace may have, never 0
-    static std::atomic<uint64_t> counter{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() ^
-                                         reinterpret_cast<uintptr_t>(&call_token)};
-    uint64_t z = counter.fetch_add(1, std::memory_order_relaxed) * 0x9E3779B97F4A7C15ull;
-    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
-    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
-    z ^= z >> 31;
-    return z != 0 ? z : 1;
-}
-
-}  // namespace iq2
 
 extern "C" {
 

@@ -26,9 +26,6 @@ struct Divisor {
 #endif
 };
 
-// A number for a call that no earlier flag in any workspace holds: flags of parts (below) are compared with it.
-uint64_t call_token();
-
 // A paged cache (iq2_kv_cache): k, v [pages][heads][page_size][d], k_scale, v_scale f32 [pages][heads][page_size]
 // for int8 codes. Token `pos` of a sequence lives in page block_table[pos / page_size], row pos % page_size.
 struct KvCacheView {

@@ -75,7 +75,7 @@ constexpr uint32_t part_floats(int dp) { return AP_ITEM_ROWS * (dp + 2); }
 struct PrefillArgs {
     RowsView v;
     void* out;
-    unsigned long long *flags, token;  // see attention_parts.cuh
+    uint32_t* flags;  // see attention_parts.cuh
     float* parts;
     const int32_t *cu_q, *cu_k;
     unsigned int* status;
@@ -476,7 +476,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     auto part_empty = [&](uint32_t s) { return more + 120 + (AP_PARTS + s) * 8; };
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
 
-    if (threadIdx.x < 2 * PART_WARPS) p.flags[blockIdx.x * 2 * PART_WARPS + threadIdx.x] = 0ull;  // (this block's own)
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(q_full(i), 1), mbar_init(q_empty(i), 1), mbar_init(s_full(i), 1), mbar_init(o_full(i), 1);
@@ -490,6 +489,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         *odd_values = 0u;
     }
     if (warp == AP_MMA_WARP) tmem_alloc<false>(smem_u32(const_cast<uint32_t*>(words)), 512);
+    pdl_wait();  // (the flags are down)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             const uint32_t item_row = i * AP_ROWS + row;
             uint16_t* const out = static_cast<uint16_t*>(p.out) +
                                   ((int64_t)(w.row0 + row_tok) * p.q_heads + w.kv_head * (int)p.group + (int)row_head) * p.d;
-            const PartSet set{p.flags, p.token, w.c0, w.c1, w.slot, blockIdx.x, warp};
+            const PartSet set{p.flags, w.c0, w.c1, w.slot, blockIdx.x, warp};
             auto part_at = [&](uint32_t c) { return p.parts + (uint64_t)set.part(c) * part_floats(DP) + item_row; };
             // (one loop for all three, since code that is not cached costs more than its branches)
             enum { WHOLE, LEAVE, JOIN };
@@ -904,7 +904,6 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 if (what != LEAVE || !set.show()) break;
                 what = JOIN;
             }
-            if (what == JOIN) set.clear();
             if (any) {
                 tc_fence_before();
                 __syncwarp();
@@ -923,6 +922,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         for (uint32_t x = issued > SLOTS ? issued - SLOTS : 0; x < issued; ++x)
             mbar_wait(full(x % SLOTS), (x / SLOTS) & 1, p.status, AP_LOAD, p.wait_ns);
     }
+}
+
+// Before every call's kernel, whose blocks start beside it and wait for its end.
+constexpr int CLEAR_THREADS = 608;
+__global__ void __launch_bounds__(CLEAR_THREADS) clear_flags(uint32_t* flags, uint32_t sixteens) {
+    pdl_launch_dependents();
+    for (uint32_t i = threadIdx.x; i < sixteens; i += CLEAR_THREADS) reinterpret_cast<uint4*>(flags)[i] = make_uint4(0, 0, 0, 0);
 }
 
 // The tensor map of [tokens][heads][d] rows as dims {d, inner, outer, tokens} (inner x outer = heads), box {64, bi, 1, bt}.
@@ -957,7 +963,7 @@ cudaError_t launch(const PrefillParams& p, uint8_t* workspace, unsigned blocks, 
     if (e != cudaSuccess) return e;
     if (encode_fn() == nullptr) return cudaErrorNotSupported;
     a.v = p.v, a.out = p.out, a.cu_q = p.cu_q, a.cu_k = p.cu_k;
-    a.flags = reinterpret_cast<unsigned long long*>(workspace), a.token = call_token();
+    a.flags = reinterpret_cast<uint32_t*>(workspace);
     a.parts = reinterpret_cast<float*>(workspace + part_flags_bytes(blocks));
     a.seqs = p.seqs, a.q_tokens = p.q_tokens, a.k_tokens = p.k_tokens, a.q_heads = p.q_heads, a.kv_heads = p.kv_heads;
     a.group = p.q_heads / p.kv_heads, a.tpt = AP_ROWS / a.group, a.d = p.d;
@@ -972,8 +978,22 @@ cudaError_t launch(const PrefillParams& p, uint8_t* workspace, unsigned blocks, 
         return cudaErrorInvalidValue;
     e = cudaFuncSetAttribute(prefill_kernel<DP, BF>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
     if (e != cudaSuccess) return e;
-    prefill_kernel<DP, BF><<<blocks, AP_THREADS, S::SMEM, stream>>>(qm, km, vm, a);
-    return cudaGetLastError();
+    // (one split of shared memory for both: changing it would drain an SM)
+    e = cudaFuncSetAttribute(clear_flags, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    clear_flags<<<1, CLEAR_THREADS, 0, stream>>>(a.flags, (uint32_t)(part_flags_bytes(blocks) / 16));
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(AP_THREADS);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prefill_kernel<DP, BF>, qm, km, vm, a);
 }
 
 }  // namespace
