@@ -810,6 +810,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             // (one loop for all three, since code that is not cached costs more than its branches)
             enum { WHOLE, LEAVE, JOIN };
             int what = whole ? WHOLE : set.others_done() ? JOIN : LEAVE;
+            // A part that is left and then joined after all is taken from the workspace like the others': two warps that
+            // finish together then write the same values, once each, the infinities of the guard among them.
+            bool left = false;
             const float mine = m * p.c;
             for (;;) {
                 float top = mine, sum = l;
@@ -858,7 +861,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                                     const float* const src = part_at(b) - item_row + (c / 4 * AP_ITEM_ROWS + item_row) * 4;
 #pragma unroll
                                     for (int x = 0; x < 32; x += 4) {
-                                        const float4 z = b == set.self ? make_float4(o[x], o[x + 1], o[x + 2], o[x + 3])
+                                        const float4 z = b == set.self && !left ? make_float4(o[x], o[x + 1], o[x + 2], o[x + 3])
                                                                        : __ldcg(reinterpret_cast<const float4*>(src + x * AP_ITEM_ROWS));
                                         y[x] += z.x * wb, y[x + 1] += z.y * wb, y[x + 2] += z.z * wb, y[x + 3] += z.w * wb;
                                     }
@@ -882,7 +885,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                     }
                 }
                 // infinities and NaN that the guard took out, back into the rows that see them
-                if (odd && valid) {
+                if (odd && valid && !left) {
 #pragma unroll 1
                     for (int32_t key = max(w.least, w.j0 * AP_KEYS); key < min(seen, w.j1 * AP_KEYS); ++key) {
                         const uint16_t* const v = static_cast<const uint16_t*>(p.v.p) + (int64_t)(w.k0 + key) * p.v.token_stride +
@@ -902,7 +905,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 }
                 __syncwarp();
                 if (what != LEAVE || !set.show()) break;
-                what = JOIN;
+                what = JOIN, left = true;
             }
             if (any) {
                 tc_fence_before();

@@ -46,3 +46,31 @@ def test_prefill_sink(lens, before, dtype, gap):
     want, size = ref.prefill(q, k, v, cu_q.tolist(), cu_k.tolist())
     worst = ((got - want).abs() - 3 * ref.UNIT[dtype] * size - (2.0 ** -25 if dtype == F16 else 0.0)).max()
     assert worst <= 0, worst
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lens,before", [([700], 0), ([64], 9000), ([333, 901], 0), ([17, 450], 3000)])
+def test_prefill_infinities_in_items_cut_between_blocks(lens, before, dtype):
+    """Values of both infinities and NaN that some rows of a tile see and others do not, in items that several blocks have parts
+    of: each row has what the formula gives, every time."""
+    keys = [n + before for n in lens]
+    q, k, v = (randn((n, h, 16), 3 + i, dtype) for i, (n, h) in enumerate([(sum(lens), 32), (sum(keys), 8), (sum(keys), 8)]))
+    end = torch.tensor(keys).cumsum(0)
+    for i, back in enumerate([1, 2, 9, 30, 60, 130, 200]):  # places from each sequence's end, where the causal mask cuts
+        for e, n in zip(end.tolist(), keys):
+            if back < n:
+                v[e - back, i % 8, i::5] = (float("inf"), -float("inf"), float("nan"))[i % 3]
+                v[e - back, (i + 1) % 8, i::7] = (-float("inf"), float("inf"), float("inf"))[i % 3]
+    cu_q = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    cu_k = torch.tensor([0] + keys).cumsum(0).to(torch.int32)
+    want, _ = ref.prefill(q, k, v, cu_q.tolist(), cu_k.tolist())
+    first = None
+    for _ in range(10):
+        got = c.attention_prefill(q, k, v, cu_q.cuda(), cu_k.cuda())
+        first = got if first is None else first
+        assert torch.equal(got.view(torch.int16), first.view(torch.int16))
+    got = got.double().cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isposinf(), want.isposinf()) and torch.equal(got.isneginf(), want.isneginf())
+    finite = want.isfinite()
+    clean, size = ref.prefill(q, k, v.nan_to_num(0, 0, 0), cu_q.tolist(), cu_k.tolist())
+    assert ((got - clean).abs() <= 3 * ref.UNIT[dtype] * size + (2.0 ** -25 if dtype == F16 else 0.0))[finite].all()
