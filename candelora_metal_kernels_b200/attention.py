@@ -80,7 +80,9 @@ def _out(op: str, index: int, out, shape, dtype, near: torch.Tensor) -> torch.Te
 class KvCache:
     """A paged key-value cache over tensors k, v [num_pages, kv_heads, page_size, head_dim] (f16, bf16 or int8) and, for
     int8, k_scale, v_scale f32 [num_pages, kv_heads, page_size]. Token `pos` of a sequence lies in page
-    block_table[sequence, pos // page_size], row pos % page_size. Holds no state besides the tensors."""
+    block_table[sequence, pos // page_size], row pos % page_size. The calls take the tensors' addresses from here, so that k, v
+    and the scales cannot be replaced (a cache of other tensors is another KvCache), and calls refuse ones whose memory has
+    moved since. Holds no other state."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None):
@@ -103,13 +105,28 @@ class KvCache:
             _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: only an int8 cache takes scales")
         if not k.is_contiguous() or not v.is_contiguous():
             _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op} expects contiguous layouts")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
         self.dtype, self.device, self._index = k.dtype, k.device, k.get_device()
-        self._struct = _lib.KvCacheStruct(
-            k.data_ptr(), v.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
-            None if v_scale is None else v_scale.data_ptr(), *k.shape, _KV_DTYPES[k.dtype])
+        self._addresses = self._now()
+        self._struct = _lib.KvCacheStruct(*self._addresses, *k.shape, _KV_DTYPES[k.dtype])
         self._ptr = ctypes.addressof(self._struct)
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scale = property(lambda self: self._k_scale)
+    v_scale = property(lambda self: self._v_scale)
+
+    def _now(self) -> tuple:
+        if self._k_scale is None:
+            return self._k.data_ptr(), self._v.data_ptr(), None, None
+        return self._k.data_ptr(), self._v.data_ptr(), self._k_scale.data_ptr(), self._v_scale.data_ptr()
+
+    def _checked(self, op: str) -> int:
+        """The address of the C struct, if the tensors still lie where they did."""
+        if self._now() != self._addresses:
+            _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: the cache's tensors have moved since the KvCache was made")
+        return self._ptr
 
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
@@ -172,7 +189,7 @@ def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     if tokens:
         args = _lib.KV_TOKENS.pack(k.data_ptr(), k_strides[0], k_strides[1], v.data_ptr(), v_strides[0], v_strides[1], *rows_q[:3],
                                    _X_DTYPES[dtype], tokens, rows_q[3], slots.data_ptr(), *rope, interleaved, out_ptr, out_code)
-        _call(index, _lib.load().iq2_kv_cache_write, cache._ptr, args)
+        _call(index, _lib.load().iq2_kv_cache_write, cache._checked(op), args)
     return q_out
 
 
@@ -196,7 +213,7 @@ def kv_cache_read(cache: KvCache, block_table: torch.Tensor, cu_seqlens: torch.T
     k_out = _out(op, index, k_out, shape, dtype, cache.k)
     v_out = _out(op, index, v_out, shape, dtype, k_out)
     if total_tokens:
-        _call(index, _lib.load().iq2_kv_cache_read, cache._ptr, table.data_ptr(), width, seqs,
+        _call(index, _lib.load().iq2_kv_cache_read, cache._checked(op), table.data_ptr(), width, seqs,
               None if starts is None else starts.data_ptr(), cu.data_ptr(), total_tokens, k_out.data_ptr(),
               v_out.data_ptr(), _X_DTYPES[dtype])
     return k_out, v_out
@@ -296,5 +313,5 @@ def attention_decode(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor,
     lib = _lib.load()
     if workspace is None:
         workspace = _scratch(attention_decode_workspace_bytes(q, cache, block_table), q)
-    _call(index, lib.iq2_attention_decode, cache._ptr, args, *_buffer(workspace))
+    _call(index, lib.iq2_attention_decode, cache._checked(op), args, *_buffer(workspace))
     return out
