@@ -208,8 +208,7 @@ int iq2_attention_decode(const iq2_kv_cache* cache, const iq2_attention_tokens* 
     if ((rc = check_scale(op, t->scale, cache->head_dim, &scale)) != IQ2_OK) return rc;
     if (t->batch == 0) return IQ2_OK;
     if (t->table_width == 0) return capi_fail(IQ2_ERR_ZERO_DIM, "%s expects non-zero dimensions", op);
-    // the units of a sequence's items (128 tokens or more each) are numbered in 32 bits
-    if (((uint64_t)t->table_width * cache->page_size / 128 + 1) * t->q_heads > (uint64_t)UINT32_MAX)
+    if (!iq2::attention_decode_fits(view(cache), t->table_width, t->q_heads))
         return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u pages of %u tokens are too long a sequence", op, t->table_width, cache->page_size);
     if (t->batch > 65535u) return capi_fail(IQ2_ERR_OVERFLOW, "%s: a batch of %u is too large", op, t->batch);
     const size_t e = size_of(t->dtype);

@@ -754,6 +754,13 @@ cudaError_t launch_kind(const DecodeArgs& a, uint32_t blocks, cudaStream_t strea
 
 }  // namespace
 
+bool attention_decode_fits(const KvCacheView& c, uint32_t table_width, uint32_t q_heads) {
+    const uint32_t unit = c.dtype == kInt8 ? DecodeShape<64, CK_INT8, false>::UNIT : DecodeShape<64, CK_F16, false>::UNIT;
+    const uint64_t tokens = std::min<uint64_t>((uint64_t)table_width * c.page_size, INT32_MAX);
+    const uint64_t items = (uint64_t)c.heads * ((q_heads / c.heads + AD_HEADS - 1) / AD_HEADS);
+    return ((tokens + unit - 1) / unit + AD_ITEM_COST) * items <= (uint64_t)UINT32_MAX;
+}
+
 size_t attention_decode_workspace(uint32_t, uint32_t, uint32_t, uint32_t d, int num_sms) {
     return records_bytes(num_sms) + (size_t)num_sms * 2 * AD_HEADS * ((d > 64 ? 128 : 64) + 2) * sizeof(float);
 }

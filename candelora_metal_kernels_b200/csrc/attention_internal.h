@@ -73,6 +73,8 @@ struct DecodeParams {
     int dtype;
     float scale;
 };
+// Whether the units of a sequence's items can be numbered in 32 bits.
+bool attention_decode_fits(const KvCacheView& c, uint32_t table_width, uint32_t q_heads);
 size_t attention_decode_workspace(uint32_t batch, uint32_t q_heads, uint32_t kv_heads, uint32_t d, int num_sms);
 cudaError_t launch_attention_decode(const DecodeParams& p, void* workspace, int num_sms, cudaStream_t stream);
 
