@@ -167,11 +167,11 @@ int iq2_attention_prefill(const iq2_attention_prompts* t, void* workspace, size_
     if ((rc = check_scale(op, t->scale, t->head_dim, &scale)) != IQ2_OK) return rc;
     if (t->q_tokens == 0) return IQ2_OK;
     if (t->sequences == 0) return capi_fail(IQ2_ERR_ZERO_DIM, "%s expects non-zero dimensions", op);
-    // work items are numbered in 32 bits
-    if (t->q_tokens > (uint32_t)INT32_MAX || t->k_tokens > (uint32_t)INT32_MAX ||
+    // work items are numbered in 32 bits; tokens, with a tile past the end and an item's cost on top, in 31
+    if ((uint64_t)t->q_tokens + t->k_tokens + 1024 > (uint64_t)INT32_MAX ||
         ((uint64_t)t->q_tokens + t->sequences) * t->q_heads > (uint64_t)INT32_MAX ||
         ((uint64_t)t->k_tokens + 1024) * t->kv_heads > (uint64_t)UINT32_MAX)
-        return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u queries of %u heads are too large", op, t->q_tokens, t->q_heads);
+        return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u queries of %u heads over %u keys are too large", op, t->q_tokens, t->q_heads, t->k_tokens);
     if ((rc = check_pointers(op, {{"q", t->q.data, 16}, {"out", t->out, 16}, {"cu_seqlens_q", t->cu_seqlens_q, 4},
                                   {"cu_seqlens_k", t->cu_seqlens_k, 4}})) != IQ2_OK)
         return rc;
