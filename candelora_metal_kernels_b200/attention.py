@@ -27,14 +27,18 @@ _KV_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, to
 # These calls last a few microseconds on the GPU, so the host side counts: device indices are compared instead of device
 # objects, the stream is taken without its wrapper, and arguments are packed as bytes.
 
-def _call(index: int, fn, *args) -> None:
-    """fn(*args, stream) on GPU `index`, which the C ABI expects to be the current one."""
-    stream = torch._C._cuda_getCurrentRawStream(index)  # current_stream(device).cuda_stream without the Stream object
+def _on(index: int, fn, *args) -> int:
+    """fn(*args) with GPU `index` as the current one, which the C ABI expects."""
     if index == torch._C._cuda_getDevice():
-        rc = fn(*args, stream)
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, stream)
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def _call(index: int, fn, *args) -> None:
+    """fn(*args, stream) on GPU `index`."""
+    # (current_stream(device).cuda_stream without the Stream object)
+    rc = _on(index, fn, *args, torch._C._cuda_getCurrentRawStream(index))
     if rc != _lib.IQ2_OK:
         _lib.check(rc)
 
@@ -263,7 +267,7 @@ def attention_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
         _scale(op, scale), out.data_ptr())
     lib = _lib.load()
     if workspace is None:
-        workspace = _scratch(lib.iq2_attention_prefill_workspace_size(args), q)
+        workspace = _scratch(_on(index, lib.iq2_attention_prefill_workspace_size, args), q)
     _call(index, lib.iq2_attention_prefill, args, *_buffer(workspace))
     return out
 
@@ -286,8 +290,7 @@ def _buffer(workspace: torch.Tensor | None):
 
 def attention_decode_workspace_bytes(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor) -> int:
     """Device scratch attention_decode needs for q [batch, q_heads, head_dim], whatever the lengths."""
-    with torch.cuda.device(cache.device):
-        return int(_lib.load().iq2_attention_decode_workspace_size(cache._ptr, q.shape[0], q.shape[1]))
+    return int(_on(cache._index, _lib.load().iq2_attention_decode_workspace_size, cache._ptr, q.shape[0], q.shape[1]))
 
 
 def attention_decode(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, seq_lens: torch.Tensor, *,
