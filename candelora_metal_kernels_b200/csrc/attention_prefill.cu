@@ -25,11 +25,13 @@
 //     rows see become zeros too, and the epilogue adds them back to exactly the rows that see them.
 // What bounds it: per pair of key tiles the four products take 2048 cycles of the tensor core; the step takes 3100 to 3400,
 // since a row's softmax (load, maximum, 128 exponentials and their rounding, store: about 2000, of which the exponentials
-// are 1500 of instruction latency and issue) and its products with their handshakes (about 1080) follow one another and the
+// are 1500: 1024 at the exponential unit's own rate, which needs 2048 for both row tiles, as the tensor core does, and the
+// rest latency and issue) and its products with their handshakes (about 1080) follow one another and the
 // other tile fills only part of the gap. Two tiles of 128 rows and five K or V tiles of 32 KB are what shared memory and
-// TMEM hold. Measured (32 query heads, 8 key heads, 128 elements, bf16, causal): 16384 tokens 1.72 to 1.89 ms, 1160 to 1280
-// TFLOP/s, with the tensor pipe busy 61 % of the time; 2048 tokens 54 us, where an item's start and end (3 tiles' time) and
-// the kernel's (about 4 us) are a third; a batch of nine prompts of up to 200 tokens 24.5 us, all of it such latencies.
+// TMEM hold at 128 elements (at 64, TMEM has 128 columns to spare). Measured (32 query heads, 8 key heads, 128 elements, bf16, causal): 16384 tokens 1.73 to 1.89 ms, 1160 to 1270
+// TFLOP/s, with the tensor pipe busy 62 % of the time; 2048 tokens 56 us, where an item's start and end (3 tiles' time) and
+// the kernel's (about 4 us) are a third; a batch of nine prompts of up to 200 tokens 26.4 us, all of it such latencies.
+// 64 elements: 8192 tokens 375 us, 730 TFLOP/s; 2048 tokens 45 us.
 // Every wait is bounded by wall time (device_status); a block that gives up still drains its copies and frees its TMEM.
 #include "attention_internal.h"
 #include "attention_parts.cuh"

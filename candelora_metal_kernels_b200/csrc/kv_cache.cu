@@ -6,9 +6,10 @@
 // with every product and sum rounded by itself in f32, so that a result does not depend on how the compiler fuses.
 // int8 rows (one token and head): m = max |x|, scale = m / 127, code = rint(x * (127 / m)); m < 2^-100 gives zeros (the
 // quotient would overflow), and a row with an infinity or NaN gets a NaN scale, so that it reads back as NaN.
-// Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 12.8 to 13.3 us, 5980 GB/s at best of bytes in
-// and out; of 8800 tokens, f32 into an int8 cache, with the read back 66.9 us, 5420 GB/s; read of 89091 tokens of an int8 cache
-// to bf16 96 us, 5750 GB/s.
+// Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 18.3 us over 0.9 GB of inputs and
+// outputs in turn, 4190 GB/s (12.8 over 0.2 GB, where the L2 keeps part of the outputs); of 8800 tokens, f32 into an int8 cache,
+// with the read back 67.5 us, 5380 GB/s; read of 89091 tokens to bf16, of an int8 cache 97 us, 5680 GB/s, of a bf16 one 117 us,
+// 6220 GB/s.
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"
 

@@ -346,9 +346,10 @@ typedef struct iq2_attention_prompts {
 size_t iq2_attention_prefill_workspace_size(const iq2_attention_prompts* prompts);
 
 /*
- * out = softmax(scale q k^T) v for every sequence, f32 statistics and accumulation. Keys may be
- * more than queries (a later chunk of a prompt) or fewer; a query that sees no key gets zeros, and
- * so do rows of no sequence (before cu_seqlens_q[0], or from cu_seqlens_q[sequences] on).
+ * out = softmax(scale q k^T) v for every sequence; scores, maxima, sums and accumulation in f32, the
+ * probabilities rounded to dtype for their product with v (f16: kept to 2^-35 of the row's largest).
+ * Keys may be more than queries (a later chunk of a prompt) or fewer; a query that sees no key gets
+ * zeros, and so do rows of no sequence (before cu_seqlens_q[0], or from cu_seqlens_q[sequences] on).
  * What a masked key or value holds (other sequences' tokens, infinities, NaN) has no effect.
  */
 int iq2_attention_prefill(const iq2_attention_prompts* prompts, void* workspace, size_t workspace_bytes,
@@ -370,7 +371,8 @@ typedef struct iq2_attention_tokens {
 size_t iq2_attention_decode_workspace_size(const iq2_kv_cache* cache, uint32_t batch, uint32_t q_heads);
 
 /*
- * out = softmax(scale q k^T) v, f32 statistics and accumulation, any q type over any cache type.
+ * out = softmax(scale q k^T) v, any q type over any cache type; scores, maxima, sums and accumulation
+ * in f32, q and the probabilities as sums of two 16-bit pieces (three for f32 q over a bf16 cache).
  * A sequence of length 0 gets zeros.
  */
 int iq2_attention_decode(const iq2_kv_cache* cache, const iq2_attention_tokens* tokens, void* workspace,
