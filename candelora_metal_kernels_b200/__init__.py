@@ -14,6 +14,7 @@ from .attention import (
     kv_cache_read,
     kv_cache_write,
 )
+from .pages import KvPages, KvStep, kv_pages_step
 from .iq2_matmul import (
     Iq2MatmulOp,
     Iq2MatmulVariant,
@@ -38,6 +39,8 @@ __all__ = [
     "Iq2MatmulOp",
     "Iq2MatmulVariant",
     "KvCache",
+    "KvPages",
+    "KvStep",
     "LIB_PATH",
     "attention_decode",
     "attention_decode_workspace_bytes",
@@ -55,5 +58,6 @@ __all__ = [
     "iq3_s_matmul",
     "kv_cache_read",
     "kv_cache_write",
+    "kv_pages_step",
     "workspace_bytes",
 ]

@@ -27,7 +27,7 @@ IQ2_ERR_TIMEOUT = 11
 IQ2_COMM_ID_BYTES = 128
 
 DTYPE_F32, DTYPE_F16, DTYPE_BF16 = 0, 1, 2
-KV_INT8 = 3
+KV_INT8, KV_INT4 = 3, 4
 ACT_QUANT_OFF, ACT_QUANT_W8A8, ACT_QUANT_W4A8 = 0, 1, 2
 
 # Every symbol the headers (include/candelora_iq2.h, include/candelora_iq2_testing.h) declare,
@@ -58,6 +58,8 @@ SIGNATURES = {
     "iq2_matmul_grouped_sharded_workspace_size": ([_vp, _u32, _u32, _int, _int], _sz),
     "iq2_matmul_grouped_sharded": ([_vp, _vp, _u32, _u32, _int, _vp, _sz, _vp], _int),
     "iq2_kv_cache_write": ([_vp, _vp, _vp], _int),
+    "iq2_kv_cache_write_normed": ([_vp, _vp, _vp, _vp], _int),
+    "iq2_kv_pages_step": ([_vp, _vp, _vp], _int),
     "iq2_kv_cache_read": ([_vp, _vp, _u32, _u32, _vp, _vp, _u32, _vp, _vp, _int, _vp], _int),
     "iq2_attention_prefill_workspace_size": ([_vp], _sz),
     "iq2_attention_prefill": ([_vp, _vp, _sz, _vp], _int),
@@ -78,13 +80,22 @@ class KvCacheStruct(ctypes.Structure):
     """struct iq2_kv_cache."""
 
     _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("num_pages", _u32), ("kv_heads", _u32),
-                ("page_size", _u32), ("head_dim", _u32), ("dtype", _int)]
+                ("page_size", _u32), ("head_dim", _u32), ("dtype", _int), ("k_group", _vp), ("v_group", _vp)]
+
+
+class KvPagesStruct(ctypes.Structure):
+    """struct iq2_kv_pages."""
+
+    _fields_ = [("block_table", _vp), ("seq_lens", _vp), ("free_pages", _vp), ("free_count", _vp), ("sequences", _u32),
+                ("table_width", _u32), ("num_pages", _u32), ("page_size", _u32)]
 
 
 # The attention operators' argument structs, packed in the header's field order with C alignment (iq2_rows: a pointer and
 # two int64 strides). Packing bytes is several times cheaper than filling a ctypes.Structure, and these calls are short.
 _ROWS = "Pqq"
 KV_TOKENS = struct.Struct("@" + 3 * _ROWS + "iIIPPPPIiPi0q")           # iq2_kv_tokens
+HEAD_NORMS = struct.Struct("@PPiif0q")                                 # iq2_head_norms
+KV_STEP = struct.Struct("@PPIPPPPP")                                   # iq2_kv_step
 ATTENTION_PROMPTS = struct.Struct("@" + 3 * _ROWS + "iIIIIIIPPifP")    # iq2_attention_prompts
 ATTENTION_TOKENS = struct.Struct("@" + _ROWS + "iIIIPPfP")             # iq2_attention_tokens
 

@@ -1,8 +1,8 @@
 """Tensor-level host API of the attention operators over the CUDA C ABI (no reference counterpart: the reference ends at
 the projections). They take the projections' outputs as [tokens, heads, head_dim] CUDA tensors:
 
-  KvCache               a paged cache: 16-bit, or int8 with a scale for each token and head
-  kv_cache_write        rotates q and k, writes k and v into the cache
+  KvCache               a paged cache: 16-bit, int8 with a scale for each token and head, or 4-bit with group scales
+  kv_cache_write        norms and rotates q and k, writes k and v into the cache
   kv_cache_read         cached tokens back into packed 16- or 32-bit tensors
   attention_prefill     attention of packed prompts (causal or not, grouped heads)
   attention_decode      attention of one new token a sequence over the cache
@@ -21,7 +21,8 @@ from ._lib import Iq2Error
 from .iq2_matmul import _X_DTYPES, _bail
 
 _PREFILL_DTYPES = (torch.float16, torch.bfloat16)
-_KV_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.int8: _lib.KV_INT8}
+_KV_DTYPES = {torch.float16: _lib.DTYPE_F16, torch.bfloat16: _lib.DTYPE_BF16, torch.int8: _lib.KV_INT8,
+              torch.uint8: _lib.KV_INT4}
 
 
 # These calls last a few microseconds on the GPU, so the host side counts: device indices are compared instead of device
@@ -86,45 +87,65 @@ class KvCache:
     int8, k_scale, v_scale f32 [num_pages, kv_heads, page_size]. Token `pos` of a sequence lies in page
     block_table[sequence, pos // page_size], row pos % page_size. The calls take the tensors' addresses from here, so that k, v
     and the scales cannot be replaced (a cache of other tensors is another KvCache), and calls refuse ones whose memory has
-    moved since. Holds no other state."""
+    moved since. Holds no other state.
+
+    A 4-bit cache has k, v uint8 [num_pages, kv_heads, page_size, head_dim / 2] (head_dim a multiple of 32), element 2i in the
+    low half of byte i, 2i + 1 in the high half, as code + 8; the scales above, and k_group, v_group
+    [num_pages, kv_heads, page_size, 4] float8_e4m3fn, of which the first head_dim / 32 are the (not negative) scales of a
+    row's groups of 32 elements: an element is code * group scale * row scale."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
-                 v_scale: torch.Tensor | None = None):
+                 v_scale: torch.Tensor | None = None, k_group: torch.Tensor | None = None, v_group: torch.Tensor | None = None):
         op = "KvCache"
         if k.dim() != 4 or k.shape != v.shape:
             _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op} expects k and v of one shape [num_pages, kv_heads, page_size, "
                                                  f"head_dim], got {list(k.shape)} and {list(v.shape)}")
         if k.device.type != "cuda":
             _bail(_lib.IQ2_ERR_DEVICE, f"{op} requires a CUDA device")
-        for name, t in (("v", v), ("k_scale", k_scale), ("v_scale", v_scale)):
+        for name, t in (("v", v), ("k_scale", k_scale), ("v_scale", v_scale), ("k_group", k_group), ("v_group", v_group)):
             if t is not None and t.device != k.device:
                 _elsewhere(op, k.get_device(), name, t)
         if k.dtype not in _KV_DTYPES or v.dtype != k.dtype:
             _bail(_lib.IQ2_ERR_DTYPE, f"{op} unsupported cache dtype: {k.dtype}, {v.dtype}")
-        if k.dtype == torch.int8:
+        int4 = k.dtype == torch.uint8
+        if int4 or k.dtype == torch.int8:
             for s in (k_scale, v_scale):
                 if s is None or s.dtype != torch.float32 or s.shape != k.shape[:3] or not s.is_contiguous():
-                    _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: an int8 cache takes contiguous f32 scales {list(k.shape[:3])}")
+                    _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: {'a 4-bit' if int4 else 'an int8'} cache takes contiguous f32 "
+                                                         f"scales {list(k.shape[:3])}")
         elif k_scale is not None or v_scale is not None:
-            _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: only an int8 cache takes scales")
+            _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: only an int8 or 4-bit cache takes scales")
+        if int4:
+            for s in (k_group, v_group):
+                if s is None or s.dtype != torch.float8_e4m3fn or s.shape != (*k.shape[:3], 4) or not s.is_contiguous():
+                    _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: a 4-bit cache takes contiguous float8_e4m3fn group scales "
+                                                         f"{[*k.shape[:3], 4]}")
+            if k.shape[3] % 16 != 0:
+                _bail(_lib.IQ2_ERR_UNSUPPORTED, f"{op}: head_dim={2 * k.shape[3]} of a 4-bit cache is not a multiple of 32")
+        elif k_group is not None or v_group is not None:
+            _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: only a 4-bit cache takes group scales")
         if not k.is_contiguous() or not v.is_contiguous():
             _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op} expects contiguous layouts")
-        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
+        self._k, self._v, self._k_scale, self._v_scale, self._k_group, self._v_group = k, v, k_scale, v_scale, k_group, v_group
+        self._tensors = tuple(t for t in (k, v, k_scale, v_scale, k_group, v_group) if t is not None)
         self.num_pages, self.kv_heads, self.page_size, self.head_dim = k.shape
+        if int4:
+            self.head_dim *= 2
         self.dtype, self.device, self._index = k.dtype, k.device, k.get_device()
         self._addresses = self._now()
-        self._struct = _lib.KvCacheStruct(*self._addresses, *k.shape, _KV_DTYPES[k.dtype])
+        held = (*self._addresses, *[None] * (6 - len(self._addresses)))
+        self._struct = _lib.KvCacheStruct(*held[:4], *k.shape[:3], self.head_dim, _KV_DTYPES[k.dtype], *held[4:])
         self._ptr = ctypes.addressof(self._struct)
 
     k = property(lambda self: self._k)
     v = property(lambda self: self._v)
     k_scale = property(lambda self: self._k_scale)
     v_scale = property(lambda self: self._v_scale)
+    k_group = property(lambda self: self._k_group)
+    v_group = property(lambda self: self._v_group)
 
     def _now(self) -> tuple:
-        if self._k_scale is None:
-            return self._k.data_ptr(), self._v.data_ptr(), None, None
-        return self._k.data_ptr(), self._v.data_ptr(), self._k_scale.data_ptr(), self._v_scale.data_ptr()
+        return tuple([t.data_ptr() for t in self._tensors])
 
     def _checked(self, op: str) -> int:
         """The address of the C struct, if the tensors still lie where they did."""
@@ -135,23 +156,42 @@ class KvCache:
     @classmethod
     def empty(cls, num_pages: int, kv_heads: int, page_size: int, head_dim: int, dtype: torch.dtype = torch.bfloat16,
               device="cuda") -> "KvCache":
-        """A cache of zeros."""
-        shape = (num_pages, kv_heads, page_size, head_dim)
-        k, v = (torch.zeros(shape, dtype=dtype, device=device) for _ in range(2))
-        if dtype != torch.int8:
-            return cls(k, v)
-        return cls(k, v, *(torch.zeros(shape[:3], dtype=torch.float32, device=device) for _ in range(2)))
+        """A cache of zeros. dtype torch.uint8: a 4-bit cache."""
+        shape = (num_pages, kv_heads, page_size)
+        if dtype == torch.uint8:
+            if head_dim % 32 != 0:
+                _bail(_lib.IQ2_ERR_UNSUPPORTED, f"KvCache: head_dim={head_dim} of a 4-bit cache is not a multiple of 32")
+            k, v = (torch.full((*shape, head_dim // 2), 0x88, dtype=dtype, device=device) for _ in range(2))
+            groups = [torch.zeros((*shape, 4), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn) for _ in range(2)]
+        else:
+            k, v = (torch.zeros((*shape, head_dim), dtype=dtype, device=device) for _ in range(2))
+            groups = []
+            if dtype != torch.int8:
+                return cls(k, v)
+        return cls(k, v, *(torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2)), *groups)
+
+
+def _weights(op: str, index: int, name: str, t: torch.Tensor, heads: int, dim: int):
+    """Norm weights f32 [dim] or [heads, dim], contiguous, and whether they are each head's own."""
+    if t.get_device() != index:
+        _elsewhere(op, index, name, t)
+    shape = t.shape
+    if t.dtype != torch.float32 or shape[-1:] != (dim,) or len(shape) > 2 or (len(shape) == 2 and shape[0] != heads):
+        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op} expects {name} as f32 [{dim}] or [{heads}, {dim}], got {t.dtype} {list(shape)}")
+    return t if t.is_contiguous() else t.contiguous(), len(shape) == 2
 
 
 def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, *, q: torch.Tensor | None = None,
                    q_dtype: torch.dtype | None = None, positions: torch.Tensor | None = None,
                    cos: torch.Tensor | None = None, sin: torch.Tensor | None = None, interleaved: bool = False,
-                   q_out: torch.Tensor | None = None) -> torch.Tensor | None:
+                   q_out: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                   k_norm: torch.Tensor | None = None, norm_eps: float = 1e-6) -> torch.Tensor | None:
     """Write k, v [tokens, kv_heads, head_dim] (f32, f16 or bf16) to the cache's `slots` (int32 [tokens],
     page * page_size + row; a slot outside the cache, e.g. -1, writes nothing). With cos, sin f32
     [rows, head_dim / 2] and positions int32 [tokens], k and q are rotated first: pairs (i, i + head_dim / 2), or
     (2i, 2i + 1) with `interleaved`; without cos and sin, positions are not read. q [tokens, q_heads, head_dim], of k's
-    dtype, is returned as q_dtype (its own by default)."""
+    dtype, is returned as q_dtype (its own by default). With q_norm or k_norm (f32 [head_dim], or a row for each head), each
+    head's q or k becomes x / sqrt(mean(x^2) + norm_eps) * weight before its rotation."""
     op = "kv_cache_write"
     d, index, kv_heads = cache.head_dim, cache._index, cache.kv_heads
     k, k_strides, (tokens, _, _) = _rows(op, index, "k", k, kv_heads, d)
@@ -186,6 +226,17 @@ def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
         positions = _indices(op, index, "positions", positions, 1)
         same = same and positions.shape[0] == tokens
         rope = (positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), shape[0])
+    norms = None
+    if q_norm is not None or k_norm is not None:
+        if q_norm is not None and q is None:
+            _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: q_norm goes with q")
+        if not 0.0 < norm_eps < 3e38:  # (an f32 in the C ABI)
+            _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: norm_eps is not positive")
+        # (the names keep copies alive until the call)
+        q_norm, q_own = (None, False) if q_norm is None else _weights(op, index, "q_norm", q_norm, q_shape[1], d)
+        k_norm, k_own = (None, False) if k_norm is None else _weights(op, index, "k_norm", k_norm, kv_heads, d)
+        norms = _lib.HEAD_NORMS.pack(0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(),
+                                     q_own, k_own, norm_eps)
     if not same:
         _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: k has {tokens} tokens, v {v.shape[0]}, slots {slots.shape[0]}"
                                              f"{'' if q is None else f', q {q.shape[0]}'}"
@@ -193,13 +244,16 @@ def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     if tokens:
         args = _lib.KV_TOKENS.pack(k.data_ptr(), k_strides[0], k_strides[1], v.data_ptr(), v_strides[0], v_strides[1], *rows_q[:3],
                                    _X_DTYPES[dtype], tokens, rows_q[3], slots.data_ptr(), *rope, interleaved, out_ptr, out_code)
-        _call(index, _lib.load().iq2_kv_cache_write, cache._checked(op), args)
+        if norms is None:
+            _call(index, _lib.load().iq2_kv_cache_write, cache._checked(op), args)
+        else:
+            _call(index, _lib.load().iq2_kv_cache_write_normed, cache._checked(op), args, norms)
     return q_out
 
 
 def kv_cache_read(cache: KvCache, block_table: torch.Tensor, cu_seqlens: torch.Tensor, total_tokens: int, *,
                   starts: torch.Tensor | None = None, dtype: torch.dtype | None = None, k_out=None, v_out=None):
-    """Packed (k, v) [total_tokens, kv_heads, head_dim] in `dtype` (the cache's own, bf16 for an int8 cache): rows
+    """Packed (k, v) [total_tokens, kv_heads, head_dim] in `dtype` (the cache's own, bf16 for an int8 or 4-bit cache): rows
     [cu_seqlens[b], cu_seqlens[b + 1]) are the tokens starts[b], starts[b] + 1, ... (from 0 without `starts`) of the
     sequence whose pages are block_table[b] (int32 [sequences, width]). Rows of no sequence are zeros."""
     op = "kv_cache_read"
@@ -210,7 +264,7 @@ def kv_cache_read(cache: KvCache, block_table: torch.Tensor, cu_seqlens: torch.T
     if cu.shape[0] != seqs + 1 or (starts is not None and starts.shape[0] != seqs):
         _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: block_table has {seqs} sequences, cu_seqlens {cu.shape[0]} entries")
     if dtype is None:
-        dtype = torch.bfloat16 if cache.dtype == torch.int8 else cache.dtype
+        dtype = cache.dtype if cache.k_scale is None else torch.bfloat16
     if dtype not in _X_DTYPES:
         _bail(_lib.IQ2_ERR_DTYPE, f"{op} unsupported out dtype: {dtype}")
     shape = (total_tokens, cache.kv_heads, cache.head_dim)

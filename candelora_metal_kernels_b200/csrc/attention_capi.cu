@@ -1,5 +1,6 @@
 // C ABI of the attention operators (declared in include/candelora_iq2.h): the checks of their arguments, in the order
-// dimensions, device, types, layout, buffers; the kernels are in kv_cache.cu, attention_prefill.cu and attention_decode.cu.
+// dimensions, device, types, layout, buffers; the kernels are in kv_cache.cu, kv_pages.cu, attention_prefill.cu and
+// attention_decode.cu.
 #include <cinttypes>
 #include <cmath>
 #include <initializer_list>
@@ -57,17 +58,22 @@ int check_cache(const char* op, const iq2_kv_cache* c) {
     int rc = check_heads(op, c->kv_heads, c->kv_heads, c->head_dim);
     if (rc != IQ2_OK) return rc;
     if (c->num_pages == 0 || c->page_size == 0) return capi_fail(IQ2_ERR_ZERO_DIM, "%s expects non-zero dimensions", op);
-    if (c->dtype != IQ2_DTYPE_F16 && c->dtype != IQ2_DTYPE_BF16 && c->dtype != IQ2_KV_INT8)
+    if (c->dtype != IQ2_DTYPE_F16 && c->dtype != IQ2_DTYPE_BF16 && c->dtype != IQ2_KV_INT8 && c->dtype != IQ2_KV_INT4)
         return capi_fail(IQ2_ERR_DTYPE, "%s unsupported cache dtype: %d", op, c->dtype);
+    if (c->dtype == IQ2_KV_INT4 && c->head_dim % iq2::I4_GROUP != 0)
+        return capi_fail(IQ2_ERR_UNSUPPORTED, "%s: head_dim=%u of a 4-bit cache is not a multiple of %u", op, c->head_dim, iq2::I4_GROUP);
     if ((uint64_t)c->num_pages * c->page_size > (uint64_t)INT32_MAX)  // slots are int32
         return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u pages of %u tokens are too large", op, c->num_pages, c->page_size);
     if ((rc = check_pointers(op, {{"cache k", c->k, 16}, {"cache v", c->v, 16}})) != IQ2_OK) return rc;
-    if (c->dtype != IQ2_KV_INT8) return IQ2_OK;
-    return check_pointers(op, {{"cache k_scale", c->k_scale, 4}, {"cache v_scale", c->v_scale, 4}});
+    if (c->dtype != IQ2_KV_INT8 && c->dtype != IQ2_KV_INT4) return IQ2_OK;
+    if ((rc = check_pointers(op, {{"cache k_scale", c->k_scale, 4}, {"cache v_scale", c->v_scale, 4}})) != IQ2_OK) return rc;
+    if (c->dtype == IQ2_KV_INT8) return IQ2_OK;
+    return check_pointers(op, {{"cache k_group", c->k_group, 4}, {"cache v_group", c->v_group, 4}});
 }
 
 iq2::KvCacheView view(const iq2_kv_cache* c) {
-    return {c->k, c->v, c->k_scale, c->v_scale, c->num_pages, c->kv_heads, c->page_size, c->head_dim, c->dtype};
+    return {c->k, c->v, c->k_scale, c->v_scale, c->num_pages, c->kv_heads, c->page_size, c->head_dim, c->dtype,
+            c->dtype == IQ2_KV_INT4 ? c->k_group : nullptr, c->dtype == IQ2_KV_INT4 ? c->v_group : nullptr};
 }
 iq2::RowsView view(const iq2_rows& r) { return {r.data, r.token_stride, r.head_stride}; }
 
@@ -93,8 +99,7 @@ int check_workspace(const char* op, const void* workspace, size_t bytes, size_t 
 
 extern "C" {
 
-int iq2_kv_cache_write(const iq2_kv_cache* cache, const iq2_kv_tokens* t, iq2_stream_t stream) {
-    const char* op = "iq2_kv_cache_write";
+static int cache_write(const char* op, const iq2_kv_cache* cache, const iq2_kv_tokens* t, const iq2_head_norms* norms, iq2_stream_t stream) {
     iq2::capi_ok();
     if (t == nullptr) return capi_fail(IQ2_ERR_INVALID_ARGUMENT, "%s: NULL tokens", op);
     int rc = check_cache(op, cache);
@@ -103,6 +108,9 @@ int iq2_kv_cache_write(const iq2_kv_cache* cache, const iq2_kv_tokens* t, iq2_st
     if (has_q && (rc = check_heads(op, t->q_heads, cache->kv_heads, cache->head_dim)) != IQ2_OK) return rc;
     if (!float_dtype(t->dtype)) return capi_fail(IQ2_ERR_DTYPE, "%s unsupported k/v dtype: %d", op, t->dtype);
     if (has_q && !float_dtype(t->q_out_dtype)) return capi_fail(IQ2_ERR_DTYPE, "%s unsupported q_out dtype: %d", op, t->q_out_dtype);
+    const bool norm = norms != nullptr && (norms->q_norm != nullptr || norms->k_norm != nullptr);
+    if (norm && !(norms->eps > 0.f && std::isfinite(norms->eps))) return capi_fail(IQ2_ERR_INVALID_ARGUMENT, "%s: eps is not positive", op);
+    if (norm && norms->q_norm != nullptr && !has_q) return capi_fail(IQ2_ERR_INVALID_ARGUMENT, "%s: q_norm goes with q", op);
     if (t->tokens == 0) return IQ2_OK;
     if (t->tokens > (uint32_t)INT32_MAX) return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u tokens are too many", op, t->tokens);
     const size_t e = size_of(t->dtype);
@@ -112,6 +120,8 @@ int iq2_kv_cache_write(const iq2_kv_cache* cache, const iq2_kv_tokens* t, iq2_st
         if (t->rope_len == 0) return capi_fail(IQ2_ERR_ZERO_DIM, "%s: empty cos / sin", op);
         if ((rc = check_pointers(op, {{"positions", t->positions, 4}, {"cos", t->cos, 4}, {"sin", t->sin, 4}})) != IQ2_OK) return rc;
     }
+    if (norm && norms->q_norm != nullptr && (rc = check_pointers(op, {{"q_norm", norms->q_norm, 4}})) != IQ2_OK) return rc;
+    if (norm && norms->k_norm != nullptr && (rc = check_pointers(op, {{"k_norm", norms->k_norm, 4}})) != IQ2_OK) return rc;
     iq2::KvWriteParams p{};
     p.c = view(cache);
     p.k = view(t->k), p.v = view(t->v), p.q = view(t->q);
@@ -120,8 +130,22 @@ int iq2_kv_cache_write(const iq2_kv_cache* cache, const iq2_kv_tokens* t, iq2_st
     p.dtype = t->dtype, p.q_out_dtype = t->q_out_dtype, p.interleaved = t->interleaved != 0;
     p.vec = rows_aligned(t->k, e, 16) && rows_aligned(t->v, e, 16) && (!has_q || rows_aligned(t->q, e, 16)) &&
             (!rope || (reinterpret_cast<uintptr_t>(t->cos) % 16 == 0 && reinterpret_cast<uintptr_t>(t->sin) % 16 == 0));
+    if (norm) {
+        p.q_norm = norms->q_norm, p.k_norm = norms->k_norm;
+        p.q_norm_stride = norms->q_per_head ? cache->head_dim : 0, p.k_norm_stride = norms->k_per_head ? cache->head_dim : 0;
+        p.eps = norms->eps, p.inv_d = 1.0 / cache->head_dim;
+        p.vec = p.vec && reinterpret_cast<uintptr_t>(p.q_norm) % 16 == 0 && reinterpret_cast<uintptr_t>(p.k_norm) % 16 == 0;
+    }
     const cudaError_t err = iq2::launch_kv_write(p, reinterpret_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? IQ2_OK : capi_cuda_fail(op, err);
+}
+
+int iq2_kv_cache_write(const iq2_kv_cache* cache, const iq2_kv_tokens* tokens, iq2_stream_t stream) {
+    return cache_write("iq2_kv_cache_write", cache, tokens, nullptr, stream);
+}
+
+int iq2_kv_cache_write_normed(const iq2_kv_cache* cache, const iq2_kv_tokens* tokens, const iq2_head_norms* norms, iq2_stream_t stream) {
+    return cache_write("iq2_kv_cache_write_normed", cache, tokens, norms, stream);
 }
 
 int iq2_kv_cache_read(const iq2_kv_cache* cache, const int32_t* block_table, uint32_t table_width, uint32_t sequences,
@@ -141,6 +165,31 @@ int iq2_kv_cache_read(const iq2_kv_cache* cache, const int32_t* block_table, uin
     if (starts != nullptr && (rc = check_pointers(op, {{"starts", starts, 4}})) != IQ2_OK) return rc;
     const iq2::KvReadParams p{view(cache), block_table, starts, cu_seqlens, table_width, sequences, total, k_out, v_out, out_dtype};
     const cudaError_t err = iq2::launch_kv_read(p, reinterpret_cast<cudaStream_t>(stream));
+    return err == cudaSuccess ? IQ2_OK : capi_cuda_fail(op, err);
+}
+
+int iq2_kv_pages_step(const iq2_kv_pages* pages, const iq2_kv_step* step, iq2_stream_t stream) {
+    const char* op = "iq2_kv_pages_step";
+    iq2::capi_ok();
+    if (pages == nullptr || step == nullptr) return capi_fail(IQ2_ERR_INVALID_ARGUMENT, "%s: NULL pages or step", op);
+    const iq2_kv_pages& g = *pages;
+    const iq2_kv_step& t = *step;
+    if (g.sequences == 0 || g.table_width == 0 || g.num_pages == 0 || g.page_size == 0)
+        return capi_fail(IQ2_ERR_ZERO_DIM, "%s expects non-zero dimensions", op);
+    if (g.sequences > iq2::PAGES_MOST_SEQS)
+        return capi_fail(IQ2_ERR_UNSUPPORTED, "%s: %u sequences are more than %u", op, g.sequences, iq2::PAGES_MOST_SEQS);
+    if ((uint64_t)g.num_pages * g.page_size > (uint64_t)INT32_MAX)
+        return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u pages of %u tokens are too large", op, g.num_pages, g.page_size);
+    if (t.total > (uint32_t)INT32_MAX) return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u tokens are too many", op, t.total);
+    int rc = check_pointers(op, {{"block_table", g.block_table, 4}, {"seq_lens", g.seq_lens, 4}, {"free_pages", g.free_pages, 4},
+                                 {"free_count", g.free_count, 4}, {"new_lens", t.new_lens, 4}, {"cu_seqlens_q", t.cu_seqlens_q, 4},
+                                 {"cu_seqlens_k", t.cu_seqlens_k, 4}, {"granted", t.granted, 4}});
+    if (rc == IQ2_OK && t.keep != nullptr) rc = check_pointers(op, {{"keep", t.keep, 4}});
+    if (rc == IQ2_OK && t.total > 0) rc = check_pointers(op, {{"slots", t.slots, 4}, {"positions", t.positions, 4}});
+    if (rc != IQ2_OK) return rc;
+    iq2::PagesParams p{g.block_table, g.seq_lens, g.free_pages, g.free_count, g.sequences, g.table_width, g.num_pages, g.page_size,
+                       t.keep, t.new_lens, t.total, t.slots, t.positions, t.cu_seqlens_q, t.cu_seqlens_k, t.granted, {}};
+    const cudaError_t err = iq2::launch_kv_pages_step(p, reinterpret_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? IQ2_OK : capi_cuda_fail(op, err);
 }
 

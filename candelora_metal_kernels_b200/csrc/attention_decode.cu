@@ -25,6 +25,10 @@
 //     the keys have little there), which the 2^-8 of bf16 activations hides. For f32 and f16 ones (8e-6 against 1e-6 over
 //     the whole) a byte with 0x64 above it is 1024 + code + 128, and a subtraction makes it the code itself: 51.0 instead of
 //     49.2 us for 100001 tokens.
+//   * 4-bit codes become f16 values code g 2^-12 by one AND-OR and one multiply-add a pair: four bits u under the exponent of 1
+//     are 1 + u / 16 or 1 + u / 256, and A = G, B = -1.5 G or A = 16 G, B = -16.5 G make (u - 8) G / 16 of them, exactly, since g has
+//     four significant bits; G = g 2^-8 are the e4m3 bits moved by seven places. A thread's 16 bytes of a key row are one
+//     group, so that it needs one scale a key; of the values it needs those of two tokens and each group at a time.
 //   * The key scale multiplies s, the value scale w multiplies p. The reference m of a head's exponents moves when a product
 //     p w has grown by more than 2^8, so that p w keeps to the range of f16; the sum of p itself is f32 (int8 caches: held by
 //     2^-16 of itself, since p alone may reach 2^122).
@@ -55,6 +59,9 @@ constexpr uint32_t AD_ITEM_COST = 3;
 // 2^-107, just below the smallest value scale that a row of the cache has (its largest value, 2^-100 or more, over 127). A row of
 // zeros has 0 and counts as this, so that the reference stays finite; its codes are zeros.
 constexpr float AD_MIN_SCALE = 6.16297582e-33f;
+// 4-bit rows' scales, 2^-111 or more, multiply p as 2^9 of themselves (2^126 at most); a row of zeros counts as 2^-103.
+constexpr float AD_I4_UP = 512.f, AD_I4_MIN_SCALE = 9.86076132e-32f;
+constexpr float AD_I4_UNIT = 4096.f;             // 2^12: what 4-bit values are held by
 // p times the value scale: the power of two that it has at the reference, and how far it may grow before that moves.
 template <bool BF>
 constexpr float AD_TOP = BF ? 0.f : 7.f;
@@ -67,17 +74,18 @@ constexpr uint32_t CODE_ZERO = 0x00800080u;      // two codes of 0 as f16: 128 2
 constexpr float CODE_UNIT = 16777216.f;          // 2^24
 constexpr float LOG2E = 1.44269504f;
 
-enum CacheKind { CK_F16, CK_BF16, CK_INT8 };
+enum CacheKind { CK_F16, CK_BF16, CK_INT8, CK_INT4 };
 
 template <int DP, int KIND, bool WIDE>
 struct DecodeShape {
     static constexpr int PIECES = WIDE && KIND == CK_BF16 ? 3 : 2;
-    static constexpr int ESIZE = KIND == CK_INT8 ? 1 : 2;
-    static constexpr int TOK = KIND == CK_INT8 ? 32 : 16;  // tokens of a warp's stage: 8 KB of K and V at DP = 128
-    static constexpr int UNIT = TOK * 4;                   // tokens that the line of work is cut at: 32 KB at DP = 128
-    static constexpr int ROW = DP * ESIZE;                 // bytes of a padded K or V row
+    static constexpr int EBITS = KIND == CK_INT4 ? 4 : KIND == CK_INT8 ? 8 : 16;
+    static constexpr int TOK = EBITS < 16 ? 32 : 16;       // tokens of a warp's stage: 8 KB of K and V at DP = 128 (4 bits: 4 KB)
+    static constexpr int UNIT = TOK * 4;                   // tokens that the line of work is cut at: 32 KB at DP = 128 (16 KB)
+    static constexpr int ROW = DP * EBITS / 8;             // bytes of a padded K or V row
     static constexpr int CHUNKS = ROW / 16;
-    static constexpr int SCALES = KIND == CK_INT8 ? TOK * 8 : 0;
+    // scales of the rows of K and V, then of their groups (a word a row)
+    static constexpr int SCALES = KIND == CK_INT4 ? TOK * 16 : KIND == CK_INT8 ? TOK * 8 : 0;
     static constexpr int STAGE = 2 * TOK * ROW + SCALES;
     static constexpr int RING = AD_STAGES * STAGE;
     static constexpr int Q_BYTES = PIECES * AD_HEADS * DP * 2;
@@ -170,6 +178,28 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t bytes, uint32_t sel) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What makes f16 values of 4-bit codes: (a, b) of the upper and the lower bits of a byte, for the two halves of a word.
+struct CodeScale {
+    __half2 a_hi, b_hi, a_lo, b_lo;
+};
+// bytes: the e4m3 scales of the two halves in bytes 1 and 3, zeros in 0 and 2.
+__device__ __forceinline__ CodeScale code_scale(uint32_t bytes) {
+    const uint32_t moved = bytes >> 1;
+    const __half2 g = *reinterpret_cast<const __half2*>(&moved);
+    return {g, __hmul2(g, __float2half2_rn(-1.5f)), __hmul2(g, __float2half2_rn(16.f)), __hmul2(g, __float2half2_rn(-16.5f))};
+}
+// The values of a word's codes: v[0], v[1] the lower and upper bits of bytes 0 and 2, v[2], v[3] of bytes 1 and 3.
+__device__ __forceinline__ void code_values(uint32_t w, const CodeScale& s, uint32_t (&v)[4]) {
+    const uint32_t even = w << 2, odd = w >> 6;
+    const uint32_t u[4] = {(even & 0x003C003Cu) | 0x3C003C00u, (even & 0x03C003C0u) | 0x3C003C00u, (odd & 0x003C003Cu) | 0x3C003C00u,
+                           (odd & 0x03C003C0u) | 0x3C003C00u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&u[i]), i % 2 ? s.a_hi : s.a_lo, i % 2 ? s.b_hi : s.b_lo);
+        v[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -179,10 +209,12 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // Byte offset of 16-byte chunk c of row r in a K or V stage. The readers of a phase must meet eight different 16-byte
 // columns of the 128-byte bank line:
 //   ldmatrix (16-bit K and V, int8 V) reads eight rows of one chunk: column ^ row;
-//   int8 K is read by plain 16-byte loads, two rows of four chunks at a time: odd rows swap the halves of their line.
-// 64-byte rows (int8, DP = 64) share a line in pairs: ldmatrix needs column ^ (row / 2) inside each half.
+//   int8 and 4-bit K is read by plain 16-byte loads, two rows of four chunks at a time: odd rows swap the halves of their line.
+// 64-byte rows (int8 at DP = 64, 4 bits at 128) share a line in pairs: ldmatrix needs column ^ (row / 2) inside each half.
+// 32-byte rows (4 bits at DP = 64) share it in fours: column ^ (row / 4).
 template <int CHUNKS, bool PLAIN>
 __device__ __forceinline__ uint32_t stage_offset(uint32_t r, uint32_t c) {
+    if (CHUNKS == 2) return r * 32 + (PLAIN ? c : c ^ ((r >> 2) & 1)) * 16;
     if (CHUNKS == 4) return r * 64 + (PLAIN ? c : c ^ ((r >> 1) & 3)) * 16;
     return (r * CHUNKS + (PLAIN ? c ^ ((r & 1) * 4) : c ^ (r & 7))) * 16;
 }
@@ -229,7 +261,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     decode_kernel(const __grid_constant__ DecodeArgs a) {
     using S = DecodeShape<DP, KIND, WIDE>;
     // WIDE: f32 activations, and f16 ones over int8 codes
-    constexpr bool BF = KIND == CK_BF16, I8 = KIND == CK_INT8, THIRD = BF && WIDE, SHIFTED = I8 && !WIDE;
+    constexpr bool BF = KIND == CK_BF16, I8 = KIND == CK_INT8, I4 = KIND == CK_INT4, CODES = I8 || I4, THIRD = BF && WIDE, SHIFTED = I8 && !WIDE;
     constexpr int TOK = S::TOK, UNIT = S::UNIT, NT = DP / 8, KS = DP / 16, ST = TOK / 8;
     constexpr uint32_t ALL = TOK == 32 ? 0xFFFFFFFFu : (1u << TOK) - 1;
     const DecodeParams& p = a.p;
@@ -312,7 +344,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     if (d < DP) __syncwarp();
     // a tile's rows lie side by side in one page, or each lane looks one row up
     const bool side_by_side = p.c.page_size % TOK == 0;
-    const uint32_t row_bytes = d * S::ESIZE, chunk = lane % S::CHUNKS, row0 = lane / S::CHUNKS;
+    const uint32_t row_bytes = d * S::EBITS / 8, chunk = lane % S::CHUNKS, row0 = lane / S::CHUNKS;
     constexpr int ROWS = 32 / S::CHUNKS;  // rows that the warp copies at a time
     auto page_of = [&](uint32_t tok) { return a.by_page.quotient(tok); };
     uint32_t pre_i = warp, pre_page = 0, pre_first = 0;  // the tile to copy next, its page, the first token of that page
@@ -352,13 +384,17 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             if (inside) {
 #pragma unroll
                 for (int i = 0; i < TOK / ROWS; ++i, pk += ROWS * row_bytes, pv += ROWS * row_bytes) {
-                    cp_async_16(dst + stage_offset<S::CHUNKS, I8>(row0 + i * ROWS, chunk), pk);
+                    cp_async_16(dst + stage_offset<S::CHUNKS, CODES>(row0 + i * ROWS, chunk), pk);
                     cp_async_16(dst + TOK * S::ROW + stage_offset<S::CHUNKS, false>(row0 + i * ROWS, chunk), pv);
                 }
             }
-            if (I8) {
+            if (CODES) {
                 cp_async_4(dst + 2 * TOK * S::ROW + lane * 4, p.c.k_scale + row + lane, 4);
                 cp_async_4(dst + 2 * TOK * S::ROW + TOK * 4 + lane * 4, p.c.v_scale + row + lane, 4);
+            }
+            if (I4) {
+                cp_async_4(dst + 2 * TOK * S::ROW + TOK * 8 + lane * 4, p.c.k_group + (row + lane) * 4, 4);
+                cp_async_4(dst + 2 * TOK * S::ROW + TOK * 12 + lane * 4, p.c.v_group + (row + lane) * 4, 4);
             }
         } else {
             const bool valid = lane < TOK && lane < left && pre_page < p.c.pages;
@@ -370,13 +406,17 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                 const int64_t src = __shfl_sync(0xFFFFFFFFu, mine, r);
                 const int64_t off = src < 0 ? 0 : src * row_bytes + chunk * 16;
                 if (inside) {
-                    cp_async_16(dst + stage_offset<S::CHUNKS, I8>(r, chunk), k + off, src < 0 ? 0 : 16);
+                    cp_async_16(dst + stage_offset<S::CHUNKS, CODES>(r, chunk), k + off, src < 0 ? 0 : 16);
                     cp_async_16(dst + TOK * S::ROW + stage_offset<S::CHUNKS, false>(r, chunk), v + off, src < 0 ? 0 : 16);
                 }
             }
-            if (I8) {
+            if (CODES) {
                 cp_async_4(dst + 2 * TOK * S::ROW + lane * 4, p.c.k_scale + (valid ? mine : 0), valid ? 4 : 0);
                 cp_async_4(dst + 2 * TOK * S::ROW + TOK * 4 + lane * 4, p.c.v_scale + (valid ? mine : 0), valid ? 4 : 0);
+            }
+            if (I4) {
+                cp_async_4(dst + 2 * TOK * S::ROW + TOK * 8 + lane * 4, p.c.k_group + (valid ? mine * 4 : 0), valid ? 4 : 0);
+                cp_async_4(dst + 2 * TOK * S::ROW + TOK * 12 + lane * 4, p.c.v_group + (valid ? mine * 4 : 0), valid ? 4 : 0);
             }
         }
         pre_i += AD_WARPS;
@@ -428,22 +468,24 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 #pragma unroll
                 for (int piece = 0; piece < S::PIECES; ++piece) {
                     const uint32_t h = pack_pair<BF>(rest, 0.f);
-                    q[piece * DP + lane + i * 32] = (uint16_t)h;
+                    // (4 bits: the pairs that a word's codes come out in, elements j and j + 4 of eight, side by side)
+                    const uint32_t e = lane + i * 32, at = I4 ? (e & ~7u) | ((e & 3) * 2 + ((e >> 2) & 1)) : e;
+                    q[piece * DP + at] = (uint16_t)h;
                     rest = (rest - unpack_pair<BF>(h).x) * AD_LOW<BF>;
                 }
             }
-            if (lane == 0) q_factor[warp] = p.scale * LOG2E * up * (SHIFTED ? CODE_UNIT : 1.f);
+            if (lane == 0) q_factor[warp] = p.scale * LOG2E * up * (SHIFTED ? CODE_UNIT : I4 ? AD_I4_UNIT : 1.f);
         }
         __syncthreads();
         // A fragments of S: k index 16 ks + 2t (+1, +8, +9). For int8 the k index is a relabelled dimension, so that a
-        // thread's codes of four k steps are 16 consecutive bytes of its row.
-        auto k_lo = [&](int ks) { return I8 ? (t + 4 * (ks / 4)) * 16 + (ks % 4) * 4 : ks * 16 + t * 2; };
+        // thread's codes of four k steps are 16 consecutive bytes of its row; for 4 bits, of two k steps a word of its DP / 8.
+        auto k_lo = [&](int ks) { return I4 ? t * (DP / 4) + ks * 4 : I8 ? (t + 4 * (ks / 4)) * 16 + (ks % 4) * 4 : ks * 16 + t * 2; };
         const uint32_t* const q_row = reinterpret_cast<const uint32_t*>(q_smem) + g * S::PIECES * (DP / 2);
         uint32_t qa[KS][4];
         float minus[4] = {0.f, 0.f, 0.f, 0.f};  // where S starts: minus its products with the 128s
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const uint32_t lo = k_lo(ks) / 2, hi = lo + (I8 ? 1 : 4);
+            const uint32_t lo = k_lo(ks) / 2, hi = lo + (CODES ? 1 : 4);
             qa[ks][0] = q_row[lo], qa[ks][1] = q_row[DP / 2 + lo];
             qa[ks][2] = q_row[hi], qa[ks][3] = q_row[DP / 2 + hi];
             if (SHIFTED) mma16816<BF>(minus, qa[ks], CODE_ZERO, CODE_ZERO);
@@ -452,6 +494,8 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         for (int j = 0; j < 4; ++j) minus[j] = -minus[j];
         auto joined = [](float high, float low) { return fmaf(low, 1.f / AD_LOW<BF>, high); };
         const float factor = q_factor[g];
+        // 4 bits: this thread's group of a key row, as bytes 1 and 3 of a word (all zeros past head_dim)
+        const uint32_t group_of = t * (DP / 4) / I4_GROUP, group_sel = group_of * I4_GROUP < d ? 0x0404u | group_of * 0x1010u : 0x4444u;
         float o[NT][4], o_off[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
@@ -473,7 +517,28 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             for (int n = 0; n < ST; ++n)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s[n][j] = minus[j];
-            if (I8) {
+            const uint32_t* const groups = reinterpret_cast<const uint32_t*>(ring + stage * S::STAGE + 2 * TOK * S::ROW + TOK * 8);
+            if (I4) {
+#pragma unroll
+                for (int n = 0; n < ST; ++n) {
+                    uint32_t w[DP / 32];
+                    if (DP == 128) {
+                        const uint4 u = ld_shared_v4<0>(k_at + stage_offset<S::CHUNKS, true>(n * 8 + g, t));
+                        w[0] = u.x, w[1] = u.y, w[2 % (DP / 32)] = u.z, w[3 % (DP / 32)] = u.w;
+                    } else {
+                        const uint2 u = ld_shared_v2_volatile(k_at + (n * 8 + g) * S::ROW + t * 8);
+                        w[0] = u.x, w[1] = u.y;
+                    }
+                    const CodeScale scale = code_scale(prmt(groups[n * 8 + g], 0u, group_sel));
+#pragma unroll
+                    for (int j = 0; j < DP / 32; ++j) {
+                        uint32_t v[4];
+                        code_values(w[j], scale, v);
+                        mma16816<BF>(s[n], qa[2 * j], v[0], v[1]);
+                        mma16816<BF>(s[n], qa[2 * j + 1], v[2], v[3]);
+                    }
+                }
+            } else if (I8) {
 #pragma unroll
                 for (int q4 = 0; q4 < KS / 4; ++q4) {
                     uint4 w[ST];
@@ -508,10 +573,11 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 #pragma unroll
             for (int n = 0; n < ST; ++n) {
                 float2 ks2 = make_float2(factor, factor), vs2 = make_float2(1.f, 1.f);
-                if (I8) {
+                if (CODES) {
+                    constexpr float UP = I4 ? AD_I4_UP : 1.f, LEAST = I4 ? AD_I4_MIN_SCALE : AD_MIN_SCALE;
                     const float2 sk = scales[n * 4], sv = scales[TOK / 2 + n * 4];
                     ks2 = make_float2(sk.x * factor, sk.y * factor);
-                    vs2 = make_float2(max_nan(sv.x, AD_MIN_SCALE), max_nan(sv.y, AD_MIN_SCALE));
+                    vs2 = make_float2(max_nan(sv.x * UP, LEAST), max_nan(sv.y * UP, LEAST));
                 }
                 x[n][0] = joined(s[n][0], s[n][2]) * ks2.x, x[n][1] = joined(s[n][1], s[n][3]) * ks2.y;
                 vs[n][0] = vs2.x, vs[n][1] = vs2.y;
@@ -532,7 +598,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         e[n][j] = exp2_approx(x[n][j] - base);
-                        w[n][j] = I8 ? e[n][j] * vs[n][j] : e[n][j];
+                        w[n][j] = CODES ? e[n][j] * vs[n][j] : e[n][j];
                         top = fmaxf(top, w[n][j]);
                     }
                 if (!__any_sync(0xFFFFFFFFu, top > AD_LAZY<BF> || m == -INFINITY)) break;
@@ -541,7 +607,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
 #pragma unroll
                 for (int n = 0; n < ST; ++n)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) most = fmaxf(most, I8 ? x[n][j] + __log2f(vs[n][j]) : x[n][j]);
+                    for (int j = 0; j < 2; ++j) most = fmaxf(most, CODES ? x[n][j] + __log2f(vs[n][j]) : x[n][j]);
                 most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
                 most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
                 const float next = fmaxf(m, most), keep = m == -INFINITY ? 0.f : exp2_approx(m - next);
@@ -561,7 +627,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             uint32_t pa[TOK / 16][4], pa3[TOK / 16][4];
 #pragma unroll
             for (int n = 0; n < ST; ++n) {
-                l = fmaf(e[n][0] + e[n][1], I8 ? AD_SUM : 1.f, l);
+                l = fmaf(e[n][0] + e[n][1], CODES ? AD_SUM : 1.f, l);
                 const uint32_t high = pack_pair<BF>(w[n][0], w[n][1]);
                 const float2 h = unpack_pair<BF>(high);
                 const uint32_t low = pack_pair<BF>((w[n][0] - h.x) * AD_LOW<BF>, (w[n][1] - h.y) * AD_LOW<BF>);
@@ -574,7 +640,25 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                 }
             }
 
-            if (I8) {
+            if (I4) {
+                uint2 gw[ST];  // the groups' scales of tokens 8 n + 2t, + 1
+#pragma unroll
+                for (int n = 0; n < ST; ++n) gw[n] = *reinterpret_cast<const uint2*>(groups + TOK + n * 8 + t * 2);
+#pragma unroll
+                for (int c = 0; c < S::CHUNKS; ++c) {
+                    uint32_t r[4];  // group c of tokens 0-7, 8-15, 16-23, 24-31; each word: dimensions 4g to 4g + 3 of two tokens
+                    ldmatrix4_trans(r, v_at + stage_offset<S::CHUNKS, false>(lane, c));
+#pragma unroll
+                    for (int ks = 0; ks < TOK / 16; ++ks) {
+                        uint32_t v0[4], v1[4];
+                        // (a selector of 8 + i is the sign of byte i in all bits: none)
+                        code_values(r[ks * 2], code_scale(prmt(gw[ks * 2].x, gw[ks * 2].y, 0x4C08u + c * 0x1111u)), v0);
+                        code_values(r[ks * 2 + 1], code_scale(prmt(gw[ks * 2 + 1].x, gw[ks * 2 + 1].y, 0x4C08u + c * 0x1111u)), v1);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma16816<BF>(o[(c * 4 + j) % NT], pa[ks], v0[j], v1[j]);
+                    }
+                }
+            } else if (I8) {
 #pragma unroll
                 for (int ks = 0; ks < TOK / 16; ++ks)
                     if (SHIFTED) mma16816<BF>(o_off, pa[ks], CODE_ZERO, CODE_ZERO);
@@ -606,11 +690,11 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             __syncwarp();
             stage = stage == AD_STAGES - 1 ? 0 : stage + 1;
         }
-        if (I8) {  // the 128s off, and the codes' unit and the sums' on
+        if (CODES) {  // the 128s off, and the codes' unit and the sums' on
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[n][j] = SHIFTED ? (o[n][j] - o_off[j]) * (CODE_UNIT * AD_SUM) : o[n][j] * AD_SUM;
+                for (int j = 0; j < 4; ++j) o[n][j] = SHIFTED ? (o[n][j] - o_off[j]) * (CODE_UNIT * AD_SUM) : o[n][j] * (I4 ? AD_SUM * (AD_I4_UNIT / AD_I4_UP) : AD_SUM);
         }
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
         l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
@@ -620,11 +704,13 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         if (!next.done()) load_q(next);
 
         // ---- the eight warps' (o, m, l) of the item, through four slots of shared memory ----
+        // accumulator n's columns of this thread: int8, the even or odd dimensions of a 16-dimension chunk; 4 bits, every fourth of 32
+        constexpr uint32_t STEP = I4 ? 4 : I8 ? 2 : 1;
+        auto column = [&](int n) { return I4 ? (n / 4) * 32 + n % 4 + t * 8 : I8 ? (n / 2) * 16 + n % 2 + t * 4 : n * 8 + t * 2; };
         auto put = [&](float* slot) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                // int8: accumulator columns are the even and odd dimensions of a 16-dimension chunk
-                const uint32_t e0 = KIND == CK_INT8 ? (n / 2) * 16 + n % 2 + t * 4 : n * 8 + t * 2, e1 = e0 + (KIND == CK_INT8 ? 2 : 1);
+                const uint32_t e0 = column(n), e1 = e0 + STEP;
                 slot[g * DP + e0] = joined(o[n][0], o[n][2]);
                 slot[g * DP + e1] = joined(o[n][1], o[n][3]);
             }
@@ -639,7 +725,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             l = l * f1 + l2 * f2, m = both;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const uint32_t e0 = KIND == CK_INT8 ? (n / 2) * 16 + n % 2 + t * 4 : n * 8 + t * 2, e1 = e0 + (KIND == CK_INT8 ? 2 : 1);
+                const uint32_t e0 = column(n), e1 = e0 + STEP;
                 o[n][0] = joined(o[n][0], o[n][2]) * f1 + slot[g * DP + e0] * f2, o[n][2] = 0.f;
                 o[n][1] = joined(o[n][1], o[n][3]) * f1 + slot[g * DP + e1] * f2, o[n][3] = 0.f;
             }
@@ -749,6 +835,7 @@ cudaError_t launch(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
 template <int DP>
 cudaError_t launch_kind(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
     const bool wide = a.p.dtype == kF32;
+    if (a.p.c.dtype == kInt4) return launch<DP, CK_INT4, false>(a, blocks, stream);
     if (a.p.c.dtype == kInt8) return a.p.dtype != kBf16 ? launch<DP, CK_INT8, true>(a, blocks, stream) : launch<DP, CK_INT8, false>(a, blocks, stream);
     if (a.p.c.dtype == kF16) return launch<DP, CK_F16, false>(a, blocks, stream);
     return wide ? launch<DP, CK_BF16, true>(a, blocks, stream) : launch<DP, CK_BF16, false>(a, blocks, stream);
@@ -757,7 +844,7 @@ cudaError_t launch_kind(const DecodeArgs& a, uint32_t blocks, cudaStream_t strea
 }  // namespace
 
 bool attention_decode_fits(const KvCacheView& c, uint32_t table_width, uint32_t q_heads) {
-    const uint32_t unit = c.dtype == kInt8 ? DecodeShape<64, CK_INT8, false>::UNIT : DecodeShape<64, CK_F16, false>::UNIT;
+    const uint32_t unit = c.dtype == kInt8 || c.dtype == kInt4 ? DecodeShape<64, CK_INT8, false>::UNIT : DecodeShape<64, CK_F16, false>::UNIT;
     const uint64_t tokens = std::min<uint64_t>((uint64_t)table_width * c.page_size, INT32_MAX);
     const uint64_t items = (uint64_t)c.heads * ((q_heads / c.heads + AD_HEADS - 1) / AD_HEADS);
     return ((tokens + unit - 1) / unit + AD_ITEM_COST) * items <= (uint64_t)UINT32_MAX;

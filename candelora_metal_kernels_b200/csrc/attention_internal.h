@@ -7,8 +7,9 @@
 
 namespace iq2 {
 
-// Element types, numbered as IQ2_DTYPE_* of the C ABI; a cache adds int8 (IQ2_KV_INT8).
-constexpr int kF32 = 0, kF16 = 1, kBf16 = 2, kInt8 = 3;
+// Element types, numbered as IQ2_DTYPE_* of the C ABI; a cache adds int8 (IQ2_KV_INT8) and 4-bit codes (IQ2_KV_INT4).
+constexpr int kF32 = 0, kF16 = 1, kBf16 = 2, kInt8 = 3, kInt4 = 4;
+constexpr uint32_t I4_GROUP = 32;  // elements of a 4-bit row that share a scale
 
 // Division of n < 2^31 by a divisor that is known before the launch, as a product: with 2^s the power of two at or above
 // the divisor, floor(n / divisor) = (n magic) >> (31 + s) for magic = floor(2^(31 + s) / divisor) + 1.
@@ -27,12 +28,14 @@ struct Divisor {
 };
 
 // A paged cache (iq2_kv_cache): k, v [pages][heads][page_size][d], k_scale, v_scale f32 [pages][heads][page_size]
-// for int8 codes. Token `pos` of a sequence lives in page block_table[pos / page_size], row pos % page_size.
+// for int8 codes; 4-bit codes, two a byte, have them too and e4m3 scales k_group, v_group [pages][heads][page_size][4] of
+// I4_GROUP elements each. Token `pos` of a sequence lives in page block_table[pos / page_size], row pos % page_size.
 struct KvCacheView {
     void *k, *v;
     float *k_scale, *v_scale;
     uint32_t pages, heads, page_size, d;
     int dtype;
+    uint8_t *k_group, *v_group;
 };
 
 // Rows of a [tokens][heads][d] tensor: element strides of the first two dimensions, the last one contiguous.
@@ -50,7 +53,10 @@ struct KvWriteParams {
     uint32_t tokens, q_heads, rope_len;
     int dtype, q_out_dtype;
     bool interleaved;
-    bool vec;  // every row of the inputs and tables starts on a 16-byte boundary
+    bool vec;  // every row of the inputs, tables and norm weights starts on a 16-byte boundary
+    const float *q_norm, *k_norm;                 // weights of the heads' norms, null: none
+    uint32_t q_norm_stride, k_norm_stride;        // from one head's weights to the next's: 0 or d
+    double eps, inv_d;                            // inv_d: 1 / d
     Divisor by_heads, by_page;  // set by the launch: heads of a token (q, k and v), tokens of a page
 };
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);
@@ -63,6 +69,18 @@ struct KvReadParams {
     int out_dtype;
 };
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream);
+
+// The pages of a batch's sequences (iq2_kv_pages) and a step of them (iq2_kv_step).
+struct PagesParams {
+    int32_t *table, *lens, *free_pages, *free_count;
+    uint32_t seqs, width, pages, page_size;
+    const int32_t *keep, *new_lens;  // keep: null = all
+    uint32_t total;
+    int32_t *slots, *positions, *cu_q, *cu_k, *granted;
+    Divisor by_page;  // set by the launch
+};
+constexpr uint32_t PAGES_MOST_SEQS = 8192;
+cudaError_t launch_kv_pages_step(const PagesParams& p, cudaStream_t stream);
 
 struct DecodeParams {
     KvCacheView c;

@@ -6,6 +6,12 @@
 // with every product and sum rounded by itself in f32, so that a result does not depend on how the compiler fuses.
 // int8 rows (one token and head): m = max |x|, scale = m / 127, code = rint(x * (127 / m)); m < 2^-100 gives zeros (the
 // quotient would overflow), and a row with an infinity or NaN gets a NaN scale, so that it reads back as NaN.
+// 4-bit rows: s = the power of two with 224 < m / 7s <= 448, a group's g = e4m3(m_g / 7s), code = the integer nearest to
+// x / (s g), ties to even, at most 7 (g may be 2^-4 of itself below m_g / 7s: 7.44 still rounds to 7). Steps s g of four
+// significant bits make the values exact in 16 bits, and codes of 16-bit inputs are those of the quotient itself, whatever the
+// arithmetic: a code is taken from the product with 1 / (s g) and the remainder x - code s g, exact in f32, says where that is off.
+// Norms: y = (x r) w, r = 1 / sqrt(mean(x^2) + eps) summed and taken in 64 bits and rounded to f32, so that r, and with it the
+// codes next to borders, does not depend on the order of the sum.
 // Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 18.3 us over 0.9 GB of inputs and
 // outputs in turn, 4190 GB/s (12.8 over 0.2 GB, where the L2 keeps part of the outputs); of 8800 tokens, f32 into an int8 cache,
 // with the read back 67.5 us, 5380 GB/s; read of 89091 tokens to bf16, of an int8 cache 97 us, 5680 GB/s, of a bf16 one 117 us,
@@ -116,6 +122,87 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
     return prmt(prmt(code(x[0]), code(x[1]), 0x0040u), prmt(code(x[2]), code(x[3]), 0x0040u), 0x5410u);
 }
 
+// The cosines and sines of a thread's V pairs: (a[i], b[i]), or interleaved those of a and then those of b.
+template <int V>
+__device__ __forceinline__ void load_turns(const KvWriteParams& p, int64_t row, uint32_t lane, float (&c)[V], float (&s)[V]) {
+    if (!p.interleaved) {
+        load_angles(p.cos + row + lane * V, p.vec, c), load_angles(p.sin + row + lane * V, p.vec, s);
+        return;
+    }
+    const int64_t i0 = row + lane * (V / 2), i1 = i0 + p.c.d / 4;
+    float c0[V / 2], s0[V / 2], c1[V / 2], s1[V / 2];
+    load_angles(p.cos + i0, p.vec, c0), load_angles(p.sin + i0, p.vec, s0);
+    load_angles(p.cos + i1, p.vec, c1), load_angles(p.sin + i1, p.vec, s1);
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) c[i] = c0[i], s[i] = s0[i], c[V / 2 + i] = c1[i], s[V / 2 + i] = s1[i];
+}
+
+// The value of e4m3 bits without a sign, and the bits nearest to x >= 0.
+__device__ __forceinline__ float e4m3_value(uint32_t bits) { return __uint_as_float(bits << 20) * 1.32922800e36f; }  // 2^120
+__device__ __forceinline__ uint32_t e4m3_pair(float low, float high) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
+    return r;
+}
+
+// V codes of a group with the step s g (0: all of them are 0) as nibbles.
+template <int V>
+__device__ __forceinline__ uint32_t codes_int4(const float (&x)[V], float step) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        float c = __fadd_rn(__fadd_rn(__fmul_rn(x[i], inv), 12582912.0f), -12582912.0f);
+        const float rest = __fmaf_rn(-c, step, x[i]), over = fabsf(rest) - 0.5f * step;
+        if (over > 0.f || (over == 0.f && ((int)c & 1))) c += copysignf(1.f, rest);
+        c = fminf(fmaxf(c, -7.f), 7.f);
+        if (step == 0.f) c = 0.f;
+        w |= (__float_as_uint(c + 12582920.0f) & 15u) << (4 * i);
+    }
+    return w;
+}
+
+// A row of the 4-bit cache: m is the row's maximum, a thread has V elements from lane V of each half, which lie in one group.
+// Called by whole warps.
+template <int LANES, int V>
+__device__ __forceinline__ void store_int4(const KvCacheView& cache, int64_t row, uint32_t half, uint32_t lane, bool is_v, bool wanted, float m,
+                                           const float (&a)[V], const float (&b)[V]) {
+    constexpr uint32_t PIECES = I4_GROUP / V;  // threads' pieces of a group
+    __shared__ float4 held[KW_THREADS / LANES][2 * LANES / 4 + 1];
+    float* const piece = reinterpret_cast<float*>(held[threadIdx.x / LANES]);
+    const uint32_t at_a = lane * V, at_b = half + lane * V;
+    float ma = 0.f, mb = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; ++i) ma = max_nan(ma, fabsf(a[i])), mb = max_nan(mb, fabsf(b[i]));
+    if (at_a < half) piece[at_a / V] = ma, piece[at_b / V] = mb;
+    __syncwarp();
+    if (!wanted) return;
+#pragma unroll
+    for (uint32_t i = 0; i < PIECES; ++i) {
+        ma = max_nan(ma, piece[at_a / I4_GROUP * PIECES + i]);
+        mb = max_nan(mb, piece[at_b / I4_GROUP * PIECES + i]);
+    }
+    const bool finite = m < __int_as_float(0x7F800000), some = finite && m >= MIN_AMAX;
+    // s and 1 / s: the exponent of m, less 11, and one more where m's fraction passes 3136 / 2048
+    const uint32_t bits = __float_as_uint(m), e = some ? (bits >> 23) - 11 + ((bits & 0x7FFFFFu) > 0x440000u) : 127u;
+    const float s = some ? __uint_as_float(e << 23) : 0.f, up = __uint_as_float((254u - e) << 23);
+    const uint32_t g = some ? e4m3_pair(__fdiv_rn(ma, 7.f) * up, __fdiv_rn(mb, 7.f) * up) : 0u;
+    const uint32_t wa = codes_int4(a, some ? s * e4m3_value(g & 0xFFu) : 0.f), wb = codes_int4(b, some ? s * e4m3_value(g >> 8) : 0.f);
+    uint8_t* const dst = static_cast<uint8_t*>(is_v ? cache.v : cache.k) + row * half;
+    if (V == 4) {
+        *reinterpret_cast<uint16_t*>(dst + at_a / 2) = (uint16_t)wa;
+        *reinterpret_cast<uint16_t*>(dst + at_b / 2) = (uint16_t)wb;
+    } else {
+        *reinterpret_cast<uint32_t*>(dst + at_a / 2) = wa;
+        *reinterpret_cast<uint32_t*>(dst + at_b / 2) = wb;
+    }
+    uint8_t* const groups = (is_v ? cache.v_group : cache.k_group) + row * 4;
+    if (at_a % I4_GROUP == 0) groups[at_a / I4_GROUP] = (uint8_t)g;
+    if (at_b % I4_GROUP == 0) groups[at_b / I4_GROUP] = (uint8_t)(g >> 8);
+    if (lane == 0) (is_v ? cache.v_scale : cache.k_scale)[row] = finite ? s : __int_as_float(0x7FC00000);
+}
+
 // LANES threads (a power of two >= d / 2V) take a row: lane l holds the V elements from Vl of each half, 16 bytes of the input,
 // so that a pair of either rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head)
 // with the heads of q, then k, then v. A thread has one row (two or three in flight: 2048 tokens 16.5 / 18.5 against 14.5 us);
@@ -123,8 +210,8 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
 // the kernel's (widened as it came, in pieces of eight bytes, bf16 rows of 8800 tokens took 61.5 us into a bf16 cache, not 43.6).
 // Blocks of an SM: eight for f32 rows (8800 tokens into a bf16 cache 54.0 us; with all the registers that the compiler likes
 // 58.8), six for the 16 values of a thread that 16-bit rows make (43.6 us; five 45.0, seven 44.9, with spills).
-template <int LANES, int IN>
-__global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
+template <int LANES, int IN, bool NORM, bool I4>
+__global__ void __launch_bounds__(KW_THREADS, NORM || I4 ? 4 : IN == kF32 ? 8 : 6) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
     constexpr int V = IN == kF32 ? 4 : 8;
     const uint32_t lane = threadIdx.x % LANES, r = blockIdx.x * (KW_THREADS / LANES) + threadIdx.x / LANES;
     const uint32_t heads = p.q_heads + 2 * p.c.heads, half = p.c.d / 2;
@@ -134,7 +221,43 @@ __global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kerne
     const uint32_t h = head - (is_q ? 0 : is_v ? p.q_heads + p.c.heads : p.q_heads);
     float a[V] = {}, b[V] = {};
     int32_t slot = 0;
-    if (active) {
+    if (NORM) {
+        uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;  // (rows that are not there add up to nothing)
+        float c[V], s[V];
+        const float* const weights = !active || is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
+        const bool rotated = active && p.cos != nullptr && !is_v;
+        if (active) {
+            const RowsView& in = is_q ? p.q : is_v ? p.v : p.k;
+            const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * V;
+            wa = load16<IN>(in.p, at, p.vec), wb = load16<IN>(in.p, at + half, p.vec);
+            if (!is_q) slot = __ldg(p.slots + t);
+            if (rotated) load_turns(p, (int64_t)min((uint32_t)max(__ldg(p.positions + t), 0), p.rope_len - 1) * half, lane, c, s);
+        }
+        widen<IN>(wa, a), widen<IN>(wb, b);
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) sum = fma((double)a[i], (double)a[i], sum), sum = fma((double)b[i], (double)b[i], sum);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (weights != nullptr) {
+            const float r = (float)rsqrt(sum * p.inv_d + p.eps);
+            const float* const at = weights + h * (is_q ? p.q_norm_stride : p.k_norm_stride) + lane * V;
+            float w[V];
+            load_angles(at, p.vec, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) a[i] = __fmul_rn(__fmul_rn(a[i], r), w[i]);
+            load_angles(at + half, p.vec, w);
+#pragma unroll
+            for (int i = 0; i < V; ++i) b[i] = __fmul_rn(__fmul_rn(b[i], r), w[i]);
+        }
+        if (rotated && p.interleaved) {
+#pragma unroll
+            for (int i = 0; i < V / 2; ++i) rotate(a[2 * i], a[2 * i + 1], c[i], s[i]), rotate(b[2 * i], b[2 * i + 1], c[V / 2 + i], s[V / 2 + i]);
+        } else if (rotated) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) rotate(a[i], b[i], c[i], s[i]);
+        }
+    } else if (active) {
         const RowsView& in = is_q ? p.q : is_v ? p.v : p.k;
         const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * V;
         const uint4 wa = load16<IN>(in.p, at, p.vec), wb = load16<IN>(in.p, at + half, p.vec);
@@ -164,7 +287,7 @@ __global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kerne
         store_values(p.q_out, at, p.q_out_dtype, a);
         store_values(p.q_out, at + half, p.q_out_dtype, b);
     }
-    if (p.c.dtype != kInt8) {
+    if (!I4 && p.c.dtype != kInt8) {
         if (is_q) return;
     } else if (__all_sync(0xFFFFFFFFu, is_q)) {  // (a warp that goes on shuffles as a whole)
         return;
@@ -173,7 +296,7 @@ __global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kerne
     const uint32_t page = p.by_page.quotient((uint32_t)slot & 0x7FFFFFFFu);
     const int64_t row = ((int64_t)page * p.c.heads + h) * p.c.page_size + ((uint32_t)slot - page * p.c.page_size);
     void* const cache = is_v ? p.c.v : p.c.k;
-    if (p.c.dtype != kInt8) {
+    if (!I4 && p.c.dtype != kInt8) {
         if (wanted) {
             store_values(cache, row * p.c.d + lane * V, p.c.dtype, a);
             store_values(cache, row * p.c.d + lane * V + half, p.c.dtype, b);
@@ -185,6 +308,10 @@ __global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kerne
     for (int i = 0; i < V; ++i) m = max_nan(m, max_nan(fabsf(a[i]), fabsf(b[i])));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    if (I4) {
+        store_int4<LANES, V>(p.c, row, half, lane, is_v, wanted, m, a, b);
+        return;
+    }
     if (!wanted) return;
     const bool finite = m < __int_as_float(0x7F800000), zero = m < MIN_AMAX;
     const float inv = finite && !zero ? __fdiv_rn(127.0f, m) : 0.0f;
@@ -203,23 +330,30 @@ __global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kerne
         (is_v ? p.c.v_scale : p.c.k_scale)[row] = !finite ? __int_as_float(0x7FC00000) : zero ? 0.0f : __fdiv_rn(m, 127.0f);
 }
 
-template <int LANES, int IN>
+template <int LANES, int IN, bool NORM, bool I4>
 cudaError_t launch_write(const KvWriteParams& p, cudaStream_t stream) {
     const uint32_t heads = p.q_heads + 2 * p.c.heads;
     const uint32_t chunk = std::max(1u, 0x7FFFFFFFu / heads);  // rows of a launch stay below 2^31
     for (uint64_t t0 = 0; t0 < p.tokens; t0 += chunk) {
         const uint32_t rows = std::min<uint64_t>(chunk, p.tokens - t0) * heads, per = KW_THREADS / LANES;
-        kv_write_kernel<LANES, IN><<<rows / per + (rows % per != 0), KW_THREADS, 0, stream>>>(p, (uint32_t)t0, rows);
+        kv_write_kernel<LANES, IN, NORM, I4><<<rows / per + (rows % per != 0), KW_THREADS, 0, stream>>>(p, (uint32_t)t0, rows);
     }
     return cudaGetLastError();
 }
 
+template <int IN, bool NORM, bool I4>
+cudaError_t launch_write_rows(const KvWriteParams& p, cudaStream_t stream) {
+    constexpr int MOST = IN == kF32 ? 16 : 8;  // lanes of a row of 128 elements
+    if (p.c.d > 64) return launch_write<MOST, IN, NORM, I4>(p, stream);
+    if (p.c.d > 32) return launch_write<MOST / 2, IN, NORM, I4>(p, stream);
+    return launch_write<MOST / 4, IN, NORM, I4>(p, stream);
+}
+
 template <int IN>
 cudaError_t launch_write_of(const KvWriteParams& p, cudaStream_t stream) {
-    constexpr int MOST = IN == kF32 ? 16 : 8;  // lanes of a row of 128 elements
-    if (p.c.d > 64) return launch_write<MOST, IN>(p, stream);
-    if (p.c.d > 32) return launch_write<MOST / 2, IN>(p, stream);
-    return launch_write<MOST / 4, IN>(p, stream);
+    const bool norm = p.q_norm != nullptr || p.k_norm != nullptr;
+    if (p.c.dtype == kInt4) return norm ? launch_write_rows<IN, true, true>(p, stream) : launch_write_rows<IN, false, true>(p, stream);
+    return norm ? launch_write_rows<IN, true, false>(p, stream) : launch_write_rows<IN, false, false>(p, stream);
 }
 
 // ---- read ----
@@ -230,11 +364,15 @@ cudaError_t launch_write_of(const KvWriteParams& p, cudaStream_t stream) {
 constexpr int KR_MOST = 32, KR_BATCH = 4;
 
 struct Eight {
-    uint4 w;  // 8 16-bit elements; or the 8 codes in x, y and the scale in z
+    uint4 w;  // 8 16-bit elements; or the 8 codes in x, y and the scale in z; or 8 4-bit codes in x, their group's scale in y, the row's in z
 };
-__device__ __forceinline__ Eight read8(const KvCacheView& c, const void* src, const float* scale, int64_t row, uint32_t col) {
+template <bool I4>
+__device__ __forceinline__ Eight read8(const KvCacheView& c, const void* src, const float* scale, const uint8_t* group, int64_t row, uint32_t col) {
     Eight e;
-    if (c.dtype == kInt8) {
+    if (I4) {
+        const uint32_t w = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(src) + (row * c.d + col) / 2));
+        e.w = make_uint4(w, __ldg(group + row * 4 + col / I4_GROUP), __float_as_uint(__ldg(scale + row)), 0u);
+    } else if (c.dtype == kInt8) {
         const uint2 w = __ldg(reinterpret_cast<const uint2*>(static_cast<const int8_t*>(src) + row * c.d + col));
         e.w = make_uint4(w.x, w.y, __float_as_uint(__ldg(scale + row)), 0u);
     } else {
@@ -243,13 +381,18 @@ __device__ __forceinline__ Eight read8(const KvCacheView& c, const void* src, co
     return e;
 }
 
+template <bool I4>
 __device__ __forceinline__ void write8(void* out, int64_t at, int out_dtype, const Eight& e, int dtype) {
-    if (out_dtype == dtype) {  // 16-bit to the same type: the bits
+    if (!I4 && out_dtype == dtype) {  // 16-bit to the same type: the bits
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(out) + at) = e.w;
         return;
     }
     float x[8];
-    if (dtype == kInt8) {
+    if (I4) {  // code times group's scale is exact, so that a value is rounded once whatever the row's scale is
+        const float g = e4m3_value(e.w.y), s = __uint_as_float(e.w.z);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn((float)((int)((e.w.x >> (4 * i)) & 15u) - 8), g), s);
+    } else if (dtype == kInt8) {
         const float s = __uint_as_float(e.w.z);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = __fmul_rn((float)(int8_t)((i < 4 ? e.w.x : e.w.y) >> (8 * (i & 3))), s);
@@ -266,7 +409,7 @@ __device__ __forceinline__ void write8(void* out, int64_t at, int out_dtype, con
         make_uint4(pack16(x[0], x[1], out_dtype), pack16(x[2], x[3], out_dtype), pack16(x[4], x[5], out_dtype), pack16(x[6], x[7], out_dtype));
 }
 
-template <int LANES>
+template <int LANES, bool I4>
 __global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const __grid_constant__ KvReadParams p, uint32_t tokens) {
     __shared__ int64_t first[KR_MOST];  // each token's row of head 0 in the cache, -1: none (its rows are zeros)
     const uint32_t t0 = blockIdx.x * tokens;
@@ -299,11 +442,11 @@ __global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const __grid_consta
 #pragma unroll
         for (int i = 0; i < KR_BATCH; ++i) {
             const uint32_t r = r0 + i * GROUPS, t = r / p.c.heads;
-            k[i].w = v[i].w = make_uint4(0, 0, 0, 0);
+            k[i].w = v[i].w = make_uint4(I4 ? 0x88888888u : 0u, 0, 0, 0);
             if (r < rows && first[t] >= 0) {
                 const int64_t row = first[t] + (int64_t)(r - t * p.c.heads) * p.c.page_size;
-                k[i] = read8(p.c, p.c.k, p.c.k_scale, row, col);
-                v[i] = read8(p.c, p.c.v, p.c.v_scale, row, col);
+                k[i] = read8<I4>(p.c, p.c.k, p.c.k_scale, p.c.k_group, row, col);
+                v[i] = read8<I4>(p.c, p.c.v, p.c.v_scale, p.c.v_group, row, col);
             }
         }
 #pragma unroll
@@ -311,18 +454,18 @@ __global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const __grid_consta
             const uint32_t r = r0 + i * GROUPS;
             if (r >= rows) break;
             const int64_t at = ((int64_t)t0 * p.c.heads + r) * p.c.d + col;
-            write8(p.k_out, at, p.out_dtype, k[i], p.c.dtype);
-            write8(p.v_out, at, p.out_dtype, v[i], p.c.dtype);
+            write8<I4>(p.k_out, at, p.out_dtype, k[i], p.c.dtype);
+            write8<I4>(p.v_out, at, p.out_dtype, v[i], p.c.dtype);
         }
     }
 }
 
-template <int LANES>
+template <int LANES, bool I4>
 cudaError_t launch_read(const KvReadParams& p, cudaStream_t stream) {
     // up to 32 tokens a block (the look-up of their rows is done once for all heads), fewer where that leaves the SMs idle
     uint32_t tokens = KR_MOST;
     while (tokens > 1 && (p.total + tokens - 1) / tokens < 4 * 148) tokens /= 2;
-    kv_read_kernel<LANES><<<(p.total + tokens - 1) / tokens, KW_THREADS, 0, stream>>>(p, tokens);
+    kv_read_kernel<LANES, I4><<<(p.total + tokens - 1) / tokens, KW_THREADS, 0, stream>>>(p, tokens);
     return cudaGetLastError();
 }
 
@@ -335,10 +478,15 @@ cudaError_t launch_kv_write(const KvWriteParams& params, cudaStream_t stream) {
     return p.dtype == kF16 ? launch_write_of<kF16>(p, stream) : launch_write_of<kBf16>(p, stream);
 }
 
+template <bool I4>
+static cudaError_t launch_read_rows(const KvReadParams& p, cudaStream_t stream) {
+    if (p.c.d > 64) return launch_read<16, I4>(p, stream);
+    if (p.c.d > 32) return launch_read<8, I4>(p, stream);
+    return launch_read<4, I4>(p, stream);
+}
+
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream) {
-    if (p.c.d > 64) return launch_read<16>(p, stream);
-    if (p.c.d > 32) return launch_read<8>(p, stream);
-    return launch_read<4>(p, stream);
+    return p.c.dtype == kInt4 ? launch_read_rows<true>(p, stream) : launch_read_rows<false>(p, stream);
 }
 
 }  // namespace iq2

@@ -15,6 +15,7 @@ const SOURCES: &[&str] = &[
     "iq2_variants.cu",
     "attention_capi.cu",
     "kv_cache.cu",
+    "kv_pages.cu",
     "attention_decode.cu",
     "attention_prefill.cu",
 ];

@@ -45,6 +45,7 @@ pub struct Iq2MatmulProblem {
 }
 
 pub const IQ2_KV_INT8: c_int = 3;
+pub const IQ2_KV_INT4: c_int = 4;
 
 /// struct iq2_kv_cache (a paged key-value cache).
 #[repr(C)]
@@ -59,6 +60,8 @@ pub struct Iq2KvCache {
     pub page_size: u32,
     pub head_dim: u32,
     pub dtype: c_int,
+    pub k_group: *mut u8,
+    pub v_group: *mut u8,
 }
 
 /// struct iq2_rows (a [tokens, heads, head_dim] tensor, strides in elements).
@@ -88,6 +91,45 @@ pub struct Iq2KvTokens {
     pub interleaved: c_int,
     pub q_out: *mut c_void,
     pub q_out_dtype: c_int,
+}
+
+/// struct iq2_head_norms (norms of queries and keys for each head).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Iq2HeadNorms {
+    pub q_norm: *const f32,
+    pub k_norm: *const f32,
+    pub q_per_head: c_int,
+    pub k_per_head: c_int,
+    pub eps: f32,
+}
+
+/// struct iq2_kv_pages (the pages of a batch's sequences).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Iq2KvPages {
+    pub block_table: *mut i32,
+    pub seq_lens: *mut i32,
+    pub free_pages: *mut i32,
+    pub free_count: *mut i32,
+    pub sequences: u32,
+    pub table_width: u32,
+    pub num_pages: u32,
+    pub page_size: u32,
+}
+
+/// struct iq2_kv_step (one step of the sequences).
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct Iq2KvStep {
+    pub keep: *const i32,
+    pub new_lens: *const i32,
+    pub total: u32,
+    pub slots: *mut i32,
+    pub positions: *mut i32,
+    pub cu_seqlens_q: *mut i32,
+    pub cu_seqlens_k: *mut i32,
+    pub granted: *mut i32,
 }
 
 /// struct iq2_attention_prompts (packed prompts).
@@ -261,6 +303,13 @@ extern "C" {
         stream: *mut c_void,
     ) -> c_int;
     pub fn iq2_kv_cache_write(cache: *const Iq2KvCache, tokens: *const Iq2KvTokens, stream: *mut c_void) -> c_int;
+    pub fn iq2_kv_cache_write_normed(
+        cache: *const Iq2KvCache,
+        tokens: *const Iq2KvTokens,
+        norms: *const Iq2HeadNorms,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub fn iq2_kv_pages_step(pages: *const Iq2KvPages, step: *const Iq2KvStep, stream: *mut c_void) -> c_int;
     pub fn iq2_kv_cache_read(
         cache: *const Iq2KvCache,
         block_table: *const i32,

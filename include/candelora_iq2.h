@@ -271,13 +271,19 @@ int iq2_matmul_grouped_sharded(iq2_comm_t comm, const iq2_matmul_problem* proble
  * as many. head_dim is a multiple of 16, at most 128.
  */
 
-/* Element type of a cache: IQ2_DTYPE_F16, IQ2_DTYPE_BF16, or int8 codes with one f32 scale for
- * each token and head. */
+/* Element type of a cache: IQ2_DTYPE_F16, IQ2_DTYPE_BF16, int8 codes with one f32 scale for each
+ * token and head, or 4-bit codes with that and one e4m3 scale for each 32 elements of a row. */
 #define IQ2_KV_INT8 3
+#define IQ2_KV_INT4 4
 
 /*
  * A paged key-value cache: k and v [num_pages, kv_heads, page_size, head_dim], contiguous and
- * 16-byte aligned; k_scale and v_scale f32 [num_pages, kv_heads, page_size], for IQ2_KV_INT8 only.
+ * 16-byte aligned; k_scale and v_scale f32 [num_pages, kv_heads, page_size], for IQ2_KV_INT8 and
+ * IQ2_KV_INT4 only. IQ2_KV_INT4 rows are head_dim / 2 bytes (head_dim a multiple of 32): element 2i
+ * in the low half of byte i, element 2i + 1 in the high half, each as its code -7..7 plus 8; and
+ * k_group and v_group [num_pages, kv_heads, page_size, 4] hold the e4m3 scales (not negative, no
+ * NaN) of a row's groups of 32 elements, 4-byte aligned, of which the first head_dim / 32 count. An
+ * element is code * group scale * row scale. k_group and v_group are not read for other types.
  * Any page_size. Token `pos` of a sequence lies in page block_table[pos / page_size], row
  * pos % page_size. A block table is int32 [sequences, table_width] on the device; entries outside
  * [0, num_pages) are never followed: their tokens take no part in an attention and read as zeros.
@@ -288,7 +294,9 @@ typedef struct iq2_kv_cache {
     float* k_scale;
     float* v_scale;
     uint32_t num_pages, kv_heads, page_size, head_dim;
-    int dtype; /* IQ2_DTYPE_F16, IQ2_DTYPE_BF16 or IQ2_KV_INT8 */
+    int dtype; /* IQ2_DTYPE_F16, IQ2_DTYPE_BF16, IQ2_KV_INT8 or IQ2_KV_INT4 */
+    uint8_t* k_group;
+    uint8_t* v_group;
 } iq2_kv_cache;
 
 /* Rows of a [tokens, heads, head_dim] tensor whose last dimension is contiguous: strides in
@@ -318,8 +326,28 @@ typedef struct iq2_kv_tokens {
  * Rotates q and k by their positions, writes q to q_out and k and v to their slots of the cache,
  * in one launch. 16-bit caches round once; int8 rows (one token and head) hold
  * rint(x * (127 / max|x|)) and the scale max|x| / 127, a row with an infinity or NaN a NaN scale.
+ * IQ2_KV_INT4 rows: the row scale s is the power of two with 224 < max|x| / 7s <= 448, a group's
+ * scale g the e4m3 number nearest to its max|x| / 7s, a code the integer nearest to x / (s g), ties
+ * to even, at most 7; rows whose largest value is below 2^-100 are zeros, a row with an infinity or
+ * NaN gets a NaN row scale.
  */
 int iq2_kv_cache_write(const iq2_kv_cache* cache, const iq2_kv_tokens* tokens, iq2_stream_t stream);
+
+/* Norms of queries and keys for each head (iq2_kv_cache_write_normed). */
+typedef struct iq2_head_norms {
+    const float* q_norm;        /* weights [head_dim], or [q_heads, head_dim] with q_per_head; NULL: q has no norm  */
+    const float* k_norm;        /* weights [head_dim], or [kv_heads, head_dim] with k_per_head; NULL: k has no norm */
+    int q_per_head, k_per_head;
+    float eps;                  /* positive */
+} iq2_head_norms;
+
+/*
+ * iq2_kv_cache_write with x / sqrt(mean(x^2) + eps) * weight of each head's q and k before their
+ * rotation, in the same launch. The sum of squares and the root are taken in 64 bits, the root's
+ * reciprocal and each product are rounded to f32. norms NULL: none.
+ */
+int iq2_kv_cache_write_normed(const iq2_kv_cache* cache, const iq2_kv_tokens* tokens,
+                              const iq2_head_norms* norms, iq2_stream_t stream);
 
 /*
  * Cached tokens -> packed k_out, v_out [total, kv_heads, head_dim] in out_dtype: rows
@@ -377,6 +405,43 @@ size_t iq2_attention_decode_workspace_size(const iq2_kv_cache* cache, uint32_t b
  */
 int iq2_attention_decode(const iq2_kv_cache* cache, const iq2_attention_tokens* tokens, void* workspace,
                          size_t workspace_bytes, iq2_stream_t stream);
+
+/*
+ * The pages of a batch's sequences, on the device. A page belongs to one sequence or is free:
+ * block_table int32 [sequences, table_width] has the pages of sequence b's seq_lens[b] tokens in its
+ * first columns (the others are not read), free_pages int32 [num_pages] the free ones in its first
+ * free_count[0] places, the next one to be taken last.
+ */
+typedef struct iq2_kv_pages {
+    int32_t* block_table;
+    int32_t* seq_lens;          /* [sequences] */
+    int32_t* free_pages;
+    int32_t* free_count;        /* [1] */
+    uint32_t sequences, table_width, num_pages, page_size;
+} iq2_kv_pages;
+
+/* One step of the sequences (iq2_kv_pages_step). */
+typedef struct iq2_kv_step {
+    const int32_t* keep;        /* [sequences] or NULL: a sequence keeps at most so many of its tokens (0: it has ended) */
+    const int32_t* new_lens;    /* [sequences] tokens that it gets then                                                  */
+    uint32_t total;             /* rows of slots and positions: the new tokens, packed in the order of the sequences     */
+    int32_t* slots;             /* [total] for iq2_kv_cache_write; -1: no place                                          */
+    int32_t* positions;         /* [total]                                                                               */
+    int32_t* cu_seqlens_q;      /* [sequences + 1] first row of each sequence, at most total                             */
+    int32_t* cu_seqlens_k;      /* [sequences + 1] sums of the new seq_lens (at most 2^31 - 1)                           */
+    int32_t* granted;           /* [sequences] new_lens, or 0 where there is no place                                    */
+} iq2_kv_step;
+
+/*
+ * Cuts every sequence to `keep`, whose pages behind go back to the free ones in the order of sequences
+ * and columns, gives every sequence the pages of its new tokens in the same order, and writes
+ * where they go, in one launch. All of a sequence's new tokens get a place or none: none where they
+ * pass `total` rows or the table's width, and none from the first sequence on whose pages are more
+ * than are left (but for those that need no new page). Such a sequence keeps the tokens it had, its
+ * rows get slot -1 and position 0, as do rows of no sequence. Negative counts are 0. At most 8192
+ * sequences.
+ */
+int iq2_kv_pages_step(const iq2_kv_pages* pages, const iq2_kv_step* step, iq2_stream_t stream);
 
 #ifdef __cplusplus
 }
