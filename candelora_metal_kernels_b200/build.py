@@ -20,9 +20,9 @@ LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libcandelora_iq2.so"
 SOURCES = ["iq2xxs_capi.cu", "iq2xxs_gemv.cu", "iq2xxs_gemm.cu", "iq2xxs_dequant.cu", "iq2xxs_noalloc.cu",
            "iq2xxs_sharded.cu", "iq2_variants.cu", "attention_capi.cu", "kv_cache.cu", "kv_pages.cu", "attention_decode.cu",
-           "attention_prefill.cu"]
+           "attention_decode_int4.cu", "attention_prefill.cu"]
 HEADERS = ["iq2xxs_common.cuh", "iq2xxs_codebook.h", "iq2xxs_internal.h", "iq2_variant_grids.h", "attention_internal.h",
-           "tcgen05.cuh", "attention_parts.cuh"]
+           "tcgen05.cuh", "attention_parts.cuh", "attention_decode.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -1,0 +1,602 @@
+// Attention of one new token a sequence over a 4-bit paged cache: the line of work, its parts and their join are those of
+// attention_decode.cu, the products are turned round.
+//
+// A cached element is code g s (iq2_kv_cache): 72 bytes for a row of 128, so that the widening of the codes decides, not HBM. The
+// products have the tokens (or the values' dimensions) as the sixteen rows of mma.sync m16n8k16 and eight query heads as its columns:
+//   S^T = K Q^T  (32 tokens x 8 heads a warp's tile),  O^T = V^T P^T  (DP dimensions x 8 heads)
+// so that all rows of an accumulator are in use: 32 + 8 registers at 128 elements, half of what heads as rows take, which
+// leaves room for twice the warps.
+//   * Codes become f16 values code g 2^-15 by one AND and one multiply-add a pair: four bits u among the lowest ten are the f16
+//     numbers u 2^-22 or u 2^-18, which A = G 2^15 or G 2^11 and B = -G 2^-4 make (u - 8) G 2^-7 of, exactly (g has four significant
+//     bits and is a multiple of 2^-9); G = g 2^-8 are the e4m3 bits moved by seven places.
+//   * A product's inner index may be relabelled as long as both sides agree. For S a thread's inner elements are DP / 4 consecutive
+//     ones of a key row, one group: one wide load and one scale a key. For O a thread's rows are DP / 8 consecutive dimensions, again
+//     one group, of the two tokens whose p it holds; tokens are relabelled so that both kinds of loads are free of bank conflicts.
+//   * q of 32 bits and its p are sums of two f16 pieces in one accumulator: q is held times the power of two that brings a head's
+//     largest |q| to 2^14, so that its 22 bits end at 2^-39 of it; p times its value's row scale is 2^7 at the reference, up to
+//     2^15, and its 22 bits end at 2^-31 of the largest. q of 16 bits is one piece exactly, and its p is rounded to f16 once.
+//   * The row scales of keys multiply s, those of values multiply p.
+// The maxima, sums, s, p and o are f32.
+#include "attention_decode.cuh"
+
+#include <type_traits>
+
+namespace iq2 {
+
+namespace {
+
+constexpr int A4_WARPS = 12, A4_THREADS = A4_WARPS * 32, A4_STAGES = 2;
+static_assert(2 * A4_WARPS <= 32, "a lane a piece");
+constexpr int A4_TOK = 32, A4_NT = A4_TOK / 8;  // tokens of a warp's stage, and eights of them
+constexpr int A4_RUN = 8;                // tokens that lie side by side in a page of a multiple of these
+constexpr float A4_TOP = 7.f;            // log2 of p times the value scale at the reference
+constexpr float A4_LAZY = 32768.f;       // how far it may grow before that moves
+constexpr float A4_SUM = 1.f / 65536.f;  // what the sums of p, and with them o, are held times: p alone may reach 2^118
+// The values' row scales, 2^-111 or more, multiply p as 2^9 of themselves (2^126 at most); a row of zeros counts as 2^-103.
+constexpr float A4_UP = 512.f, A4_MIN_SCALE = 9.86076132e-32f;
+constexpr float A4_VALUE = 32768.f;      // 2^15: what values are held by
+
+template <int DP>
+struct Shape4 {
+    static constexpr int ROW = DP / 2, CHUNKS = ROW / 16;  // bytes and 16-byte chunks of a padded row
+    static constexpr int KS = DP / 16, MT = DP / 16;       // steps of S's inner index, row tiles of O
+    static constexpr int SCALES = 2 * A4_TOK * ROW;        // of a stage: row scales of K and V, then group scales, a word a token
+    static constexpr int STAGE = SCALES + 4 * A4_TOK * 4;
+    static constexpr int RING = A4_STAGES * STAGE;
+    static constexpr int HEAD = DP + 4;                    // floats of a head in a piece's slot
+    static constexpr int MAXIMA = AD_HEADS * HEAD, SUMS = MAXIMA + AD_HEADS, SLOT = SUMS + AD_HEADS;  // floats of one (o, max, sum)
+    static constexpr int PART = AD_HEADS * (DP + 2);       // and in the workspace
+    static constexpr int SMEM = A4_WARPS * (RING + SLOT * 4);
+    static_assert(SLOT * 4 <= RING, "a warp's last piece lies in its ring");
+};
+
+// Where a token of a tile lies among the eight that share an accumulator's rows: a thread's pairs 2t, 2t + 1 are the rows
+// (0, 3), (1, 2), (4, 7), (5, 6), of which rows 4 to 7 have the halves of their 64 bytes swapped. So the four rows that the
+// threads of a column read together, 0 1 4 5 or 2 3 6 7, fall to different banks, and so do two rows side by side.
+__device__ __forceinline__ uint32_t row_of(uint32_t i) { return (0x65742130u >> (i * 4)) & 7u; }
+
+// Byte offset of 16-byte chunk c of row r in a K or V stage.
+template <int CHUNKS>
+__device__ __forceinline__ uint32_t chunk_offset(uint32_t r, uint32_t c) {
+    return r * (CHUNKS * 16) + (CHUNKS == 4 ? c ^ ((r >> 1) & 2) : c) * 16;
+}
+
+// What makes f16 values of codes: A for the lower and the upper bits of a byte, and B, for the two halves of a word.
+struct CodeScale {
+    __half2 lo, hi, off;
+};
+// bytes: the e4m3 scales of the two halves in bytes 1 and 3, zeros in 0 and 2.
+__device__ __forceinline__ CodeScale code_scale(uint32_t bytes) {
+    const uint32_t moved = bytes >> 1;
+    const __half2 g = *reinterpret_cast<const __half2*>(&moved);
+    return {__hmul2(g, __float2half2_rn(32768.f)), __hmul2(g, __float2half2_rn(2048.f)), __hmul2(g, __float2half2_rn(-0.0625f))};
+}
+// The values of a word's codes: v[0], v[1] the lower and upper bits of bytes 0 and 2, v[2], v[3] of bytes 1 and 3.
+__device__ __forceinline__ void code_values(uint32_t w, const CodeScale& s, uint32_t (&v)[4]) {
+    const uint32_t even = w << 2, odd = w >> 6;
+    const uint32_t u[4] = {even & 0x003C003Cu, even & 0x03C003C0u, odd & 0x003C003Cu, odd & 0x03C003C0u};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&u[i]), i % 2 ? s.hi : s.lo, s.off);
+        v[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+}
+
+// An 8 x 8 matrix of 16-bit elements, a row's pairs in the four lanes of a column of threads, turned round.
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+    return v;
+}
+
+// N consecutive elements of a row of q as f32, zeros unless `there`; `vec`: rows start on 16-byte boundaries.
+template <int N>
+__device__ __forceinline__ void load_row(const void* base, int64_t at, int dtype, bool there, bool vec, float (&x)[N]) {
+    if (!there) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = 0.f;
+    } else if (!vec) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = load_elem(base, at + i, dtype);
+    } else if (dtype == kF32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const float4 f = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(base) + at + i));
+            x[i] = f.x, x[i + 1] = f.y, x[i + 2] = f.z, x[i + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 8) {
+            const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + at + i));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = dtype == kF16 ? unpack_pair<false>(u[j]) : unpack_pair<true>(u[j]);
+                x[i + 2 * j] = f.x, x[i + 2 * j + 1] = f.y;
+            }
+        }
+    }
+}
+
+// N consecutive elements of a 16-byte aligned output row.
+template <int N>
+__device__ __forceinline__ void store_row(void* base, int64_t at, int dtype, const float (&y)[N]) {
+    if (dtype == kF32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) *reinterpret_cast<float4*>(static_cast<float*>(base) + at + i) = make_float4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; i += 8) {
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = dtype == kF16 ? pack_pair<false>(y[i + 2 * j], y[i + 2 * j + 1]) : pack_pair<true>(y[i + 2 * j], y[i + 2 * j + 1]);
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at + i) = make_uint4(u[0], u[1], u[2], u[3]);
+    }
+}
+
+// A warp's piece of an item that is not all of it. valid: 0, or 1, and 2 where it has the item's first token, 4 its last one, 8
+// where the item is the first of the block.
+struct Piece {
+    uint32_t b, item, valid;
+};
+// Where piece `i` lies: a warp's first one behind the rings, its last one in its ring.
+template <typename S>
+__device__ __forceinline__ float* slot_of(uint8_t* smem, uint32_t i) {
+    return reinterpret_cast<float*>(smem + (i % 2 == 0 ? A4_WARPS * S::RING + i / 2 * (S::SLOT * 4) : i / 2 * S::RING));
+}
+
+// WIDE: q of 32 bits, and two pieces of q and p; of 16 bits, q is one piece exactly and p is rounded to f16 once.
+template <int DP, bool WIDE>
+__global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_constant__ DecodeArgs a) {
+    using S = Shape4<DP>;
+    constexpr int TOK = A4_TOK, NT = A4_NT, KS = S::KS, MT = S::MT;
+    using Tokens = std::conditional_t<TOK == 64, uint64_t, uint32_t>;  // a bit a token of a tile
+    using Cursor = iq2::Cursor<AD_I4_UNIT, AD_I4_ITEM_COST>;
+    constexpr Tokens ALL = ~(Tokens)0;
+    const DecodeParams& p = a.p;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Piece pieces[2 * A4_WARPS];  // of each warp its first and its last, of those that are not a whole item
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    const uint32_t d = p.c.d, group = p.q_heads / p.c.heads, items = p.c.heads * a.chunks_of_heads;
+    pdl_launch_dependents();
+
+    // the ring starts as zeros: chunks past head_dim are never copied, and the matrix instructions read them
+    if (d < DP)
+        for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
+    if (lane < 2) pieces[warp * 2 + lane].valid = 0;
+    typename Cursor::Part of;
+    Cursor cur = Cursor::of_part(a, blockIdx.x * A4_WARPS + warp, gridDim.x * A4_WARPS, a.inv_blocks * (1.0 / A4_WARPS), lane, 32, of);
+    if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(of.u0, of.each * A4_WARPS);
+    const uint64_t block_u0 = of.u0 - min(of.u0, warp * of.each);
+    if (cur.t0 == cur.t1) cur.unit = cur.end;  // nothing, or nothing but an item's start
+    Cursor pre = cur;
+
+    // ---- the copies: tile `i` (TOK tokens) of pre's piece of an item, one page lookup ahead ----
+    const uint32_t ring = smem_u32(smem + warp * S::RING);
+    __syncwarp();
+    // a tile's rows lie side by side in one page, or in runs of eight, or each lane looks its rows up
+    const bool whole_tiles = p.c.page_size % TOK == 0, runs = p.c.page_size % A4_RUN == 0;
+    const uint32_t row_bytes = d / 2, chunk = lane % S::CHUNKS, row0 = lane / S::CHUNKS;
+    constexpr int ROWS = 32 / S::CHUNKS;  // rows that the warp copies at a time
+    uint32_t pre_i = 0, page0 = 0, page1 = 0, ahead = 0;  // the tile to copy next; pages looked up, and tiles since
+    auto look_up = [&](uint32_t tok) {
+        return tok < pre.t1 ? (uint32_t)__ldg(p.block_table + (int64_t)pre.b * p.table_width + a.by_page.quotient(tok)) : 0xFFFFFFFFu;
+    };
+    auto find_tile = [&]() {  // the next tile of this warp, and its page numbers under way
+        bool fresh = ahead == 32;
+        while (!pre.done() && pre.t0 + pre_i * TOK >= pre.t1) {
+            pre.next(p, items);
+            pre_i = 0, fresh = true;
+        }
+        if (pre.done()) return;
+        const uint32_t tok = pre.t0 + pre_i * TOK;
+        if (whole_tiles) {  // lanes hold the pages of this warp's next 32 tiles
+            if (fresh || pre_i == 0) page0 = look_up(tok + lane * TOK), ahead = 0;
+        } else if (runs) {  // of the tile's runs
+            page0 = look_up(tok + lane % (TOK / A4_RUN) * A4_RUN);
+        } else {            // of its tokens
+            page0 = look_up(tok + lane);
+            if (TOK == 64) page1 = look_up(tok + lane + 32);
+        }
+    };
+    // Copies the tile and returns a bit for each token that takes part: rows of tokens past the end, or of pages outside
+    // the cache, are zeros, and what such pages hold cannot matter.
+    auto copy_tile = [&](uint32_t stage) {
+        const uint32_t tok = pre.t0 + pre_i * TOK, h = pre.item / a.chunks_of_heads, dst = ring + stage * S::STAGE, left = pre.t1 - tok;
+        const uint8_t *const k = static_cast<const uint8_t*>(p.c.k), *const v = static_cast<const uint8_t*>(p.c.v);
+        const bool inside = chunk * 16 < row_bytes;
+        auto cache_row = [&](uint32_t page, uint32_t at) {  // of token `at`, -1: none
+            const uint32_t in_page = at - a.by_page.quotient(at) * p.c.page_size;
+            return page < p.c.pages ? ((int64_t)page * p.c.heads + h) * p.c.page_size + in_page : (int64_t)-1;
+        };
+        // 16 bytes of scales a lane and turn: row scales of K and V, then group scales
+        auto scales_of = [&](int turn) {
+            const uint32_t kind = (turn * 32 + lane) / (TOK / 4);
+            return kind == 0 ? reinterpret_cast<const uint8_t*>(p.c.k_scale) : kind == 1 ? reinterpret_cast<const uint8_t*>(p.c.v_scale)
+                 : kind == 2 ? p.c.k_group : p.c.v_group;
+        };
+        int64_t mine0, mine1;  // the rows of tokens `lane` and `lane` + 32
+        ++pre_i;
+        if (whole_tiles) {
+            const int64_t row = cache_row(__shfl_sync(0xFFFFFFFFu, page0, ahead++), tok);
+            if (row >= 0 && left >= TOK) {
+                const int64_t off = (row + row0) * row_bytes + chunk * 16;
+                const uint8_t *pk = k + off, *pv = v + off;
+                if (inside) {
+#pragma unroll
+                    for (int i = 0; i < TOK / ROWS; ++i, pk += ROWS * row_bytes, pv += ROWS * row_bytes) {
+                        cp_async_16(dst + chunk_offset<S::CHUNKS>(row0 + i * ROWS, chunk), pk);
+                        cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(row0 + i * ROWS, chunk), pv);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < TOK / 32; ++i) cp_async_16(dst + S::SCALES + (i * 32 + lane) * 16, scales_of(i) + row * 4 + lane % (TOK / 4) * 16);
+                return ALL;
+            }
+            mine0 = row >= 0 && lane < left ? row + lane : -1;
+            mine1 = row >= 0 && lane + 32 < left ? row + lane + 32 : -1;
+        } else if (runs) {
+            const int64_t run = cache_row(page0, tok + lane % (TOK / A4_RUN) * A4_RUN);
+            if (left >= TOK && __all_sync(0xFFFFFFFFu, run >= 0)) {
+#pragma unroll
+                for (int i = 0; i < TOK / ROWS; ++i) {
+                    const uint32_t r = row0 + i * ROWS;
+                    const int64_t off = (__shfl_sync(0xFFFFFFFFu, run, r / A4_RUN) + r % A4_RUN) * row_bytes + chunk * 16;
+                    if (inside) {
+                        cp_async_16(dst + chunk_offset<S::CHUNKS>(r, chunk), k + off);
+                        cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(r, chunk), v + off);
+                    }
+                }
+                const int64_t at = __shfl_sync(0xFFFFFFFFu, run, lane % (TOK / 4) / 2) * 4 + lane % 2 * 16;
+#pragma unroll
+                for (int i = 0; i < TOK / 32; ++i) cp_async_16(dst + S::SCALES + (i * 32 + lane) * 16, scales_of(i) + at);
+                return ALL;
+            }
+            const int64_t run0 = __shfl_sync(0xFFFFFFFFu, run, lane / A4_RUN), run1 = __shfl_sync(0xFFFFFFFFu, run, lane / A4_RUN + 4);
+            mine0 = run0 >= 0 && lane < left ? run0 + lane % A4_RUN : -1;
+            mine1 = run1 >= 0 && lane + 32 < left ? run1 + lane % A4_RUN : -1;
+        } else {
+            mine0 = cache_row(page0, tok + lane), mine1 = cache_row(page1, tok + lane + 32);
+        }
+#pragma unroll 1
+        for (int i = 0; i < TOK / ROWS; ++i) {
+            const uint32_t r = row0 + i * ROWS;
+            const int64_t src = __shfl_sync(0xFFFFFFFFu, i * ROWS < 32 ? mine0 : mine1, r % 32);
+            const int64_t off = src < 0 ? 0 : src * row_bytes + chunk * 16;
+            if (inside) {
+                cp_async_16(dst + chunk_offset<S::CHUNKS>(r, chunk), k + off, src < 0 ? 0 : 16);
+                cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(r, chunk), v + off, src < 0 ? 0 : 16);
+            }
+        }
+#pragma unroll 1
+        for (int i = 0; i < TOK / 32; ++i) {
+            const int64_t src = i == 0 ? mine0 : mine1, at = max(src, (int64_t)0);
+            const uint32_t bytes = src < 0 ? 0 : 4, to = dst + S::SCALES + (i * 32 + lane) * 4;
+            cp_async_4(to, p.c.k_scale + at, bytes);
+            cp_async_4(to + TOK * 4, p.c.v_scale + at, bytes);
+            cp_async_4(to + TOK * 8, p.c.k_group + at * 4, bytes);
+            cp_async_4(to + TOK * 12, p.c.v_group + at * 4, bytes);
+        }
+        const Tokens low = __ballot_sync(0xFFFFFFFFu, mine0 >= 0);
+        return TOK == 64 ? low | (Tokens)((uint64_t)__ballot_sync(0xFFFFFFFFu, mine1 >= 0) << 32) : low;
+    };
+    Tokens present[A4_STAGES] = {};
+    auto copy_and_find = [&](int stage) {
+        if (!pre.done()) {
+            const Tokens here = copy_tile(stage);
+#pragma unroll
+            for (int s = 0; s < A4_STAGES; ++s)
+                if (s == stage) present[s] = here;
+            find_tile();
+        }
+        cp_async_commit();
+    };
+    find_tile();
+#pragma unroll 1
+    for (int s = 0; s < A4_STAGES - 1; ++s) copy_and_find(s);
+    int stage = 0;
+
+    // this thread's places: its key row and chunk, its two value rows and their bytes, its groups' scales as bytes 1 and 3
+    const uint32_t k_row = row_of(g), v_row0 = row_of(2 * t), v_row1 = row_of(2 * t + 1);
+    const uint32_t k_at = DP == 128 ? chunk_offset<S::CHUNKS>(k_row, t) : k_row * S::ROW + t * 8;
+    const uint32_t v_at0 = TOK * S::ROW + (DP == 128 ? chunk_offset<S::CHUNKS>(v_row0, g / 2) + g % 2 * 8 : v_row0 * S::ROW + g * 4);
+    const uint32_t v_at1 = TOK * S::ROW + (DP == 128 ? chunk_offset<S::CHUNKS>(v_row1, g / 2) + g % 2 * 8 : v_row1 * S::ROW + g * 4);
+    const uint32_t k_group = t * (DP / 4) / I4_GROUP, v_group = g * (DP / 8) / I4_GROUP;
+    const uint32_t k_sel = k_group * I4_GROUP < d ? 0x0404u | k_group * 0x1010u : 0x4444u;  // (zeros past head_dim)
+    const uint32_t v_sel = 0x4C08u + v_group * 0x1111u;  // (8 + i is the sign of byte i in all bits: none)
+
+    while (!cur.done()) {
+        // ---- q of the item: the pieces of head g, elements t DP / 4 and on ----
+        const uint32_t kv_head = cur.item / a.chunks_of_heads, head0 = kv_head * group + (cur.item % a.chunks_of_heads) * AD_HEADS;
+        const uint32_t heads = min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
+        uint32_t q_high[KS][2], q_low[KS][2];
+        float2 factor;  // scale log2(e) 2^e of the heads 2t, 2t + 1
+        {
+            float x[DP / 4], top = 0.f, unit = A4_VALUE, down = 1.f;  // 2^e and 2^(15 - e)
+            load_row<DP / 4>(p.q.p, (int64_t)cur.b * p.q.token_stride + (int64_t)(head0 + g) * p.q.head_stride + t * (DP / 4), p.dtype,
+                             g < heads && t * (DP / 4) < d, a.q_vec, x);
+#pragma unroll
+            for (int i = 0; i < DP / 4; ++i) top = fmaxf(top, fabsf(x[i]));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+            const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -110), 126);
+            if (top > 0.f && top < INFINITY) unit = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(142 - e) << 23);
+            const float f = p.scale * LOG2E * unit;
+            factor = make_float2(__shfl_sync(0xFFFFFFFFu, f, t * 8), __shfl_sync(0xFFFFFFFFu, f, t * 8 + 4));
+            // elements j and j + 4 of a word's eight are a pair: j = 0, 1 of one step, j = 2, 3 of the next
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x0 = x[i * 8 + j] * down, x1 = x[i * 8 + j + 4] * down;
+                    const uint32_t high = pack_pair<false>(x0, x1);
+                    const float2 back = unpack_pair<false>(high);
+                    q_high[i * 2 + j / 2][j % 2] = high;
+                    q_low[i * 2 + j / 2][j % 2] = WIDE ? pack_pair<false>(x0 - back.x, x1 - back.y) : 0u;
+                }
+        }
+        float o[MT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < MT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+
+        const uint32_t tokens = cur.t1 - cur.t0;
+#pragma unroll 1
+        for (uint32_t i = 0; i * TOK < tokens; ++i) {
+            cp_async_wait<A4_STAGES - 2>();
+            __syncwarp();
+            const uint32_t at = ring + stage * S::STAGE;
+            Tokens here = 0;
+#pragma unroll
+            for (int s = 0; s < A4_STAGES; ++s)
+                if (s == stage) here = present[s];
+            copy_and_find(stage == 0 ? A4_STAGES - 1 : stage - 1);  // the stage the last tile freed
+
+            // ---- S^T: rows are tokens row_of(g) of each eight, columns the heads 2t, 2t + 1 ----
+            float x[NT][2];
+#pragma unroll
+            for (int mt = 0; mt < NT / 2; ++mt) {
+                uint32_t w[2][DP / 32];
+                CodeScale scale[2];
+                float s[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const uint32_t from = at + k_at + (mt * 2 + r) * 8 * S::ROW;
+                    if (DP == 128) {
+                        const uint4 u = ld_shared_v4<0>(from);
+                        w[r][0] = u.x, w[r][1] = u.y, w[r][2 % (DP / 32)] = u.z, w[r][3 % (DP / 32)] = u.w;
+                    } else {
+                        const uint2 u = ld_shared_v2_volatile(from);
+                        w[r][0] = u.x, w[r][1] = u.y;
+                    }
+                    scale[r] = code_scale(prmt(ld_shared(at + S::SCALES + TOK * 8 + ((mt * 2 + r) * 8 + k_row) * 4), 0u, k_sel));
+                }
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    uint32_t v0[4], v1[4];
+                    code_values(w[0][j], scale[0], v0), code_values(w[1][j], scale[1], v1);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t k[4] = {v0[2 * h], v1[2 * h], v0[2 * h + 1], v1[2 * h + 1]};
+                        mma16816<false>(s, k, q_high[2 * j + h][0], q_high[2 * j + h][1]);
+                        if (WIDE) mma16816<false>(s, k, q_low[2 * j + h][0], q_low[2 * j + h][1]);
+                    }
+                }
+                x[mt * 2][0] = s[0], x[mt * 2][1] = s[1], x[mt * 2 + 1][0] = s[2], x[mt * 2 + 1][1] = s[3];
+            }
+
+            // x = log2(e) scale q . k; w = 2^(x - m) times the value scale
+            float e[NT][2], w[NT][2], vs[NT];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const uint32_t from = at + S::SCALES + (n * 8 + k_row) * 4;
+                const float ks = __uint_as_float(ld_shared(from));
+                vs[n] = max_nan(__uint_as_float(ld_shared(from + TOK * 4)) * A4_UP, A4_MIN_SCALE);
+                x[n][0] *= ks * factor.x, x[n][1] *= ks * factor.y;
+            }
+            if (here != ALL) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    if (!((here >> (n * 8 + k_row)) & 1u)) x[n][0] = x[n][1] = -INFINITY;
+            }
+            // The reference does as a rule: the products are made with it, and made again in the rare case that it moves.
+            bool fresh = __any_sync(0xFFFFFFFFu, m[0] == -INFINITY || m[1] == -INFINITY);
+            for (;;) {
+                if (!fresh) {
+                    float top = 0.f;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float base = m[h] == -INFINITY ? 0.f : m[h] - A4_TOP;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            e[n][h] = exp2_approx(x[n][h] - base);
+                            w[n][h] = e[n][h] * vs[n];
+                            top = fmaxf(top, w[n][h]);
+                        }
+                    }
+                    if (!__any_sync(0xFFFFFFFFu, top > A4_LAZY)) break;
+                }
+                // the largest x + log2(value scale) of the heads' tokens
+                float keep[2];
+                bool moved = false;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float most = -INFINITY;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) most = fmaxf(most, x[n][h] + __log2f(vs[n]));
+#pragma unroll
+                    for (int b = 4; b < 32; b *= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, b));
+                    const float next = fmaxf(m[h], most);
+                    keep[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - next);
+                    moved = moved || next > m[h];
+                    m[h] = next;
+                }
+                if (!__any_sync(0xFFFFFFFFu, moved) && !fresh) break;
+                fresh = false;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    l[h] *= keep[h];
+#pragma unroll
+                    for (int n = 0; n < MT; ++n) o[n][h] *= keep[h], o[n][2 + h] *= keep[h];
+                }
+            }
+            uint32_t high[NT], low[NT];  // the pieces of p, with heads as rows and tokens as columns
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) l[h] = fmaf(e[n][h], A4_SUM, l[h]);
+                const uint32_t hi = pack_pair<false>(w[n][0], w[n][1]);
+                high[n] = transposed(hi);
+                if (WIDE) {
+                    const float2 back = unpack_pair<false>(hi);
+                    low[n] = transposed(pack_pair<false>(w[n][0] - back.x, w[n][1] - back.y));
+                }
+            }
+
+            // ---- O^T: rows are this thread's DP / 8 dimensions, two a tile ----
+#pragma unroll
+            for (int ks = 0; ks < NT / 2; ++ks) {
+                uint32_t y[2][DP / 32];  // the codes of the two tokens of eight, four of one in the lower half and of the other in the upper
+                CodeScale scale[2];
+#pragma unroll
+                for (int r = 0; r < 2; ++r) {
+                    const int n = ks * 2 + r;
+                    const uint32_t from0 = at + v_at0 + n * 8 * S::ROW, from1 = at + v_at1 + n * 8 * S::ROW;
+                    if (DP == 128) {
+                        const uint2 u0 = ld_shared_v2_volatile(from0), u1 = ld_shared_v2_volatile(from1);
+                        y[r][0] = prmt(u0.x, u1.x, 0x5410u), y[r][1] = prmt(u0.x, u1.x, 0x7632u);
+                        y[r][2 % (DP / 32)] = prmt(u0.y, u1.y, 0x5410u), y[r][3 % (DP / 32)] = prmt(u0.y, u1.y, 0x7632u);
+                    } else {
+                        const uint32_t u0 = ld_shared(from0), u1 = ld_shared(from1);
+                        y[r][0] = prmt(u0, u1, 0x5410u), y[r][1] = prmt(u0, u1, 0x7632u);
+                    }
+                    const uint32_t groups = at + S::SCALES + TOK * 12 + n * 32;
+                    scale[r] = code_scale(prmt(ld_shared(groups + v_row0 * 4), ld_shared(groups + v_row1 * 4), v_sel));
+                }
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    uint32_t v0[4], v1[4];
+                    code_values(y[0][j], scale[0], v0), code_values(y[1][j], scale[1], v1);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t v[4] = {v0[2 * h], v0[2 * h + 1], v1[2 * h], v1[2 * h + 1]};
+                        mma16816<false>(o[2 * j + h], v, high[ks * 2], high[ks * 2 + 1]);
+                        if (WIDE) mma16816<false>(o[2 * j + h], v, low[ks * 2], low[ks * 2 + 1]);
+                    }
+                }
+            }
+            __syncwarp();
+            stage = stage == A4_STAGES - 1 ? 0 : stage + 1;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int b = 4; b < 32; b *= 2) l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], b);
+
+        // ---- the end of the piece: a whole item's output, or (o, m, l) for the block to add up ----
+        constexpr float UNIT_OF_O = A4_SUM * (A4_VALUE / A4_UP);
+        if (cur.whole()) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                if (2 * t + h < heads && g * (DP / 8) < d) {
+                    auto value = [&](float x) { return l[h] == 0.f ? 0.f : x * UNIT_OF_O / l[h]; };
+                    float y[DP / 8];
+#pragma unroll
+                    for (int j = 0; j < DP / 32; ++j)
+                        y[4 * j] = value(o[2 * j][h]), y[4 * j + 1] = value(o[2 * j][2 + h]), y[4 * j + 2] = value(o[2 * j + 1][h]), y[4 * j + 3] = value(o[2 * j + 1][2 + h]);
+                    store_row<DP / 8>(p.out, ((int64_t)cur.b * p.q_heads + head0 + 2 * t + h) * d + g * (DP / 8), p.dtype, y);
+                }
+            }
+        } else {
+            const bool first = cur.unit == of.u0;
+            // (the last piece takes the ring: all of the warp's copies are done then)
+            float* const slot = slot_of<S>(smem, warp * 2 + !first);
+            if (!first) {
+                cp_async_wait<0>();
+                __syncwarp();
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j)
+                    *reinterpret_cast<float4*>(slot + (2 * t + h) * S::HEAD + g * (DP / 8) + j * 4) =
+                        make_float4(o[2 * j][h], o[2 * j][2 + h], o[2 * j + 1][h], o[2 * j + 1][2 + h]);
+                if (g == 0) slot[S::MAXIMA + 2 * t + h] = m[h], slot[S::SUMS + 2 * t + h] = l[h];
+            }
+            if (lane == 0)
+                pieces[warp * 2 + !first] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.unit - cur.k <= block_u0 ? 8u : 0u)};
+        }
+        cur.next(p, items);
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+
+    // ---- the warps' pieces: those of one item follow one another. A warp an item and head ----
+    const Piece mine = lane < 2 * A4_WARPS ? pieces[lane] : Piece{0, 0, 0};
+    const uint32_t there = __ballot_sync(0xFFFFFFFFu, mine.valid != 0);
+    const int before = 31 - __clz(there & ((1u << lane) - 1));  // the piece before this lane's, -1: none
+    const uint32_t b_before = __shfl_sync(0xFFFFFFFFu, mine.b, max(before, 0)), item_before = __shfl_sync(0xFFFFFFFFu, mine.item, max(before, 0));
+    uint32_t starts = __ballot_sync(0xFFFFFFFFu, mine.valid != 0 && (before < 0 || b_before != mine.b || item_before != mine.item));
+    uint32_t turn = warp;  // (item, head) pairs until this warp's next
+#pragma unroll 1
+    while (starts != 0) {
+        const int at = __ffs(starts) - 1;
+        starts &= starts - 1;
+        const uint32_t ours = there & ~((1u << at) - 1) & (starts != 0 ? (starts & -starts) - 1 : 0xFFFFFFFFu);
+        const int last = 31 - __clz(ours);
+        const uint32_t b = __shfl_sync(0xFFFFFFFFu, mine.b, at), item = __shfl_sync(0xFFFFFFFFu, mine.item, at);
+        const uint32_t from = __shfl_sync(0xFFFFFFFFu, mine.valid, at), to = __shfl_sync(0xFFFFFFFFu, mine.valid, last);
+        const bool whole = (from & 2u) != 0 && (to & 4u) != 0;
+        const uint32_t kv_head = item / a.chunks_of_heads, head0 = kv_head * group + (item % a.chunks_of_heads) * AD_HEADS;
+        const uint32_t heads = min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
+        float* const part = a.parts + ((uint64_t)blockIdx.x * 2 + ((from & 8u) != 0 ? 0 : 1)) * S::PART;
+        for (; turn < AD_HEADS; turn += A4_WARPS) {
+            const uint32_t h = turn;
+            if (h >= heads) continue;
+            float mx = -INFINITY, sum = 0.f, y[DP / 32] = {};
+            for (uint32_t rest = ours; rest != 0; rest &= rest - 1) mx = fmaxf(mx, slot_of<S>(smem, __ffs(rest) - 1)[S::MAXIMA + h]);
+#pragma unroll 2
+            for (uint32_t rest = ours; rest != 0; rest &= rest - 1) {
+                const float* const slot = slot_of<S>(smem, __ffs(rest) - 1);
+                const float w = mx == -INFINITY ? 0.f : exp2_approx(slot[S::MAXIMA + h] - mx);
+                sum += slot[S::SUMS + h] * w;
+#pragma unroll
+                for (int i = 0; i < DP / 32; ++i) y[i] += slot[h * S::HEAD + lane + i * 32] * w;
+            }
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) {
+                const uint32_t el = lane + i * 32;
+                constexpr float UNIT_OF_O = A4_SUM * (A4_VALUE / A4_UP);
+                if (!whole) part[h * DP + el] = y[i] * UNIT_OF_O;
+                else if (el < d) store_elem(p.out, ((int64_t)b * p.q_heads + head0 + h) * d + el, p.dtype, sum == 0.f ? 0.f : y[i] * UNIT_OF_O / sum);
+            }
+            if (!whole && lane == 0) part[AD_HEADS * DP + h] = mx, part[AD_HEADS * DP + AD_HEADS + h] = sum;
+        }
+        turn -= AD_HEADS;
+    }
+}
+
+template <int DP, bool WIDE>
+cudaError_t launch4(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
+    cudaError_t e = cudaFuncSetAttribute(decode4_kernel<DP, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape4<DP>::SMEM);
+    if (e != cudaSuccess) return e;
+    decode4_kernel<DP, WIDE><<<blocks, A4_THREADS, Shape4<DP>::SMEM, stream>>>(a);
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    return launch_join<DP>(a, blocks, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_attention_decode_int4(const DecodeParams& p, void* workspace, int num_sms, cudaStream_t stream) {
+    const DecodeArgs a = decode_args(p, workspace, num_sms);
+    if (p.dtype == kF32) return p.c.d > 64 ? launch4<128, true>(a, num_sms, stream) : launch4<64, true>(a, num_sms, stream);
+    return p.c.d > 64 ? launch4<128, false>(a, num_sms, stream) : launch4<64, false>(a, num_sms, stream);
+}
+
+}  // namespace iq2

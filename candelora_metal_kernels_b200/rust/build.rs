@@ -17,6 +17,7 @@ const SOURCES: &[&str] = &[
     "kv_cache.cu",
     "kv_pages.cu",
     "attention_decode.cu",
+    "attention_decode_int4.cu",
     "attention_prefill.cu",
 ];
 
@@ -55,6 +56,7 @@ fn main() {
         "attention_internal.h",
         "tcgen05.cuh",
         "attention_parts.cuh",
+        "attention_decode.cuh",
     ] {
         println!("cargo:rerun-if-changed={}", csrc.join(h).display());
     }

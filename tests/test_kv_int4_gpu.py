@@ -4,10 +4,14 @@ The writer's codes and scales are those of the quotients themselves, which the r
 compared exactly (f32 rows whose quotients lie within 2^-50 of a border would not be, and there are none here). The reader
 rounds code x group's scale x row's scale once, or twice to 16 bits: exact where eight bits fit.
 
-attention_decode, element by element, with A = sum_j p_j |v_j|: the output's rounding, u |o|; q in two f16 pieces (22 bits) moves a
-score by 2^-23 scale sum |q k|, and the f32 sums of its products by up to ten roundings of that, 2^-16 in all at scale
-sum |q k| <= 13 (normal values, head_dim 128); the exponential is good to 2^-22 and its f32 argument below 2^5 to 2^-20; p keeps
-22 bits. A relative change of p by e moves o by 2 e A at most: 2^-15 A.
+attention_decode, element by element, with A = sum_j p_j |v_j|: the output's rounding, u |o|; q in two f16 pieces (22 bits; one piece
+is exact for 16-bit q) moves a score by 2^-23 scale sum |q k|, and the f32 sums of its products by up to ten roundings of that,
+2^-16 in all at scale sum |q k| <= 13 (normal values, head_dim 128); the exponential is good to 2^-22 and its f32 argument below
+2^5 to 2^-20; p keeps 22 bits under f32 q. A relative change of p by e moves o by 2 e A at most: 2^-15 A, and in proportion where
+scale sum |q k| is more than 13. Under 16-bit q p is rounded to f16 once more, 2^-11 of itself at most: 2^-11 A (its sum is that
+of p itself). Then, p s (s a row's scale) is made of f16 numbers, which have steps of 2^-24 at least: it is off by half of one, where
+the largest p s is 2^7 or more, so by 2^-32 of the largest. An element is at most 3136 s, which is less than twice its row's
+largest, so that each of n tokens may move o by 2^-31 of the largest p max |v|.
 """
 import pytest
 import torch
@@ -200,8 +204,8 @@ def check_decode(q, cache, table, lens, got, scale=None, most=None):
     want, size = step_ref.decode4(q, cache, table, lens, scale)
     # |q| |k| >= sum |q k|, |k| of normal rows with larger channels at most 20 at head_dim 128
     scores = (q.double().norm(dim=-1).max().item() * 20 * (128 ** -0.5 if scale is None else scale))
-    part = 2.0 ** -15 * max(1.0, scores / 13)
-    floor = max(lens) * 2.0 ** -42 * (8.0 if most is None else most)
+    part = 2.0 ** -15 * max(1.0, scores / 13) + (0.0 if q.dtype == F32 else ref.UNIT[F16])
+    floor = max(lens) * 2.0 ** -31 * (8.0 if most is None else most)
     got = got.double().cpu()
     assert torch.isfinite(got).all()
     worst = ((got - want).abs() - ref.UNIT[q.dtype] * want.abs() - part * size - floor).max()
