@@ -19,13 +19,11 @@
 // The maxima, sums, s, p and o are f32.
 #include "attention_decode.cuh"
 
-#include <type_traits>
-
 namespace iq2 {
 
 namespace {
 
-constexpr int A4_WARPS = 12, A4_THREADS = A4_WARPS * 32, A4_STAGES = 2;
+constexpr int A4_WARPS = 12, A4_THREADS = A4_WARPS * 32;
 static_assert(2 * A4_WARPS <= 32, "a lane a piece");
 constexpr int A4_TOK = 32, A4_NT = A4_TOK / 8;  // tokens of a warp's stage, and eights of them
 constexpr int A4_RUN = 8;                // tokens that lie side by side in a page of a multiple of these
@@ -42,7 +40,7 @@ struct Shape4 {
     static constexpr int KS = DP / 16, MT = DP / 16;       // steps of S's inner index, row tiles of O
     static constexpr int SCALES = 2 * A4_TOK * ROW;        // of a stage: row scales of K and V, then group scales, a word a token
     static constexpr int STAGE = SCALES + 4 * A4_TOK * 4;
-    static constexpr int RING = A4_STAGES * STAGE;
+    static constexpr int RING = 2 * STAGE;
     static constexpr int HEAD = DP + 4;                    // floats of a head in a piece's slot
     static constexpr int MAXIMA = AD_HEADS * HEAD, SUMS = MAXIMA + AD_HEADS, SLOT = SUMS + AD_HEADS;  // floats of one (o, max, sum)
     static constexpr int PART = AD_HEADS * (DP + 2);       // and in the workspace
@@ -152,23 +150,22 @@ __device__ __forceinline__ float* slot_of(uint8_t* smem, uint32_t i) {
     return reinterpret_cast<float*>(smem + (i % 2 == 0 ? A4_WARPS * S::RING + i / 2 * (S::SLOT * 4) : i / 2 * S::RING));
 }
 
-// WIDE: q of 32 bits, and two pieces of q and p; of 16 bits, q is one piece exactly and p is rounded to f16 once.
-template <int DP, bool WIDE>
+// WIDE: q of 32 bits, and two pieces of q and p; of 16 bits, q is one piece exactly and p is rounded to f16 once. FULL: head_dim
+// is DP.
+template <int DP, bool WIDE, bool FULL>
 __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_constant__ DecodeArgs a) {
     using S = Shape4<DP>;
     constexpr int TOK = A4_TOK, NT = A4_NT, KS = S::KS, MT = S::MT;
-    using Tokens = std::conditional_t<TOK == 64, uint64_t, uint32_t>;  // a bit a token of a tile
     using Cursor = iq2::Cursor<AD_I4_UNIT, AD_I4_ITEM_COST>;
-    constexpr Tokens ALL = ~(Tokens)0;
     const DecodeParams& p = a.p;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Piece pieces[2 * A4_WARPS];  // of each warp its first and its last, of those that are not a whole item
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
-    const uint32_t d = p.c.d, group = p.q_heads / p.c.heads, items = p.c.heads * a.chunks_of_heads;
+    const uint32_t d = FULL ? DP : p.c.d, group = p.q_heads / p.c.heads, items = p.c.heads * a.chunks_of_heads;
     pdl_launch_dependents();
 
     // the ring starts as zeros: chunks past head_dim are never copied, and the matrix instructions read them
-    if (d < DP)
+    if (!FULL)
         for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
     if (lane < 2) pieces[warp * 2 + lane].valid = 0;
     typename Cursor::Part of;
@@ -178,130 +175,115 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     if (cur.t0 == cur.t1) cur.unit = cur.end;  // nothing, or nothing but an item's start
     Cursor pre = cur;
 
-    // ---- the copies: tile `i` (TOK tokens) of pre's piece of an item, one page lookup ahead ----
+    // ---- the copies: pre's tile from token pre_tok on, whose pages have been looked up ----
     const uint32_t ring = smem_u32(smem + warp * S::RING);
     __syncwarp();
-    // a tile's rows lie side by side in one page, or in runs of eight, or each lane looks its rows up
+    // a tile's rows lie side by side in one page, or in runs of eight, or each lane looks its row up
     const bool whole_tiles = p.c.page_size % TOK == 0, runs = p.c.page_size % A4_RUN == 0;
-    const uint32_t row_bytes = d / 2, chunk = lane % S::CHUNKS, row0 = lane / S::CHUNKS;
     constexpr int ROWS = 32 / S::CHUNKS;  // rows that the warp copies at a time
-    uint32_t pre_i = 0, page0 = 0, page1 = 0, ahead = 0;  // the tile to copy next; pages looked up, and tiles since
+    const uint32_t row_bytes = d / 2, chunk = lane % S::CHUNKS, row0 = lane / S::CHUNKS;
+    const uint32_t page_rows = p.c.heads * p.c.page_size;
+    const bool inside = FULL || chunk * 16 < row_bytes;
+    const uint8_t* const k_from = static_cast<const uint8_t*>(p.c.k) + chunk * 16;
+    const int64_t v_less_k = static_cast<const uint8_t*>(p.c.v) - static_cast<const uint8_t*>(p.c.k);
+    // 32 words of each kind of scale, 16 bytes a lane: row scales of K and V, then group scales
+    const uint8_t* const scales_from = (lane < 8 ? reinterpret_cast<const uint8_t*>(p.c.k_scale) : lane < 16 ? reinterpret_cast<const uint8_t*>(p.c.v_scale)
+                                        : lane < 24 ? p.c.k_group : p.c.v_group);
+    uint32_t pre_tok = cur.t0, pre_in = 0, pre_head = 0;  // the tile to copy next, its place in its page (whole tiles), rows of the heads before
+    uint32_t page = 0, ahead = 0;                         // this lane's page of those looked up; tiles since
+    bool live = !pre.done(), fresh = true;
     auto look_up = [&](uint32_t tok) {
         return tok < pre.t1 ? (uint32_t)__ldg(p.block_table + (int64_t)pre.b * p.table_width + a.by_page.quotient(tok)) : 0xFFFFFFFFu;
     };
+    auto in_page = [&](uint32_t tok) { return tok - a.by_page.quotient(tok) * p.c.page_size; };
     auto find_tile = [&]() {  // the next tile of this warp, and its page numbers under way
-        bool fresh = ahead == 32;
-        while (!pre.done() && pre.t0 + pre_i * TOK >= pre.t1) {
+        if (pre_tok >= pre.t1) {
             pre.next(p, items);
-            pre_i = 0, fresh = true;
+            live = !pre.done();
+            pre_tok = pre.t0, fresh = true;
         }
-        if (pre.done()) return;
-        const uint32_t tok = pre.t0 + pre_i * TOK;
+        if (!live) return;
+        if (fresh) pre_head = pre.item / a.chunks_of_heads * p.c.page_size;
         if (whole_tiles) {  // lanes hold the pages of this warp's next 32 tiles
-            if (fresh || pre_i == 0) page0 = look_up(tok + lane * TOK), ahead = 0;
-        } else if (runs) {  // of the tile's runs
-            page0 = look_up(tok + lane % (TOK / A4_RUN) * A4_RUN);
-        } else {            // of its tokens
-            page0 = look_up(tok + lane);
-            if (TOK == 64) page1 = look_up(tok + lane + 32);
+            if (fresh || ahead == 32) page = look_up(pre_tok + lane * TOK), pre_in = in_page(pre_tok), ahead = 0;
+        } else {            // of the tile's runs, or of its tokens
+            page = look_up(pre_tok + (runs ? lane % (TOK / A4_RUN) * A4_RUN : lane));
         }
+        fresh = false;
     };
     // Copies the tile and returns a bit for each token that takes part: rows of tokens past the end, or of pages outside
     // the cache, are zeros, and what such pages hold cannot matter.
-    auto copy_tile = [&](uint32_t stage) {
-        const uint32_t tok = pre.t0 + pre_i * TOK, h = pre.item / a.chunks_of_heads, dst = ring + stage * S::STAGE, left = pre.t1 - tok;
-        const uint8_t *const k = static_cast<const uint8_t*>(p.c.k), *const v = static_cast<const uint8_t*>(p.c.v);
-        const bool inside = chunk * 16 < row_bytes;
-        auto cache_row = [&](uint32_t page, uint32_t at) {  // of token `at`, -1: none
-            const uint32_t in_page = at - a.by_page.quotient(at) * p.c.page_size;
-            return page < p.c.pages ? ((int64_t)page * p.c.heads + h) * p.c.page_size + in_page : (int64_t)-1;
-        };
-        // 16 bytes of scales a lane and turn: row scales of K and V, then group scales
-        auto scales_of = [&](int turn) {
-            const uint32_t kind = (turn * 32 + lane) / (TOK / 4);
-            return kind == 0 ? reinterpret_cast<const uint8_t*>(p.c.k_scale) : kind == 1 ? reinterpret_cast<const uint8_t*>(p.c.v_scale)
-                 : kind == 2 ? p.c.k_group : p.c.v_group;
-        };
-        int64_t mine0, mine1;  // the rows of tokens `lane` and `lane` + 32
-        ++pre_i;
+    auto copy_tile = [&](uint32_t dst) {
+        const uint32_t left = pre.t1 - pre_tok;
+        int64_t mine;  // the row of token `lane`, -1: none
         if (whole_tiles) {
-            const int64_t row = cache_row(__shfl_sync(0xFFFFFFFFu, page0, ahead++), tok);
-            if (row >= 0 && left >= TOK) {
-                const int64_t off = (row + row0) * row_bytes + chunk * 16;
-                const uint8_t *pk = k + off, *pv = v + off;
+            const uint32_t at = __shfl_sync(0xFFFFFFFFu, page, ahead++);
+            const int64_t row = (int64_t)((uint64_t)at * page_rows + (pre_head + pre_in));
+            pre_in = pre_in + TOK == p.c.page_size ? 0 : pre_in + TOK;
+            if (at < p.c.pages && left >= TOK) {
+                const uint8_t* const pk = k_from + (row + row0) * row_bytes;
+                const uint8_t* const pv = pk + v_less_k;
                 if (inside) {
 #pragma unroll
-                    for (int i = 0; i < TOK / ROWS; ++i, pk += ROWS * row_bytes, pv += ROWS * row_bytes) {
-                        cp_async_16(dst + chunk_offset<S::CHUNKS>(row0 + i * ROWS, chunk), pk);
-                        cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(row0 + i * ROWS, chunk), pv);
+                    for (int i = 0; i < TOK / ROWS; ++i) {
+                        cp_async_16(dst + chunk_offset<S::CHUNKS>(row0 + i * ROWS, chunk), pk + i * ROWS * row_bytes);
+                        cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(row0 + i * ROWS, chunk), pv + i * ROWS * row_bytes);
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < TOK / 32; ++i) cp_async_16(dst + S::SCALES + (i * 32 + lane) * 16, scales_of(i) + row * 4 + lane % (TOK / 4) * 16);
-                return ALL;
+                cp_async_16(dst + S::SCALES + lane * 16, scales_from + (row * 4 + lane % 8 * 16));
+                return 0xFFFFFFFFu;
             }
-            mine0 = row >= 0 && lane < left ? row + lane : -1;
-            mine1 = row >= 0 && lane + 32 < left ? row + lane + 32 : -1;
+            mine = at < p.c.pages && lane < left ? row + lane : -1;
         } else if (runs) {
-            const int64_t run = cache_row(page0, tok + lane % (TOK / A4_RUN) * A4_RUN);
+            const int64_t run = page < p.c.pages ? (int64_t)((uint64_t)page * page_rows + (pre_head + in_page(pre_tok + lane % (TOK / A4_RUN) * A4_RUN))) : -1;
             if (left >= TOK && __all_sync(0xFFFFFFFFu, run >= 0)) {
 #pragma unroll
                 for (int i = 0; i < TOK / ROWS; ++i) {
                     const uint32_t r = row0 + i * ROWS;
-                    const int64_t off = (__shfl_sync(0xFFFFFFFFu, run, r / A4_RUN) + r % A4_RUN) * row_bytes + chunk * 16;
+                    const uint8_t* const pk = k_from + (__shfl_sync(0xFFFFFFFFu, run, r / A4_RUN) + r % A4_RUN) * row_bytes;
                     if (inside) {
-                        cp_async_16(dst + chunk_offset<S::CHUNKS>(r, chunk), k + off);
-                        cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(r, chunk), v + off);
+                        cp_async_16(dst + chunk_offset<S::CHUNKS>(r, chunk), pk);
+                        cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(r, chunk), pk + v_less_k);
                     }
                 }
-                const int64_t at = __shfl_sync(0xFFFFFFFFu, run, lane % (TOK / 4) / 2) * 4 + lane % 2 * 16;
-#pragma unroll
-                for (int i = 0; i < TOK / 32; ++i) cp_async_16(dst + S::SCALES + (i * 32 + lane) * 16, scales_of(i) + at);
-                return ALL;
+                cp_async_16(dst + S::SCALES + lane * 16, scales_from + (__shfl_sync(0xFFFFFFFFu, run, lane % 8 / 2) * 4 + lane % 2 * 16));
+                return 0xFFFFFFFFu;
             }
-            const int64_t run0 = __shfl_sync(0xFFFFFFFFu, run, lane / A4_RUN), run1 = __shfl_sync(0xFFFFFFFFu, run, lane / A4_RUN + 4);
-            mine0 = run0 >= 0 && lane < left ? run0 + lane % A4_RUN : -1;
-            mine1 = run1 >= 0 && lane + 32 < left ? run1 + lane % A4_RUN : -1;
+            const int64_t from = __shfl_sync(0xFFFFFFFFu, run, lane / A4_RUN);
+            mine = from >= 0 && lane < left ? from + lane % A4_RUN : -1;
         } else {
-            mine0 = cache_row(page0, tok + lane), mine1 = cache_row(page1, tok + lane + 32);
+            mine = page < p.c.pages ? (int64_t)((uint64_t)page * page_rows + (pre_head + in_page(pre_tok + lane))) : -1;
         }
 #pragma unroll 1
         for (int i = 0; i < TOK / ROWS; ++i) {
             const uint32_t r = row0 + i * ROWS;
-            const int64_t src = __shfl_sync(0xFFFFFFFFu, i * ROWS < 32 ? mine0 : mine1, r % 32);
-            const int64_t off = src < 0 ? 0 : src * row_bytes + chunk * 16;
+            const int64_t src = __shfl_sync(0xFFFFFFFFu, mine, r);
+            const uint8_t* const pk = k_from + (src < 0 ? 0 : src * row_bytes);
             if (inside) {
-                cp_async_16(dst + chunk_offset<S::CHUNKS>(r, chunk), k + off, src < 0 ? 0 : 16);
-                cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(r, chunk), v + off, src < 0 ? 0 : 16);
+                cp_async_16(dst + chunk_offset<S::CHUNKS>(r, chunk), pk, src < 0 ? 0 : 16);
+                cp_async_16(dst + TOK * S::ROW + chunk_offset<S::CHUNKS>(r, chunk), pk + v_less_k, src < 0 ? 0 : 16);
             }
         }
-#pragma unroll 1
-        for (int i = 0; i < TOK / 32; ++i) {
-            const int64_t src = i == 0 ? mine0 : mine1, at = max(src, (int64_t)0);
-            const uint32_t bytes = src < 0 ? 0 : 4, to = dst + S::SCALES + (i * 32 + lane) * 4;
-            cp_async_4(to, p.c.k_scale + at, bytes);
-            cp_async_4(to + TOK * 4, p.c.v_scale + at, bytes);
-            cp_async_4(to + TOK * 8, p.c.k_group + at * 4, bytes);
-            cp_async_4(to + TOK * 12, p.c.v_group + at * 4, bytes);
-        }
-        const Tokens low = __ballot_sync(0xFFFFFFFFu, mine0 >= 0);
-        return TOK == 64 ? low | (Tokens)((uint64_t)__ballot_sync(0xFFFFFFFFu, mine1 >= 0) << 32) : low;
+        const int64_t at = max(mine, (int64_t)0);
+        const uint32_t bytes = mine < 0 ? 0 : 4, to = dst + S::SCALES + lane * 4;
+        cp_async_4(to, p.c.k_scale + at, bytes);
+        cp_async_4(to + TOK * 4, p.c.v_scale + at, bytes);
+        cp_async_4(to + TOK * 8, p.c.k_group + at * 4, bytes);
+        cp_async_4(to + TOK * 12, p.c.v_group + at * 4, bytes);
+        return __ballot_sync(0xFFFFFFFFu, mine >= 0);
     };
-    Tokens present[A4_STAGES] = {};
-    auto copy_and_find = [&](int stage) {
-        if (!pre.done()) {
-            const Tokens here = copy_tile(stage);
-#pragma unroll
-            for (int s = 0; s < A4_STAGES; ++s)
-                if (s == stage) present[s] = here;
+    uint32_t there = 0;  // the tokens of the tile that was copied last
+    auto copy_and_find = [&](uint32_t dst) {
+        if (live) {
+            there = copy_tile(dst);
+            pre_tok += TOK;
             find_tile();
         }
         cp_async_commit();
     };
-    find_tile();
-#pragma unroll 1
-    for (int s = 0; s < A4_STAGES - 1; ++s) copy_and_find(s);
-    int stage = 0;
+    if (live) find_tile();
+    copy_and_find(ring);
+    uint32_t at = ring;  // the stage to take next
 
     // this thread's places: its key row and chunk, its two value rows and their bytes, its groups' scales as bytes 1 and 3
     const uint32_t k_row = row_of(g), v_row0 = row_of(2 * t), v_row1 = row_of(2 * t + 1);
@@ -317,7 +299,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
         const uint32_t kv_head = cur.item / a.chunks_of_heads, head0 = kv_head * group + (cur.item % a.chunks_of_heads) * AD_HEADS;
         const uint32_t heads = min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
         uint32_t q_high[KS][2], q_low[KS][2];
-        float2 factor;  // scale log2(e) 2^e of the heads 2t, 2t + 1
+        float factor[2];  // scale log2(e) 2^e of the heads 2t, 2t + 1
         {
             float x[DP / 4], top = 0.f, unit = A4_VALUE, down = 1.f;  // 2^e and 2^(15 - e)
             load_row<DP / 4>(p.q.p, (int64_t)cur.b * p.q.token_stride + (int64_t)(head0 + g) * p.q.head_stride + t * (DP / 4), p.dtype,
@@ -328,8 +310,8 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -110), 126);
             if (top > 0.f && top < INFINITY) unit = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(142 - e) << 23);
-            const float f = p.scale * LOG2E * unit;
-            factor = make_float2(__shfl_sync(0xFFFFFFFFu, f, t * 8), __shfl_sync(0xFFFFFFFFu, f, t * 8 + 4));
+            const float f = fmaxf(p.scale * LOG2E * unit, 1.17549435e-38f);  // (not 0: times -infinity it stays that)
+            factor[0] = __shfl_sync(0xFFFFFFFFu, f, t * 8), factor[1] = __shfl_sync(0xFFFFFFFFu, f, t * 8 + 4);
             // elements j and j + 4 of a word's eight are a pair: j = 0, 1 of one step, j = 2, 3 of the next
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i)
@@ -346,17 +328,12 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
 #pragma unroll
         for (int n = 0; n < MT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
-        const uint32_t tokens = cur.t1 - cur.t0;
 #pragma unroll 1
-        for (uint32_t i = 0; i * TOK < tokens; ++i) {
-            cp_async_wait<A4_STAGES - 2>();
+        for (uint32_t tok = cur.t0; tok < cur.t1; tok += TOK) {
+            cp_async_wait<0>();
             __syncwarp();
-            const uint32_t at = ring + stage * S::STAGE;
-            Tokens here = 0;
-#pragma unroll
-            for (int s = 0; s < A4_STAGES; ++s)
-                if (s == stage) here = present[s];
-            copy_and_find(stage == 0 ? A4_STAGES - 1 : stage - 1);  // the stage the last tile freed
+            const uint32_t here = there;
+            copy_and_find(2 * ring + S::STAGE - at);  // the stage that the last tile freed
 
             // ---- S^T: rows are tokens row_of(g) of each eight, columns the heads 2t, 2t + 1 ----
             float x[NT][2];
@@ -391,31 +368,31 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 x[mt * 2][0] = s[0], x[mt * 2][1] = s[1], x[mt * 2 + 1][0] = s[2], x[mt * 2 + 1][1] = s[3];
             }
 
-            // x = log2(e) scale q . k; w = 2^(x - m) times the value scale
+            // factor x = log2(e) scale q . k; w = 2^(factor x - m) times the value scale
             float e[NT][2], w[NT][2], vs[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint32_t from = at + S::SCALES + (n * 8 + k_row) * 4;
                 const float ks = __uint_as_float(ld_shared(from));
                 vs[n] = max_nan(__uint_as_float(ld_shared(from + TOK * 4)) * A4_UP, A4_MIN_SCALE);
-                x[n][0] *= ks * factor.x, x[n][1] *= ks * factor.y;
+                x[n][0] *= ks, x[n][1] *= ks;
             }
-            if (here != ALL) {
+            if (here != 0xFFFFFFFFu) {
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
                     if (!((here >> (n * 8 + k_row)) & 1u)) x[n][0] = x[n][1] = -INFINITY;
             }
             // The reference does as a rule: the products are made with it, and made again in the rare case that it moves.
-            bool fresh = __any_sync(0xFFFFFFFFu, m[0] == -INFINITY || m[1] == -INFINITY);
+            bool first = __any_sync(0xFFFFFFFFu, m[0] == -INFINITY || m[1] == -INFINITY);
             for (;;) {
-                if (!fresh) {
+                if (!first) {
                     float top = 0.f;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const float base = m[h] == -INFINITY ? 0.f : m[h] - A4_TOP;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            e[n][h] = exp2_approx(x[n][h] - base);
+                            e[n][h] = exp2_approx(fmaf(x[n][h], factor[h], -base));
                             w[n][h] = e[n][h] * vs[n];
                             top = fmaxf(top, w[n][h]);
                         }
@@ -429,7 +406,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 for (int h = 0; h < 2; ++h) {
                     float most = -INFINITY;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) most = fmaxf(most, x[n][h] + __log2f(vs[n]));
+                    for (int n = 0; n < NT; ++n) most = fmaxf(most, fmaf(x[n][h], factor[h], __log2f(vs[n])));
 #pragma unroll
                     for (int b = 4; b < 32; b *= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, b));
                     const float next = fmaxf(m[h], most);
@@ -437,8 +414,8 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                     moved = moved || next > m[h];
                     m[h] = next;
                 }
-                if (!__any_sync(0xFFFFFFFFu, moved) && !fresh) break;
-                fresh = false;
+                if (!__any_sync(0xFFFFFFFFu, moved) && !first) break;
+                first = false;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     l[h] *= keep[h];
@@ -492,7 +469,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 }
             }
             __syncwarp();
-            stage = stage == A4_STAGES - 1 ? 0 : stage + 1;
+            at = 2 * ring + S::STAGE - at;
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
@@ -539,8 +516,8 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
 
     // ---- the warps' pieces: those of one item follow one another. A warp an item and head ----
     const Piece mine = lane < 2 * A4_WARPS ? pieces[lane] : Piece{0, 0, 0};
-    const uint32_t there = __ballot_sync(0xFFFFFFFFu, mine.valid != 0);
-    const int before = 31 - __clz(there & ((1u << lane) - 1));  // the piece before this lane's, -1: none
+    const uint32_t held = __ballot_sync(0xFFFFFFFFu, mine.valid != 0);
+    const int before = 31 - __clz(held & ((1u << lane) - 1));  // the piece before this lane's, -1: none
     const uint32_t b_before = __shfl_sync(0xFFFFFFFFu, mine.b, max(before, 0)), item_before = __shfl_sync(0xFFFFFFFFu, mine.item, max(before, 0));
     uint32_t starts = __ballot_sync(0xFFFFFFFFu, mine.valid != 0 && (before < 0 || b_before != mine.b || item_before != mine.item));
     uint32_t turn = warp;  // (item, head) pairs until this warp's next
@@ -548,7 +525,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     while (starts != 0) {
         const int at = __ffs(starts) - 1;
         starts &= starts - 1;
-        const uint32_t ours = there & ~((1u << at) - 1) & (starts != 0 ? (starts & -starts) - 1 : 0xFFFFFFFFu);
+        const uint32_t ours = held & ~((1u << at) - 1) & (starts != 0 ? (starts & -starts) - 1 : 0xFFFFFFFFu);
         const int last = 31 - __clz(ours);
         const uint32_t b = __shfl_sync(0xFFFFFFFFu, mine.b, at), item = __shfl_sync(0xFFFFFFFFu, mine.item, at);
         const uint32_t from = __shfl_sync(0xFFFFFFFFu, mine.valid, at), to = __shfl_sync(0xFFFFFFFFu, mine.valid, last);
@@ -582,21 +559,27 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     }
 }
 
-template <int DP, bool WIDE>
+template <int DP, bool WIDE, bool FULL>
 cudaError_t launch4(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(decode4_kernel<DP, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape4<DP>::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(decode4_kernel<DP, WIDE, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape4<DP>::SMEM);
     if (e != cudaSuccess) return e;
-    decode4_kernel<DP, WIDE><<<blocks, A4_THREADS, Shape4<DP>::SMEM, stream>>>(a);
+    decode4_kernel<DP, WIDE, FULL><<<blocks, A4_THREADS, Shape4<DP>::SMEM, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess) return e;
     return launch_join<DP>(a, blocks, stream);
+}
+
+template <int DP>
+cudaError_t launch4_of(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
+    const bool full = a.p.c.d == DP;
+    if (a.p.dtype == kF32) return full ? launch4<DP, true, true>(a, blocks, stream) : launch4<DP, true, false>(a, blocks, stream);
+    return full ? launch4<DP, false, true>(a, blocks, stream) : launch4<DP, false, false>(a, blocks, stream);
 }
 
 }  // namespace
 
 cudaError_t launch_attention_decode_int4(const DecodeParams& p, void* workspace, int num_sms, cudaStream_t stream) {
     const DecodeArgs a = decode_args(p, workspace, num_sms);
-    if (p.dtype == kF32) return p.c.d > 64 ? launch4<128, true>(a, num_sms, stream) : launch4<64, true>(a, num_sms, stream);
-    return p.c.d > 64 ? launch4<128, false>(a, num_sms, stream) : launch4<64, false>(a, num_sms, stream);
+    return p.c.d > 64 ? launch4_of<128>(a, num_sms, stream) : launch4_of<64>(a, num_sms, stream);
 }
 
 }  // namespace iq2
