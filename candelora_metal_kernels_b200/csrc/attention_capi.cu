@@ -163,7 +163,7 @@ int iq2_kv_cache_read(const iq2_kv_cache* cache, const int32_t* block_table, uin
                                   {"v_out", v_out, 16}})) != IQ2_OK)
         return rc;
     if (starts != nullptr && (rc = check_pointers(op, {{"starts", starts, 4}})) != IQ2_OK) return rc;
-    const iq2::KvReadParams p{view(cache), block_table, starts, cu_seqlens, table_width, sequences, total, k_out, v_out, out_dtype};
+    const iq2::KvReadParams p{view(cache), block_table, starts, cu_seqlens, table_width, sequences, total, k_out, v_out, out_dtype, {}};
     const cudaError_t err = iq2::launch_kv_read(p, reinterpret_cast<cudaStream_t>(stream));
     return err == cudaSuccess ? IQ2_OK : capi_cuda_fail(op, err);
 }

@@ -129,11 +129,11 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     // the ring starts as zeros: chunks past head_dim are never copied, and the matrix instructions read them
     if (d < DP)
         for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
-    using Cursor = iq2::Cursor<UNIT, AD_ITEM_COST>;
-    typename Cursor::Part part_of;
-    Cursor cur = Cursor::of_part(a, blockIdx.x, gridDim.x, a.inv_blocks, threadIdx.x, AD_THREADS, part_of);
-    const uint64_t u0 = part_of.u0;
-    if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(u0, part_of.each);
+    using Cursor = iq2::Cursor<UNIT, AD_ITEM_COST, false>;
+    typename Cursor::Parts line;
+    Cursor cur = Cursor::of_part(a, blockIdx.x, gridDim.x, a.inv_blocks, threadIdx.x, AD_THREADS, line);
+    const uint64_t u0 = line.begin(blockIdx.x);
+    if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, blockIdx.x, 1);
     if (cur.t0 == cur.t1) return;  // nothing, or nothing but an item's start
     Cursor pre = cur;
 

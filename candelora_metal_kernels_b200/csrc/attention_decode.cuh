@@ -16,7 +16,8 @@ constexpr int AD_HEADS = 8;  // query heads of an item
 // 1 x 100001 49.7 / 48.6 / 47.9 us.
 constexpr uint32_t AD_ITEM_COST = 3;
 constexpr uint32_t AD_I4_UNIT = 32;  // tokens that the line of work is cut at for 4-bit caches: a warp's tile
-constexpr uint32_t AD_I4_ITEM_COST = 2;
+// Measured with 0 / 1 / 2 / 4: 128 x 4096 tokens 94.7 / 92.9 / 93.7 / 95.3 us, 1 x 333 11.4 / 9.4 / 10.8 / 11.2 us.
+constexpr uint32_t AD_I4_ITEM_COST = 1;
 constexpr float LOG2E = 1.44269504f;
 
 // What join_kernel's block of the same number has to join: the parts of blocks c0 to c1 of one item, block c0's being its
@@ -100,7 +101,9 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 
 // The line of work from one unit on: the item it is in and the tokens [t0, t1) of that item in the part. The line's units are UNIT
 // tokens; an item's first COST units have no tokens, and a part that ends inside them has none (the next part has the item).
-template <uint32_t UNIT, uint32_t COST>
+// EVEN: parts differ by a unit at most, of one unit at least, so that none is empty but behind the line's end (the parts of an item
+// follow one another); otherwise all but the last ones are of the same length, rounded up.
+template <uint32_t UNIT, uint32_t COST, bool EVEN>
 struct Cursor {
     uint64_t unit, end;
     uint32_t b, item, len, units;  // the sequence, its item (key head, group of query heads), tokens and units an item
@@ -132,14 +135,20 @@ struct Cursor {
         if (t0 == t1) unit = end;
     }
 
-    // The first unit and the units of part `part` of `parts` equal ones.
-    struct Part {
-        uint64_t u0, each;
+    // Where the parts of the line begin: EVEN at multiples of a fraction, rounded down, the same for whoever asks.
+    struct Parts {
+        uint64_t units, each;  // of the line; of a part
+        uint32_t parts;
+        double share;          // units / parts
+        __device__ __forceinline__ uint64_t begin(uint32_t part) const {
+            if (EVEN) return part >= parts ? units : min((uint64_t)(part * share), units);
+            return min(part * each, units);
+        }
     };
     // Part `part` of `parts` as a cursor (done at once where there is nothing). A warp works it out by itself, from the lengths.
     // Sequences of length 0 get their zeros here, a part a sequence, from the `threads` threads that take the part.
     static __device__ __forceinline__ Cursor of_part(const DecodeArgs& a, uint32_t part, uint32_t parts, double inv_parts, uint32_t thread,
-                                                     uint32_t threads, Part& of) {
+                                                     uint32_t threads, Parts& line) {
         const DecodeParams& p = a.p;
         const uint32_t lane = threadIdx.x % 32, d = p.c.d, items = p.c.heads * a.chunks_of_heads;
         uint64_t units = 0;
@@ -160,10 +169,12 @@ struct Cursor {
 #pragma unroll
         for (int o = 16; o > 0; o /= 2) units += __shfl_xor_sync(0xFFFFFFFFu, units, o);
         units *= items;
-        uint64_t each = (uint64_t)((double)units * inv_parts);  // units / parts, rounded up
-        while (each * parts < units) ++each;
-        const uint64_t u0 = min(part * each, units), u1 = min(u0 + each, units);
-        of = {u0, each};
+        line = {units, 0, parts, EVEN ? max((double)units * inv_parts, 1.0) : (double)units * inv_parts};
+        if (!EVEN) {
+            line.each = (uint64_t)line.share;  // units / parts, rounded up
+            while (line.each * parts < units) ++line.each;
+        }
+        const uint64_t u0 = line.begin(part), u1 = line.begin(part + 1);
         Cursor cur{};
         if (u0 < u1) {
             uint64_t before = 0;  // units of the sequences before
@@ -194,14 +205,15 @@ struct Cursor {
         return cur;
     }
 
-    // What the block of a part that begins with this cursor (`each` units a block) has to join.
-    __device__ __forceinline__ JoinRecord record(uint64_t u0, uint64_t each) const {
+    // What the block has to join whose part, `per_block` ones of the line from `part` on, begins with this cursor.
+    __device__ __forceinline__ JoinRecord record(const Parts& line, uint32_t part, uint32_t per_block) const {
         // the first block whose part begins inside an item's tokens joins it: the block before it has the first of them
-        const uint64_t unit0 = u0 - k;
         JoinRecord r{b, item, blockIdx.x - 1, 0, 0};
-        if (t0 > 0 && u0 - each <= unit0 + COST) {
-            r.c1 = blockIdx.x, r.slot = u0 - each >= unit0 ? 0 : 1;
-            while ((r.c1 + 1) * each < unit0 + units) ++r.c1;
+        if (t0 == 0) return r;
+        const uint64_t unit0 = unit - k, before = line.begin(part - per_block);
+        if (before <= unit0 + COST) {
+            r.c1 = blockIdx.x, r.slot = before >= unit0 ? 0 : 1;
+            while (line.begin((r.c1 + 1) * per_block) < unit0 + units) ++r.c1;
         }
         return r;
     }

@@ -156,7 +156,7 @@ template <int DP, bool WIDE, bool FULL>
 __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_constant__ DecodeArgs a) {
     using S = Shape4<DP>;
     constexpr int TOK = A4_TOK, NT = A4_NT, KS = S::KS, MT = S::MT;
-    using Cursor = iq2::Cursor<AD_I4_UNIT, AD_I4_ITEM_COST>;
+    using Cursor = iq2::Cursor<AD_I4_UNIT, AD_I4_ITEM_COST, true>;
     const DecodeParams& p = a.p;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ Piece pieces[2 * A4_WARPS];  // of each warp its first and its last, of those that are not a whole item
@@ -168,10 +168,11 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     if (!FULL)
         for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
     if (lane < 2) pieces[warp * 2 + lane].valid = 0;
-    typename Cursor::Part of;
-    Cursor cur = Cursor::of_part(a, blockIdx.x * A4_WARPS + warp, gridDim.x * A4_WARPS, a.inv_blocks * (1.0 / A4_WARPS), lane, 32, of);
-    if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(of.u0, of.each * A4_WARPS);
-    const uint64_t block_u0 = of.u0 - min(of.u0, warp * of.each);
+    typename Cursor::Parts line;
+    const uint32_t part0 = blockIdx.x * A4_WARPS;  // the block's parts of the line, one a warp
+    Cursor cur = Cursor::of_part(a, part0 + warp, gridDim.x * A4_WARPS, a.inv_blocks * (1.0 / A4_WARPS), lane, 32, line);
+    if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, part0, A4_WARPS);
+    const uint64_t first_unit = cur.unit, block_u0 = line.begin(part0);
     if (cur.t0 == cur.t1) cur.unit = cur.end;  // nothing, or nothing but an item's start
     Cursor pre = cur;
 
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 }
             }
         } else {
-            const bool first = cur.unit == of.u0;
+            const bool first = cur.unit == first_unit;
             // (the last piece takes the ring: all of the warp's copies are done then)
             float* const slot = slot_of<S>(smem, warp * 2 + !first);
             if (!first) {

@@ -58,6 +58,8 @@ struct KvWriteParams {
     uint32_t q_norm_stride, k_norm_stride;        // from one head's weights to the next's: 0 or d
     double eps, inv_d;                            // inv_d: 1 / d
     Divisor by_heads, by_page;  // set by the launch: heads of a token (q, k and v), tokens of a page
+    Divisor by_q, by_kv;        // (with norms or a 4-bit cache) heads of q and of k, and blocks that have rows of them
+    uint32_t blocks_q, blocks_kv;
 };
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);
 
@@ -67,6 +69,7 @@ struct KvReadParams {
     uint32_t table_width, seqs, total;
     void *k_out, *v_out;  // [total][heads][d]
     int out_dtype;
+    Divisor by_heads;  // set by the launch
 };
 cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream);
 

@@ -122,87 +122,6 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
     return prmt(prmt(code(x[0]), code(x[1]), 0x0040u), prmt(code(x[2]), code(x[3]), 0x0040u), 0x5410u);
 }
 
-// The cosines and sines of a thread's V pairs: (a[i], b[i]), or interleaved those of a and then those of b.
-template <int V>
-__device__ __forceinline__ void load_turns(const KvWriteParams& p, int64_t row, uint32_t lane, float (&c)[V], float (&s)[V]) {
-    if (!p.interleaved) {
-        load_angles(p.cos + row + lane * V, p.vec, c), load_angles(p.sin + row + lane * V, p.vec, s);
-        return;
-    }
-    const int64_t i0 = row + lane * (V / 2), i1 = i0 + p.c.d / 4;
-    float c0[V / 2], s0[V / 2], c1[V / 2], s1[V / 2];
-    load_angles(p.cos + i0, p.vec, c0), load_angles(p.sin + i0, p.vec, s0);
-    load_angles(p.cos + i1, p.vec, c1), load_angles(p.sin + i1, p.vec, s1);
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) c[i] = c0[i], s[i] = s0[i], c[V / 2 + i] = c1[i], s[V / 2 + i] = s1[i];
-}
-
-// The value of e4m3 bits without a sign, and the bits nearest to x >= 0.
-__device__ __forceinline__ float e4m3_value(uint32_t bits) { return __uint_as_float(bits << 20) * 1.32922800e36f; }  // 2^120
-__device__ __forceinline__ uint32_t e4m3_pair(float low, float high) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
-    return r;
-}
-
-// V codes of a group with the step s g (0: all of them are 0) as nibbles.
-template <int V>
-__device__ __forceinline__ uint32_t codes_int4(const float (&x)[V], float step) {
-    float inv;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        float c = __fadd_rn(__fadd_rn(__fmul_rn(x[i], inv), 12582912.0f), -12582912.0f);
-        const float rest = __fmaf_rn(-c, step, x[i]), over = fabsf(rest) - 0.5f * step;
-        if (over > 0.f || (over == 0.f && ((int)c & 1))) c += copysignf(1.f, rest);
-        c = fminf(fmaxf(c, -7.f), 7.f);
-        if (step == 0.f) c = 0.f;
-        w |= (__float_as_uint(c + 12582920.0f) & 15u) << (4 * i);
-    }
-    return w;
-}
-
-// A row of the 4-bit cache: m is the row's maximum, a thread has V elements from lane V of each half, which lie in one group.
-// Called by whole warps.
-template <int LANES, int V>
-__device__ __forceinline__ void store_int4(const KvCacheView& cache, int64_t row, uint32_t half, uint32_t lane, bool is_v, bool wanted, float m,
-                                           const float (&a)[V], const float (&b)[V]) {
-    constexpr uint32_t PIECES = I4_GROUP / V;  // threads' pieces of a group
-    __shared__ float4 held[KW_THREADS / LANES][2 * LANES / 4 + 1];
-    float* const piece = reinterpret_cast<float*>(held[threadIdx.x / LANES]);
-    const uint32_t at_a = lane * V, at_b = half + lane * V;
-    float ma = 0.f, mb = 0.f;
-#pragma unroll
-    for (int i = 0; i < V; ++i) ma = max_nan(ma, fabsf(a[i])), mb = max_nan(mb, fabsf(b[i]));
-    if (at_a < half) piece[at_a / V] = ma, piece[at_b / V] = mb;
-    __syncwarp();
-    if (!wanted) return;
-#pragma unroll
-    for (uint32_t i = 0; i < PIECES; ++i) {
-        ma = max_nan(ma, piece[at_a / I4_GROUP * PIECES + i]);
-        mb = max_nan(mb, piece[at_b / I4_GROUP * PIECES + i]);
-    }
-    const bool finite = m < __int_as_float(0x7F800000), some = finite && m >= MIN_AMAX;
-    // s and 1 / s: the exponent of m, less 11, and one more where m's fraction passes 3136 / 2048
-    const uint32_t bits = __float_as_uint(m), e = some ? (bits >> 23) - 11 + ((bits & 0x7FFFFFu) > 0x440000u) : 127u;
-    const float s = some ? __uint_as_float(e << 23) : 0.f, up = __uint_as_float((254u - e) << 23);
-    const uint32_t g = some ? e4m3_pair(__fdiv_rn(ma, 7.f) * up, __fdiv_rn(mb, 7.f) * up) : 0u;
-    const uint32_t wa = codes_int4(a, some ? s * e4m3_value(g & 0xFFu) : 0.f), wb = codes_int4(b, some ? s * e4m3_value(g >> 8) : 0.f);
-    uint8_t* const dst = static_cast<uint8_t*>(is_v ? cache.v : cache.k) + row * half;
-    if (V == 4) {
-        *reinterpret_cast<uint16_t*>(dst + at_a / 2) = (uint16_t)wa;
-        *reinterpret_cast<uint16_t*>(dst + at_b / 2) = (uint16_t)wb;
-    } else {
-        *reinterpret_cast<uint32_t*>(dst + at_a / 2) = wa;
-        *reinterpret_cast<uint32_t*>(dst + at_b / 2) = wb;
-    }
-    uint8_t* const groups = (is_v ? cache.v_group : cache.k_group) + row * 4;
-    if (at_a % I4_GROUP == 0) groups[at_a / I4_GROUP] = (uint8_t)g;
-    if (at_b % I4_GROUP == 0) groups[at_b / I4_GROUP] = (uint8_t)(g >> 8);
-    if (lane == 0) (is_v ? cache.v_scale : cache.k_scale)[row] = finite ? s : __int_as_float(0x7FC00000);
-}
-
 // LANES threads (a power of two >= d / 2V) take a row: lane l holds the V elements from Vl of each half, 16 bytes of the input,
 // so that a pair of either rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head)
 // with the heads of q, then k, then v. A thread has one row (two or three in flight: 2048 tokens 16.5 / 18.5 against 14.5 us);
@@ -210,8 +129,8 @@ __device__ __forceinline__ void store_int4(const KvCacheView& cache, int64_t row
 // the kernel's (widened as it came, in pieces of eight bytes, bf16 rows of 8800 tokens took 61.5 us into a bf16 cache, not 43.6).
 // Blocks of an SM: eight for f32 rows (8800 tokens into a bf16 cache 54.0 us; with all the registers that the compiler likes
 // 58.8), six for the 16 values of a thread that 16-bit rows make (43.6 us; five 45.0, seven 44.9, with spills).
-template <int LANES, int IN, bool NORM, bool I4>
-__global__ void __launch_bounds__(KW_THREADS, NORM || I4 ? 4 : IN == kF32 ? 8 : 6) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
+template <int LANES, int IN>
+__global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
     constexpr int V = IN == kF32 ? 4 : 8;
     const uint32_t lane = threadIdx.x % LANES, r = blockIdx.x * (KW_THREADS / LANES) + threadIdx.x / LANES;
     const uint32_t heads = p.q_heads + 2 * p.c.heads, half = p.c.d / 2;
@@ -221,43 +140,7 @@ __global__ void __launch_bounds__(KW_THREADS, NORM || I4 ? 4 : IN == kF32 ? 8 : 
     const uint32_t h = head - (is_q ? 0 : is_v ? p.q_heads + p.c.heads : p.q_heads);
     float a[V] = {}, b[V] = {};
     int32_t slot = 0;
-    if (NORM) {
-        uint4 wa = make_uint4(0, 0, 0, 0), wb = wa;  // (rows that are not there add up to nothing)
-        float c[V], s[V];
-        const float* const weights = !active || is_v ? nullptr : is_q ? p.q_norm : p.k_norm;
-        const bool rotated = active && p.cos != nullptr && !is_v;
-        if (active) {
-            const RowsView& in = is_q ? p.q : is_v ? p.v : p.k;
-            const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * V;
-            wa = load16<IN>(in.p, at, p.vec), wb = load16<IN>(in.p, at + half, p.vec);
-            if (!is_q) slot = __ldg(p.slots + t);
-            if (rotated) load_turns(p, (int64_t)min((uint32_t)max(__ldg(p.positions + t), 0), p.rope_len - 1) * half, lane, c, s);
-        }
-        widen<IN>(wa, a), widen<IN>(wb, b);
-        double sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum = fma((double)a[i], (double)a[i], sum), sum = fma((double)b[i], (double)b[i], sum);
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-        if (weights != nullptr) {
-            const float r = (float)rsqrt(sum * p.inv_d + p.eps);
-            const float* const at = weights + h * (is_q ? p.q_norm_stride : p.k_norm_stride) + lane * V;
-            float w[V];
-            load_angles(at, p.vec, w);
-#pragma unroll
-            for (int i = 0; i < V; ++i) a[i] = __fmul_rn(__fmul_rn(a[i], r), w[i]);
-            load_angles(at + half, p.vec, w);
-#pragma unroll
-            for (int i = 0; i < V; ++i) b[i] = __fmul_rn(__fmul_rn(b[i], r), w[i]);
-        }
-        if (rotated && p.interleaved) {
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) rotate(a[2 * i], a[2 * i + 1], c[i], s[i]), rotate(b[2 * i], b[2 * i + 1], c[V / 2 + i], s[V / 2 + i]);
-        } else if (rotated) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) rotate(a[i], b[i], c[i], s[i]);
-        }
-    } else if (active) {
+    if (active) {
         const RowsView& in = is_q ? p.q : is_v ? p.v : p.k;
         const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * V;
         const uint4 wa = load16<IN>(in.p, at, p.vec), wb = load16<IN>(in.p, at + half, p.vec);
@@ -287,7 +170,7 @@ __global__ void __launch_bounds__(KW_THREADS, NORM || I4 ? 4 : IN == kF32 ? 8 : 
         store_values(p.q_out, at, p.q_out_dtype, a);
         store_values(p.q_out, at + half, p.q_out_dtype, b);
     }
-    if (!I4 && p.c.dtype != kInt8) {
+    if (p.c.dtype != kInt8) {
         if (is_q) return;
     } else if (__all_sync(0xFFFFFFFFu, is_q)) {  // (a warp that goes on shuffles as a whole)
         return;
@@ -296,7 +179,7 @@ __global__ void __launch_bounds__(KW_THREADS, NORM || I4 ? 4 : IN == kF32 ? 8 : 
     const uint32_t page = p.by_page.quotient((uint32_t)slot & 0x7FFFFFFFu);
     const int64_t row = ((int64_t)page * p.c.heads + h) * p.c.page_size + ((uint32_t)slot - page * p.c.page_size);
     void* const cache = is_v ? p.c.v : p.c.k;
-    if (!I4 && p.c.dtype != kInt8) {
+    if (p.c.dtype != kInt8) {
         if (wanted) {
             store_values(cache, row * p.c.d + lane * V, p.c.dtype, a);
             store_values(cache, row * p.c.d + lane * V + half, p.c.dtype, b);
@@ -308,10 +191,6 @@ __global__ void __launch_bounds__(KW_THREADS, NORM || I4 ? 4 : IN == kF32 ? 8 : 
     for (int i = 0; i < V; ++i) m = max_nan(m, max_nan(fabsf(a[i]), fabsf(b[i])));
 #pragma unroll
     for (int o = LANES / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
-    if (I4) {
-        store_int4<LANES, V>(p.c, row, half, lane, is_v, wanted, m, a, b);
-        return;
-    }
     if (!wanted) return;
     const bool finite = m < __int_as_float(0x7F800000), zero = m < MIN_AMAX;
     const float inv = finite && !zero ? __fdiv_rn(127.0f, m) : 0.0f;
@@ -330,30 +209,252 @@ __global__ void __launch_bounds__(KW_THREADS, NORM || I4 ? 4 : IN == kF32 ? 8 : 
         (is_v ? p.c.v_scale : p.c.k_scale)[row] = !finite ? __int_as_float(0x7FC00000) : zero ? 0.0f : __fdiv_rn(m, 127.0f);
 }
 
-template <int LANES, int IN, bool NORM, bool I4>
+template <int LANES, int IN>
 cudaError_t launch_write(const KvWriteParams& p, cudaStream_t stream) {
     const uint32_t heads = p.q_heads + 2 * p.c.heads;
     const uint32_t chunk = std::max(1u, 0x7FFFFFFFu / heads);  // rows of a launch stay below 2^31
     for (uint64_t t0 = 0; t0 < p.tokens; t0 += chunk) {
         const uint32_t rows = std::min<uint64_t>(chunk, p.tokens - t0) * heads, per = KW_THREADS / LANES;
-        kv_write_kernel<LANES, IN, NORM, I4><<<rows / per + (rows % per != 0), KW_THREADS, 0, stream>>>(p, (uint32_t)t0, rows);
+        kv_write_kernel<LANES, IN><<<rows / per + (rows % per != 0), KW_THREADS, 0, stream>>>(p, (uint32_t)t0, rows);
     }
     return cudaGetLastError();
 }
 
-template <int IN, bool NORM, bool I4>
-cudaError_t launch_write_rows(const KvWriteParams& p, cudaStream_t stream) {
-    constexpr int MOST = IN == kF32 ? 16 : 8;  // lanes of a row of 128 elements
-    if (p.c.d > 64) return launch_write<MOST, IN, NORM, I4>(p, stream);
-    if (p.c.d > 32) return launch_write<MOST / 2, IN, NORM, I4>(p, stream);
-    return launch_write<MOST / 4, IN, NORM, I4>(p, stream);
-}
-
 template <int IN>
 cudaError_t launch_write_of(const KvWriteParams& p, cudaStream_t stream) {
+    constexpr int MOST = IN == kF32 ? 16 : 8;  // lanes of a row of 128 elements
+    if (p.c.d > 64) return launch_write<MOST, IN>(p, stream);
+    if (p.c.d > 32) return launch_write<MOST / 2, IN>(p, stream);
+    return launch_write<MOST / 4, IN>(p, stream);
+}
+
+// ---- write with norms, and into 4-bit caches ----
+// As above, but a thread has eight elements of each half whatever the input's type (fewer threads share a row's sums, maxima and
+// addresses), a block has rows of one of q, k and v, and rows off the 16-byte boundaries are a kernel of their own (their
+// loads element by element are predicated away in one that has both, but issued all the same).
+constexpr int KN = 8;
+enum RowKind { ROW_Q, ROW_K, ROW_V };
+
+// Eight elements of a row in f32.
+template <int IN, bool VEC>
+__device__ __forceinline__ void load_eight(const void* base, int64_t i, float (&x)[KN]) {
+    if (IN == kF32) {
+        const uint4 a = load16<IN>(base, i, VEC), b = load16<IN>(base, i + 4, VEC);
+        float y[4], z[4];
+        widen<IN>(a, y), widen<IN>(b, z);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = y[j], x[4 + j] = z[j];
+    } else {
+        widen<IN>(load16<IN>(base, i, VEC), x);
+    }
+}
+
+// The value of e4m3 bits without a sign, and the bits nearest to two numbers >= 0.
+__device__ __forceinline__ float e4m3_value(uint32_t bits) { return __uint_as_float(bits << 20) * 1.32922800e36f; }  // 2^120
+__device__ __forceinline__ uint32_t e4m3_pair(float low, float high) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(high), "f"(low));
+    return r;
+}
+
+// Eight codes of a group as nibbles. `g` are the bits of the group's scale, `s` the row's. The product with 1 / (s g) is off by
+// three roundings, 2^-20 at most.
+// SHORT: x are 16-bit numbers. Their quotients by a step of four bits are ties or 2^-12 and more from one, so that rounding them to
+// multiples of 2^-15 first makes ties of ties. Otherwise the remainder x - code s g says where the code may be the neighbour's,
+// or a tie that goes to the even one: those threads go over their codes again. Where g is no normal number codes may pass 7.
+template <bool SHORT>
+__device__ __forceinline__ uint32_t codes_int4(const float (&x)[KN], uint32_t g, float s) {
+    const float step = s * e4m3_value(g);
+    float inv, c[KN];
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
+    if (g == 0) inv = 0.f;
+    auto whole = [](float q) { return __fadd_rn(__fadd_rn(q, 12582912.0f), -12582912.0f); };
+    if (SHORT) {
+#pragma unroll
+        for (int i = 0; i < KN; ++i) c[i] = whole(__fadd_rn(__fadd_rn(__fmul_rn(x[i], inv), 384.0f), -384.0f));
+    } else {
+        float worst = 0.f;
+#pragma unroll
+        for (int i = 0; i < KN; ++i) {
+            c[i] = whole(__fmul_rn(x[i], inv));
+            worst = fmaxf(worst, fabsf(__fmaf_rn(-c[i], step, x[i])));
+        }
+        if (g != 0 && worst >= 0.5f * step) {
+#pragma unroll
+            for (int i = 0; i < KN; ++i) {
+                const float rest = __fmaf_rn(-c[i], step, x[i]), over = fabsf(rest) - 0.5f * step;
+                if (over > 0.f || (over == 0.f && ((int)c[i] & 1))) c[i] += copysignf(1.f, rest);
+            }
+        }
+    }
+    if (g < 8) {
+#pragma unroll
+        for (int i = 0; i < KN; ++i) c[i] = fminf(fmaxf(c[i], -7.f), 7.f);
+    }
+    uint32_t byte[KN / 2];  // 8 + code in each half: 2^23 + 2^22 more leaves them in the lowest bits
+#pragma unroll
+    for (int i = 0; i < KN / 2; ++i) byte[i] = __float_as_uint(__fmaf_rn(c[2 * i + 1], 16.f, c[2 * i]) + (12582912.0f + 136.0f));
+    return prmt(prmt(byte[0], byte[1], 0x0040u), prmt(byte[2], byte[3], 0x0040u), 0x5410u);
+}
+
+template <int LANES, int IN, bool NORM, bool I4, bool VEC>
+__global__ void __launch_bounds__(KW_THREADS, 4) kv_write_rows_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t tokens) {
+    constexpr uint32_t PER = KW_THREADS / LANES;
+    const uint32_t lane = threadIdx.x % LANES, half = p.c.d / 2;
+    const int kind = blockIdx.x < p.blocks_q ? ROW_Q : blockIdx.x < p.blocks_q + p.blocks_kv ? ROW_K : ROW_V;
+    const uint32_t block = blockIdx.x - (kind == ROW_Q ? 0 : kind == ROW_K ? p.blocks_q : p.blocks_q + p.blocks_kv);
+    const uint32_t heads = kind == ROW_Q ? p.q_heads : p.c.heads, r = block * PER + threadIdx.x / LANES;
+    const uint32_t in_launch = kind == ROW_Q ? p.by_q.quotient(r) : p.by_kv.quotient(r), t = token0 + in_launch, h = r - in_launch * heads;
+    const bool active = in_launch < tokens && lane * (2 * KN) < p.c.d;
+    const RowsView& in = kind == ROW_Q ? p.q : kind == ROW_K ? p.k : p.v;
+    const bool rotated = p.cos != nullptr && kind != ROW_V;
+    const float* const weights = kind == ROW_Q ? p.q_norm : kind == ROW_K ? p.k_norm : nullptr;
+    float a[KN] = {}, b[KN] = {}, c[KN], s[KN];  // (rows that are not there add up to nothing)
+    int32_t slot = -1;
+    if (active) {
+        const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * KN;
+        load_eight<IN, VEC>(in.p, at, a), load_eight<IN, VEC>(in.p, at + half, b);
+        if (kind != ROW_Q) slot = __ldg(p.slots + t);
+        if (rotated) {
+            const int64_t row = (int64_t)min((uint32_t)max(__ldg(p.positions + t), 0), p.rope_len - 1) * half;
+            if (p.interleaved) {  // the pairs of a, then those of b
+                float c0[KN / 2], s0[KN / 2], c1[KN / 2], s1[KN / 2];
+                const int64_t i0 = row + lane * (KN / 2), i1 = i0 + half / 2;
+                load_angles(p.cos + i0, VEC, c0), load_angles(p.sin + i0, VEC, s0);
+                load_angles(p.cos + i1, VEC, c1), load_angles(p.sin + i1, VEC, s1);
+#pragma unroll
+                for (int i = 0; i < KN / 2; ++i) c[i] = c0[i], s[i] = s0[i], c[KN / 2 + i] = c1[i], s[KN / 2 + i] = s1[i];
+            } else {
+                load_angles(p.cos + row + lane * KN, VEC, c), load_angles(p.sin + row + lane * KN, VEC, s);
+            }
+        }
+    }
+    if (NORM && weights != nullptr) {
+        double sum = 0.0;
+#pragma unroll
+        for (int i = 0; i < KN; ++i) sum = fma((double)a[i], (double)a[i], sum), sum = fma((double)b[i], (double)b[i], sum);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o /= 2) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
+        if (active) {
+            const float root = (float)rsqrt(sum * p.inv_d + p.eps);
+            const float* const at = weights + h * (kind == ROW_Q ? p.q_norm_stride : p.k_norm_stride) + lane * KN;
+            float w[KN];
+            load_angles(at, VEC, w);
+#pragma unroll
+            for (int i = 0; i < KN; ++i) a[i] = __fmul_rn(__fmul_rn(a[i], root), w[i]);
+            load_angles(at + half, VEC, w);
+#pragma unroll
+            for (int i = 0; i < KN; ++i) b[i] = __fmul_rn(__fmul_rn(b[i], root), w[i]);
+        }
+    }
+    if (active && rotated) {
+        if (p.interleaved) {
+#pragma unroll
+            for (int i = 0; i < KN / 2; ++i) rotate(a[2 * i], a[2 * i + 1], c[i], s[i]), rotate(b[2 * i], b[2 * i + 1], c[KN / 2 + i], s[KN / 2 + i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < KN; ++i) rotate(a[i], b[i], c[i], s[i]);
+        }
+    }
+    if (kind == ROW_Q) {
+        if (active) {
+            const int64_t at = ((int64_t)t * p.q_heads + h) * p.c.d + lane * KN;
+            store_values(p.q_out, at, p.q_out_dtype, a);
+            store_values(p.q_out, at + half, p.q_out_dtype, b);
+        }
+        return;
+    }
+    const bool wanted = slot >= 0 && (uint64_t)slot < (uint64_t)p.c.pages * p.c.page_size;
+    const uint32_t page = p.by_page.quotient((uint32_t)slot & 0x7FFFFFFFu);
+    const int64_t row = ((int64_t)page * p.c.heads + h) * p.c.page_size + ((uint32_t)slot - page * p.c.page_size);
+    void* const cache = kind == ROW_V ? p.c.v : p.c.k;
+    float* const scales = kind == ROW_V ? p.c.v_scale : p.c.k_scale;
+    const uint32_t at_a = lane * KN, at_b = half + lane * KN;
+    if (!I4 && p.c.dtype != kInt8) {
+        if (wanted) {
+            store_values(cache, row * p.c.d + at_a, p.c.dtype, a);
+            store_values(cache, row * p.c.d + at_b, p.c.dtype, b);
+        }
+        return;
+    }
+    float ma = 0.f, mb = 0.f;
+#pragma unroll
+    for (int i = 0; i < KN; ++i) ma = max_nan(ma, fabsf(a[i])), mb = max_nan(mb, fabsf(b[i]));
+    float m = max_nan(ma, mb);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o /= 2) m = max_nan(m, __shfl_xor_sync(0xFFFFFFFFu, m, o));
+    const bool finite = m < __int_as_float(0x7F800000), some = finite && m >= MIN_AMAX;
+    if (!I4) {
+        if (!wanted) return;
+        const float inv = some ? __fdiv_rn(127.0f, m) : 0.0f;
+        int8_t* const dst = static_cast<int8_t*>(cache) + row * p.c.d;
+        *reinterpret_cast<uint2*>(dst + at_a) = finite ? make_uint2(codes4(a, inv), codes4(a + 4, inv)) : make_uint2(0u, 0u);
+        *reinterpret_cast<uint2*>(dst + at_b) = finite ? make_uint2(codes4(b, inv), codes4(b + 4, inv)) : make_uint2(0u, 0u);
+        if (lane == 0) scales[row] = !finite ? __int_as_float(0x7FC00000) : some ? __fdiv_rn(m, 127.0f) : 0.0f;
+        return;
+    }
+    // the groups' maxima: of four threads side by side, or, where the halves do not begin on a group, of pieces of eight in
+    // shared memory
+    if (half % I4_GROUP == 0) {
+#pragma unroll
+        for (int o = 1; o < (int)I4_GROUP / KN; o *= 2) {
+            ma = max_nan(ma, __shfl_xor_sync(0xFFFFFFFFu, ma, o));
+            mb = max_nan(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, o));
+        }
+    } else {
+        __shared__ float4 held[PER][LANES / 2];
+        float* const piece = reinterpret_cast<float*>(held[threadIdx.x / LANES]);
+        if (at_a < half) piece[at_a / KN] = ma, piece[at_b / KN] = mb;
+        __syncwarp();
+        if (at_a < half) {
+            const float4 x = held[threadIdx.x / LANES][at_a / I4_GROUP], y = held[threadIdx.x / LANES][at_b / I4_GROUP];
+            ma = max_nan(max_nan(x.x, x.y), max_nan(x.z, x.w)), mb = max_nan(max_nan(y.x, y.y), max_nan(y.z, y.w));
+        }
+    }
+    if (!wanted) return;
+    // s and 1 / s: the exponent of m, less 11, and one more where m's fraction passes 3136 / 2048
+    const uint32_t bits = __float_as_uint(m), e = some ? (bits >> 23) - 11 + ((bits & 0x7FFFFFu) > 0x440000u) : 127u;
+    const float scale = some ? __uint_as_float(e << 23) : 0.f, up = __uint_as_float((254u - e) << 23);
+    const uint32_t g = some ? e4m3_pair(__fdiv_rn(ma, 7.f) * up, __fdiv_rn(mb, 7.f) * up) : 0u;
+    uint8_t* const dst = static_cast<uint8_t*>(cache) + row * half;
+    uint32_t wa = 0x88888888u, wb = wa;
+    if (some) {
+        if (IN != kF32 && kind == ROW_V) wa = codes_int4<true>(a, g & 0xFFu, scale), wb = codes_int4<true>(b, g >> 8, scale);
+        else wa = codes_int4<false>(a, g & 0xFFu, scale), wb = codes_int4<false>(b, g >> 8, scale);
+    }
+    *reinterpret_cast<uint32_t*>(dst + at_a / 2) = wa;
+    *reinterpret_cast<uint32_t*>(dst + at_b / 2) = wb;
+    uint8_t* const groups = (kind == ROW_V ? p.c.v_group : p.c.k_group) + row * 4;
+    if (at_a % I4_GROUP == 0) groups[at_a / I4_GROUP] = (uint8_t)g;
+    if (at_b % I4_GROUP == 0) groups[at_b / I4_GROUP] = (uint8_t)(g >> 8);
+    if (lane == 0) scales[row] = finite ? scale : __int_as_float(0x7FC00000);
+}
+
+template <int LANES, int IN, bool NORM, bool I4, bool VEC>
+cudaError_t launch_write_rows(KvWriteParams p, cudaStream_t stream) {
+    constexpr uint32_t PER = KW_THREADS / LANES;
+    const uint32_t chunk = std::max(1u, 0x7FFFFFFFu / (p.q_heads + 2 * p.c.heads) / 2);  // rows of a launch, and of blocks that part full, stay below 2^31
+    auto blocks = [&](uint32_t tokens, uint32_t heads) { return (uint32_t)(((uint64_t)tokens * heads + PER - 1) / PER); };
+    for (uint64_t t0 = 0; t0 < p.tokens; t0 += chunk) {
+        const uint32_t tokens = (uint32_t)std::min<uint64_t>(chunk, p.tokens - t0);
+        p.blocks_q = blocks(tokens, p.q_heads), p.blocks_kv = blocks(tokens, p.c.heads);
+        kv_write_rows_kernel<LANES, IN, NORM, I4, VEC><<<p.blocks_q + 2 * p.blocks_kv, KW_THREADS, 0, stream>>>(p, (uint32_t)t0, tokens);
+    }
+    return cudaGetLastError();
+}
+
+template <int IN, bool NORM, bool I4, bool VEC>
+cudaError_t launch_write_rows_of(const KvWriteParams& p, cudaStream_t stream) {
+    if (p.c.d > 64) return launch_write_rows<8, IN, NORM, I4, VEC>(p, stream);
+    if (p.c.d > 32) return launch_write_rows<4, IN, NORM, I4, VEC>(p, stream);
+    return launch_write_rows<2, IN, NORM, I4, VEC>(p, stream);
+}
+
+template <int IN, bool VEC>
+cudaError_t launch_write_rows_by(const KvWriteParams& p, cudaStream_t stream) {
     const bool norm = p.q_norm != nullptr || p.k_norm != nullptr;
-    if (p.c.dtype == kInt4) return norm ? launch_write_rows<IN, true, true>(p, stream) : launch_write_rows<IN, false, true>(p, stream);
-    return norm ? launch_write_rows<IN, true, false>(p, stream) : launch_write_rows<IN, false, false>(p, stream);
+    if (p.c.dtype != kInt4) return launch_write_rows_of<IN, true, false, VEC>(p, stream);
+    return norm ? launch_write_rows_of<IN, true, true, VEC>(p, stream) : launch_write_rows_of<IN, false, true, VEC>(p, stream);
 }
 
 // ---- read ----
@@ -388,10 +489,25 @@ __device__ __forceinline__ void write8(void* out, int64_t at, int out_dtype, con
         return;
     }
     float x[8];
-    if (I4) {  // code times group's scale is exact, so that a value is rounded once whatever the row's scale is
-        const float g = e4m3_value(e.w.y), s = __uint_as_float(e.w.z);
+    if (I4) {  // (code + 8) as the f16 number of its bits, times the group's scale, exactly: code g 2^-15; then one rounding in f32
+        const uint32_t moved = e.w.y << 7, two = moved | moved << 16, even = e.w.x << 2, odd = e.w.x >> 6;
+        const __half2 g = *reinterpret_cast<const __half2*>(&two);  // g 2^-8
+        const __half2 lo = __hmul2(g, __float2half2_rn(32768.f)), hi = __hmul2(g, __float2half2_rn(2048.f)), off = __hmul2(g, __float2half2_rn(-0.0625f));
+        const uint32_t u[4] = {even & 0x003C003Cu, even & 0x03C003C0u, odd & 0x003C003Cu, odd & 0x03C003C0u};  // elements i and i + 4
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn((float)((int)((e.w.x >> (4 * i)) & 15u) - 8), g), s);
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(__hfma2(*reinterpret_cast<const __half2*>(&u[i]), i % 2 ? hi : lo, off));
+            x[i] = f.x, x[4 + i] = f.y;
+        }
+        float s = __uint_as_float(e.w.z);
+        if (s < 5.19e33f) {  // 2^112
+            s *= 32768.f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= 32768.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], s);
     } else if (dtype == kInt8) {
         const float s = __uint_as_float(e.w.z);
 #pragma unroll
@@ -441,7 +557,7 @@ __global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const __grid_consta
         Eight k[KR_BATCH], v[KR_BATCH];
 #pragma unroll
         for (int i = 0; i < KR_BATCH; ++i) {
-            const uint32_t r = r0 + i * GROUPS, t = r / p.c.heads;
+            const uint32_t r = r0 + i * GROUPS, t = I4 ? p.by_heads.quotient(r) : r / p.c.heads;
             k[i].w = v[i].w = make_uint4(I4 ? 0x88888888u : 0u, 0, 0, 0);
             if (r < rows && first[t] >= 0) {
                 const int64_t row = first[t] + (int64_t)(r - t * p.c.heads) * p.c.page_size;
@@ -474,6 +590,12 @@ cudaError_t launch_read(const KvReadParams& p, cudaStream_t stream) {
 cudaError_t launch_kv_write(const KvWriteParams& params, cudaStream_t stream) {
     KvWriteParams p = params;
     p.by_heads = Divisor::of(p.q_heads + 2 * p.c.heads), p.by_page = Divisor::of(p.c.page_size);
+    if (p.c.dtype == kInt4 || p.q_norm != nullptr || p.k_norm != nullptr) {
+        p.by_q = Divisor::of(std::max(p.q_heads, 1u)), p.by_kv = Divisor::of(p.c.heads);
+        if (p.dtype == kF32) return p.vec ? launch_write_rows_by<kF32, true>(p, stream) : launch_write_rows_by<kF32, false>(p, stream);
+        if (p.dtype == kF16) return p.vec ? launch_write_rows_by<kF16, true>(p, stream) : launch_write_rows_by<kF16, false>(p, stream);
+        return p.vec ? launch_write_rows_by<kBf16, true>(p, stream) : launch_write_rows_by<kBf16, false>(p, stream);
+    }
     if (p.dtype == kF32) return launch_write_of<kF32>(p, stream);
     return p.dtype == kF16 ? launch_write_of<kF16>(p, stream) : launch_write_of<kBf16>(p, stream);
 }
@@ -485,7 +607,9 @@ static cudaError_t launch_read_rows(const KvReadParams& p, cudaStream_t stream) 
     return launch_read<4, I4>(p, stream);
 }
 
-cudaError_t launch_kv_read(const KvReadParams& p, cudaStream_t stream) {
+cudaError_t launch_kv_read(const KvReadParams& params, cudaStream_t stream) {
+    KvReadParams p = params;
+    p.by_heads = Divisor::of(p.c.heads);
     return p.c.dtype == kInt4 ? launch_read_rows<true>(p, stream) : launch_read_rows<false>(p, stream);
 }
 
