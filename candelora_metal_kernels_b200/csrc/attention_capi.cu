@@ -180,7 +180,7 @@ int iq2_kv_pages_step(const iq2_kv_pages* pages, const iq2_kv_step* step, iq2_st
         return capi_fail(IQ2_ERR_UNSUPPORTED, "%s: %u sequences are more than %u", op, g.sequences, iq2::PAGES_MOST_SEQS);
     if ((uint64_t)g.num_pages * g.page_size > (uint64_t)INT32_MAX)
         return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u pages of %u tokens are too large", op, g.num_pages, g.page_size);
-    if (t.total > (uint32_t)INT32_MAX) return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u tokens are too many", op, t.total);
+    if (t.total >= (uint32_t)INT32_MAX) return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u tokens are too many", op, t.total);
     int rc = check_pointers(op, {{"block_table", g.block_table, 4}, {"seq_lens", g.seq_lens, 4}, {"free_pages", g.free_pages, 4},
                                  {"free_count", g.free_count, 4}, {"new_lens", t.new_lens, 4}, {"cu_seqlens_q", t.cu_seqlens_q, 4},
                                  {"cu_seqlens_k", t.cu_seqlens_k, 4}, {"granted", t.granted, 4}});

@@ -298,7 +298,7 @@ __device__ __forceinline__ uint32_t codes_int4(const float (&x)[KN], uint32_t g,
 }
 
 template <int LANES, int IN, bool NORM, bool I4, bool VEC>
-__global__ void __launch_bounds__(KW_THREADS, 4) kv_write_rows_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t tokens) {
+__global__ void __launch_bounds__(KW_THREADS, NORM ? 4 : 5) kv_write_rows_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t tokens) {
     constexpr uint32_t PER = KW_THREADS / LANES;
     const uint32_t lane = threadIdx.x % LANES, half = p.c.d / 2;
     const int kind = blockIdx.x < p.blocks_q ? ROW_Q : blockIdx.x < p.blocks_q + p.blocks_kv ? ROW_K : ROW_V;

@@ -59,10 +59,11 @@ def test_steps_of_prompts_tokens_and_cuts(sequences, most, page):
     walk(pages, state, page, steps, reuse=page == 16)
 
 
-def test_large_steps_take_a_cluster_of_blocks():
+@pytest.mark.parametrize("page", [16, 5])
+def test_large_steps_take_a_cluster_of_blocks(page):
     """More sequences than a block's threads and more tokens than one block takes, again and again over the same pages."""
-    rng, page, n = random.Random(5), 16, 2500
-    pages, state = empty(9000, page, n, 12)
+    rng, n = random.Random(5), 2500
+    pages, state = empty(9000 if page == 16 else 20000, page, n, 12 if page == 16 else 30)
     steps = []
     for i in range(4):
         new = [rng.choice([0, 1, 3, 20, 60]) for _ in range(n)]
