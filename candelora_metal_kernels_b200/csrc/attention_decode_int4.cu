@@ -168,13 +168,31 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     if (!FULL)
         for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
     if (lane < 2) pieces[warp * 2 + lane].valid = 0;
-    typename Cursor::Parts line;
-    const uint32_t part0 = blockIdx.x * A4_WARPS;  // the block's parts of the line, one a warp
-    Cursor cur = Cursor::of_part(a, part0 + warp, gridDim.x * A4_WARPS, a.inv_blocks * (1.0 / A4_WARPS), lane, 32, line);
-    if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, part0, A4_WARPS);
-    const uint64_t first_unit = cur.unit, block_u0 = line.begin(part0);
-    if (cur.t0 == cur.t1) cur.unit = cur.end;  // nothing, or nothing but an item's start
-    Cursor pre = cur;
+    // where each warp reads and where it copies from, and the block's first unit: in shared memory, since registers are short
+    // and they change from one piece to the next only
+    __shared__ Cursor cursors[A4_WARPS][2];
+    __shared__ uint64_t block_u0;
+    Cursor& cur_held = cursors[warp][0];
+    Cursor& pre_held = cursors[warp][1];
+    bool live;  // there is a tile to copy
+    uint32_t pre_tok, pre_t1;
+    {
+        typename Cursor::Parts line;
+        const uint32_t part0 = blockIdx.x * A4_WARPS;  // the block's parts of the line, one a warp
+        Cursor cur = Cursor::of_part(a, part0 + warp, gridDim.x * A4_WARPS, a.inv_blocks * (1.0 / A4_WARPS), lane, 32, line);
+        if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, part0, A4_WARPS), block_u0 = line.begin(part0);
+        if (cur.t0 == cur.t1) cur.unit = cur.end;  // nothing, or nothing but an item's start
+        if (lane == 0) cur_held = cur, pre_held = cur;
+        live = !cur.done(), pre_tok = cur.t0, pre_t1 = cur.t1;
+    }
+    auto advance = [&](Cursor& held) {
+        Cursor c = held;
+        c.next(p, items);
+        __syncwarp();
+        if (lane == 0) held = c;
+        __syncwarp();
+        return !c.done();
+    };
 
     // ---- the copies: pre's tile from token pre_tok on, whose pages have been looked up ----
     const uint32_t ring = smem_u32(smem + warp * S::RING);
@@ -190,21 +208,24 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     // 32 words of each kind of scale, 16 bytes a lane: row scales of K and V, then group scales
     const uint8_t* const scales_from = (lane < 8 ? reinterpret_cast<const uint8_t*>(p.c.k_scale) : lane < 16 ? reinterpret_cast<const uint8_t*>(p.c.v_scale)
                                         : lane < 24 ? p.c.k_group : p.c.v_group);
-    uint32_t pre_tok = cur.t0, pre_in = 0, pre_head = 0;  // the tile to copy next, its place in its page (whole tiles), rows of the heads before
+    uint32_t pre_in = 0, pre_head = 0;  // the tile's place in its page (whole tiles), rows of the heads before
+    const int32_t* table = nullptr;     // the sequence's pages
     uint32_t page = 0, ahead = 0;                         // this lane's page of those looked up; tiles since
-    bool live = !pre.done(), fresh = true;
+    bool fresh = true;
     auto look_up = [&](uint32_t tok) {
-        return tok < pre.t1 ? (uint32_t)__ldg(p.block_table + (int64_t)pre.b * p.table_width + a.by_page.quotient(tok)) : 0xFFFFFFFFu;
+        return tok < pre_t1 ? (uint32_t)__ldg(table + a.by_page.quotient(tok)) : 0xFFFFFFFFu;
     };
     auto in_page = [&](uint32_t tok) { return tok - a.by_page.quotient(tok) * p.c.page_size; };
     auto find_tile = [&]() {  // the next tile of this warp, and its page numbers under way
-        if (pre_tok >= pre.t1) {
-            pre.next(p, items);
-            live = !pre.done();
-            pre_tok = pre.t0, fresh = true;
+        if (pre_tok >= pre_t1) {
+            live = advance(pre_held);
+            pre_tok = pre_held.t0, pre_t1 = pre_held.t1, fresh = true;
         }
         if (!live) return;
-        if (fresh) pre_head = pre.item / a.chunks_of_heads * p.c.page_size;
+        if (fresh) {
+            pre_head = pre_held.item / a.chunks_of_heads * p.c.page_size;
+            table = p.block_table + (int64_t)pre_held.b * p.table_width;
+        }
         if (whole_tiles) {  // lanes hold the pages of this warp's next 32 tiles
             if (fresh || ahead == 32) page = look_up(pre_tok + lane * TOK), pre_in = in_page(pre_tok), ahead = 0;
         } else {            // of the tile's runs, or of its tokens
@@ -215,7 +236,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     // Copies the tile and returns a bit for each token that takes part: rows of tokens past the end, or of pages outside
     // the cache, are zeros, and what such pages hold cannot matter.
     auto copy_tile = [&](uint32_t dst) {
-        const uint32_t left = pre.t1 - pre_tok;
+        const uint32_t left = pre_t1 - pre_tok;
         int64_t mine;  // the row of token `lane`, -1: none
         if (whole_tiles) {
             const uint32_t at = __shfl_sync(0xFFFFFFFFu, page, ahead++);
@@ -282,6 +303,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
         }
         cp_async_commit();
     };
+    const bool live_at_start = live;
     if (live) find_tile();
     copy_and_find(ring);
     uint32_t at = ring;  // the stage to take next
@@ -295,15 +317,22 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     const uint32_t k_sel = k_group * I4_GROUP < d ? 0x0404u | k_group * 0x1010u : 0x4444u;  // (zeros past head_dim)
     const uint32_t v_sel = 0x4C08u + v_group * 0x1111u;  // (8 + i is the sign of byte i in all bits: none)
 
-    while (!cur.done()) {
+    bool first_piece = true;
+    for (bool more = live_at_start; more; more = advance(cur_held)) {
         // ---- q of the item: the pieces of head g, elements t DP / 4 and on ----
-        const uint32_t kv_head = cur.item / a.chunks_of_heads, head0 = kv_head * group + (cur.item % a.chunks_of_heads) * AD_HEADS;
-        const uint32_t heads = min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
+        // (of the item: its first head, and how many it has)
+        auto heads_of = [&](uint32_t item, uint32_t& head0) {
+            const uint32_t kv_head = item / a.chunks_of_heads;
+            head0 = kv_head * group + (item % a.chunks_of_heads) * AD_HEADS;
+            return min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
+        };
         uint32_t q_high[KS][2], q_low[KS][2];
         float factor[2];  // scale log2(e) 2^e of the heads 2t, 2t + 1
         {
             float x[DP / 4], top = 0.f, unit = A4_VALUE, down = 1.f;  // 2^e and 2^(15 - e)
-            load_row<DP / 4>(p.q.p, (int64_t)cur.b * p.q.token_stride + (int64_t)(head0 + g) * p.q.head_stride + t * (DP / 4), p.dtype,
+            uint32_t head0;
+            const uint32_t heads = heads_of(cur_held.item, head0);
+            load_row<DP / 4>(p.q.p, (int64_t)cur_held.b * p.q.token_stride + (int64_t)(head0 + g) * p.q.head_stride + t * (DP / 4), p.dtype,
                              g < heads && t * (DP / 4) < d, a.q_vec, x);
 #pragma unroll
             for (int i = 0; i < DP / 4; ++i) top = fmaxf(top, fabsf(x[i]));
@@ -330,7 +359,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
         for (int n = 0; n < MT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
 #pragma unroll 1
-        for (uint32_t tok = cur.t0; tok < cur.t1; tok += TOK) {
+        for (uint32_t left = cur_held.t1 - cur_held.t0; left != 0; left -= min(left, (uint32_t)TOK)) {
             cp_async_wait<0>();
             __syncwarp();
             const uint32_t here = there;
@@ -479,6 +508,9 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
 
         // ---- the end of the piece: a whole item's output, or (o, m, l) for the block to add up ----
         constexpr float UNIT_OF_O = A4_SUM * (A4_VALUE / A4_UP);
+        const Cursor cur = cur_held;
+        uint32_t head0;
+        const uint32_t heads = heads_of(cur.item, head0);
         if (cur.whole()) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -492,10 +524,9 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 }
             }
         } else {
-            const bool first = cur.unit == first_unit;
             // (the last piece takes the ring: all of the warp's copies are done then)
-            float* const slot = slot_of<S>(smem, warp * 2 + !first);
-            if (!first) {
+            float* const slot = slot_of<S>(smem, warp * 2 + !first_piece);
+            if (!first_piece) {
                 cp_async_wait<0>();
                 __syncwarp();
             }
@@ -508,9 +539,9 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 if (g == 0) slot[S::MAXIMA + 2 * t + h] = m[h], slot[S::SUMS + 2 * t + h] = l[h];
             }
             if (lane == 0)
-                pieces[warp * 2 + !first] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.unit - cur.k <= block_u0 ? 8u : 0u)};
+                pieces[warp * 2 + !first_piece] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.unit - cur.k <= block_u0 ? 8u : 0u)};
         }
-        cur.next(p, items);
+        first_piece = false;
     }
     cp_async_wait<0>();
     __syncthreads();
