@@ -13,7 +13,7 @@
 //     ones of a key row, one group: one wide load and one scale a key. For O a thread's rows are DP / 8 consecutive dimensions, again
 //     one group, of the two tokens whose p it holds; tokens are relabelled so that both kinds of loads are free of bank conflicts.
 //   * q of 32 bits and its p are sums of two f16 pieces in one accumulator: q is held times the power of two that brings a head's
-//     largest |q| to 2^14, so that its 22 bits end at 2^-39 of it; p times its value's row scale is 2^7 at the reference, up to
+//     largest |q| to 2^12, so that its 22 bits end at 2^-36 of it; p times its value's row scale is 2^7 at the reference, up to
 //     2^15, and its 22 bits end at 2^-31 of the largest. q of 16 bits is one piece exactly, and its p is rounded to f16 once.
 //   * The row scales of keys multiply s, those of values multiply p.
 // The maxima, sums, s, p and o are f32.
@@ -327,9 +327,9 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
             return min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
         };
         uint32_t q_high[KS][2], q_low[KS][2];
-        float factor[2];  // scale log2(e) 2^e of the heads 2t, 2t + 1
+        float factor[2];  // scale log2(e) 2^(e + 2) of the heads 2t, 2t + 1
         {
-            float x[DP / 4], top = 0.f, unit = A4_VALUE, down = 1.f;  // 2^e and 2^(15 - e)
+            float x[DP / 4], top = 0.f, unit = A4_VALUE / 4.f, down = 1.f;  // 2^e and 2^(13 - e)
             uint32_t head0;
             const uint32_t heads = heads_of(cur_held.item, head0);
             load_row<DP / 4>(p.q.p, (int64_t)cur_held.b * p.q.token_stride + (int64_t)(head0 + g) * p.q.head_stride + t * (DP / 4), p.dtype,
@@ -339,8 +339,8 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -110), 126);
-            if (top > 0.f && top < INFINITY) unit = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(142 - e) << 23);
-            const float f = fmaxf(p.scale * LOG2E * unit, 1.17549435e-38f);  // (not 0: times -infinity it stays that)
+            if (top > 0.f && top < INFINITY) unit = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(140 - e) << 23);
+            const float f = fminf(p.scale * (4.f * LOG2E) * unit, 3e38f);  // (finite: a key row of zeros has a score of 0)
             factor[0] = __shfl_sync(0xFFFFFFFFu, f, t * 8), factor[1] = __shfl_sync(0xFFFFFFFFu, f, t * 8 + 4);
             // elements j and j + 4 of a word's eight are a pair: j = 0, 1 of one step, j = 2, 3 of the next
 #pragma unroll
@@ -398,14 +398,15 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 x[mt * 2][0] = s[0], x[mt * 2][1] = s[1], x[mt * 2 + 1][0] = s[2], x[mt * 2 + 1][1] = s[3];
             }
 
-            // factor x = log2(e) scale q . k; w = 2^(factor x - m) times the value scale
+            // x = log2(e) scale q . k, rounded before the reference is taken off (which is one of them); w = 2^(x - m) times the value
+            // scale
             float e[NT][2], w[NT][2], vs[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint32_t from = at + S::SCALES + (n * 8 + k_row) * 4;
                 const float ks = __uint_as_float(ld_shared(from));
                 vs[n] = max_nan(__uint_as_float(ld_shared(from + TOK * 4)) * A4_UP, A4_MIN_SCALE);
-                x[n][0] *= ks, x[n][1] *= ks;
+                x[n][0] *= ks * factor[0], x[n][1] *= ks * factor[1];
             }
             if (here != 0xFFFFFFFFu) {
 #pragma unroll
@@ -422,7 +423,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                         const float base = m[h] == -INFINITY ? 0.f : m[h] - A4_TOP;
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            e[n][h] = exp2_approx(fmaf(x[n][h], factor[h], -base));
+                            e[n][h] = exp2_approx(x[n][h] - base);
                             w[n][h] = e[n][h] * vs[n];
                             top = fmaxf(top, w[n][h]);
                         }
@@ -436,7 +437,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 for (int h = 0; h < 2; ++h) {
                     float most = -INFINITY;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) most = fmaxf(most, fmaf(x[n][h], factor[h], __log2f(vs[n])));
+                    for (int n = 0; n < NT; ++n) most = fmaxf(most, x[n][h] + __log2f(vs[n]));
 #pragma unroll
                     for (int b = 4; b < 32; b *= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, b));
                     const float next = fmaxf(m[h], most);

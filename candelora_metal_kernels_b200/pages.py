@@ -105,8 +105,8 @@ def kv_pages_step(pages: KvPages, new_lens: torch.Tensor, total_tokens: int, *, 
     if new.shape[0] != n or (keep is not None and keep.shape[0] != n):
         _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: block_table has {n} sequences, new_lens {new.shape[0]}"
                                              f"{'' if keep is None else f', keep {keep.shape[0]}'}")
-    if total_tokens < 0:
-        _bail(_lib.IQ2_ERR_INVALID_ARGUMENT, f"{op}: total_tokens={total_tokens} is negative")
+    if not 0 <= total_tokens < 2 ** 31 - 1:
+        _bail(_lib.IQ2_ERR_OVERFLOW, f"{op}: total_tokens={total_tokens} is negative or too large")
     if out is None:
         out = KvStep.empty(pages, total_tokens)
     elif out._total != total_tokens or out._sequences != n or out._index != index:

@@ -267,6 +267,26 @@ def test_decode_a_row_that_is_no_number_and_one_token_of_all_the_weight():
     assert torch.isfinite(c.attention_decode(q, cache, table.cuda(), torch.tensor([30], dtype=torch.int32).cuda())).all()
 
 
+@pytest.mark.parametrize("q_top,k_top", [(1e-37, 3e38), (3e38, 1e-29), (1e38, 1.0), (1e-30, 1e30), (1e30, 1e-30), (1.0, 0.0), (0.0, 1.0)])
+def test_decode_queries_and_keys_at_the_ends_of_f32(q_top, k_top):
+    """Scores of a few units from factors of any size; where they pass them by far, the largest takes all."""
+    d, n = 64, 40
+    k, v = randn((n, 1, d), 1), randn((n, 1, d), 2)
+    k, q = k / k.abs().max() * k_top, randn((1, 2, d), 3)
+    q = q / q.abs().max() * q_top
+    cache = c.KvCache.empty(2, 1, 32, d, I4)
+    c.kv_cache_write(cache, k.cuda(), v.cuda(), torch.arange(n, dtype=torch.int32).cuda())
+    table = torch.tensor([[0, 1]], dtype=torch.int32)
+    got = c.attention_decode(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda()).double().cpu()
+    want, size = step_ref.decode4(q, cache, table, [n])
+    # scores up to 30: relative errors of p of 30 times those of the docstring above
+    near = ((got - want).abs() <= 2.0 ** -14 * 30 / 13 * size + n * 2.0 ** -31 * 8).all(-1)[0]
+    # (scores are f32 numbers times log2(e): a head in which one of them passes 2^128 has no softmax in f32)
+    held = step_ref.held4(cache)[0][table[0].long()].transpose(1, 2).reshape(-1, d)[:n]
+    past = (q[0].double() @ held.T * d ** -0.5 * 1.4427).abs().amax(-1) >= 2.0 ** 128
+    assert (near | (past & got[0].isnan().all(-1))).all() and (q_top == 1e38 or not past.any())
+
+
 def test_decode_strides_scale_stream_workspace_and_repeat():
     lens, d = [300, 0, 1000], 128
     cache, table = make_cache(lens, 2, 48, d, 11)

@@ -167,7 +167,8 @@ def test_refusals():
     refused("new_lens 2", c.kv_pages_step, pages, new[:2], 3)
     refused("keep 2", c.kv_pages_step, pages, new, 3, keep=new[:2])
     refused("device mismatch", c.kv_pages_step, pages, new.cpu(), 3)
-    refused("negative", c.kv_pages_step, pages, new, -1)
+    refused("negative or too large", c.kv_pages_step, pages, new, -1)
+    refused("negative or too large", c.kv_pages_step, pages, new, 2 ** 31 - 1)
     refused("out has 4 rows", c.kv_pages_step, pages, new, 3, out=c.KvStep.empty(pages, 4))
     refused("non-zero dimensions", c.kv_pages_step, c.KvPages(t[:0], lens[:0], free, count, 4), new[:0], 3)
     refused("non-zero dimensions", c.KvPages, t, lens, free, count, 0)
