@@ -2,9 +2,10 @@
 
     python examples/attention_block.py                 (Llama-3-8B shapes: 4096 hidden, 32 / 8 heads of 128)
 
-Prompt:  q, k, v projections (one grouped call) -> rotation and cache write -> attention over the prompt -> o projection.
+Prompt:  pages for its tokens -> q, k, v projections (one grouped call) -> norms of the heads (where the layer has them), rotation
+and cache write -> attention over the prompt -> o projection.
 Token:   the same with the attention over the cache. A prompt may also come in chunks: the earlier tokens are read back
-from the cache and the chunk attends to them and itself.
+from the cache and the chunk attends to them and itself. The cache is 16-bit, int8, or 4-bit (torch.uint8).
 """
 from __future__ import annotations
 
@@ -28,10 +29,11 @@ class Shape:
     kv_heads: int = 8
     head_dim: int = 128
     theta: float = 500000.0
+    head_norms: bool = False
 
 
 class AttentionBlock:
-    """One layer's projections, its paged cache and a block table for `sequences` sequences of up to `most` tokens."""
+    """One layer's projections, its paged cache and the pages of `sequences` sequences of up to `most` tokens."""
 
     def __init__(self, shape: Shape, sequences: int, most: int, cache_dtype=torch.int8, page_size: int = 64, seed: int = 0):
         self.shape, self.page_size = shape, page_size
@@ -41,44 +43,39 @@ class AttentionBlock:
         self.weights["o"] = (*(t.cuda() for t in synth.iq2xxs_weights(shape.hidden, rows["q"], seed=seed + 9)), shape.hidden, rows["q"])
         pages = -(-most // page_size)
         self.cache = c.KvCache.empty(sequences * pages, shape.kv_heads, page_size, shape.head_dim, cache_dtype)
-        self.table = torch.arange(sequences * pages, dtype=torch.int32, device="cuda").flip(0).view(sequences, pages).contiguous()
+        self.pages = c.KvPages.empty(sequences * pages, page_size, sequences, pages)
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        weights = [1 + 0.2 * torch.randn(shape.head_dim, generator=gen, device="cuda") for _ in range(2)] if shape.head_norms else [None] * 2
+        self.q_norm, self.k_norm = weights
         half = shape.head_dim // 2
         angle = torch.arange(most, device="cuda", dtype=torch.float64)[:, None] * \
             shape.theta ** (-torch.arange(half, device="cuda", dtype=torch.float64) / half)
         self.cos, self.sin = angle.cos().float().contiguous(), angle.sin().float().contiguous()
 
-    def _project(self, x, q_dtype, sequence, position):
-        """Rotated q [tokens, heads, head_dim] in q_dtype; k and v of x [tokens, hidden] go to the cache. `sequence` and
-        `position` [tokens] say where each token belongs."""
+    def _project(self, x, q_dtype, step):
+        """Rotated q [tokens, heads, head_dim] in q_dtype; k and v of x [tokens, hidden] go to the cache, where `step` says."""
         s = self.shape
         q, k, v = c.iq2_matmul_grouped([(x, *self.weights[name]) for name in "qkv"])
-        slots = self.table[sequence, position // self.page_size] * self.page_size + position % self.page_size
         k, v = (t.view(-1, s.kv_heads, s.head_dim) for t in (k, v))
-        q = c.kv_cache_write(self.cache, k, v, slots.to(torch.int32), q=q.view(-1, s.heads, s.head_dim), q_dtype=q_dtype,
-                             positions=position.to(torch.int32), cos=self.cos, sin=self.sin)
-        return q, k, v
+        return c.kv_cache_write(self.cache, k, v, step.slots, q=q.view(-1, s.heads, s.head_dim), q_dtype=q_dtype,
+                                positions=step.positions, cos=self.cos, sin=self.sin, q_norm=self.q_norm, k_norm=self.k_norm)
 
     def _output(self, attended):
         return c.iq2_xxs_matmul(attended.flatten(1), *self.weights["o"])
 
-    def prompt(self, x, lengths, done=0):
-        """x [tokens, hidden] (bf16) of packed prompts, or of their next chunks after `done` tokens each; f32 out."""
-        dev = x.device
-        seqs = len(lengths)
-        cu = torch.tensor([0] + list(lengths), device=dev).cumsum(0).to(torch.int32)
-        sequence = torch.repeat_interleave(torch.arange(seqs, device=dev), torch.tensor(lengths, device=dev))
-        position = torch.arange(x.shape[0], device=dev) - cu[sequence].long() + done
-        q, _, _ = self._project(x, torch.bfloat16, sequence, position)
+    def prompt(self, x, lengths):
+        """x [tokens, hidden] (bf16) of packed prompts, or of their next chunks; f32 out."""
+        step = c.kv_pages_step(self.pages, torch.tensor(lengths, dtype=torch.int32, device=x.device), x.shape[0])
+        q = self._project(x, torch.bfloat16, step)
         # the keys and values as the cache holds them, so that prompts, chunks and single tokens see the same ones
-        cu_k = torch.tensor([0] + [n + done for n in lengths], device=dev).cumsum(0).to(torch.int32)
-        k, v = c.kv_cache_read(self.cache, self.table[:seqs], cu_k, x.shape[0] + done * seqs, dtype=torch.bfloat16)
-        return self._output(c.attention_prefill(q, k, v, cu, cu_k))
+        k, v = c.kv_cache_read(self.cache, self.pages.block_table, step.cu_seqlens_k, int(step.cu_seqlens_k[-1]), dtype=torch.bfloat16)
+        return self._output(c.attention_prefill(q, k, v, step.cu_seqlens_q, step.cu_seqlens_k))
 
-    def token(self, x, lengths):
-        """x [sequences, hidden] (f32) of one new token each; `lengths` int32 [sequences] counts it. f32 out."""
-        sequence = torch.arange(x.shape[0], device=x.device)
-        q, _, _ = self._project(x, torch.float32, sequence, lengths.long() - 1)
-        return self._output(c.attention_decode(q, self.cache, self.table[:x.shape[0]], lengths))
+    def token(self, x):
+        """x [sequences, hidden] (f32) of one new token each; f32 out."""
+        step = c.kv_pages_step(self.pages, torch.ones(x.shape[0], dtype=torch.int32, device=x.device), x.shape[0])
+        q = self._project(x, torch.float32, step)
+        return self._output(c.attention_decode(q, self.cache, self.pages.block_table, self.pages.seq_lens))
 
 
 def run(shape: Shape = Shape(), lengths=(700, 1200, 333), steps: int = 8, cache_dtype=torch.int8):
@@ -97,11 +94,10 @@ def run(shape: Shape = Shape(), lengths=(700, 1200, 333), steps: int = 8, cache_
     torch.cuda.synchronize()
     prompt_ms = (time.perf_counter() - start) * 1e3
 
-    lens, outs = torch.tensor(lengths, dtype=torch.int32, device="cuda"), []
+    outs = []
     start = time.perf_counter()
     for i in range(steps):
-        lens += 1
-        outs.append(block.token(torch.stack([x[n + i] for x, n in zip(xs, lengths)]), lens))
+        outs.append(block.token(torch.stack([x[n + i] for x, n in zip(xs, lengths)])))
     torch.cuda.synchronize()
     token_ms = (time.perf_counter() - start) * 1e3 / steps
 
@@ -111,7 +107,7 @@ def run(shape: Shape = Shape(), lengths=(700, 1200, 333), steps: int = 8, cache_
         want = whole.prompt(xs[b].bfloat16(), [n + steps])
         chunked = AttentionBlock(shape, 1, n + steps, cache_dtype)
         half = (n + steps) // 2
-        again = torch.cat([chunked.prompt(xs[b][:half].bfloat16(), [half]), chunked.prompt(xs[b][half:].bfloat16(), [n + steps - half], half)])
+        again = torch.cat([chunked.prompt(xs[b][:half].bfloat16(), [half]), chunked.prompt(xs[b][half:].bfloat16(), [n + steps - half])])
         for got, expected in ((torch.stack([o[b] for o in outs]), want[n:]), (again, want)):
             worst = max(worst, float((got - expected).norm() / expected.norm()))
     return worst, prompt_ms, token_ms
@@ -119,6 +115,6 @@ def run(shape: Shape = Shape(), lengths=(700, 1200, 333), steps: int = 8, cache_
 
 if __name__ == "__main__":
     run(steps=1)  # (warm-up)
-    for dtype in (torch.int8, torch.bfloat16):
-        worst, prompt_ms, token_ms = run(cache_dtype=dtype)
-        print(f"{dtype}: prompts {prompt_ms:.2f} ms, a token {token_ms:.3f} ms, tokens and chunks against whole prompts {worst:.1e}")
+    for dtype, norms in ((torch.int8, False), (torch.bfloat16, False), (torch.uint8, True)):
+        worst, prompt_ms, token_ms = run(Shape(head_norms=norms), cache_dtype=dtype)
+        print(f"{dtype}{', norms' if norms else ''}: prompts {prompt_ms:.2f} ms, a token {token_ms:.3f} ms, tokens and chunks against whole prompts {worst:.1e}")
