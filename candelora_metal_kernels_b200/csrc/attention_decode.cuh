@@ -35,6 +35,7 @@ struct DecodeArgs {
     uint32_t chunks_of_heads;
     Divisor by_page;                        // tokens of a page
     bool q_vec;                             // rows of q start on 16-byte boundaries
+    bool block_an_item;                     // (4-bit caches) not the line of work, but a block for each item
 };
 
 inline DecodeArgs decode_args(const DecodeParams& p, void* workspace, int num_sms) {
@@ -42,7 +43,8 @@ inline DecodeArgs decode_args(const DecodeParams& p, void* workspace, int num_sm
     return {p, reinterpret_cast<float*>(ws + records_bytes(num_sms)), reinterpret_cast<JoinRecord*>(ws), 1.0 / num_sms,
             (p.q_heads / p.c.heads + AD_HEADS - 1) / AD_HEADS, Divisor::of(p.c.page_size),
             reinterpret_cast<uintptr_t>(p.q.p) % 16 == 0 && p.q.token_stride * (p.dtype == kF32 ? 4 : 2) % 16 == 0 &&
-                p.q.head_stride * (p.dtype == kF32 ? 4 : 2) % 16 == 0};
+                p.q.head_stride * (p.dtype == kF32 ? 4 : 2) % 16 == 0,
+            false};
 }
 
 __device__ __forceinline__ uint32_t seq_len(const DecodeParams& p, uint32_t b) {

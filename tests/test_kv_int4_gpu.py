@@ -392,3 +392,15 @@ def test_refusals():
     cache.v_group.data = kept
     x = torch.ones((1, 2, 64), device="cuda")
     refused("have moved", c.kv_cache_write, cache, x, x, torch.zeros(1, dtype=torch.int32).cuda())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("width", [1, 12, 24, 48, 200])
+@pytest.mark.parametrize("lens,hq,hkv,d", [([1], 4, 2, 128), ([12, 0, 32, 33], 8, 1, 64), ([350, 1, 384, 385, 0, 70], 20, 2, 128), ([500, 31, 0], 9, 3, 96)])
+def test_decode_with_tables_of_any_width(lens, hq, hkv, d, width, dtype):
+    """Short tables let a block take an item, wide ones have the line of work: both give the same for lengths up to the table's."""
+    page, lens = 32, [min(n, 32 * width) for n in lens]
+    cache, table = make_cache(lens, hkv, page, d, 5, poison=float("nan"))
+    table = torch.nn.functional.pad(table, (0, max(0, width - table.shape[1])), value=-1)[:, :max(width, 1)].contiguous()
+    q = randn((len(lens), hq, d), 9, dtype).cuda()
+    check_decode(q, cache, table, lens, c.attention_decode(q, cache, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()))
