@@ -66,9 +66,10 @@ int check_cache(const char* op, const iq2_kv_cache* c) {
         return capi_fail(IQ2_ERR_OVERFLOW, "%s: %u pages of %u tokens are too large", op, c->num_pages, c->page_size);
     if ((rc = check_pointers(op, {{"cache k", c->k, 16}, {"cache v", c->v, 16}})) != IQ2_OK) return rc;
     if (c->dtype != IQ2_KV_INT8 && c->dtype != IQ2_KV_INT4) return IQ2_OK;
-    if ((rc = check_pointers(op, {{"cache k_scale", c->k_scale, 4}, {"cache v_scale", c->v_scale, 4}})) != IQ2_OK) return rc;
-    if (c->dtype == IQ2_KV_INT8) return IQ2_OK;
-    return check_pointers(op, {{"cache k_group", c->k_group, 4}, {"cache v_group", c->v_group, 4}});
+    if (c->dtype == IQ2_KV_INT8) return check_pointers(op, {{"cache k_scale", c->k_scale, 4}, {"cache v_scale", c->v_scale, 4}});
+    // (16 bytes of scales at a time)
+    return check_pointers(op, {{"cache k_scale", c->k_scale, 16}, {"cache v_scale", c->v_scale, 16}, {"cache k_group", c->k_group, 16},
+                               {"cache v_group", c->v_group, 16}});
 }
 
 iq2::KvCacheView view(const iq2_kv_cache* c) {

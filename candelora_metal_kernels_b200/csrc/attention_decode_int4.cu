@@ -168,10 +168,10 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     if (!FULL)
         for (uint32_t i = lane; i < S::RING / 16; i += 32) *reinterpret_cast<uint4*>(smem + warp * S::RING + i * 16) = make_uint4(0, 0, 0, 0);
     if (lane < 2) pieces[warp * 2 + lane].valid = 0;
-    // where each warp reads and where it copies from, and the block's first unit: in shared memory, since registers are short
-    // and they change from one piece to the next only
+    // where a warp reads and where it copies from, and the block's first unit, each warp's own: in shared memory, since registers
+    // are short and they change from one piece to the next only
     __shared__ Cursor cursors[A4_WARPS][2];
-    __shared__ uint64_t block_u0;
+    __shared__ uint64_t block_u0[A4_WARPS];
     Cursor& cur_held = cursors[warp][0];
     Cursor& pre_held = cursors[warp][1];
     bool live;  // there is a tile to copy
@@ -187,15 +187,14 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
         pre_tok = warp * tiles / A4_WARPS * TOK, pre_t1 = min((warp + 1) * tiles / A4_WARPS * TOK, len);
         live = pre_tok < pre_t1;
         const Cursor cur{0, live ? 1u : 0u, b, item, len, 1, 0, 1, pre_tok, pre_t1};
-        if (lane == 0) cur_held = cur, pre_held = cur;
-        if (threadIdx.x == 0) block_u0 = 0;
+        if (lane == 0) cur_held = cur, pre_held = cur, block_u0[warp] = 0;
     } else {
         typename Cursor::Parts line;
         const uint32_t part0 = blockIdx.x * A4_WARPS;  // the block's parts of the line, one a warp
         Cursor cur = Cursor::of_part(a, part0 + warp, gridDim.x * A4_WARPS, a.inv_blocks * (1.0 / A4_WARPS), lane, 32, line);
-        if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, part0, A4_WARPS), block_u0 = line.begin(part0);
+        if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, part0, A4_WARPS);
         if (cur.t0 == cur.t1) cur.unit = cur.end;  // nothing, or nothing but an item's start
-        if (lane == 0) cur_held = cur, pre_held = cur;
+        if (lane == 0) cur_held = cur, pre_held = cur, block_u0[warp] = line.begin(part0);
         live = !cur.done(), pre_tok = cur.t0, pre_t1 = cur.t1;
     }
     auto advance = [&](Cursor& held) {
@@ -223,7 +222,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                                         : lane < 24 ? p.c.k_group : p.c.v_group);
     uint32_t pre_in = 0, pre_head = 0;  // the tile's place in its page (whole tiles), rows of the heads before
     const int32_t* table = nullptr;     // the sequence's pages
-    uint32_t page = 0, ahead = 0;                         // this lane's page of those looked up; tiles since
+    uint32_t page = 0, ahead = 0;       // this lane's page of those looked up; tiles since
     bool fresh = true;
     auto look_up = [&](uint32_t tok) {
         return tok < pre_t1 ? (uint32_t)__ldg(table + a.by_page.quotient(tok)) : 0xFFFFFFFFu;
@@ -553,7 +552,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 if (g == 0) slot[S::MAXIMA + 2 * t + h] = m[h], slot[S::SUMS + 2 * t + h] = l[h];
             }
             if (lane == 0)
-                pieces[warp * 2 + !first_piece] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.unit - cur.k <= block_u0 ? 8u : 0u)};
+                pieces[warp * 2 + !first_piece] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.unit - cur.k <= block_u0[warp] ? 8u : 0u)};
         }
         first_piece = false;
     }

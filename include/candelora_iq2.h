@@ -282,8 +282,9 @@ int iq2_matmul_grouped_sharded(iq2_comm_t comm, const iq2_matmul_problem* proble
  * IQ2_KV_INT4 only. IQ2_KV_INT4 rows are head_dim / 2 bytes (head_dim a multiple of 32): element 2i
  * in the low half of byte i, element 2i + 1 in the high half, each as its code -7..7 plus 8; and
  * k_group and v_group [num_pages, kv_heads, page_size, 4] hold the e4m3 scales (not negative, no
- * NaN) of a row's groups of 32 elements, 4-byte aligned, of which the first head_dim / 32 count. An
- * element is code * group scale * row scale. k_group and v_group are not read for other types.
+ * NaN) of a row's groups of 32 elements, of which the first head_dim / 32 count; all scales are
+ * 16-byte aligned. An element is code * group scale * row scale. k_group and v_group are not read
+ * for other types.
  * Any page_size. Token `pos` of a sequence lies in page block_table[pos / page_size], row
  * pos % page_size. A block table is int32 [sequences, table_width] on the device; entries outside
  * [0, num_pages) are never followed: their tokens take no part in an attention and read as zeros.

@@ -383,6 +383,12 @@ def test_refusals():
     refused("head_dim=160", c.kv_cache_read, c.KvCache.empty(2, 2, 16, 160, I4), torch.zeros((1, 1), dtype=torch.int32).cuda(),
             torch.tensor([0, 1], dtype=torch.int32).cuda(), 1)
     refused("device mismatch", c.KvCache, k, k, s, s, g, g.cpu())
+    # views off the 16-byte boundaries
+    shifted = torch.zeros(s.numel() + 4, device="cuda")[1:1 + s.numel()].view(s.shape)
+    moved = torch.zeros(g.numel() + 16, dtype=torch.uint8, device="cuda")[4:4 + g.numel()].view(g.shape).view(E4M3)
+    one, x = torch.zeros(1, dtype=torch.int32).cuda(), torch.ones((1, 2, 64), device="cuda")
+    refused("v_scale is not 16-byte aligned", c.kv_cache_write, c.KvCache(k, k, s, shifted, g, g), x, x, one)
+    refused("k_group is not 16-byte aligned", c.attention_decode, x, c.KvCache(k, k, s, s, moved, g), one[None], one)
     refused("expects q of shape", c.attention_decode, torch.zeros((1, 2, 32)).cuda(), cache, torch.zeros((1, 1), dtype=torch.int32).cuda(),
             torch.ones(1, dtype=torch.int32).cuda())
     for name in ("k_group", "v_group"):
