@@ -91,7 +91,7 @@ class KvCache:
 
     A 4-bit cache has k, v uint8 [num_pages, kv_heads, page_size, head_dim / 2] (head_dim a multiple of 32), element 2i in the
     low half of byte i, 2i + 1 in the high half, as code + 8; the scales above, and k_group, v_group
-    [num_pages, kv_heads, page_size, 4] float8_e4m3fn, of which the first head_dim / 32 are the (not negative) scales of a
+    [num_pages, kv_heads, page_size, 4] float8_e4m3fn, of which the first head_dim / 32 are the scales (not negative, no NaN) of a
     row's groups of 32 elements: an element is code * group scale * row scale. Its scales start on 16-byte boundaries."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
@@ -187,7 +187,7 @@ def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
                    q_out: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
                    k_norm: torch.Tensor | None = None, norm_eps: float = 1e-6) -> torch.Tensor | None:
     """Write k, v [tokens, kv_heads, head_dim] (f32, f16 or bf16) to the cache's `slots` (int32 [tokens],
-    page * page_size + row; a slot outside the cache, e.g. -1, writes nothing). With cos, sin f32
+    page * page_size + row; a slot outside the cache, e.g. -1, writes nothing; no two tokens share one). With cos, sin f32
     [rows, head_dim / 2] and positions int32 [tokens], k and q are rotated first: pairs (i, i + head_dim / 2), or
     (2i, 2i + 1) with `interleaved`; without cos and sin, positions are not read. q [tokens, q_heads, head_dim], of k's
     dtype, is returned as q_dtype (its own by default). With q_norm or k_norm (f32 [head_dim], or a row for each head), each

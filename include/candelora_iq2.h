@@ -401,7 +401,8 @@ size_t iq2_attention_decode_workspace_size(const iq2_kv_cache* cache, uint32_t b
 
 /*
  * out = softmax(scale q k^T) v, any q type over any cache type; scores, maxima, sums and accumulation
- * in f32, q and the probabilities as sums of two 16-bit pieces (three for f32 q over a bf16 cache).
+ * in f32, q and the probabilities as sums of two 16-bit pieces (three for f32 q over a bf16 cache; over
+ * IQ2_KV_INT4 a 16-bit q is one, and its probabilities are rounded to f16 once).
  * A sequence of length 0 gets zeros.
  */
 int iq2_attention_decode(const iq2_kv_cache* cache, const iq2_attention_tokens* tokens, void* workspace,
@@ -436,7 +437,7 @@ typedef struct iq2_kv_step {
 /*
  * Cuts every sequence to `keep`, whose pages behind go back to the free ones in the order of sequences
  * and columns, gives every sequence the pages of its new tokens in the same order, and writes
- * where they go, in one launch. All of a sequence's new tokens get a place or none: none where they
+ * where they go, in one launch (two for more than 4096 rows). All of a sequence's new tokens get a place or none: none where they
  * pass `total` rows or the table's width, and none from the first sequence on whose pages are more
  * than are left (but for those that need no new page). Such a sequence keeps the tokens it had, its
  * rows get slot -1 and position 0, as do rows of no sequence. Negative counts are 0. At most 8192
