@@ -191,7 +191,7 @@ def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
     [rows, head_dim / 2] and positions int32 [tokens], k and q are rotated first: pairs (i, i + head_dim / 2), or
     (2i, 2i + 1) with `interleaved`; without cos and sin, positions are not read. q [tokens, q_heads, head_dim], of k's
     dtype, is returned as q_dtype (its own by default). With q_norm or k_norm (f32 [head_dim], or a row for each head), each
-    head's q or k becomes x / sqrt(mean(x^2) + norm_eps) * weight before its rotation."""
+    head's q or k becomes x / sqrt(mean(x^2) + norm_eps) * weight before its rotation (norm_eps rounded to f32)."""
     op = "kv_cache_write"
     d, index, kv_heads = cache.head_dim, cache._index, cache.kv_heads
     k, k_strides, (tokens, _, _) = _rows(op, index, "k", k, kv_heads, d)

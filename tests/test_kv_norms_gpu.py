@@ -127,6 +127,14 @@ def test_without_norms_it_is_the_plain_write():
     assert torch.equal(normed.cpu(), step_ref.normed(q.cpu(), ones.cpu(), 1e-6).bfloat16())
 
 
+def test_eps_is_an_f32():
+    """Rows next to eps: they show in one of some ten whether eps is an f32 (0.1 is off by 1.5e-8) or has 64 bits."""
+    x, w, eps = 0.01 * randn((500, 4, 32), 1), weights(4, 32, 2, True), float(torch.tensor(0.1))
+    cache = c.KvCache.empty(1, 4, 8, 32, I4)
+    out = c.kv_cache_write(cache, x.cuda(), x.cuda(), torch.full((500,), -1, dtype=torch.int32).cuda(), q=x.cuda(), q_norm=w.cuda(), norm_eps=0.1).cpu()
+    assert torch.equal(out, step_ref.normed(x, w, eps)) and not torch.equal(out, step_ref.normed(x, w, 0.1))
+
+
 def test_refusals():
     cache = c.KvCache.empty(2, 2, 16, 64)
     kv, q, one = torch.ones((4, 2, 64)).cuda(), torch.ones((4, 6, 64)).cuda(), torch.arange(4, dtype=torch.int32).cuda()
