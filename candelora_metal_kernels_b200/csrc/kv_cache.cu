@@ -15,9 +15,9 @@
 // Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 18.3 us over 0.9 GB of inputs and
 // outputs in turn, 4190 GB/s (12.8 over 0.2 GB, where the L2 keeps part of the outputs); of 8800 tokens, f32 into an int8 cache,
 // with the read back 67.5 us, 5380 GB/s; read of 89091 tokens to bf16, of an int8 cache 97 us, 5680 GB/s, of a bf16 one 117 us,
-// 6220 GB/s, of a 4-bit one 96 us, 4860 GB/s (a fill of the 365 MB that the read of an int8 or 4-bit cache writes takes 97 us: the
-// writes bind). With norms the write of 2048 tokens takes 18.4 us; 8800 tokens into a 4-bit cache with the read back 66 us from
-// f32, and 75 us from bf16 with norms, of which the write is 60: instructions, 400 for four rows at 67 % of the issue slots.
+// 6220 GB/s, of a 4-bit one 85 us, 5510 GB/s, 365 MB of the 467 written. With norms the write of 2048 tokens takes 17.6 us; 8800
+// tokens into a 4-bit cache with the read back 63 us from f32, and 71 us from bf16 with norms, of which the write is 57:
+// instructions, 400 for four rows at two thirds of the issue slots.
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"
 
@@ -234,8 +234,11 @@ cudaError_t launch_write_of(const KvWriteParams& p, cudaStream_t stream) {
 // As above, but a thread has eight elements of each half whatever the input's type (fewer threads share a row's sums, maxima and
 // addresses), a block has rows of one of q, k and v, and rows off the 16-byte boundaries are a kernel of their own (their
 // loads element by element are predicated away in one that has both, but issued all the same: 28 instead of 12 loads a warp; all
-// of it 22.5 -> 18.4 us for 2048 tokens with norms). Blocks of an SM: four with norms (five 19.2, three 18.2 us), five without (8800
-// tokens from f32 into a 4-bit cache and back 65.4 us; four 69.5, six 67.0).
+// of it 22.5 -> 18.4 us for 2048 tokens with norms). Threads of an SM: 1024 with norms (1280: 19.2 us), 1280 without (8800 tokens
+// from f32 into a 4-bit cache and back 65.4 us; 1024: 69.5, 1536: 67.0). Of a block, whose rows end together: 32 / 64 / 96 / 128 / 256
+// threads 17.6 / 17.7 / 18.0 / 17.8 / 18.4 us and, 8800 tokens from bf16 with norms into a 4-bit cache and back, 73.7 / 72.0 / 74.3 /
+// 73.1 / 75.1.
+constexpr int KN_THREADS = 64;
 constexpr int KN = 8;
 enum RowKind { ROW_Q, ROW_K, ROW_V };
 
@@ -302,8 +305,8 @@ __device__ __forceinline__ uint32_t codes_int4(const float (&x)[KN], uint32_t g,
 }
 
 template <int LANES, int IN, bool NORM, bool I4, bool VEC>
-__global__ void __launch_bounds__(KW_THREADS, NORM ? 4 : 5) kv_write_rows_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t tokens) {
-    constexpr uint32_t PER = KW_THREADS / LANES;
+__global__ void __launch_bounds__(KN_THREADS, (NORM ? 1024 : 1280) / KN_THREADS) kv_write_rows_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t tokens) {
+    constexpr uint32_t PER = KN_THREADS / LANES;
     const uint32_t lane = threadIdx.x % LANES, half = p.c.d / 2;
     const int kind = blockIdx.x < p.blocks_q ? ROW_Q : blockIdx.x < p.blocks_q + p.blocks_kv ? ROW_K : ROW_V;
     const uint32_t block = blockIdx.x - (kind == ROW_Q ? 0 : kind == ROW_K ? p.blocks_q : p.blocks_q + p.blocks_kv);
@@ -436,13 +439,13 @@ __global__ void __launch_bounds__(KW_THREADS, NORM ? 4 : 5) kv_write_rows_kernel
 
 template <int LANES, int IN, bool NORM, bool I4, bool VEC>
 cudaError_t launch_write_rows(KvWriteParams p, cudaStream_t stream) {
-    constexpr uint32_t PER = KW_THREADS / LANES;
+    constexpr uint32_t PER = KN_THREADS / LANES;
     const uint32_t chunk = std::max(1u, 0x7FFFFFFFu / (p.q_heads + 2 * p.c.heads) / 2);  // rows of a launch, and of blocks that part full, stay below 2^31
     auto blocks = [&](uint32_t tokens, uint32_t heads) { return (uint32_t)(((uint64_t)tokens * heads + PER - 1) / PER); };
     for (uint64_t t0 = 0; t0 < p.tokens; t0 += chunk) {
         const uint32_t tokens = (uint32_t)std::min<uint64_t>(chunk, p.tokens - t0);
         p.blocks_q = blocks(tokens, p.q_heads), p.blocks_kv = blocks(tokens, p.c.heads);
-        kv_write_rows_kernel<LANES, IN, NORM, I4, VEC><<<p.blocks_q + 2 * p.blocks_kv, KW_THREADS, 0, stream>>>(p, (uint32_t)t0, tokens);
+        kv_write_rows_kernel<LANES, IN, NORM, I4, VEC><<<p.blocks_q + 2 * p.blocks_kv, KN_THREADS, 0, stream>>>(p, (uint32_t)t0, tokens);
     }
     return cudaGetLastError();
 }
@@ -465,8 +468,14 @@ cudaError_t launch_write_rows_by(const KvWriteParams& p, cudaStream_t stream) {
 // A block takes `tokens` tokens: it finds their rows in the cache, then groups of LANES threads (a power of two >= d / 8)
 // copy a row of K and V each, eight elements a thread, KR_BATCH rows' loads in flight. An int8 cache is read at one byte for
 // two written, and the stores bind (codes widened by byte permutes instead of conversions: 96.0 us as well; stores that give
-// way in the cache: 96.6).
-constexpr int KR_MOST = 32, KR_BATCH = 4;
+// way in the cache: 96.6). Threads of a block, an eighth as many tokens: of a 4-bit cache 96 / 128 / 160 / 192 / 224 / 256 / 384 take
+// 85.2 / 92.4 / 84.8 / 85.3 / 91 / 96.2 / 87.8 us for 89091 tokens, 14.9 / - / 13.2 / 13.4 / - / 15.5 / - for 8800 (rows that are
+// in flight together are no power of two apart), of an int8 cache 160 / 192 / 256 / 384 take 100.0 / 100.2 / 97.1 / 113.4.
+constexpr int KR_BATCH = 4;
+template <bool I4>
+struct ReadShape {
+    static constexpr uint32_t THREADS = I4 ? 160 : 256, MOST = THREADS / 8;  // of a block, and its tokens at most
+};
 
 struct Eight {
     uint4 w;  // 8 16-bit elements; or the 8 codes in x, y and the scale in z; or 8 4-bit codes in x, their group's scale in y, the row's in z
@@ -530,8 +539,8 @@ __device__ __forceinline__ void write8(void* out, int64_t at, int out_dtype, con
 }
 
 template <int LANES, bool I4>
-__global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const __grid_constant__ KvReadParams p, uint32_t tokens) {
-    __shared__ int64_t first[KR_MOST];  // each token's row of head 0 in the cache, -1: none (its rows are zeros)
+__global__ void __launch_bounds__(ReadShape<I4>::THREADS) kv_read_kernel(const __grid_constant__ KvReadParams p, uint32_t tokens) {
+    __shared__ int64_t first[ReadShape<I4>::MOST];  // each token's row of head 0 in the cache, -1: none (its rows are zeros)
     const uint32_t t0 = blockIdx.x * tokens;
     if (threadIdx.x < tokens && t0 + threadIdx.x < p.total) {
         const int32_t t = (int32_t)(t0 + threadIdx.x);
@@ -554,7 +563,7 @@ __global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const __grid_consta
         first[threadIdx.x] = row;
     }
     __syncthreads();
-    constexpr uint32_t GROUPS = KW_THREADS / LANES;
+    constexpr uint32_t GROUPS = ReadShape<I4>::THREADS / LANES;
     const uint32_t col = threadIdx.x % LANES * 8, rows = min(tokens, p.total - t0) * p.c.heads;
     if (col >= p.c.d) return;
     for (uint32_t r0 = threadIdx.x / LANES; r0 < rows; r0 += GROUPS * KR_BATCH) {
@@ -582,10 +591,10 @@ __global__ void __launch_bounds__(KW_THREADS) kv_read_kernel(const __grid_consta
 
 template <int LANES, bool I4>
 cudaError_t launch_read(const KvReadParams& p, cudaStream_t stream) {
-    // up to 32 tokens a block (the look-up of their rows is done once for all heads), fewer where that leaves the SMs idle
-    uint32_t tokens = KR_MOST;
+    // up to 32 (20) tokens a block (the look-up of their rows is done once for all heads), fewer where that leaves the SMs idle
+    uint32_t tokens = ReadShape<I4>::MOST;
     while (tokens > 1 && (p.total + tokens - 1) / tokens < 4 * 148) tokens /= 2;
-    kv_read_kernel<LANES, I4><<<(p.total + tokens - 1) / tokens, KW_THREADS, 0, stream>>>(p, tokens);
+    kv_read_kernel<LANES, I4><<<(p.total + tokens - 1) / tokens, ReadShape<I4>::THREADS, 0, stream>>>(p, tokens);
     return cudaGetLastError();
 }
 
