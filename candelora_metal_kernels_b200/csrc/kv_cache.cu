@@ -15,8 +15,8 @@
 // Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 18.3 us over 0.9 GB of inputs and
 // outputs in turn, 4190 GB/s (12.8 over 0.2 GB, where the L2 keeps part of the outputs); of 8800 tokens, f32 into an int8 cache,
 // with the read back 67.5 us, 5380 GB/s; read of 89091 tokens to bf16, of an int8 cache 97 us, 5680 GB/s, of a bf16 one 117 us,
-// 6220 GB/s, of a 4-bit one 85 us, 5510 GB/s, 365 MB of the 467 written. With norms the write of 2048 tokens takes 17.6 us; 8800
-// tokens into a 4-bit cache with the read back 63 us from f32, and 71 us from bf16 with norms, of which the write is 57:
+// 6220 GB/s, of a 4-bit one 85 us, 5510 GB/s, 365 MB of the 467 written. With norms the write of 2048 tokens takes 17.3 us; 8800
+// tokens into a 4-bit cache with the read back 62 us from f32, and 68 us from bf16 with norms, of which the write is 55:
 // instructions, 400 for four rows at two thirds of the issue slots.
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"
@@ -234,10 +234,10 @@ cudaError_t launch_write_of(const KvWriteParams& p, cudaStream_t stream) {
 // As above, but a thread has eight elements of each half whatever the input's type (fewer threads share a row's sums, maxima and
 // addresses), a block has rows of one of q, k and v, and rows off the 16-byte boundaries are a kernel of their own (their
 // loads element by element are predicated away in one that has both, but issued all the same: 28 instead of 12 loads a warp; all
-// of it 22.5 -> 18.4 us for 2048 tokens with norms). Threads of an SM: 1024 with norms (1280: 19.2 us), 1280 without (8800 tokens
-// from f32 into a 4-bit cache and back 65.4 us; 1024: 69.5, 1536: 67.0). Of a block, whose rows end together: 32 / 64 / 96 / 128 / 256
-// threads 17.6 / 17.7 / 18.0 / 17.8 / 18.4 us and, 8800 tokens from bf16 with norms into a 4-bit cache and back, 73.7 / 72.0 / 74.3 /
-// 73.1 / 75.1.
+// of it 22.5 -> 18.4 us for 2048 tokens with norms). Of a block, whose rows end together, 32 / 64 / 96 / 128 / 256 threads take 17.6 /
+// 17.7 / 18.0 / 17.8 / 18.4 us and, 8800 tokens from bf16 with norms into a 4-bit cache and back, 73.7 / 72.0 / 74.3 / 73.1 / 75.1.
+// Threads of an SM, then: with norms 896 / 1024 / 1152 (56 registers) 17.7 / 17.9 / 17.3 and 70.2 / 70.2 / 67.7 us; without, 8800 tokens
+// from f32 into a 4-bit cache and back, 1152 / 1280 / 1344 (48 registers) / 1408 64.3 / 62.7 / 61.8 / 64.0.
 constexpr int KN_THREADS = 64;
 constexpr int KN = 8;
 enum RowKind { ROW_Q, ROW_K, ROW_V };
@@ -305,7 +305,7 @@ __device__ __forceinline__ uint32_t codes_int4(const float (&x)[KN], uint32_t g,
 }
 
 template <int LANES, int IN, bool NORM, bool I4, bool VEC>
-__global__ void __launch_bounds__(KN_THREADS, (NORM ? 1024 : 1280) / KN_THREADS) kv_write_rows_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t tokens) {
+__global__ void __launch_bounds__(KN_THREADS, (NORM ? 1152 : 1344) / KN_THREADS) kv_write_rows_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t tokens) {
     constexpr uint32_t PER = KN_THREADS / LANES;
     const uint32_t lane = threadIdx.x % LANES, half = p.c.d / 2;
     const int kind = blockIdx.x < p.blocks_q ? ROW_Q : blockIdx.x < p.blocks_q + p.blocks_kv ? ROW_K : ROW_V;
