@@ -237,7 +237,8 @@ cudaError_t launch_write_of(const KvWriteParams& p, cudaStream_t stream) {
 // of it 22.5 -> 18.4 us for 2048 tokens with norms). Of a block, whose rows end together, 32 / 64 / 96 / 128 / 256 threads take 17.6 /
 // 17.7 / 18.0 / 17.8 / 18.4 us and, 8800 tokens from bf16 with norms into a 4-bit cache and back, 73.7 / 72.0 / 74.3 / 73.1 / 75.1.
 // Threads of an SM, then: with norms 896 / 1024 / 1152 (56 registers) 17.7 / 17.9 / 17.3 and 70.2 / 70.2 / 67.7 us; without, 8800 tokens
-// from f32 into a 4-bit cache and back, 1152 / 1280 / 1344 (48 registers) / 1408 64.3 / 62.7 / 61.8 / 64.0.
+// from f32 into a 4-bit cache and back, 1152 / 1280 / 1344 (40 registers, aligned rows without
+// spills) / 1408 64.3 / 62.7 / 61.5 / 63.5.
 constexpr int KN_THREADS = 64;
 constexpr int KN = 8;
 enum RowKind { ROW_Q, ROW_K, ROW_V };
