@@ -13,9 +13,12 @@
 //     ones of a key row, one group: one wide load and one scale a key. For O a thread's rows are DP / 8 consecutive dimensions, again
 //     one group, of the two tokens whose p it holds; tokens are relabelled so that both kinds of loads are free of bank conflicts.
 //   * q of 32 bits and its p are sums of two f16 pieces in one accumulator: q is held times the power of two that brings a head's
-//     largest |q| to 2^12, so that its 22 bits end at 2^-36 of it; p times its value's row scale is 2^7 at the reference, up to
-//     2^15, and its 22 bits end at 2^-31 of the largest. q of 16 bits is one piece exactly, and its p is rounded to f16 once.
-//   * The row scales of keys multiply s, those of values multiply p.
+//     largest |q| to 2^12, so that its 22 bits end at 2^-36 of it. q of 16 bits is one piece exactly, and its p is rounded to f16 once.
+//   * The row scales of keys multiply s, those of values multiply p. p next to the largest score's, whose sum is l, ends at 2^-126 as
+//     f32's exponential does, whatever the values; what f16 pieces are taken of is p times the value's row scale times 2^level, a
+//     head's own power of two that makes the largest of these 2^7 to 2^8 (they may grow to 2^15), so that 22 bits end at 2^-31 of the
+//     largest. (The row scales in the reference instead: one exponential less to look at, 2 % faster, but rows of 3e38 lost the tokens below
+//     2^-7 of the largest weight, and rows of zeros all of their weight beside rows of 1e9.)
 // The maxima, sums, s, p and o are f32.
 //
 // A warp has a part of the line of its own, copies its tiles into two stages by itself and waits for nobody; at the end the block
@@ -38,12 +41,11 @@ constexpr int A4_WARPS = 12, A4_THREADS = A4_WARPS * 32;
 static_assert(2 * A4_WARPS <= 32, "a lane a piece");
 constexpr int A4_TOK = 32, A4_NT = A4_TOK / 8;  // tokens of a warp's stage, and eights of them
 constexpr int A4_RUN = 8;                // tokens that lie side by side in a page of a multiple of these
-constexpr float A4_TOP = 7.f;            // log2 of p times the value scale at the reference
-constexpr float A4_LAZY = 32768.f;       // how far it may grow before that moves
-constexpr float A4_SUM = 1.f / 65536.f;  // what the sums of p, and with them o, are held times: p alone may reach 2^118
-// The values' row scales, 2^-111 or more, multiply p as 2^9 of themselves (2^126 at most); a row of zeros counts as 2^-103.
-constexpr float A4_UP = 512.f, A4_MIN_SCALE = 9.86076132e-32f;
+constexpr float A4_TOP = 7.f;            // log2 of the largest p times its value scale where the head's level is set
+constexpr float A4_LAZY = 32768.f;       // how far that, or p from 1, may grow before reference and level move
+constexpr float A4_MOST = 112.f;         // log2 of the highest level: p times it stays below 2^127
 constexpr float A4_VALUE = 32768.f;      // 2^15: what values are held by
+constexpr uint32_t A4_NORM = 13;         // a piece's sum of p is held in [2^-13, 2^-12): 24 pieces in each of 148 parts add up to less than 1
 
 template <int DP>
 struct Shape4 {
@@ -103,6 +105,11 @@ __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
     return v;
 }
+
+// 2^x of an integer x in -126..127, its logarithm, and one over it.
+__device__ __forceinline__ float power_of_two(float x) { return __uint_as_float((uint32_t)((int)x + 127) << 23); }
+__device__ __forceinline__ float log2_of_power(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
+__device__ __forceinline__ float over_power(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
 // N consecutive elements of a row of q as f32, zeros unless `there`; `vec`: rows start on 16-byte boundaries.
 template <int N>
@@ -377,7 +384,8 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                     q_low[i * 2 + j / 2][j % 2] = WIDE ? pack_pair<false>(x0 - back.x, x1 - back.y) : 0u;
                 }
         }
-        float o[MT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+        // o is held times 2^level of the head, f = 2^level
+        float o[MT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, f[2] = {power_of_two(A4_MOST), power_of_two(A4_MOST)};
 #pragma unroll
         for (int n = 0; n < MT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
@@ -421,14 +429,14 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 x[mt * 2][0] = s[0], x[mt * 2][1] = s[1], x[mt * 2 + 1][0] = s[2], x[mt * 2 + 1][1] = s[3];
             }
 
-            // x = log2(e) scale q . k, rounded before the reference is taken off (which is one of them); w = 2^(x - m) times the value
-            // scale
-            float e[NT][2], w[NT][2], vs[NT];
+            // x = log2(e) scale q . k, rounded before the reference is taken off (which is one of them); e = 2^(x - m), w = e f times
+            // the value scale
+            float e[NT][2], w[NT][2], sum[2] = {0.f, 0.f}, vs[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const uint32_t from = at + S::SCALES + (n * 8 + k_row) * 4;
                 const float ks = __uint_as_float(ld_shared(from));
-                vs[n] = max_nan(__uint_as_float(ld_shared(from + TOK * 4)) * A4_UP, A4_MIN_SCALE);
+                vs[n] = __uint_as_float(ld_shared(from + TOK * 4));
                 x[n][0] *= ks * factor[0], x[n][1] *= ks * factor[1];
             }
             if (here != 0xFFFFFFFFu) {
@@ -436,52 +444,55 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 for (int n = 0; n < NT; ++n)
                     if (!((here >> (n * 8 + k_row)) & 1u)) x[n][0] = x[n][1] = -INFINITY;
             }
-            // The reference does as a rule: the products are made with it, and made again in the rare case that it moves.
+            // Reference and level do as a rule: the products are made with them, and made again in the rare case that they move.
             bool first = __any_sync(0xFFFFFFFFu, m[0] == -INFINITY || m[1] == -INFINITY);
             for (;;) {
                 if (!first) {
                     float top = 0.f;
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const float base = m[h] == -INFINITY ? 0.f : m[h] - A4_TOP;
+                        const float base = m[h] == -INFINITY ? 0.f : m[h];
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
                             e[n][h] = exp2_approx(x[n][h] - base);
-                            w[n][h] = e[n][h] * vs[n];
-                            top = fmaxf(top, w[n][h]);
+                            w[n][h] = e[n][h] * f[h] * vs[n];
+                            top = fmaxf(top, fabsf(w[n][h]));
                         }
+                        sum[h] = (e[0][h] + e[1][h]) + (e[2][h] + e[3][h]);
+                        top = fmaxf(top, sum[h]);
                     }
                     if (!__any_sync(0xFFFFFFFFu, top > A4_LAZY)) break;
                 }
-                // the largest x + log2(value scale) of the heads' tokens
-                float keep[2];
                 bool moved = false;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    float most = -INFINITY;
+                    // the largest x of the head's tokens, and the largest x + log2 |value scale|
+                    float most = -INFINITY, weighed = -INFINITY;
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) most = fmaxf(most, x[n][h] + __log2f(vs[n]));
+                    for (int n = 0; n < NT; ++n) most = fmaxf(most, x[n][h]), weighed = fmaxf(weighed, x[n][h] + __log2f(fabsf(vs[n])));
 #pragma unroll
-                    for (int b = 4; b < 32; b *= 2) most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, b));
-                    const float next = fmaxf(m[h], most);
-                    keep[h] = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - next);
-                    moved = moved || next > m[h];
-                    m[h] = next;
+                    for (int b = 4; b < 32; b *= 2) {
+                        most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, b));
+                        weighed = fmaxf(weighed, __shfl_xor_sync(0xFFFFFFFFu, weighed, b));
+                    }
+                    // the level takes the tile's largest w to 2^A4_TOP, but never makes o larger than it is
+                    // (whole numbers, so that what is there is taken times powers of two; nothing yet: `up` is infinite)
+                    const float next = fmaxf(m[h], ceilf(most)), level = log2_of_power(f[h]), up = next - m[h];
+                    const float to = fmaxf(fminf(fminf(ceilf(A4_TOP - (weighed - next)), level + up), A4_MOST), -126.f);
+                    const float keep = m[h] == -INFINITY ? 0.f : exp2_approx(-up), keep_o = m[h] == -INFINITY ? 0.f : exp2_approx(to - level - up);
+                    moved = moved || next > m[h] || to != level;
+                    m[h] = next, f[h] = power_of_two(to);
+                    l[h] *= keep;
+#pragma unroll
+                    for (int n = 0; n < MT; ++n) o[n][h] *= keep_o, o[n][2 + h] *= keep_o;
                 }
                 if (!__any_sync(0xFFFFFFFFu, moved) && !first) break;
                 first = false;
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    l[h] *= keep[h];
-#pragma unroll
-                    for (int n = 0; n < MT; ++n) o[n][h] *= keep[h], o[n][2 + h] *= keep[h];
-                }
             }
+            l[0] += sum[0], l[1] += sum[1];
             uint32_t high[NT], low[NT];  // the pieces of p, with heads as rows and tokens as columns
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) l[h] = fmaf(e[n][h], A4_SUM, l[h]);
                 const uint32_t hi = pack_pair<false>(w[n][0], w[n][1]);
                 high[n] = transposed(hi);
                 if (WIDE) {
@@ -531,7 +542,6 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
             for (int b = 4; b < 32; b *= 2) l[h] += __shfl_xor_sync(0xFFFFFFFFu, l[h], b);
 
         // ---- the end of the piece: a whole item's output, or (o, m, l) for the block to add up ----
-        constexpr float UNIT_OF_O = A4_SUM * (A4_VALUE / A4_UP);
         const Cursor cur = cur_held;
         uint32_t head0;
         const uint32_t heads = heads_of(cur.item, head0);
@@ -539,7 +549,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if (2 * t + h < heads && g * (DP / 8) < d) {
-                    auto value = [&](float x) { return l[h] == 0.f ? 0.f : x * UNIT_OF_O / l[h]; };
+                    auto value = [&](float x) { return l[h] == 0.f ? 0.f : x * A4_VALUE / l[h] * over_power(f[h]); };
                     float y[DP / 8];
 #pragma unroll
                     for (int j = 0; j < DP / 32; ++j)
@@ -554,13 +564,18 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 cp_async_wait<0>();
                 __syncwarp();
             }
+            // Its level goes, or values of any size would not meet in one sum: l = 2^k l' with l' in [2^-13, 2^-12), o' = o / 2^(level + k)
+            // is about the output times l', and the reference m + k.
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
+                const uint32_t k = min(max(__float_as_uint(l[h]) >> 23, 100u), 240u);  // + 127 - A4_NORM
+                const float down = __uint_as_float((254u - A4_NORM - k) << 23), off = over_power(f[h]);
+                auto value = [&](float x) { return x * (down * A4_VALUE) * off; };
 #pragma unroll
                 for (int j = 0; j < DP / 32; ++j)
                     *reinterpret_cast<float4*>(slot + (2 * t + h) * S::HEAD + g * (DP / 8) + j * 4) =
-                        make_float4(o[2 * j][h], o[2 * j][2 + h], o[2 * j + 1][h], o[2 * j + 1][2 + h]);
-                if (g == 0) slot[S::MAXIMA + 2 * t + h] = m[h], slot[S::SUMS + 2 * t + h] = l[h];
+                        make_float4(value(o[2 * j][h]), value(o[2 * j][2 + h]), value(o[2 * j + 1][h]), value(o[2 * j + 1][2 + h]));
+                if (g == 0) slot[S::MAXIMA + 2 * t + h] = m[h] + ((float)k - (127.f - A4_NORM)), slot[S::SUMS + 2 * t + h] = l[h] * down;
             }
             if (lane == 0)
                 pieces[warp * 2 + !first_piece] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.unit - cur.k <= block_u0[warp] ? 8u : 0u)};
@@ -605,9 +620,8 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
 #pragma unroll
             for (int i = 0; i < DP / 32; ++i) {
                 const uint32_t el = lane + i * 32;
-                constexpr float UNIT_OF_O = A4_SUM * (A4_VALUE / A4_UP);
-                if (!whole) part[h * DP + el] = y[i] * UNIT_OF_O;
-                else if (el < d) store_elem(p.out, ((int64_t)b * p.q_heads + head0 + h) * d + el, p.dtype, sum == 0.f ? 0.f : y[i] * UNIT_OF_O / sum);
+                if (!whole) part[h * DP + el] = y[i];
+                else if (el < d) store_elem(p.out, ((int64_t)b * p.q_heads + head0 + h) * d + el, p.dtype, sum == 0.f ? 0.f : y[i] / sum);
             }
             if (!whole && lane == 0) part[AD_HEADS * DP + h] = mx, part[AD_HEADS * DP + AD_HEADS + h] = sum;
         }
