@@ -12,8 +12,8 @@
 //   * A product's inner index may be relabelled as long as both sides agree. For S a thread's inner elements are DP / 4 consecutive
 //     ones of a key row, one group: one wide load and one scale a key. For O a thread's rows are DP / 8 consecutive dimensions, again
 //     one group, of the two tokens whose p it holds; tokens are relabelled so that both kinds of loads are free of bank conflicts.
-//   * q of 32 bits and its p are sums of two f16 pieces in one accumulator: q is held times the power of two that brings a head's
-//     largest |q| to 2^12, so that its 22 bits end at 2^-36 of it. q of 16 bits is one piece exactly, and its p is rounded to f16 once.
+//   * q of 32 bits and p are sums of two f16 pieces in one accumulator: q is held times the power of two that brings a head's
+//     largest |q| to 2^12, so that its 22 bits end at 2^-36 of it. q of 16 bits is one piece exactly; p of bf16 q is rounded to f16 once.
 //   * The row scales of keys multiply s, those of values multiply p. p next to the largest score's, whose sum is l, ends at 2^-126 as
 //     f32's exponential does, whatever the values; what f16 pieces are taken of is p times the value's row scale times 2^level, a
 //     head's own power of two that makes the largest of these 2^7 to 2^8 (they may grow to 2^15), so that 22 bits end at 2^-31 of the
@@ -168,9 +168,9 @@ __device__ __forceinline__ float* slot_of(uint8_t* smem, uint32_t i) {
     return reinterpret_cast<float*>(smem + (i % 2 == 0 ? A4_WARPS * S::RING + i / 2 * (S::SLOT * 4) : i / 2 * S::RING));
 }
 
-// WIDE: q of 32 bits, and two pieces of q and p; of 16 bits, q is one piece exactly and p is rounded to f16 once. FULL: head_dim
-// is DP.
-template <int DP, bool WIDE, bool FULL>
+// WIDE: q of 32 bits, in two pieces (of 16 bits it is one). FINE: p in two pieces. One piece is for bf16 outputs, which are rounded
+// to 2^-8 of themselves anyway, p to 2^-11: 50.9 us against 55.0 for 64 x 4096 tokens. FULL: head_dim is DP.
+template <int DP, bool WIDE, bool FINE, bool FULL>
 __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_constant__ DecodeArgs a) {
     using S = Shape4<DP>;
     constexpr int TOK = A4_TOK, NT = A4_NT, KS = S::KS, MT = S::MT;
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
             for (int n = 0; n < NT; ++n) {
                 const uint32_t hi = pack_pair<false>(w[n][0], w[n][1]);
                 high[n] = transposed(hi);
-                if (WIDE) {
+                if (FINE) {
                     const float2 back = unpack_pair<false>(hi);
                     low[n] = transposed(pack_pair<false>(w[n][0] - back.x, w[n][1] - back.y));
                 }
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                     for (int h = 0; h < 2; ++h) {
                         const uint32_t v[4] = {v0[2 * h], v0[2 * h + 1], v1[2 * h], v1[2 * h + 1]};
                         mma16816<false>(o[2 * j + h], v, high[ks * 2], high[ks * 2 + 1]);
-                        if (WIDE) mma16816<false>(o[2 * j + h], v, low[ks * 2], low[ks * 2 + 1]);
+                        if (FINE) mma16816<false>(o[2 * j + h], v, low[ks * 2], low[ks * 2 + 1]);
                     }
                 }
             }
@@ -629,11 +629,11 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     }
 }
 
-template <int DP, bool WIDE, bool FULL>
+template <int DP, bool WIDE, bool FINE, bool FULL>
 cudaError_t launch4(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
-    cudaError_t e = cudaFuncSetAttribute(decode4_kernel<DP, WIDE, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape4<DP>::SMEM);
+    cudaError_t e = cudaFuncSetAttribute(decode4_kernel<DP, WIDE, FINE, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape4<DP>::SMEM);
     if (e != cudaSuccess) return e;
-    decode4_kernel<DP, WIDE, FULL><<<blocks, A4_THREADS, Shape4<DP>::SMEM, stream>>>(a);
+    decode4_kernel<DP, WIDE, FINE, FULL><<<blocks, A4_THREADS, Shape4<DP>::SMEM, stream>>>(a);
     if ((e = cudaGetLastError()) != cudaSuccess || a.block_an_item) return e;
     return launch_join<DP>(a, blocks, stream);
 }
@@ -641,8 +641,9 @@ cudaError_t launch4(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
 template <int DP>
 cudaError_t launch4_of(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream) {
     const bool full = a.p.c.d == DP;
-    if (a.p.dtype == kF32) return full ? launch4<DP, true, true>(a, blocks, stream) : launch4<DP, true, false>(a, blocks, stream);
-    return full ? launch4<DP, false, true>(a, blocks, stream) : launch4<DP, false, false>(a, blocks, stream);
+    if (a.p.dtype == kF32) return full ? launch4<DP, true, true, true>(a, blocks, stream) : launch4<DP, true, true, false>(a, blocks, stream);
+    if (a.p.dtype == kF16) return full ? launch4<DP, false, true, true>(a, blocks, stream) : launch4<DP, false, true, false>(a, blocks, stream);
+    return full ? launch4<DP, false, false, true>(a, blocks, stream) : launch4<DP, false, false, false>(a, blocks, stream);
 }
 
 }  // namespace

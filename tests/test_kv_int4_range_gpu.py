@@ -20,13 +20,13 @@ BF16, F16, F32, I4 = torch.bfloat16, torch.float16, torch.float32, torch.uint8
 LOG2E = 1.4426950408889634
 
 
-def assert_near(q, k, v, got, scale, dtype):
-    """q, got [heads, d] of one sequence and key head over k, v [n, d] as they are held, in 64 bits."""
+def assert_near(q, k, v, got, scale, dtype, fine=False):
+    """q, got [heads, d] of one sequence and key head over k, v [n, d] as they are held, in 64 bits. `fine`: 22 bits of p."""
     q, got = q.double().cpu(), got.double().cpu()
     p = torch.softmax(q @ k.T * scale, -1)
     want, size = p @ v, p @ v.abs()
     part = 2.0 ** -15 * ((q.abs() @ k.abs().T * scale).amax(-1, keepdim=True) / 13).clamp(min=1)
-    if dtype != F32:
+    if dtype != F32 and not fine:
         part = part + ref.UNIT[F16]
     floor = len(k) * 2.0 ** -31 * (p * v.abs().amax(-1)).amax(-1, keepdim=True)
     assert torch.isfinite(got).all()
