@@ -44,6 +44,7 @@ constexpr int A4_RUN = 8;                // tokens that lie side by side in a pa
 constexpr float A4_TOP = 7.f;            // log2 of the largest p times its value scale where the head's level is set
 constexpr float A4_LAZY = 32768.f;       // how far that, or p from 1, may grow before reference and level move
 constexpr float A4_MOST = 112.f;         // log2 of the highest level: p times it stays below 2^127
+constexpr float A4_FACTOR = 1024.f;      // factors of scores above this are applied in two steps
 constexpr float A4_VALUE = 32768.f;      // 2^15: what values are held by
 constexpr uint32_t A4_NORM = 13;         // a piece's sum of p is held in [2^-13, 2^-12): 24 pieces in each of 148 parts add up to less than 1
 
@@ -190,6 +191,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
     // are short and they change from one piece to the next only
     __shared__ Cursor cursors[A4_WARPS][2];
     __shared__ uint64_t block_u0[A4_WARPS];
+    __shared__ __align__(8) float factor_rest[A4_WARPS][AD_HEADS];  // how many times A4_FACTOR the heads' factors are, 1 or more
     Cursor& cur_held = cursors[warp][0];
     Cursor& pre_held = cursors[warp][1];
     bool live;  // there is a tile to copy
@@ -357,9 +359,9 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
             return min((uint32_t)AD_HEADS, (kv_head + 1) * group - head0);
         };
         uint32_t q_high[KS][2], q_low[KS][2];
-        float factor[2];  // scale log2(e) 2^(e + 2) of the heads 2t, 2t + 1
+        float factor[2];  // scale log2(e) 2^(e + 2) of the heads 2t, 2t + 1, or A4_FACTOR where it is more
         {
-            float x[DP / 4], top = 0.f, unit = A4_VALUE / 4.f, down = 1.f;  // 2^e and 2^(13 - e)
+            float x[DP / 4], top = 0.f, unit = 1.f, down = 1.f;  // 2^e and 2^(13 - e); q of zeros has any
             uint32_t head0;
             const uint32_t heads = heads_of(cur_held.item, head0);
             load_row<DP / 4>(p.q.p, (int64_t)cur_held.b * p.q.token_stride + (int64_t)(head0 + g) * p.q.head_stride + t * (DP / 4), p.dtype,
@@ -370,7 +372,10 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
             top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
             const int e = min(max((int)(__float_as_uint(top) >> 23) - 126, -110), 126);
             if (top > 0.f && top < INFINITY) unit = __uint_as_float((uint32_t)(e + 127) << 23), down = __uint_as_float((uint32_t)(140 - e) << 23);
-            const float f = fminf(p.scale * (4.f * LOG2E) * unit, 3e38f);  // (finite: a key row of zeros has a score of 0)
+            // (times a key's row scale, 2^117 at most, what is left of it is finite: where s is 0 the score is)
+            const float all = fminf(p.scale * (4.f * LOG2E) * unit, 3e38f), f = fminf(all, A4_FACTOR);
+            if (t == 0) factor_rest[warp][g] = fmaxf(all * (1.f / A4_FACTOR), 1.f);
+            __syncwarp();
             factor[0] = __shfl_sync(0xFFFFFFFFu, f, t * 8), factor[1] = __shfl_sync(0xFFFFFFFFu, f, t * 8 + 4);
             // elements j and j + 4 of a word's eight are a pair: j = 0, 1 of one step, j = 2, 3 of the next
 #pragma unroll
@@ -445,7 +450,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                     if (!((here >> (n * 8 + k_row)) & 1u)) x[n][0] = x[n][1] = -INFINITY;
             }
             // Reference and level do as a rule: the products are made with them, and made again in the rare case that they move.
-            bool first = __any_sync(0xFFFFFFFFu, m[0] == -INFINITY || m[1] == -INFINITY);
+            bool first = __any_sync(0xFFFFFFFFu, m[0] == -INFINITY || m[1] == -INFINITY || factor[0] >= A4_FACTOR || factor[1] >= A4_FACTOR);
             for (;;) {
                 if (!first) {
                     float top = 0.f;
@@ -462,6 +467,11 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                         top = fmaxf(top, sum[h]);
                     }
                     if (!__any_sync(0xFFFFFFFFu, top > A4_LAZY)) break;
+                }
+                if (first) {  // (x is not whole yet where the factor is more than A4_FACTOR)
+                    const float2 rest = *reinterpret_cast<const float2*>(factor_rest[warp] + 2 * t);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) x[n][0] *= rest.x, x[n][1] *= rest.y;
                 }
                 bool moved = false;
 #pragma unroll

@@ -1,5 +1,5 @@
 """Attention of single tokens over 4-bit caches whose value rows are of any size: every token counts by its weight, whatever
-the sizes of the values beside it.
+the sizes of the values beside it; and queries and keys whose sizes' product passes f32.
 
 Tolerance, element by element, as test_kv_int4_gpu.py derives it, with what f16 steps may do taken from the tokens' own weights and
 rows: u |o| + 2^-15 max(1, scale sum |q k| / 13) A (2^-11 A more under 16-bit q) + n 2^-31 max_j p_j max |v_j|, A = sum_j p_j |v_j|. The
@@ -117,3 +117,23 @@ def test_sequences_of_different_sizes_in_a_batch(dtype):
     for b in range(batch):
         rows = [x[table[b].long()].transpose(1, 2).reshape(-1, d)[:n] for x in held]
         assert_near(q[b], *rows, got[b], d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("q_top,k_top", [(1e30, 1e20), (3e38, 3e38), (1e19, 1e19), (1.0, 3e38), (3e38, 1.0)])
+def test_large_keys_that_large_queries_do_not_see(q_top, k_top, dtype):
+    """Products of the sizes of q and k that pass f32, where q . k is 0: the score is 0, beside scores of a few units."""
+    d, n = 128, 70
+    q, k, v = (randn(shape, i) for i, shape in enumerate(((1, 8, d), (n, 1, d), (n, 1, d))))
+    q[..., 32:], k[..., :32] = 0, 0
+    q, k = q / q.abs().max() * q_top, k / k.abs().max() * k_top
+    if 1e3 < q_top < 1e31:  # these see q, by a few units
+        k[::3, :, :32] = randn((len(k[::3]), 1, 32), 5) / q_top
+        k[::3, :, 32:] = 0
+    q = q.to(dtype)
+    cache = c.KvCache.empty(5, 1, 16, d, I4)
+    c.kv_cache_write(cache, k.cuda(), v.cuda(), torch.arange(n, dtype=torch.int32).cuda())
+    table = torch.arange(5, dtype=torch.int32)[None]
+    got = c.attention_decode(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda())
+    held = [x.transpose(1, 2).reshape(-1, d)[:n] for x in step_ref.held4(cache)]
+    assert_near(q[0], *held, got[0], d ** -0.5, dtype)
