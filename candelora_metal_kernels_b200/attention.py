@@ -92,7 +92,8 @@ class KvCache:
     A 4-bit cache has k, v uint8 [num_pages, kv_heads, page_size, head_dim / 2] (head_dim a multiple of 32), element 2i in the
     low half of byte i, 2i + 1 in the high half, as code + 8; the scales above, and k_group, v_group
     [num_pages, kv_heads, page_size, 4] float8_e4m3fn, of which the first head_dim / 32 are the scales (not negative, no NaN) of a
-    row's groups of 32 elements: an element is code * group scale * row scale. Its scales start on 16-byte boundaries."""
+    row's groups of 32 elements: an element is code * group scale * row scale, a finite f32 number (row scales have either sign
+    and any size, those of keys up to 2^117), or NaN where the row scale is. Its scales start on 16-byte boundaries."""
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor | None = None,
                  v_scale: torch.Tensor | None = None, k_group: torch.Tensor | None = None, v_group: torch.Tensor | None = None):

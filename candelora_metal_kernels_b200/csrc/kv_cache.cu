@@ -514,7 +514,7 @@ __device__ __forceinline__ void write8(void* out, int64_t at, int out_dtype, con
             x[i] = f.x, x[4 + i] = f.y;
         }
         float s = __uint_as_float(e.w.z);
-        if (s < 5.19e33f) {  // 2^112
+        if (fabsf(s) < 5.19e33f) {  // 2^112
             s *= 32768.f;
         } else {
 #pragma unroll

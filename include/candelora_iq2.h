@@ -283,8 +283,9 @@ int iq2_matmul_grouped_sharded(iq2_comm_t comm, const iq2_matmul_problem* proble
  * in the low half of byte i, element 2i + 1 in the high half, each as its code -7..7 plus 8; and
  * k_group and v_group [num_pages, kv_heads, page_size, 4] hold the e4m3 scales (not negative, no
  * NaN) of a row's groups of 32 elements, of which the first head_dim / 32 count; all scales are
- * 16-byte aligned. An element is code * group scale * row scale. k_group and v_group are not read
- * for other types.
+ * 16-byte aligned. An element is code * group scale * row scale, a finite f32 number, or NaN where the
+ * row scale is. Row scales have either sign and any size, up to 2^117 those of keys (the write makes
+ * none above that, and none below 0). k_group and v_group are not read for other types.
  * Any page_size. Token `pos` of a sequence lies in page block_table[pos / page_size], row
  * pos % page_size. A block table is int32 [sequences, table_width] on the device; entries outside
  * [0, num_pages) are never followed: their tokens take no part in an attention and read as zeros.

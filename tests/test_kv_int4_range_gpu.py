@@ -20,15 +20,16 @@ BF16, F16, F32, I4 = torch.bfloat16, torch.float16, torch.float32, torch.uint8
 LOG2E = 1.4426950408889634
 
 
-def assert_near(q, k, v, got, scale, dtype, fine=False):
-    """q, got [heads, d] of one sequence and key head over k, v [n, d] as they are held, in 64 bits. `fine`: 22 bits of p."""
+def assert_near(q, k, v, got, scale, dtype, fine=False, lost=0.0):
+    """q, got [heads, d] of one sequence and key head over k, v [n, d] as they are held, in 64 bits. `fine`: 22 bits of p. `lost`: the
+    tokens' products that are too small, and half of the smallest number of the output's type."""
     q, got = q.double().cpu(), got.double().cpu()
     p = torch.softmax(q @ k.T * scale, -1)
     want, size = p @ v, p @ v.abs()
     part = 2.0 ** -15 * ((q.abs() @ k.abs().T * scale).amax(-1, keepdim=True) / 13).clamp(min=1)
     if dtype != F32 and not fine:
         part = part + ref.UNIT[F16]
-    floor = len(k) * 2.0 ** -31 * (p * v.abs().amax(-1)).amax(-1, keepdim=True)
+    floor = len(k) * 2.0 ** -31 * (p * v.abs().amax(-1)).amax(-1, keepdim=True) + lost
     assert torch.isfinite(got).all()
     over = (got - want).abs() - ref.UNIT[dtype] * want.abs() - part * size - floor
     assert (over <= 0).all(), (over / size.clamp(min=1e-300)).max()
@@ -137,3 +138,41 @@ def test_large_keys_that_large_queries_do_not_see(q_top, k_top, dtype):
     got = c.attention_decode(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda())
     held = [x.transpose(1, 2).reshape(-1, d)[:n] for x in step_ref.held4(cache)]
     assert_near(q[0], *held, got[0], d ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n,width", [(3, 1), (32, 2), (77, 5), (1000, 200)])
+@pytest.mark.parametrize("kind", ["either sign", "any size", "subnormal", "one of 2^120", "zero"])
+def test_row_scales_that_the_write_does_not_make(kind, n, width, dtype):
+    """Read and decode agree on every cache that the format allows: row scales below zero, of any size, no powers of two, zero under
+    codes that are not. Products below 2^-125 may be lost (a level ends at 2^112)."""
+    if dtype == F16 and kind == "one of 2^120":
+        pytest.skip("f16 outputs end at 65504")
+    d, page, pages = 64, 16, -(-n // 16)
+    gen = torch.Generator().manual_seed(n)
+    codes = [torch.randint(0, 256, (pages, 1, page, d // 2), generator=gen).to(torch.uint8) for _ in range(2)]
+    groups = [torch.randint(40, 80, (pages, 1, page, 4), generator=gen).to(torch.uint8) for _ in range(2)]
+    either = torch.randint(0, 2, (2, pages, 1, page), generator=gen) * 2.0 - 1
+    scales = either * (0.5 + torch.rand(either.shape, generator=gen)) * 0.02
+    size = torch.zeros(either.shape[1:], dtype=torch.float64)
+    if kind == "any size":
+        size = torch.randint(-140, 10 if dtype == F16 else 100, size.shape, generator=gen).double()
+    elif kind == "subnormal":
+        size -= 130
+    elif kind == "one of 2^120":
+        groups[1].view(-1, 4)[n // 2] = torch.tensor([0, 1, 2, 3])  # so that the elements stay finite
+        size.view(-1)[n // 2] = 123
+    elif kind == "zero":
+        scales[:, ::2] = 0
+    scales = [scales[0].contiguous(), (scales[1].double() * torch.exp2(size)).float()]
+    (k, v), (kg, vg), (ks, vs) = ([x.cuda() for x in t] for t in (codes, groups, scales))
+    cache = c.KvCache(k, v, ks, vs, kg.view(torch.float8_e4m3fn), vg.view(torch.float8_e4m3fn))
+    table = torch.full((1, max(width, pages)), -1, dtype=torch.int32)
+    table[0, :pages] = torch.arange(pages)
+    held = [x.transpose(1, 2).reshape(-1, d)[:n] for x in step_ref.held4(cache)]
+    assert torch.isfinite(held[1].float()).all()
+    got = c.kv_cache_read(cache, table.cuda(), torch.tensor([0, n], dtype=torch.int32).cuda(), n, dtype=F32)
+    assert all(torch.equal(g[:, 0].cpu(), h.float()) for g, h in zip(got, held))
+    q = 0.1 * randn((1, 8, d), 3, dtype)
+    got = c.attention_decode(q.cuda(), cache, table.cuda(), torch.tensor([n], dtype=torch.int32).cuda())
+    assert_near(q[0], *held, got[0], d ** -0.5, dtype, lost=n * 2.0 ** -125 + (2.0 ** -25 if dtype == F16 else 0.0))
