@@ -25,9 +25,9 @@
 //     the keys have little there), which the 2^-8 of bf16 activations hides. For f32 and f16 ones (8e-6 against 1e-6 over
 //     the whole) a byte with 0x64 above it is 1024 + code + 128, and a subtraction makes it the code itself: 51.0 instead of
 //     49.2 us for 100001 tokens.
-//   * The key scale multiplies s, the value scale w multiplies p. The reference m of a head's exponents moves when a product
-//     p w has grown by more than 2^8, so that p w keeps to the range of f16; the sum of p itself is f32 (int8 caches: held by
-//     2^-16 of itself, since p alone may reach 2^122).
+//   * The key scale multiplies s, the value scale multiplies p, and a power of two of the head keeps these products to the range of
+//     f16 (attention_decode.cuh). The reference m of a head's exponents moves when one of them, or p, has grown past 2^15 (16-bit
+//     caches: when p has grown by more than 2^8).
 // The maxima, sums, s, p and o are f32.
 //
 // Measured (8 key heads, 128 elements): 128 sequences of up to 4096 tokens, bf16 cache, 214 us: 6260 GB/s, 0.96 of the copy
@@ -45,17 +45,13 @@ namespace iq2 {
 namespace {
 
 constexpr int AD_WARPS = 8, AD_THREADS = AD_WARPS * 32, AD_STAGES = 3;
-// 2^-107, just below the smallest value scale that a row of the cache has (its largest value, 2^-100 or more, over 127). A row of
-// zeros has 0 and counts as this, so that the reference stays finite; its codes are zeros.
-constexpr float AD_MIN_SCALE = 6.16297582e-33f;
-// p times the value scale: the power of two that it has at the reference, and how far it may grow before that moves.
+// 16-bit caches: the power of two that p has at the reference, and how far it may grow before that moves.
 template <bool BF>
 constexpr float AD_TOP = BF ? 0.f : 7.f;
 template <bool BF>
 constexpr float AD_LAZY = BF ? 256.f : 32768.f;
 template <bool BF>
 constexpr float AD_LOW = BF ? 1.f : 2048.f;      // what low pieces are held times
-constexpr float AD_SUM = 1.f / 65536.f;          // int8 caches: what the sums of p, and with them o, are held times
 constexpr uint32_t CODE_ZERO = 0x00800080u;      // two codes of 0 as f16: 128 2^-24
 constexpr float CODE_UNIT = 16777216.f;          // 2^24
 enum CacheKind { CK_F16, CK_BF16, CK_INT8 };
@@ -283,7 +279,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         for (int j = 0; j < 4; ++j) minus[j] = -minus[j];
         auto joined = [](float high, float low) { return fmaf(low, 1.f / AD_LOW<BF>, high); };
         const float factor = q_factor[g];
-        float o[NT][4], o_off[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f;
+        float o[NT][4], o_off[4] = {0.f, 0.f, 0.f, 0.f}, m = -INFINITY, l = 0.f, f = power_of_two(AD_MOST);  // (int8 caches: f)
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
@@ -333,8 +329,8 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                 }
             }
 
-            // x = log2(e) scale q . k, this thread's tokens 8 n + 2 t, + 1 of head g; w = 2^(x - m) times the value scale
-            float x[ST][2], e[ST][2], w[ST][2], vs[ST][2];
+            // x = log2(e) scale q . k, this thread's tokens 8 n + 2 t, + 1 of head g; w = 2^(x - m), times f and the value scale
+            float x[ST][2], e[ST][2], w[ST][2], vs[ST][2], sum;
             const float2* const scales = reinterpret_cast<const float2*>(ring + stage * S::STAGE + 2 * TOK * S::ROW) + t;
 #pragma unroll
             for (int n = 0; n < ST; ++n) {
@@ -342,7 +338,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
                 if (I8) {
                     const float2 sk = scales[n * 4], sv = scales[TOK / 2 + n * 4];
                     ks2 = make_float2(sk.x * factor, sk.y * factor);
-                    vs2 = make_float2(max_nan(sv.x, AD_MIN_SCALE), max_nan(sv.y, AD_MIN_SCALE));
+                    vs2 = sv;
                 }
                 x[n][0] = joined(s[n][0], s[n][2]) * ks2.x, x[n][1] = joined(s[n][1], s[n][3]) * ks2.y;
                 vs[n][0] = vs2.x, vs[n][1] = vs2.y;
@@ -356,43 +352,53 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             }
             // The reference does as a rule: the products are made with it, and made again in the rare case that it moves.
             for (;;) {
-                const float base = m == -INFINITY ? 0.f : m - AD_TOP<BF>;
+                const float base = m == -INFINITY ? 0.f : I8 ? m : m - AD_TOP<BF>;
                 float top = 0.f;
+                sum = 0.f;
 #pragma unroll
                 for (int n = 0; n < ST; ++n)
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         e[n][j] = exp2_approx(x[n][j] - base);
-                        w[n][j] = I8 ? e[n][j] * vs[n][j] : e[n][j];
-                        top = fmaxf(top, w[n][j]);
+                        w[n][j] = I8 ? e[n][j] * f * vs[n][j] : e[n][j];
+                        top = fmaxf(top, I8 ? fabsf(w[n][j]) : w[n][j]);
+                        if (I8) sum += e[n][j];
                     }
-                if (!__any_sync(0xFFFFFFFFu, top > AD_LAZY<BF> || m == -INFINITY)) break;
-                // the largest x + log2(value scale) of the head's tokens
-                float most = -INFINITY;
+                if (I8) top = fmaxf(top, sum);
+                if (!__any_sync(0xFFFFFFFFu, top > (I8 ? AD_SCALED_LAZY : AD_LAZY<BF>) || m == -INFINITY)) break;
+                // the largest x of the head's tokens, and the largest x + log2 |value scale|
+                float most = -INFINITY, weighed = -INFINITY;
 #pragma unroll
                 for (int n = 0; n < ST; ++n)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) most = fmaxf(most, I8 ? x[n][j] + __log2f(vs[n][j]) : x[n][j]);
-                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 1));
-                most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, 2));
+                    for (int j = 0; j < 2; ++j) {
+                        most = fmaxf(most, x[n][j]);
+                        if (I8) weighed = fmaxf(weighed, x[n][j] + __log2f(fabsf(vs[n][j])));
+                    }
+#pragma unroll
+                for (int b = 1; b < 4; b *= 2) {
+                    most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, b));
+                    if (I8) weighed = fmaxf(weighed, __shfl_xor_sync(0xFFFFFFFFu, weighed, b));
+                }
                 const float next = fmaxf(m, most), keep = m == -INFINITY ? 0.f : exp2_approx(m - next);
-                const bool moved = next > m;
-                if (!__any_sync(0xFFFFFFFFu, moved)) break;
-                if (moved) {
-                    m = next;
-                    l *= keep;
+                const Moved to = I8 ? Moved::from(m, f, most, weighed) : Moved{next, f, keep, keep, next > m};
+                if (!__any_sync(0xFFFFFFFFu, to.moved)) break;
+                if (to.moved) {
+                    m = to.m, f = to.f;
+                    l *= to.keep;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) o[n][j] *= keep;
+                        for (int j = 0; j < 4; ++j) o[n][j] *= to.keep_o;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o_off[j] *= keep;
+                    for (int j = 0; j < 4; ++j) o_off[j] *= to.keep_o;
                 }
             }
+            if (I8) l += sum;
             uint32_t pa[TOK / 16][4], pa3[TOK / 16][4];
 #pragma unroll
             for (int n = 0; n < ST; ++n) {
-                l = fmaf(e[n][0] + e[n][1], I8 ? AD_SUM : 1.f, l);
+                if (!I8) l += e[n][0] + e[n][1];
                 const uint32_t high = pack_pair<BF>(w[n][0], w[n][1]);
                 const float2 h = unpack_pair<BF>(high);
                 const uint32_t low = pack_pair<BF>((w[n][0] - h.x) * AD_LOW<BF>, (w[n][1] - h.y) * AD_LOW<BF>);
@@ -437,14 +443,16 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
             __syncwarp();
             stage = stage == AD_STAGES - 1 ? 0 : stage + 1;
         }
-        if (I8) {  // the 128s off, and the codes' unit and the sums' on
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
+        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
+        if (I8) {  // the 128s and the level off, and the codes' unit on
+            const Leveled piece = Leveled::of(l, f, SHIFTED ? CODE_UNIT : 1.f);
+            m += piece.k, l = piece.l;
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) o[n][j] = SHIFTED ? (o[n][j] - o_off[j]) * (CODE_UNIT * AD_SUM) : o[n][j] * AD_SUM;
+                for (int j = 0; j < 4; ++j) o[n][j] = (SHIFTED ? o[n][j] - o_off[j] : o[n][j]) * piece.down * piece.off;
         }
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 1);
-        l += __shfl_xor_sync(0xFFFFFFFFu, l, 2);
 
         Cursor next = cur;
         next.next(p, items);

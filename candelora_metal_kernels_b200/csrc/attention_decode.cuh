@@ -101,6 +101,42 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
+// 2^x of an integer x in -126..127, its logarithm, and one over it.
+__device__ __forceinline__ float power_of_two(float x) { return __uint_as_float((uint32_t)((int)x + 127) << 23); }
+__device__ __forceinline__ float log2_of_power(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
+__device__ __forceinline__ float over_power(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+
+// ---- values with row scales (int8 and 4-bit caches) ----
+// Next to the largest score, held as a whole number m, a token has p = 2^(x - m), and l is the sum of these whatever the values
+// are. What f16 pieces are taken of, and o with it, is w = p |value scale| 2^level, a head's own power of two f that makes the largest
+// of them 2^7 to 2^8. m and f do as a rule, and move where a w, or a sum of p, has grown past AD_SCALED_LAZY.
+constexpr float AD_SCALED_TOP = 7.f, AD_SCALED_LAZY = 32768.f;
+constexpr float AD_MOST = 112.f;  // the highest level: p times it stays below 2^127
+struct Moved {
+    float m, f, keep, keep_o;  // and what l and o are taken times
+    bool moved;
+    // most: the largest x of the tokens to come, weighed: the largest x + log2 |value scale|.
+    static __device__ __forceinline__ Moved from(float m, float f, float most, float weighed) {
+        // (the level never makes o larger than it is; nothing yet: `up` is infinite)
+        const float next = fmaxf(m, ceilf(most)), level = log2_of_power(f), up = next - m;
+        const float to = fmaxf(fminf(fminf(ceilf(AD_SCALED_TOP - (weighed - next)), level + up), AD_MOST), -126.f);
+        const bool none = m == -INFINITY;
+        return {next, power_of_two(to), none ? 0.f : exp2_approx(-up), none ? 0.f : exp2_approx(to - level - up), next > m || to != level};
+    }
+};
+// (o, m, l) as others add it up: the level goes, or values of any size would not meet in one sum. l = 2^k l' with l' in [2^-13, 2^-12),
+// so that 24 of these in each of 148 parts add up to less than 1; o' = o / 2^(level + k), about the output times l'; and m + k.
+struct Leveled {
+    float k, l, down, off;  // o' = o * down * off
+    // unit: what o is held by.
+    static __device__ __forceinline__ Leveled of(float l, float f, float unit) {
+        constexpr uint32_t NORM = 13;
+        const uint32_t e = min(max(__float_as_uint(l) >> 23, 100u), 240u);
+        const float down = __uint_as_float((254u - NORM - e) << 23);
+        return {(float)e - (127.f - NORM), l * down, down * unit, over_power(f)};
+    }
+};
+
 // The line of work from one unit on: the item it is in and the tokens [t0, t1) of that item in the part. The line's units are UNIT
 // tokens; an item's first COST units have no tokens, and a part that ends inside them has none (the next part has the item).
 // EVEN: parts differ by a unit at most, of one unit at least, so that none is empty but behind the line's end (the parts of an item

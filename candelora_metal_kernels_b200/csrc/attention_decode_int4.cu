@@ -41,12 +41,8 @@ constexpr int A4_WARPS = 12, A4_THREADS = A4_WARPS * 32;
 static_assert(2 * A4_WARPS <= 32, "a lane a piece");
 constexpr int A4_TOK = 32, A4_NT = A4_TOK / 8;  // tokens of a warp's stage, and eights of them
 constexpr int A4_RUN = 8;                // tokens that lie side by side in a page of a multiple of these
-constexpr float A4_TOP = 7.f;            // log2 of the largest p times its value scale where the head's level is set
-constexpr float A4_LAZY = 32768.f;       // how far that, or p from 1, may grow before reference and level move
-constexpr float A4_MOST = 112.f;         // log2 of the highest level: p times it stays below 2^127
 constexpr float A4_FACTOR = 1024.f;      // factors of scores above this are applied in two steps
 constexpr float A4_VALUE = 32768.f;      // 2^15: what values are held by
-constexpr uint32_t A4_NORM = 13;         // a piece's sum of p is held in [2^-13, 2^-12): 24 pieces in each of 148 parts add up to less than 1
 
 template <int DP>
 struct Shape4 {
@@ -106,11 +102,6 @@ __device__ __forceinline__ uint32_t ld_shared(uint32_t addr) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
     return v;
 }
-
-// 2^x of an integer x in -126..127, its logarithm, and one over it.
-__device__ __forceinline__ float power_of_two(float x) { return __uint_as_float((uint32_t)((int)x + 127) << 23); }
-__device__ __forceinline__ float log2_of_power(float x) { return (float)((int)(__float_as_uint(x) >> 23) - 127); }
-__device__ __forceinline__ float over_power(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
 // N consecutive elements of a row of q as f32, zeros unless `there`; `vec`: rows start on 16-byte boundaries.
 template <int N>
@@ -390,7 +381,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 }
         }
         // o is held times 2^level of the head, f = 2^level
-        float o[MT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, f[2] = {power_of_two(A4_MOST), power_of_two(A4_MOST)};
+        float o[MT][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, f[2] = {power_of_two(AD_MOST), power_of_two(AD_MOST)};
 #pragma unroll
         for (int n = 0; n < MT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 
@@ -466,7 +457,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                         sum[h] = (e[0][h] + e[1][h]) + (e[2][h] + e[3][h]);
                         top = fmaxf(top, sum[h]);
                     }
-                    if (!__any_sync(0xFFFFFFFFu, top > A4_LAZY)) break;
+                    if (!__any_sync(0xFFFFFFFFu, top > AD_SCALED_LAZY)) break;
                 }
                 if (first) {  // (x is not whole yet where the factor is more than A4_FACTOR)
                     const float2 rest = *reinterpret_cast<const float2*>(factor_rest[warp] + 2 * t);
@@ -485,16 +476,12 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                         most = fmaxf(most, __shfl_xor_sync(0xFFFFFFFFu, most, b));
                         weighed = fmaxf(weighed, __shfl_xor_sync(0xFFFFFFFFu, weighed, b));
                     }
-                    // the level takes the tile's largest w to 2^A4_TOP, but never makes o larger than it is
-                    // (whole numbers, so that what is there is taken times powers of two; nothing yet: `up` is infinite)
-                    const float next = fmaxf(m[h], ceilf(most)), level = log2_of_power(f[h]), up = next - m[h];
-                    const float to = fmaxf(fminf(fminf(ceilf(A4_TOP - (weighed - next)), level + up), A4_MOST), -126.f);
-                    const float keep = m[h] == -INFINITY ? 0.f : exp2_approx(-up), keep_o = m[h] == -INFINITY ? 0.f : exp2_approx(to - level - up);
-                    moved = moved || next > m[h] || to != level;
-                    m[h] = next, f[h] = power_of_two(to);
-                    l[h] *= keep;
+                    const Moved to = Moved::from(m[h], f[h], most, weighed);
+                    moved = moved || to.moved;
+                    m[h] = to.m, f[h] = to.f;
+                    l[h] *= to.keep;
 #pragma unroll
-                    for (int n = 0; n < MT; ++n) o[n][h] *= keep_o, o[n][2 + h] *= keep_o;
+                    for (int n = 0; n < MT; ++n) o[n][h] *= to.keep_o, o[n][2 + h] *= to.keep_o;
                 }
                 if (!__any_sync(0xFFFFFFFFu, moved) && !first) break;
                 first = false;
@@ -574,18 +561,15 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 cp_async_wait<0>();
                 __syncwarp();
             }
-            // Its level goes, or values of any size would not meet in one sum: l = 2^k l' with l' in [2^-13, 2^-12), o' = o / 2^(level + k)
-            // is about the output times l', and the reference m + k.
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t k = min(max(__float_as_uint(l[h]) >> 23, 100u), 240u);  // + 127 - A4_NORM
-                const float down = __uint_as_float((254u - A4_NORM - k) << 23), off = over_power(f[h]);
-                auto value = [&](float x) { return x * (down * A4_VALUE) * off; };
+                const Leveled piece = Leveled::of(l[h], f[h], A4_VALUE);
+                auto value = [&](float x) { return x * piece.down * piece.off; };
 #pragma unroll
                 for (int j = 0; j < DP / 32; ++j)
                     *reinterpret_cast<float4*>(slot + (2 * t + h) * S::HEAD + g * (DP / 8) + j * 4) =
                         make_float4(value(o[2 * j][h]), value(o[2 * j][2 + h]), value(o[2 * j + 1][h]), value(o[2 * j + 1][2 + h]));
-                if (g == 0) slot[S::MAXIMA + 2 * t + h] = m[h] + ((float)k - (127.f - A4_NORM)), slot[S::SUMS + 2 * t + h] = l[h] * down;
+                if (g == 0) slot[S::MAXIMA + 2 * t + h] = m[h] + piece.k, slot[S::SUMS + 2 * t + h] = piece.l;
             }
             if (lane == 0)
                 pieces[warp * 2 + !first_piece] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.unit - cur.k <= block_u0[warp] ? 8u : 0u)};
