@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
     typename Cursor::Parts line;
     Cursor cur = Cursor::of_part(a, blockIdx.x, gridDim.x, a.inv_blocks, threadIdx.x, AD_THREADS, line);
     const uint64_t u0 = line.begin(blockIdx.x);
-    if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, blockIdx.x, 1);
+    if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, blockIdx.x, blockIdx.x, 1);
     if (cur.t0 == cur.t1) return;  // nothing, or nothing but an item's start
     Cursor pre = cur;
 
@@ -488,7 +488,7 @@ __global__ void __launch_bounds__(AD_THREADS, 1)
         __syncthreads();
         {
             const bool whole = cur.whole();
-            float* const part = a.parts + ((uint64_t)blockIdx.x * 2 + (cur.unit == u0 ? 0 : 1)) * S::PART;
+            float* const part = a.parts + ((uint64_t)blockIdx.x * 2 + (cur.first_of(u0) ? 0 : 1)) * S::PART;
             const uint32_t h = warp;  // a warp a head
             float mx = -INFINITY, w[4], sum = 0.f;
 #pragma unroll

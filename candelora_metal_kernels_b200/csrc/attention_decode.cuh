@@ -18,6 +18,7 @@ constexpr uint32_t AD_ITEM_COST = 3;
 constexpr uint32_t AD_I4_UNIT = 32;  // tokens that the line of work is cut at for 4-bit caches: a warp's tile
 // Measured with 0 / 1 / 2 / 4: 128 x 4096 tokens 94.7 / 92.9 / 93.7 / 95.3 us, 1 x 333 11.4 / 9.4 / 10.8 / 11.2 us.
 constexpr uint32_t AD_I4_ITEM_COST = 1;
+constexpr int AD_I4_WARPS = 12;  // of a block for 4-bit caches, each with a part of its own
 constexpr float LOG2E = 1.44269504f;
 
 // What join_kernel's block of the same number has to join: the parts of blocks c0 to c1 of one item, block c0's being its
@@ -47,9 +48,14 @@ inline DecodeArgs decode_args(const DecodeParams& p, void* workspace, int num_sm
             false};
 }
 
-__device__ __forceinline__ uint32_t seq_len(const DecodeParams& p, uint32_t b) {
+__host__ __device__ __forceinline__ uint32_t seq_len(const DecodeParams& p, uint32_t b) {
     const uint64_t most = min((uint64_t)p.table_width * p.c.page_size, (uint64_t)0x7FFFFFFF);
-    return (uint32_t)min((uint64_t)max(__ldg(p.seq_lens + b), 0), most);
+#ifdef __CUDA_ARCH__
+    const int32_t len = __ldg(p.seq_lens + b);
+#else
+    const int32_t len = p.seq_lens[b];
+#endif
+    return (uint32_t)min((uint64_t)max(len, 0), most);
 }
 
 __device__ __forceinline__ float load_elem(const void* p, int64_t i, int dtype) {
@@ -140,21 +146,22 @@ struct Leveled {
 // The line of work from one unit on: the item it is in and the tokens [t0, t1) of that item in the part. The line's units are UNIT
 // tokens; an item's first COST units have no tokens, and a part that ends inside them has none (the next part has the item).
 // EVEN: parts differ by a unit at most, of one unit at least, so that none is empty but behind the line's end (the parts of an item
-// follow one another); otherwise all but the last ones are of the same length, rounded up.
+// follow one another); otherwise all but the last ones are of the same length, rounded up. What deals the work is callable on the
+// host too, for tests without a GPU.
 template <uint32_t UNIT, uint32_t COST, bool EVEN>
 struct Cursor {
     uint64_t unit, end;
     uint32_t b, item, len, units;  // the sequence, its item (key head, group of query heads), tokens and units an item
     uint32_t k, n;                 // first unit of the item in the part, and how many
     uint32_t t0, t1;
-    __device__ __forceinline__ void cut() {
+    __host__ __device__ __forceinline__ void cut() {
         n = (uint32_t)min((uint64_t)(units - k), end - unit);
         t0 = (max(k, COST) - COST) * UNIT, t1 = min((max(k + n, COST) - COST) * UNIT, len);
     }
-    static __device__ __forceinline__ uint32_t units_of(uint32_t len_) { return len_ == 0 ? 0 : (len_ + UNIT - 1) / UNIT + COST; }
-    __device__ __forceinline__ bool done() const { return unit >= end; }
-    __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == len; }
-    __device__ __forceinline__ void next(const DecodeParams& p, uint32_t items) {
+    static __host__ __device__ __forceinline__ uint32_t units_of(uint32_t len_) { return len_ == 0 ? 0 : (len_ + UNIT - 1) / UNIT + COST; }
+    __host__ __device__ __forceinline__ bool done() const { return unit >= end; }
+    __host__ __device__ __forceinline__ bool whole() const { return t0 == 0 && t1 == len; }
+    __host__ __device__ __forceinline__ void next(const DecodeParams& p, uint32_t items) {
         unit += n;
         k = 0;
         if (done()) return;
@@ -178,11 +185,31 @@ struct Cursor {
         uint64_t units, each;  // of the line; of a part
         uint32_t parts;
         double share;          // units / parts
-        __device__ __forceinline__ uint64_t begin(uint32_t part) const {
+        __host__ __device__ __forceinline__ uint64_t begin(uint32_t part) const {
             if (EVEN) return part >= parts ? units : min((uint64_t)(part * share), units);
             return min(part * each, units);
         }
+        static __host__ __device__ __forceinline__ Parts of(uint64_t units, uint32_t parts, double inv_parts) {
+            Parts line{units, 0, parts, EVEN ? max((double)units * inv_parts, 1.0) : (double)units * inv_parts};
+            if (!EVEN) {
+                line.each = (uint64_t)line.share;  // units / parts, rounded up
+                while (line.each * parts < units) ++line.each;
+            }
+            return line;
+        }
     };
+    // The part [u0, u1) of the line, which begins in sequence b_ of len_ tokens and own units an item, `before` units into the line.
+    static __host__ __device__ __forceinline__ Cursor at(uint64_t u0, uint64_t u1, uint32_t b_, uint32_t len_, uint32_t own, uint64_t before) {
+        Cursor cur{};
+        cur.b = b_, cur.len = len_, cur.units = own;
+        const uint32_t rest = (uint32_t)(u0 - before);
+        cur.item = rest / own, cur.k = rest % own;
+        cur.unit = u0, cur.end = u1;
+        cur.cut();
+        return cur;
+    }
+    // Whether the item is the first one of the block whose first unit is u0: its part of it is the block's number 0, others number 1.
+    __host__ __device__ __forceinline__ bool first_of(uint64_t u0) const { return unit - k <= u0; }
     // Part `part` of `parts` as a cursor (done at once where there is nothing). A warp works it out by itself, from the lengths.
     // Sequences of length 0 get their zeros here, a part a sequence, from the `threads` threads that take the part.
     static __device__ __forceinline__ Cursor of_part(const DecodeArgs& a, uint32_t part, uint32_t parts, double inv_parts, uint32_t thread,
@@ -207,11 +234,7 @@ struct Cursor {
 #pragma unroll
         for (int o = 16; o > 0; o /= 2) units += __shfl_xor_sync(0xFFFFFFFFu, units, o);
         units *= items;
-        line = {units, 0, parts, EVEN ? max((double)units * inv_parts, 1.0) : (double)units * inv_parts};
-        if (!EVEN) {
-            line.each = (uint64_t)line.share;  // units / parts, rounded up
-            while (line.each * parts < units) ++line.each;
-        }
+        line = Parts::of(units, parts, inv_parts);
         const uint64_t u0 = line.begin(part), u1 = line.begin(part + 1);
         Cursor cur{};
         if (u0 < u1) {
@@ -228,13 +251,9 @@ struct Cursor {
                 }
                 const uint32_t hit = __ballot_sync(0xFFFFFFFFu, before + upto > u0);
                 if (hit != 0) {
-                    const int at = __ffs(hit) - 1;
-                    cur.b = b0 + at;
-                    cur.len = __shfl_sync(0xFFFFFFFFu, len, at), cur.units = __shfl_sync(0xFFFFFFFFu, own, at);
-                    const uint32_t rest = (uint32_t)(u0 - before - __shfl_sync(0xFFFFFFFFu, upto - (uint64_t)own * items, at));
-                    cur.item = rest / cur.units, cur.k = rest % cur.units;
-                    cur.unit = u0, cur.end = u1;
-                    cur.cut();
+                    const int lane_of = __ffs(hit) - 1;
+                    cur = at(u0, u1, b0 + lane_of, __shfl_sync(0xFFFFFFFFu, len, lane_of), __shfl_sync(0xFFFFFFFFu, own, lane_of),
+                             before + __shfl_sync(0xFFFFFFFFu, upto - (uint64_t)own * items, lane_of));
                     break;
                 }
                 before += __shfl_sync(0xFFFFFFFFu, upto, 31);
@@ -243,14 +262,14 @@ struct Cursor {
         return cur;
     }
 
-    // What the block has to join whose part, `per_block` ones of the line from `part` on, begins with this cursor.
-    __device__ __forceinline__ JoinRecord record(const Parts& line, uint32_t part, uint32_t per_block) const {
+    // What block `block` has to join, whose part, `per_block` ones of the line from `part` on, begins with this cursor.
+    __host__ __device__ __forceinline__ JoinRecord record(const Parts& line, uint32_t block, uint32_t part, uint32_t per_block) const {
         // the first block whose part begins inside an item's tokens joins it: the block before it has the first of them
-        JoinRecord r{b, item, blockIdx.x - 1, 0, 0};
+        JoinRecord r{b, item, block - 1, 0, 0};
         if (t0 == 0) return r;
         const uint64_t unit0 = unit - k, before = line.begin(part - per_block);
         if (before <= unit0 + COST) {
-            r.c1 = blockIdx.x, r.slot = before >= unit0 ? 0 : 1;
+            r.c1 = block, r.slot = before >= unit0 ? 0 : 1;
             while (line.begin((r.c1 + 1) * per_block) < unit0 + units) ++r.c1;
         }
         return r;

@@ -37,7 +37,7 @@ namespace iq2 {
 
 namespace {
 
-constexpr int A4_WARPS = 12, A4_THREADS = A4_WARPS * 32;
+constexpr int A4_WARPS = AD_I4_WARPS, A4_THREADS = A4_WARPS * 32;
 static_assert(2 * A4_WARPS <= 32, "a lane a piece");
 constexpr int A4_TOK = 32, A4_NT = A4_TOK / 8;  // tokens of a warp's stage, and eights of them
 constexpr int A4_RUN = 8;                // tokens that lie side by side in a page of a multiple of these
@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
         typename Cursor::Parts line;
         const uint32_t part0 = blockIdx.x * A4_WARPS;  // the block's parts of the line, one a warp
         Cursor cur = Cursor::of_part(a, part0 + warp, gridDim.x * A4_WARPS, a.inv_blocks * (1.0 / A4_WARPS), lane, 32, line);
-        if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, part0, A4_WARPS);
+        if (threadIdx.x == 0) a.records[blockIdx.x] = cur.record(line, blockIdx.x, part0, A4_WARPS);
         if (cur.t0 == cur.t1) cur.unit = cur.end;  // nothing, or nothing but an item's start
         if (lane == 0) cur_held = cur, pre_held = cur, block_u0[warp] = line.begin(part0);
         live = !cur.done(), pre_tok = cur.t0, pre_t1 = cur.t1;
@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_con
                 if (g == 0) slot[S::MAXIMA + 2 * t + h] = m[h] + piece.k, slot[S::SUMS + 2 * t + h] = piece.l;
             }
             if (lane == 0)
-                pieces[warp * 2 + !first_piece] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.unit - cur.k <= block_u0[warp] ? 8u : 0u)};
+                pieces[warp * 2 + !first_piece] = {cur.b, cur.item, 1u | (cur.t0 == 0 ? 2u : 0u) | (cur.t1 == cur.len ? 4u : 0u) | (cur.first_of(block_u0[warp]) ? 8u : 0u)};
         }
         first_piece = false;
     }
