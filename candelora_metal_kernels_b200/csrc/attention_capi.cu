@@ -129,8 +129,8 @@ static int cache_write(const char* op, const iq2_kv_cache* cache, const iq2_kv_t
     p.slots = t->slots, p.positions = t->positions, p.cos = rope ? t->cos : nullptr, p.sin = t->sin, p.q_out = t->q_out;
     p.tokens = t->tokens, p.q_heads = has_q ? t->q_heads : 0, p.rope_len = t->rope_len;
     p.dtype = t->dtype, p.q_out_dtype = t->q_out_dtype, p.interleaved = t->interleaved != 0;
-    p.vec = rows_aligned(t->k, e, 16) && rows_aligned(t->v, e, 16) && (!has_q || rows_aligned(t->q, e, 16)) &&
-            (!rope || (reinterpret_cast<uintptr_t>(t->cos) % 16 == 0 && reinterpret_cast<uintptr_t>(t->sin) % 16 == 0));
+    p.vec_rows = rows_aligned(t->k, e, 16) && rows_aligned(t->v, e, 16) && (!has_q || rows_aligned(t->q, e, 16));
+    p.vec = p.vec_rows && (!rope || (reinterpret_cast<uintptr_t>(t->cos) % 16 == 0 && reinterpret_cast<uintptr_t>(t->sin) % 16 == 0));
     if (norm) {
         p.q_norm = norms->q_norm, p.k_norm = norms->k_norm;
         p.q_norm_stride = norms->q_per_head ? cache->head_dim : 0, p.k_norm_stride = norms->k_per_head ? cache->head_dim : 0;

@@ -53,13 +53,13 @@ struct KvWriteParams {
     uint32_t tokens, q_heads, rope_len;
     int dtype, q_out_dtype;
     bool interleaved;
-    bool vec;  // every row of the inputs, tables and norm weights starts on a 16-byte boundary
+    bool vec, vec_rows;  // every row of the inputs, tables and norm weights starts on a 16-byte boundary; of the inputs
     const float *q_norm, *k_norm;                 // weights of the heads' norms, null: none
     uint32_t q_norm_stride, k_norm_stride;        // from one head's weights to the next's: 0 or d
     double eps, inv_d;                            // inv_d: 1 / d
     Divisor by_heads, by_page;  // set by the launch: heads of a token (q, k and v), tokens of a page
-    Divisor by_q, by_kv;        // (with norms or a 4-bit cache) heads of q and of k, and blocks that have rows of them
-    uint32_t blocks_q, blocks_kv;
+    Divisor by_q, by_kv;        // heads of q and of k,
+    uint32_t blocks_q, blocks_kv;  // and blocks that have rows of them
 };
 cudaError_t launch_kv_write(const KvWriteParams& p, cudaStream_t stream);
 

@@ -69,14 +69,11 @@ __device__ __forceinline__ void load_angles(const float* p, bool vec, float (&x)
     if (!vec) {
 #pragma unroll
         for (int i = 0; i < N; ++i) x[i] = __ldg(p + i);
-    } else if (N == 2) {
-        const float2 f = __ldg(reinterpret_cast<const float2*>(p));
-        x[0] = f.x, x[1] = f.y;
     } else {
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
             const float4 f = __ldg(reinterpret_cast<const float4*>(p + i));
-            x[i] = f.x, x[i + 1] = f.y, x[(i + 2) % N] = f.z, x[(i + 3) % N] = f.w;
+            x[i] = f.x, x[(i + 1) % N] = f.y, x[(i + 2) % N] = f.z, x[(i + 3) % N] = f.w;
         }
     }
 }
@@ -124,13 +121,14 @@ __device__ __forceinline__ uint32_t codes4(const float* x, float inv) {
     return prmt(prmt(code(x[0]), code(x[1]), 0x0040u), prmt(code(x[2]), code(x[3]), 0x0040u), 0x5410u);
 }
 
+// ---- write of rows or tables off the 16-byte boundaries, without norms, into 16-bit and int8 caches ----
 // LANES threads (a power of two >= d / 2V) take a row: lane l holds the V elements from Vl of each half, 16 bytes of the input,
 // so that a pair of either rotation is in one thread and a row's maximum takes log2(LANES) shuffles. Rows are (token, head)
-// with the heads of q, then k, then v. A thread has one row (two or three in flight: 2048 tokens 16.5 / 18.5 against 14.5 us);
-// instructions bind next to HBM, so that divisions are products, codes are rounded by an addition, and the input's type is
-// the kernel's (widened as it came, in pieces of eight bytes, bf16 rows of 8800 tokens took 61.5 us into a bf16 cache, not 43.6).
-// Blocks of an SM: eight for f32 rows (8800 tokens into a bf16 cache 54.0 us; with all the registers that the compiler likes
-// 58.8), six for the 16 values of a thread that 16-bit rows make (43.6 us; five 45.0, seven 44.9, with spills).
+// with the heads of q, then k, then v. What is loaded element by element then lies close together: 2048 tokens from f32 into a bf16
+// cache take 15.9 us, 8800 61.2, where the kernel below takes 20.9 and 80.1 (from bf16 14.3 and 53.9 against 14.6 and 55.8). For
+// rows on the boundaries that one is the faster, 10.8 and 51.5 us against 12.1 and 58.0 (from bf16 9.4 and 43.0 against 10.5 and 48.4).
+// Blocks of an SM: eight for f32 rows (8 / 7 / 6 with element loads alone: 65.7 / 66.4 / 76.1 us for 8800 tokens), six for the 16 values
+// of a thread that 16-bit rows make (6 / 5: 52.1 / 57.1).
 template <int LANES, int IN>
 __global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kernel(const __grid_constant__ KvWriteParams p, uint32_t token0, uint32_t rows) {
     constexpr int V = IN == kF32 ? 4 : 8;
@@ -145,7 +143,7 @@ __global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kerne
     if (active) {
         const RowsView& in = is_q ? p.q : is_v ? p.v : p.k;
         const int64_t at = (int64_t)t * in.token_stride + (int64_t)h * in.head_stride + lane * V;
-        const uint4 wa = load16<IN>(in.p, at, p.vec), wb = load16<IN>(in.p, at + half, p.vec);
+        const uint4 wa = load16<IN>(in.p, at, p.vec_rows), wb = load16<IN>(in.p, at + half, p.vec_rows);
         if (!is_q) slot = __ldg(p.slots + t);
         const bool rotated = p.cos != nullptr && !is_v;
         const int64_t row = rotated ? (int64_t)min((uint32_t)max(__ldg(p.positions + t), 0), p.rope_len - 1) * half : 0;
@@ -154,14 +152,14 @@ __global__ void __launch_bounds__(KW_THREADS, IN == kF32 ? 8 : 6) kv_write_kerne
         } else if (p.interleaved) {
             const int64_t i0 = row + lane * (V / 2), i1 = i0 + half / 2;
             float c0[V / 2], s0[V / 2], c1[V / 2], s1[V / 2];
-            load_angles(p.cos + i0, p.vec, c0), load_angles(p.sin + i0, p.vec, s0);
-            load_angles(p.cos + i1, p.vec, c1), load_angles(p.sin + i1, p.vec, s1);
+            load_angles(p.cos + i0, false, c0), load_angles(p.sin + i0, false, s0);
+            load_angles(p.cos + i1, false, c1), load_angles(p.sin + i1, false, s1);
             widen<IN>(wa, a), widen<IN>(wb, b);
 #pragma unroll
             for (int i = 0; i < V / 2; ++i) rotate(a[2 * i], a[2 * i + 1], c0[i], s0[i]), rotate(b[2 * i], b[2 * i + 1], c1[i], s1[i]);
         } else {
             float c[V], s[V];
-            load_angles(p.cos + row + lane * V, p.vec, c), load_angles(p.sin + row + lane * V, p.vec, s);
+            load_angles(p.cos + row + lane * V, false, c), load_angles(p.sin + row + lane * V, false, s);
             widen<IN>(wa, a), widen<IN>(wb, b);
 #pragma unroll
             for (int i = 0; i < V; ++i) rotate(a[i], b[i], c[i], s[i]);
@@ -230,7 +228,7 @@ cudaError_t launch_write_of(const KvWriteParams& p, cudaStream_t stream) {
     return launch_write<MOST / 4, IN>(p, stream);
 }
 
-// ---- write with norms, and into 4-bit caches ----
+// ---- write: with norms, into 4-bit caches, and of rows on the 16-byte boundaries ----
 // As above, but a thread has eight elements of each half whatever the input's type (fewer threads share a row's sums, maxima and
 // addresses), a block has rows of one of q, k and v, and rows off the 16-byte boundaries are a kernel of their own (their
 // loads element by element are predicated away in one that has both, but issued all the same: 28 instead of 12 loads a warp; all
@@ -461,7 +459,11 @@ cudaError_t launch_write_rows_of(const KvWriteParams& p, cudaStream_t stream) {
 template <int IN, bool VEC>
 cudaError_t launch_write_rows_by(const KvWriteParams& p, cudaStream_t stream) {
     const bool norm = p.q_norm != nullptr || p.k_norm != nullptr;
-    if (p.c.dtype != kInt4) return launch_write_rows_of<IN, true, false, VEC>(p, stream);
+    if (p.c.dtype != kInt4) {
+        if (norm) return launch_write_rows_of<IN, true, false, VEC>(p, stream);
+        if constexpr (VEC) return launch_write_rows_of<IN, false, false, true>(p, stream);
+        else return launch_write_of<IN>(p, stream);
+    }
     return norm ? launch_write_rows_of<IN, true, true, VEC>(p, stream) : launch_write_rows_of<IN, false, true, VEC>(p, stream);
 }
 
@@ -604,14 +606,10 @@ cudaError_t launch_read(const KvReadParams& p, cudaStream_t stream) {
 cudaError_t launch_kv_write(const KvWriteParams& params, cudaStream_t stream) {
     KvWriteParams p = params;
     p.by_heads = Divisor::of(p.q_heads + 2 * p.c.heads), p.by_page = Divisor::of(p.c.page_size);
-    if (p.c.dtype == kInt4 || p.q_norm != nullptr || p.k_norm != nullptr) {
-        p.by_q = Divisor::of(std::max(p.q_heads, 1u)), p.by_kv = Divisor::of(p.c.heads);
-        if (p.dtype == kF32) return p.vec ? launch_write_rows_by<kF32, true>(p, stream) : launch_write_rows_by<kF32, false>(p, stream);
-        if (p.dtype == kF16) return p.vec ? launch_write_rows_by<kF16, true>(p, stream) : launch_write_rows_by<kF16, false>(p, stream);
-        return p.vec ? launch_write_rows_by<kBf16, true>(p, stream) : launch_write_rows_by<kBf16, false>(p, stream);
-    }
-    if (p.dtype == kF32) return launch_write_of<kF32>(p, stream);
-    return p.dtype == kF16 ? launch_write_of<kF16>(p, stream) : launch_write_of<kBf16>(p, stream);
+    p.by_q = Divisor::of(std::max(p.q_heads, 1u)), p.by_kv = Divisor::of(p.c.heads);
+    if (p.dtype == kF32) return p.vec ? launch_write_rows_by<kF32, true>(p, stream) : launch_write_rows_by<kF32, false>(p, stream);
+    if (p.dtype == kF16) return p.vec ? launch_write_rows_by<kF16, true>(p, stream) : launch_write_rows_by<kF16, false>(p, stream);
+    return p.vec ? launch_write_rows_by<kBf16, true>(p, stream) : launch_write_rows_by<kBf16, false>(p, stream);
 }
 
 template <bool I4>
