@@ -15,7 +15,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .attention import _call, _elsewhere, _indices
+from .attention import _call, _indices
 from .iq2_matmul import _bail
 
 
