@@ -32,10 +32,10 @@
 //
 // Measured (8 key heads, 128 elements): 128 sequences of up to 4096 tokens, bf16 cache, 214 us: 6260 GB/s, 0.96 of the copy
 // rate; one of 100001 tokens, int8 cache and 8 query heads a key head, 49 us: 4300 GB/s, of which about 8 us are start,
-// merge of the warps and join, and in the stream the widening of the codes binds as well (issue slots 48 % used); 16 of up to
+// merge of the warps and join, and in the stream the widening of the codes binds as well (issue slots 50 % used); 16 of up to
 // 2048, int8, f32 q, 22 us, of which the stream is 7; one of 333 tokens 9.6 us, latencies one after another. 16 of up to
-// 2048, f32 q: 24.2 us over an f16 cache, 28.0 over a bf16 one (the third piece); 64 of up to 4096, int8, bf16 q: 89.8 us with
-// pages of 64 tokens, 102 with 16 or 48 (a tile of 32 tokens then lies in several pages, and each row is looked up). The parts added
+// 2048, f32 q: 24.0 us over an f16 cache, 27.7 over a bf16 one (the third piece); 64 of up to 4096, int8, bf16 q: 91.1 us with
+// pages of 64 tokens, 103 with 16 or 48 (a tile of 32 tokens then lies in several pages, and each row is looked up). The parts added
 // up inside this kernel (by the block that finishes last) instead of by a dependent launch: 11.4 and 53.8 us for the
 // one of 333 and the one of 100001 tokens.
 #include "attention_decode.cuh"

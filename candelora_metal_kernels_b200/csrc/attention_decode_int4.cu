@@ -1,7 +1,7 @@
 // Attention of one new token a sequence over a 4-bit paged cache: the line of work, its parts and their join are those of
 // attention_decode.cu, the products are turned round.
 //
-// A cached element is code g s (iq2_kv_cache): 72 bytes for a row of 128, so that the widening of the codes decides, not HBM. The
+// A cached element is code g s (iq2_kv_cache): 72 bytes for a row of 128, so that widening the codes costs as much as HBM. The
 // products have the tokens (or the values' dimensions) as the sixteen rows of mma.sync m16n8k16 and eight query heads as its columns:
 //   S^T = K Q^T  (32 tokens x 8 heads a warp's tile),  O^T = V^T P^T  (DP dimensions x 8 heads)
 // so that all rows of an accumulator are in use: 32 + 8 registers at 128 elements, half of what heads as rows take, which
@@ -13,11 +13,12 @@
 //     ones of a key row, one group: one wide load and one scale a key. For O a thread's rows are DP / 8 consecutive dimensions, again
 //     one group, of the two tokens whose p it holds; tokens are relabelled so that both kinds of loads are free of bank conflicts.
 //   * q of 32 bits and p are sums of two f16 pieces in one accumulator: q is held times the power of two that brings a head's
-//     largest |q| to 2^12, so that its 22 bits end at 2^-36 of it. q of 16 bits is one piece exactly; p of bf16 q is rounded to f16 once.
+//     largest |q| to 2^12, so that its 22 bits end at 2^-36 of it. q of 16 bits is one piece, which has all bits of bf16 elements down to
+//     2^-29 and of f16 ones down to 2^-26 of the head's largest, and below is off by 2^-37 of that; p of bf16 q is rounded to f16 once.
 //   * The row scales of keys multiply s, those of values multiply p. p next to the largest score's, whose sum is l, ends at 2^-126 as
 //     f32's exponential does, whatever the values; what f16 pieces are taken of is p times the value's row scale times 2^level, a
 //     head's own power of two that makes the largest of these 2^7 to 2^8 (they may grow to 2^15), so that 22 bits end at 2^-31 of the
-//     largest. (The row scales in the reference instead: one exponential less to look at, 2 % faster, but rows of 3e38 lost the tokens below
+//     largest. (With the row scales in the reference instead, a product and a sum less, 2 % faster, rows of 3e38 lost the tokens below
 //     2^-7 of the largest weight, and rows of zeros all of their weight beside rows of 1e9.)
 // The maxima, sums, s, p and o are f32.
 //
@@ -26,11 +27,13 @@
 // item, 143 us for 128 x 4096 tokens in place of 104.)
 //
 // Measured (8 key heads, 128 elements, bf16 q unless said): 128 sequences of up to 4096 tokens 90 us, 4200 GB/s, 0.64 of the copy
-// rate: 685 instructions for a tile of 32 tokens and a key head at 63 % of the issue slots, ALU pipe 50 %, a third of them the
-// widening; 64 of up to 4096 51 us, with f32 q 62 us, with pages of 16 or 48 tokens 56 us, of 64 elements 39 us; one of 100001
-// tokens, 64 query heads, 37 us; 16 of up to 2048, f32 q, 18 us; one of 333 tokens 8.0 us. The first version here, heads as rows
-// as in attention_decode.cu, took 185, 55 and 22.5 us for 128 x 4096, 1 x 100001 and 16 x 2048. Warps of a block: 8 / 11 / 12 / 16
-// 103 / 98 / 93.6 / 95 us for 128 x 4096 (16 spill); tiles of 64 tokens with 8 warps 102 (with 12, of 32, 103 then).
+// rate. Latency binds: 710 instructions for a tile of 32 tokens and a key head are 52 us at full issue, less than HBM's 58, but three
+// warps a scheduler, whose loads, products and exponentials wait for one another, fill 65 % of the issue slots (ALU pipe 48 %).
+// 64 of up to 4096 50.5 us, with f16 q 55.6, with f32 q 61.5, with pages of 16 or 48 tokens 54.6, of 96 / 64 / 32 elements 59.4 / 38.4 /
+// 40; 512 of up to 512 75 us; one of 100001 tokens, 64 query heads, 36 us; 16 of up to 2048, f32 q, 18 us, f16 q 16.6. One of 333
+// tokens 8.0 us where the table has no more than 800 tokens' pages, 9.2 where it has 8192; 18 of up to 760 9.8 and 14.1. The first version here,
+// heads as rows as in attention_decode.cu, took 185, 55 and 22.5 us for 128 x 4096, 1 x 100001 and 16 x 2048. Warps of a block: 8 / 11 /
+// 12 / 16 103 / 98 / 93.6 / 95 us for 128 x 4096 (16 spill); tiles of 64 tokens with 8 warps 102 (with 12, of 32, 103 then).
 #include "attention_decode.cuh"
 
 namespace iq2 {
@@ -161,7 +164,7 @@ __device__ __forceinline__ float* slot_of(uint8_t* smem, uint32_t i) {
 }
 
 // WIDE: q of 32 bits, in two pieces (of 16 bits it is one). FINE: p in two pieces. One piece is for bf16 outputs, which are rounded
-// to 2^-8 of themselves anyway, p to 2^-11: 50.9 us against 55.0 for 64 x 4096 tokens. FULL: head_dim is DP.
+// to 2^-8 of themselves anyway, p to 2^-11: 50.5 us against 55.0 for 64 x 4096 tokens. FULL: head_dim is DP.
 template <int DP, bool WIDE, bool FINE, bool FULL>
 __global__ void __launch_bounds__(A4_THREADS, 1) decode4_kernel(const __grid_constant__ DecodeArgs a) {
     using S = Shape4<DP>;
@@ -645,10 +648,11 @@ cudaError_t launch4_of(const DecodeArgs& a, uint32_t blocks, cudaStream_t stream
 cudaError_t launch_attention_decode_int4(const DecodeParams& p, void* workspace, int num_sms, cudaStream_t stream) {
     DecodeArgs a = decode_args(p, workspace, num_sms);
     // A block an item leaves nothing to join, which saves a launch (2 us on the device and 3 on the host), but its warps wait for
-    // the longest item. It is taken where the SMs have a block for each and the tables allow no more than four tiles a warp, and no more than
-    // two above what the line of work gives (pass of it / of the line: 1 x 760 tokens of 8 key heads 12.2 / 14.3 us, 9 x 350
-    // 12.0 / 14.3, 18 x 1500 15.3 / 17.4; 1 x 1500 14.8 / 14.4, 9 x 2500 20.4 / 16.9, 16 x 2048 21.0 / 20.5, 37 x 350 in
-    // two rounds 16.8 / 16.0).
+    // the longest item. The lengths are on the device, so that the tables' width has to say how long items may be: under a server's
+    // tables, as wide as the longest sequence may become, the line of work is taken. A block an item is taken where the SMs have
+    // a block for each and the tables allow no more than four tiles a warp, and no more than two above what the line of work
+    // gives (calls by it / by the line: 1 x 760 tokens of 8 key heads 12.2 / 14.3 us, 9 x 350 12.0 / 14.3, 18 x 1500 15.3 /
+    // 17.4; 1 x 1500 14.8 / 14.4, 9 x 2500 20.4 / 16.9, 16 x 2048 21.0 / 20.5, 37 x 350 in two rounds 16.8 / 16.0).
     const uint64_t items = (uint64_t)p.batch * p.c.heads * a.chunks_of_heads, sms = num_sms;
     const uint64_t tiles = ((uint64_t)p.table_width * p.c.page_size + A4_TOK - 1) / A4_TOK;  // of a sequence at most
     a.block_an_item = items <= sms && tiles <= 4 * A4_WARPS && tiles * (sms - items) <= 2 * A4_WARPS * sms;

@@ -12,12 +12,12 @@
 // arithmetic: a code is taken from the product with 1 / (s g) and the remainder x - code s g, exact in f32, says where that is off.
 // Norms: y = (x r) w, r = 1 / sqrt(mean(x^2) + eps) summed and taken in 64 bits and rounded to f32, so that r, and with it the
 // codes next to borders, does not depend on the order of the sum.
-// Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 18.3 us over 0.9 GB of inputs and
-// outputs in turn, 4190 GB/s (12.8 over 0.2 GB, where the L2 keeps part of the outputs); of 8800 tokens, f32 into an int8 cache,
-// with the read back 67.5 us, 5380 GB/s; read of 89091 tokens to bf16, of an int8 cache 97 us, 5680 GB/s, of a bf16 one 117 us,
-// 6220 GB/s, of a 4-bit one 85 us, 5510 GB/s, 365 MB of the 467 written. With norms the write of 2048 tokens takes 17.3 us; 8800
-// tokens into a 4-bit cache with the read back 62 us from f32, and 68 us from bf16 with norms, of which the write is 55:
-// instructions, 400 for four rows at two thirds of the issue slots.
+// Measured (8 key heads, 128 elements): write of 2048 tokens with 32 query heads, f32 to bf16, 12.3 us over 0.9 GB of inputs and
+// outputs in turn, 6240 GB/s (10.7 over 0.2 GB, where the L2 keeps part of the outputs), with norms 15.9 us, as into an int8 cache
+// (bf16 to bf16 11.1 and 14.2); of 8800 tokens, f32 into an int8 cache, with the read back 61 us, 5960 GB/s, into a 4-bit cache 61 us, from
+// bf16 or f16 55 us, from bf16 with norms 66 us, of which the write is 55: with 36 warps an SM it waits for its loads in between (73 %
+// of the issue slots, 403 instructions for four rows). Read of 89091 tokens to bf16: of an int8 cache 96 us, 5750 GB/s, of a bf16 one
+// 117 us, 6220 GB/s, of a 4-bit one 84 us, 5550 GB/s, 365 MB of the 467 written.
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"
 

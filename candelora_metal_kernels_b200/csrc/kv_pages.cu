@@ -12,7 +12,7 @@
 // state is still the old one, and a barrier stands between that and what is written of the new state. A step of many tokens
 // takes a cluster of blocks for the pages, each of which works the sums out for itself, and a dependent launch over all SMs for the
 // slots, from the new table (in the cluster they took 30000 cycles of eight SMs' instructions for 123099 tokens). Measured on the
-// device: 64 sequences of five tokens 4.5 us, 512 of one 6.5 us, 123099 tokens of 96 prompts over 6265 pages 9.8 us (8.1, 8.9
+// device: 64 sequences of five tokens 4.4 us, 512 of one 6.0 us, 123099 tokens of 96 prompts over 6265 pages 9.1 us (8.1, 8.9
 // and 20.4 us by one kernel with a scan for each sum that reads the pages behind the barrier).
 #include "attention_internal.h"
 #include "iq2xxs_common.cuh"

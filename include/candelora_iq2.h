@@ -403,7 +403,8 @@ size_t iq2_attention_decode_workspace_size(const iq2_kv_cache* cache, uint32_t b
 /*
  * out = softmax(scale q k^T) v, any q type over any cache type; scores, maxima, sums and accumulation
  * in f32, q and the probabilities as sums of two 16-bit pieces (three for f32 q over a bf16 cache; over
- * IQ2_KV_INT4 a 16-bit q is one, and its probabilities are rounded to f16 once).
+ * IQ2_KV_INT4 a 16-bit q is one, and the probabilities of bf16 q are rounded to f16 once). Tokens whose
+ * probability is below 2^-126 of a head's largest take no part, whatever their values.
  * A sequence of length 0 gets zeros.
  */
 int iq2_attention_decode(const iq2_kv_cache* cache, const iq2_attention_tokens* tokens, void* workspace,
